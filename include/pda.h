@@ -557,6 +557,90 @@ int pda_paged_prefill_attention_q8(const void* queries, const void* keys,
                                    int32_t splits, void* workspace,
                                    size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Latent attention: attention over one shared latent vector per token. No
+ * counterpart in the reference (its attention layers keep keys and values per
+ * kv head, paged_kv.py:156-292); the paging, the write-before-attend order and
+ * the masking of released pages are those of the calls above.
+ *
+ *   arena    [arena_rows, latent_dim + rope_dim] fp16 (bf16 in the _bf16
+ *            entries): a token's row holds its latent c and a rotated key k
+ *            that all heads share; a page is page_size consecutive rows
+ *   kv_b     [q_heads, nope_dim + value_dim, latent_dim], the up projection:
+ *            U_h (nope_dim rows), then D_h (value_dim rows) of each head
+ *   queries  [.., q_heads, nope_dim + rope_dim], the last rope_dim rotated
+ * Head h's key is [U_h c ; k], its value D_h c; score = scale * q.key. Latents
+ * of 8..512 dims (multiples of 8), rotary parts of 0..64 dims (multiples of
+ * 16), nope_dim and value_dim of 8..128 (multiples of 8); else
+ * PDA_ERR_HEAD_DIM. Any number of query heads and any page size.
+ * ------------------------------------------------------------------------- */
+
+/* The step before either attention call, one launch for n tokens:
+ *   arena[rows[i]] = [latent_i / rms(latent_i) * norm_weight ; rope(k_rope_i)]
+ *   q_out[i, h]    = [nope part ; rope(rotary part)]
+ * rms(x) = sqrt(mean(x^2) + eps), in float32, one rounding per element;
+ * norm_weight NULL stores the latents as they are. The rotation is
+ * pda_rope_append's (element i < rope_dim / 2 pairs with i + rope_dim / 2,
+ * angle float(position) * inv_freq[i], separately rounded float32 products);
+ * inv_freq NULL: none. Row i of latent and of k_rope starts latent_stride and
+ * k_stride elements (multiples of 8) after the row before, so the two may be
+ * columns of one projection's output. q and q_out (which may be q) both NULL:
+ * no queries; latent, k_rope, arena and rows all NULL: no write. Rows outside
+ * [0, arena_rows) are not written; no two tokens may name one row. No
+ * workspace. */
+int pda_latent_append(const void* q, void* q_out, const void* latent,
+                      int64_t latent_stride, const void* k_rope, int64_t k_stride,
+                      const void* norm_weight, float eps, void* arena,
+                      const int32_t* positions, const int32_t* rows, int32_t n,
+                      int32_t q_heads, int32_t latent_dim, int32_t rope_dim,
+                      int32_t nope_dim, int64_t arena_rows, const float* inv_freq,
+                      void* stream);
+int pda_latent_append_bf16(const void* q, void* q_out, const void* latent,
+                           int64_t latent_stride, const void* k_rope,
+                           int64_t k_stride, const void* norm_weight, float eps,
+                           void* arena, const int32_t* positions,
+                           const int32_t* rows, int32_t n, int32_t q_heads,
+                           int32_t latent_dim, int32_t rope_dim, int32_t nope_dim,
+                           int64_t arena_rows, const float* inv_freq, void* stream);
+
+/* Bytes of workspace of a latent decode call (no initialisation, nothing kept
+ * between calls). `longest` as for the call. */
+int pda_latent_decode_workspace_bytes(int32_t batch, int32_t q_heads,
+                                      int32_t latent_dim, int32_t rope_dim,
+                                      int32_t page_size, int32_t table_stride,
+                                      int32_t longest, size_t* bytes);
+
+/* Decode attention over latent rows, one new token per sequence, in the
+ * absorbed form: the queries are projected into the latent (U_h^T q, rounded
+ * to the element type), all heads attend over the rows themselves, and D_h is
+ * applied to what comes out.
+ *   queries [batch, q_heads, nope_dim + rope_dim], out [batch, q_heads,
+ *   value_dim]; tables, lengths, page_size, longest and the masking of
+ *   negative or unknown pages as for pda_paged_decode_attention; a sequence
+ *   with no key to see gives zeros. arena_rows below 2^31.
+ * The split points follow from the shapes, `longest` and the lengths: repeated
+ * calls give the same bits. Three launches on `stream`; calls that share a
+ * workspace must not overlap. */
+int pda_latent_decode_attention(const void* queries, const void* arena,
+                                const void* kv_b, const int32_t* tables,
+                                const int32_t* lengths, void* out, int32_t batch,
+                                int32_t q_heads, int32_t latent_dim,
+                                int32_t rope_dim, int32_t nope_dim,
+                                int32_t value_dim, int32_t page_size,
+                                int32_t table_stride, int64_t arena_rows,
+                                int32_t longest, float scale, void* workspace,
+                                size_t workspace_bytes, void* stream);
+int pda_latent_decode_attention_bf16(const void* queries, const void* arena,
+                                     const void* kv_b, const int32_t* tables,
+                                     const int32_t* lengths, void* out,
+                                     int32_t batch, int32_t q_heads,
+                                     int32_t latent_dim, int32_t rope_dim,
+                                     int32_t nope_dim, int32_t value_dim,
+                                     int32_t page_size, int32_t table_stride,
+                                     int64_t arena_rows, int32_t longest,
+                                     float scale, void* workspace,
+                                     size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

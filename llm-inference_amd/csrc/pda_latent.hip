@@ -1,0 +1,942 @@
+// Latent attention for MI355X (gfx950): the append of latent rows and the
+// decode attention over them in the absorbed form, C-ABI in pda.h
+// (pda_latent_append, pda_latent_decode_attention). No reference counterpart:
+// the reference keeps keys and values per kv head.
+//
+// A token's cache row is [c | k]: its normalised latent c (latent_dim wide),
+// from which every head's keys and values are projected, and one rotated key k
+// (rope_dim wide) that all heads share. With W_h = kv_b[h] = [U_h; D_h]
+// (nope_dim and value_dim rows over the latent) head h has
+//   key(t) = [U_h c_t ; k_t],  value(t) = D_h c_t,
+//   score(t) = scale (q_nope . U_h c_t + q_rope . k_t).
+// Absorbed: q_nope . U_h c = (U_h^T q_nope) . c, and the weighted values are
+// D_h applied once to the weighted latents. So a step projects its queries
+// (latent_absorb_kernel), attends over the rows themselves, all heads from one
+// read (latent_decode_kernel), and projects what comes out
+// (latent_merge_kernel, which joins the parts of a sequence on the way).
+
+#include <algorithm>
+#include <type_traits>
+#include <utility>
+
+#include "pda_latent.h"
+
+namespace {
+
+using namespace pda_latent;
+using pda_internal::fail;
+using pda_internal::ok;
+
+// ---------------------------------------------------------------------------
+// Append.
+
+constexpr int kAppendHeads = 16;  // query heads of one token a workgroup takes
+
+struct LatentAppendParams {
+  const f16* q;       // [n, hq, nope + rope], or null
+  f16* q_out;
+  const f16* c;       // [n, latent], rows c_stride apart
+  const f16* k;       // [n, rope], rows k_stride apart
+  const f16* norm;    // [latent], or null: latents are stored as they are
+  f16* arena;         // [arena_rows, latent + rope]
+  const int32_t* positions;
+  const int32_t* rows;
+  const float* inv_freq;  // [rope / 2], or null: no rotation
+  int64_t c_stride;
+  int64_t k_stride;
+  int64_t arena_rows;
+  int32_t n;
+  int32_t hq;
+  int32_t latent;
+  int32_t rope;
+  int32_t nope;
+  int32_t head_groups;  // workgroups of query heads per token
+  float eps;
+};
+
+// The rotation of 8 pairs (a[i], b[i]) by the angles whose cosines and sines
+// are given: separately rounded float32 products and sums, as the other
+// append's, rounded to the element type.
+template <bool BF>
+__device__ __forceinline__ void rotate(f16x8& a, f16x8& b, const float* cs, const float* sn) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float x = widen<BF>(a[i]), y = widen<BF>(b[i]);
+    a[i] = round16<BF>(__fsub_rn(__fmul_rn(x, cs[i]), __fmul_rn(y, sn[i])));
+    b[i] = round16<BF>(__fadd_rn(__fmul_rn(y, cs[i]), __fmul_rn(x, sn[i])));
+  }
+}
+
+// The first workgroups write the rows, a wave a token (a lane 8 latent dims);
+// the others rotate the queries, kAppendHeads heads of a token each, in
+// 16-byte pieces: a piece of the nope part is copied (left alone when q_out is
+// q), a pair of pieces half the rotary part apart is rotated. A token's angles
+// are computed once a workgroup. Moves every byte once.
+template <bool BF>
+__global__ __launch_bounds__(256) void latent_append_kernel(const LatentAppendParams p) {
+  __shared__ float s_cos[4][kMaxRope / 2], s_sin[4][kMaxRope / 2];
+  const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
+  const int half = p.rope / 2;
+  const int row_groups = p.c ? (p.n + 3) / 4 : 0;
+  auto angles = [&](int token, int slot, int i) {
+    if (i < half) {
+      float sn, cs;
+      sincosf(__fmul_rn((float)p.positions[token], p.inv_freq[i]), &sn, &cs);
+      s_cos[slot][i] = cs;
+      s_sin[slot][i] = sn;
+    }
+  };
+  if ((int)blockIdx.x < row_groups) {
+    const int token = blockIdx.x * 4 + w;
+    const bool live = token < p.n;
+    if (live && p.inv_freq) angles(token, w, lane);
+    __syncthreads();
+    if (!live) return;
+    const int64_t row = p.rows[token];
+    if (row < 0 || row >= p.arena_rows) return;
+    f16* dst = p.arena + row * (p.latent + p.rope);
+    const bool mine = 8 * lane < p.latent;
+    f16x8 x = {};
+    if (mine) x = *reinterpret_cast<const f16x8*>(p.c + token * p.c_stride + 8 * lane);
+    if (p.norm) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum = fmaf(widen<BF>(x[i]), widen<BF>(x[i]), sum);
+#pragma unroll
+      for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+      const float r = 1.0f / sqrtf(sum / (float)p.latent + p.eps);
+      if (mine) {
+        const f16x8 g = *reinterpret_cast<const f16x8*>(p.norm + 8 * lane);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = round16<BF>(widen<BF>(x[i]) * r * widen<BF>(g[i]));
+      }
+    }
+    if (mine) *reinterpret_cast<f16x8*>(dst + 8 * lane) = x;
+    if (8 * lane < half) {
+      const f16* src = p.k + token * p.k_stride;
+      f16x8 a = *reinterpret_cast<const f16x8*>(src + 8 * lane);
+      f16x8 b = *reinterpret_cast<const f16x8*>(src + half + 8 * lane);
+      if (p.inv_freq) rotate<BF>(a, b, &s_cos[w][8 * lane], &s_sin[w][8 * lane]);
+      *reinterpret_cast<f16x8*>(dst + p.latent + 8 * lane) = a;
+      *reinterpret_cast<f16x8*>(dst + p.latent + half + 8 * lane) = b;
+    }
+    return;
+  }
+  const int item = blockIdx.x - row_groups;
+  const int token = item / p.head_groups, h0 = (item % p.head_groups) * kAppendHeads;
+  if (p.inv_freq) {
+    angles(token, 0, tid);
+    __syncthreads();
+  }
+  const int heads = min(kAppendHeads, p.hq - h0);
+  const int width = p.nope + p.rope;
+  const int64_t at = ((int64_t)token * p.hq + h0) * width;
+  const int pairs = half / 8, pieces = p.nope / 8 + pairs;  // a head's work items
+  const bool in_place = p.q == p.q_out;
+  for (int i = tid; i < heads * pieces; i += 256) {
+    const int h = i / pieces, j = i - h * pieces;
+    if (j >= pairs) {
+      const int64_t e = at + h * width + 8 * (j - pairs);
+      if (!in_place)
+        *reinterpret_cast<f16x8*>(p.q_out + e) = *reinterpret_cast<const f16x8*>(p.q + e);
+      continue;
+    }
+    const int64_t e = at + h * width + p.nope + 8 * j;
+    f16x8 a = *reinterpret_cast<const f16x8*>(p.q + e);
+    f16x8 b = *reinterpret_cast<const f16x8*>(p.q + e + half);
+    if (p.inv_freq) rotate<BF>(a, b, &s_cos[0][8 * j], &s_sin[0][8 * j]);
+    *reinterpret_cast<f16x8*>(p.q_out + e) = a;
+    *reinterpret_cast<f16x8*>(p.q_out + e + half) = b;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Decode.
+
+constexpr int kTileKeys = 32;     // keys per tile
+constexpr int kChunkTiles = 64;   // tiles whose rows are looked up at once
+constexpr int kChunkKeys = kTileKeys * kChunkTiles;
+constexpr int kMaxGroups = 256;   // workgroups of a launch: one per CU of an MI355X
+constexpr float kSlack = 8.0f;    // scores may pass the running max by 2^8
+
+struct LatentDecodeParams {
+  const f16* q;          // [batch, hq, nope + rope]
+  const f16* kv_b;       // [hq, nope + value, latent]
+  const f16* arena;      // [arena_rows, latent + rope]
+  const int32_t* tables; // [batch, table_stride]
+  const int32_t* lengths;
+  f16* out;              // [batch, hq, value]
+  f16* q_lat;            // [batch, hq, latent + rope]: absorbed queries
+  int32_t* prefix;       // [batch + 1] tiles before each sequence
+  float* part_o;         // [groups + batch, hq, latent] unnormalised partial sums
+  float2* part_ml;       // [groups + batch, hq] (running max, sum)
+  int64_t arena_pages;
+  int32_t table_stride;
+  int32_t page_size;
+  int32_t batch;
+  int32_t hq;
+  int32_t latent;
+  int32_t rope;
+  int32_t nope;
+  int32_t value;
+  int32_t groups;        // workgroups the stream of tiles is cut over
+  int32_t merge_batch;   // sequences a merge workgroup takes
+  float scale_log2;
+};
+
+__device__ __forceinline__ int64_t keys_of(const LatentDecodeParams& p, int b) {
+  const int64_t cap = (int64_t)p.table_stride * p.page_size;
+  return max((int64_t)0, min((int64_t)p.lengths[b], cap));
+}
+
+// Queries into the latent: q_lat[b, h] = [U_h^T q_nope | q_rope], rounded to
+// the element type (the matrix cores take 16-bit operands; the products and
+// their sum are float32). As products: (U_h^T) (32 latent dims x nope) by
+// (q_nope)^T (nope x 32 sequences); a wave has 32 latent dims, whose columns of
+// U_h it keeps in LDS and reads transposed. U_h is read once per 32 sequences.
+// The first workgroup also leaves the sequences' tile prefix for the kernels
+// after it.
+template <bool BF>
+__global__ __launch_bounds__(256) void latent_absorb_kernel(const LatentDecodeParams p) {
+  __shared__ __align__(1024) f16 s_u[4][kMaxHead * 32];
+  __shared__ int s_scan[256];
+  const int tid = threadIdx.x, w = uniform(tid >> 6), lane = tid & 63;
+  const int n = lane & 31, hh = lane >> 5;
+  const int h = blockIdx.y, b0 = blockIdx.z * 32;
+  if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) {
+    const int each = (p.batch + 255) / 256, first = min(tid * each, p.batch);
+    const int end = min(first + each, p.batch);
+    int sum = 0;
+    for (int b = first; b < end; ++b) sum += (int)((keys_of(p, b) + kTileKeys - 1) / kTileKeys);
+    s_scan[tid] = sum;
+    __syncthreads();
+    for (int d = 1; d < 256; d <<= 1) {
+      const int x = tid >= d ? s_scan[tid - d] : 0;
+      __syncthreads();
+      s_scan[tid] += x;
+      __syncthreads();
+    }
+    int at = s_scan[tid] - sum;
+    for (int b = first; b < end; ++b) {
+      p.prefix[b] = at;
+      at += (int)((keys_of(p, b) + kTileKeys - 1) / kTileKeys);
+    }
+    if (tid == 255) p.prefix[p.batch] = s_scan[255];
+  }
+  const int width = p.latent + p.rope, qwidth = p.nope + p.rope;
+  if (blockIdx.x == 0) {
+    // The rotary part is copied.
+    const int pieces = p.rope / 8;
+    for (int i = tid; i < 32 * pieces; i += 256) {
+      const int b = b0 + i / pieces, j = i % pieces;
+      if (b < p.batch) {
+        const int64_t e = (int64_t)b * p.hq + h;
+        *reinterpret_cast<f16x8*>(p.q_lat + e * width + p.latent + 8 * j) =
+            *reinterpret_cast<const f16x8*>(p.q + e * qwidth + p.nope + 8 * j);
+      }
+    }
+  }
+  const int d0 = (blockIdx.x * 4 + w) * 32;
+  if (d0 >= p.latent) return;
+  // The wave's columns of U_h: rows of 64 bytes, zeros past either edge.
+  const f16* u = p.kv_b + (int64_t)h * (p.nope + p.value) * p.latent;
+  const int steps = (p.nope + 15) / 16;
+  const int col = d0 + 8 * (lane & 3);
+  f16x8 rows[kMaxHead / 16];
+#pragma unroll
+  for (int i = 0; i < kMaxHead / 16; ++i) {
+    const int r = 16 * i + (lane >> 2);
+    rows[i] = f16x8{};
+    if (r < p.nope && col < p.latent)
+      rows[i] = *reinterpret_cast<const f16x8*>(u + (int64_t)r * p.latent + col);
+  }
+  const bool live = b0 + n < p.batch;
+  const f16* qp = p.q + ((int64_t)(live ? b0 + n : 0) * p.hq + h) * qwidth + 4 * hh;
+  f16x8 qf[kMaxHead / 16];
+#pragma unroll
+  for (int i = 0; i < kMaxHead / 16; ++i) {
+    f16x4 lo = {}, hi = {};
+    if (live && 16 * i < p.nope) lo = *reinterpret_cast<const f16x4*>(qp + 16 * i);
+    if (live && 16 * i + 8 < p.nope) hi = *reinterpret_cast<const f16x4*>(qp + 16 * i + 8);
+    qf[i] = f16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  }
+  f16* su = s_u[w];
+#pragma unroll
+  for (int i = 0; i < kMaxHead / 16; ++i)
+    *reinterpret_cast<f16x8*>(su + (16 * i + (lane >> 2)) * 32 + 8 * (lane & 3)) = rows[i];
+  // (The wave's own rows: its LDS writes are done before its reads.)
+  const int g16 = lane >> 4, s16 = lane & 15;
+  const f16* vp = su + (4 * (g16 >> 1) + (s16 >> 2)) * 32 + 16 * (g16 & 1) + 4 * (s16 & 3);
+  f32x16 acc = {};
+  for (int i = 0; i < kMaxHead / 16; ++i) {
+    if (i >= steps) break;
+    const f16x4 lo = read_tr(vp + 512 * i), hi = read_tr(vp + 512 * i + 256);
+    f16x8 q8 = qf[0];
+#pragma unroll
+    for (int j = 1; j < kMaxHead / 16; ++j)
+      if (i == j) q8 = qf[j];
+    acc = mfma16<BF>(f16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}, q8, acc);
+  }
+  if (!live) return;
+  f16* dst = p.q_lat + ((int64_t)(b0 + n) * p.hq + h) * width + d0 + 4 * hh;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    if (d0 + 8 * g >= p.latent) break;
+    f16x4 y;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) y[t] = round16<BF>(acc[4 * g + t]);
+    *reinterpret_cast<f16x4*>(dst + 8 * g) = y;
+  }
+}
+
+// Attention over the latent rows. The tiles (32 keys) of all sequences form
+// one stream, cut into `groups` equal ranges, so that ragged batches and single
+// long sequences load the CUs alike; a workgroup walks its range and writes one
+// partial (max, sum, weighted latents) per sequence it meets, to slot group +
+// sequence (both only grow along the stream, so no two share one).
+//
+// A wave holds 32 heads entire: queries (72 half2 a lane at 512 + 64 dims) and
+// weighted latents (32 x 512 in 256 accumulator registers), so the weights go
+// from the scores' registers to the next product without LDS: scores S^T = K
+// Q^T leave a lane 16 keys of one head, which are the B operand of O^T += V^T
+// P^T when V's rows are read in that order (two transposed reads). K and V are
+// the same rows: one copy in LDS serves both, swizzled in 16-byte pieces by
+// the row's group of four, which both reads undo.
+// NHG: waves side by side over heads, sharing a tile; 4 / NHG groups of waves
+// take tiles in turn. The LDS holds four tiles: a ring of NHG per group.
+template <int WP, int OB, int NHG, bool BF>
+__global__ __launch_bounds__(256, 1) void latent_decode_kernel(const LatentDecodeParams p) {
+  constexpr int kGroups = 4 / NHG;           // tiles under way side by side
+  constexpr int kPlane = kTileKeys * 32;     // halves of a 64-byte column plane
+  constexpr int kTile = WP * kPlane;
+  constexpr int kPitch = 132;                // floats of a head's 128 dims
+  constexpr int kAhead = 4;                  // operands read early
+  __shared__ __align__(1024) f16 s_t[4][kTile];
+  __shared__ int s_row[kChunkKeys];
+  __shared__ float2 s_ml[4][32];
+  __shared__ int s_at[4];
+  static_assert(4 * 32 * kPitch * 4 <= sizeof(s_t), "the joined sums use the tiles' LDS");
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = uniform(tid >> 6);
+  const int n = lane & 31, hh = lane >> 5;
+  const int hg = w % NHG, kg = w / NHG;
+  const int head0 = blockIdx.y * 32 * NHG;
+  const int h = head0 + 32 * hg + n;
+  const bool live = h < p.hq;
+  const int width = p.latent + p.rope;
+
+  const int total = p.prefix[p.batch];
+  const int per = (int)(((int64_t)total + p.groups - 1) / p.groups);
+  const int64_t from = (int64_t)blockIdx.x * per;
+  if (from >= total) return;
+  const int t0 = (int)from, t1 = (int)min((int64_t)total, from + per);
+  // The sequence that holds tile t0: those that end at or before it lie before it.
+  int before = 0;
+  for (int i = tid; i < p.batch; i += 256) before += p.prefix[i + 1] <= t0 ? 1 : 0;
+#pragma unroll
+  for (int d = 32; d; d >>= 1) before += __shfl_xor(before, d);
+  if (lane == 0) s_at[w] = before;
+  __syncthreads();
+  int b = uniform(s_at[0] + s_at[1] + s_at[2] + s_at[3]);
+
+  const int ksw = (n >> 2) & 3;
+  const int k_lane0 = 32 * n + 8 * (hh ^ ksw);
+  const int k_lane1 = 32 * n + 8 * ((2 + hh) ^ ksw);
+  const int g16 = lane >> 4, s16 = lane & 15;
+  const int vc = 2 * (g16 & 1) + ((s16 & 3) >> 1);  // 16-byte piece of the plane's row
+  const int v_row = 4 * hh + (s16 >> 2);
+  const int v_lo = 32 * v_row + 8 * (vc ^ hh) + 4 * (s16 & 1);
+  const int v_hi = 32 * (v_row + 8) + 8 * (vc ^ (2 + hh)) + 4 * (s16 & 1);
+  // The copies: lane i of an instruction moves row i / 4 (of 16), one 16-byte
+  // piece; pieces past the row's end (widths below the kernel's) are another
+  // piece of the row, whose query elements are zeros.
+  const int piece = (lane & 3) ^ ((lane >> 4) & 3);
+  const int last_piece = width / 8 - 1;
+  const bool whole = width == 32 * WP;
+  auto each_plane = [&](auto f) {
+    each(f, std::make_integer_sequence<int, (WP + NHG - 1) / NHG>{});
+  };
+  const uint32_t lds = uniform(lds_address(&s_t[0][0]));
+  const uint32_t pages = (uint32_t)min(p.arena_pages, (int64_t)INT32_MAX);
+
+  while (b < p.batch) {
+    const int seq0 = uniform(p.prefix[b]);
+    if (seq0 >= t1) break;
+    const int seq1 = uniform(p.prefix[b + 1]);
+    const int ta = max(t0, seq0) - seq0, tb = min(t1, seq1) - seq0;
+    if (ta >= tb) {  // an empty sequence
+      ++b;
+      continue;
+    }
+    const int keys = (int)keys_of(p, b);
+    f16x8 qf[2 * WP];
+    {
+      const f16* qp = p.q_lat + ((int64_t)b * p.hq + (live ? h : 0)) * width;
+#pragma unroll
+      for (int c = 0; c < 2 * WP; ++c) {
+        const int d = 16 * c + 8 * hh;
+        const f16x8 x = *reinterpret_cast<const f16x8*>(qp + min(d, width - 8));
+        qf[c] = live && d < width ? x : f16x8{};
+      }
+    }
+    f32x16 o[OB];
+#pragma unroll
+    for (int i = 0; i < OB; ++i) o[i] = f32x16{};
+    outputs_settle(o);
+    float m = -INFINITY, l = 0.0f;
+
+    for (int c0 = ta; c0 < tb; c0 += kChunkTiles) {
+      const int tiles = min(kChunkTiles, tb - c0);
+      // Arena rows of the chunk's keys; -1: no such key, or no such page.
+      __syncthreads();
+      for (int i = tid; i < tiles * kTileKeys; i += 256) {
+        const int key = c0 * kTileKeys + i;
+        int row = -1;
+        if (key < keys) {
+          const uint32_t pi = (uint32_t)key / (uint32_t)p.page_size;
+          const uint32_t page = (uint32_t)p.tables[(int64_t)b * p.table_stride + pi];
+          if (page < pages) row = (int)(page * (uint32_t)p.page_size + (key - pi * p.page_size));
+        }
+        s_row[i] = row;
+      }
+      __syncthreads();
+      // Tile `tile` of the chunk into slot `slot` of the wave's ring: this
+      // wave's planes.
+      auto copy = [&](int tile, int slot) {
+        const uint32_t dst = lds + (kg * NHG + slot) * (2 * kTile) + hg * (2 * kPlane);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int row = s_row[tile * kTileKeys + 16 * i + (lane >> 2)];
+          const f16* src = p.arena + (int64_t)max(row, 0) * width;
+          if (whole) {
+            each_plane([&](auto j) {
+              if (NHG * j.value + hg < WP)
+                copy_to_lds<64 * NHG * j.value, (2 * kPlane - 64) * NHG * j.value>(
+                    src + 32 * hg + 8 * piece, dst + 1024 * i);
+            });
+          } else {
+#pragma unroll 1
+            for (int j = 0; NHG * j + hg < WP; ++j)
+              copy_to_lds<0, 0>(src + 8 * min(4 * (NHG * j + hg) + piece, last_piece),
+                                dst + j * (NHG * 2 * kPlane) + 1024 * i);
+          }
+        }
+      };
+      // Rows of no key become zeros once they have landed (their weight is 0;
+      // zero rows keep 0 * V finite whatever the arena holds).
+      auto clean = [&](int tile, int slot) {
+        f16* t = s_t[kg * NHG + slot] + hg * kPlane;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (s_row[tile * kTileKeys + 16 * i + (lane >> 2)] >= 0) continue;
+          for (int j = 0; NHG * j + hg < WP; ++j)
+            *reinterpret_cast<f16x8*>(t + j * (NHG * kPlane) + 512 * i + 8 * lane) = f16x8{};
+        }
+      };
+      auto math = [&](int tile, int slot) {
+        const f16* t = s_t[kg * NHG + slot];
+        const uint32_t okm =
+            (uint32_t)__ballot(s_row[tile * kTileKeys + n] >= 0);
+        // Operands are read kAhead products early (the reads and products
+        // would else wait for each other in turn).
+        f32x16 s = {};
+        f16x8 a[2 * WP];
+        auto read_k = [&](int c) {
+          a[c] = *reinterpret_cast<const f16x8*>(t + (c & 1 ? k_lane1 : k_lane0) +
+                                                 kPlane * (c >> 1));
+        };
+#pragma unroll
+        for (int c = 0; c < kAhead; ++c) read_k(c);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int c = 0; c < 2 * WP; ++c) {
+          s = mfma16<BF>(a[c], qf[c], s);
+          if (c + kAhead < 2 * WP) read_k(c + kAhead);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        f16x8 va[2 * OB];
+        auto read_v = [&](int j) {
+          const f16* vp = t + kPlane * (j % OB) + 512 * (j / OB);
+          const f16x4 lo = read_tr(vp + v_lo), hi = read_tr(vp + v_hi);
+          va[j] = f16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        };
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) read_v(j);
+#pragma unroll
+        for (int v = 0; v < 16; ++v) s[v] *= p.scale_log2;
+        if (okm != 0xFFFFFFFFu) {
+          const uint32_t see = okm >> (4 * hh);
+#pragma unroll
+          for (int v = 0; v < 16; ++v)
+            if (!(see >> (8 * (v / 4) + v % 4) & 1)) s[v] = -INFINITY;
+        }
+        float top = s[0];
+#pragma unroll
+        for (int v = 1; v < 16; ++v) top = fmaxf(top, s[v]);
+        top = fmaxf(top, __shfl_xor(top, 32));
+        if (__ballot(top > m + kSlack)) {
+          float f = 1.0f;
+          if (top > m + kSlack) {
+            f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+            m = top;
+            l *= f;
+          }
+          outputs_settle(o);
+#pragma unroll
+          for (int i = 0; i < OB; ++i) {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) o[i][v] *= f;
+            asm volatile("" : "+a"(o[i]));
+          }
+        }
+        const float mu = m == -INFINITY ? 0.0f : m;
+        f16x8 pb[2];
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          pb[v / 8][v % 8] = round16<BF>(__builtin_amdgcn_exp2f(s[v] - mu));
+#pragma unroll
+        for (int v = 0; v < 16; v += 2) l = add_pair<BF>(pb[v / 8][v % 8], pb[v / 8][v % 8 + 1], l);
+        operands_settle(pb);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < 2 * OB; ++j) {
+          mfma_acc<BF>(va[j], pb[j / OB], o[j % OB]);
+          if (j + kAhead < 2 * OB) read_v(j + kAhead);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      };
+      const int rounds = (tiles + kGroups - 1) / kGroups;
+      // Copies of the first ring - 1 rounds; then per round: this round's rows
+      // have landed, everyone is past the round before, whose slot takes the
+      // next copies.
+      constexpr int kFirst = NHG > 1 ? NHG - 1 : 1;
+      for (int r = 0; r < min(kFirst, rounds); ++r)
+        if (r * kGroups + kg < tiles) copy(r * kGroups + kg, r % NHG);
+      for (int r = 0; r < rounds; ++r) {
+        const int tile = r * kGroups + kg;
+        const bool here = tile < tiles;
+        wait_vmem<0>();
+        if (here) clean(tile, r % NHG);
+        if constexpr (NHG > 1) {
+          __syncthreads();
+          const int next = tile + kFirst * kGroups;
+          if (next < tiles) copy(next, (r + kFirst) % NHG);
+        }
+        if (here) math(tile, r % NHG);
+        wait_lds();
+        if constexpr (NHG == 1)
+          if (tile + kGroups < tiles) copy(tile + kGroups, 0);
+      }
+    }
+
+    // One partial of the wave groups' sums: each scaled to their common max,
+    // 128 dims a round through LDS, added and written along the rows.
+    outputs_settle(o);
+    l += __shfl_xor(l, 32);
+    if (hh == 0) s_ml[w][n] = make_float2(m, l);
+    __syncthreads();
+    float mm = -INFINITY, ll = 0.0f;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) mm = fmaxf(mm, s_ml[g * NHG + hg][n].x);
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      const float2 x = s_ml[g * NHG + hg][n];
+      if (x.x != -INFINITY) ll += x.y * __builtin_amdgcn_exp2f(x.x - mm);
+    }
+    const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mm);
+    const int64_t slot = (int64_t)blockIdx.x + b;
+    if (kg == 0 && hh == 0 && live) p.part_ml[slot * p.hq + h] = make_float2(mm, ll);
+    float* join = reinterpret_cast<float*>(&s_t[0][0]);
+#pragma unroll
+    for (int q = 0; q < OB / 4; ++q) {
+      const int d0 = 128 * q;
+      if (d0 >= p.latent) break;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f32x16& x = o[4 * q + i];
+        asm volatile("" : "+a"(x));
+        float* at = join + (32 * w + n) * kPitch + 32 * i + 4 * hh;
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<float4*>(at + 8 * g) =
+              make_float4(x[4 * g] * f, x[4 * g + 1] * f, x[4 * g + 2] * f, x[4 * g + 3] * f);
+      }
+      __syncthreads();
+      for (int i = tid; i < 32 * NHG * 32; i += 256) {
+        const int hd = i / 32, d = 4 * (i % 32);
+        float4 x = *reinterpret_cast<const float4*>(join + hd * kPitch + d);
+#pragma unroll
+        for (int g = 1; g < kGroups; ++g) {
+          const float4 y =
+              *reinterpret_cast<const float4*>(join + (32 * NHG * g + hd) * kPitch + d);
+          x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+        }
+        if (head0 + hd < p.hq && d0 + d < p.latent)
+          *reinterpret_cast<float4*>(p.part_o + (slot * p.hq + head0 + hd) * p.latent + d0 + d) = x;
+      }
+    }
+    __syncthreads();
+    ++b;
+  }
+}
+
+// Joins the partials of each sequence and projects the result: out[b, h] = D_h
+// o / sum. A workgroup has one head and up to 32 sequences; the joined latents
+// go to LDS as two 16-bit numbers each (the value and what its rounding left),
+// so the product with D_h loses nothing that the output's rounding would show;
+// a wave takes 32 value dims at a time. D_h is read once a workgroup.
+template <bool BF>
+__global__ __launch_bounds__(256) void latent_merge_kernel(const LatentDecodeParams p) {
+  constexpr int kRow = kMaxLatent + 8;  // halves between sequences
+  __shared__ __align__(16) f16 s_hi[32 * kRow];
+  __shared__ __align__(16) f16 s_lo[32 * kRow];
+  const int tid = threadIdx.x, w = uniform(tid >> 6), lane = tid & 63;
+  const int n = lane & 31, hh = lane >> 5;
+  const int h = blockIdx.x, b0 = blockIdx.y * p.merge_batch;
+  const int count = min(p.merge_batch, p.batch - b0);
+  const int total = p.prefix[p.batch];
+  const int per = max(1, (int)(((int64_t)total + p.groups - 1) / p.groups));
+  for (int i = tid; i < count * (p.latent / 8); i += 256) {
+    const int r = i / (p.latent / 8), d = 8 * (i % (p.latent / 8));
+    const int b = b0 + r;
+    const int seq0 = p.prefix[b], seq1 = p.prefix[b + 1];
+    const int g0 = seq0 / per, g1 = seq1 > seq0 ? (seq1 - 1) / per : g0 - 1;
+    float top = -INFINITY, sum = 0.0f;
+    for (int g = g0; g <= g1; ++g)
+      top = fmaxf(top, p.part_ml[((int64_t)g + b) * p.hq + h].x);
+    float acc[8] = {};
+    if (top != -INFINITY) {
+      for (int g = g0; g <= g1; ++g) {
+        const int64_t at = ((int64_t)g + b) * p.hq + h;
+        const float2 ml = p.part_ml[at];
+        if (ml.x == -INFINITY) continue;
+        const float f = __builtin_amdgcn_exp2f(ml.x - top);
+        sum = fmaf(ml.y, f, sum);
+        const float4* src = reinterpret_cast<const float4*>(p.part_o + at * p.latent + d);
+        const float4 x = src[0], y = src[1];
+        acc[0] = fmaf(x.x, f, acc[0]);
+        acc[1] = fmaf(x.y, f, acc[1]);
+        acc[2] = fmaf(x.z, f, acc[2]);
+        acc[3] = fmaf(x.w, f, acc[3]);
+        acc[4] = fmaf(y.x, f, acc[4]);
+        acc[5] = fmaf(y.y, f, acc[5]);
+        acc[6] = fmaf(y.z, f, acc[6]);
+        acc[7] = fmaf(y.w, f, acc[7]);
+      }
+    }
+    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    f16x8 hi, lo;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float x = acc[j] * inv;
+      hi[j] = round16<BF>(x);
+      lo[j] = round16<BF>(x - widen<BF>(hi[j]));
+    }
+    *reinterpret_cast<f16x8*>(&s_hi[r * kRow + d]) = hi;
+    *reinterpret_cast<f16x8*>(&s_lo[r * kRow + d]) = lo;
+  }
+  __syncthreads();
+  const bool have = n < count;
+  const f16* down = p.kv_b + ((int64_t)h * (p.nope + p.value) + p.nope) * p.latent;
+  for (int v0 = 32 * w; v0 < p.value; v0 += 128) {
+    const int vr = v0 + n;
+    const f16* wp = down + (int64_t)min(vr, p.value - 1) * p.latent + 8 * hh;
+    f32x16 acc = {}, rest = {};
+    for (int k = 0; k < p.latent; k += 16) {
+      f16x8 a = {}, hi = {}, lo = {};
+      if (k + 8 * hh < p.latent) {
+        a = *reinterpret_cast<const f16x8*>(wp + k);
+        if (have) {
+          hi = *reinterpret_cast<const f16x8*>(&s_hi[n * kRow + k + 8 * hh]);
+          lo = *reinterpret_cast<const f16x8*>(&s_lo[n * kRow + k + 8 * hh]);
+        }
+      }
+      acc = mfma16<BF>(a, hi, acc);
+      rest = mfma16<BF>(a, lo, rest);
+    }
+    if (have) {
+      f16* dst = p.out + ((int64_t)(b0 + n) * p.hq + h) * p.value + v0 + 4 * hh;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        if (v0 + 8 * g >= p.value) break;
+        f16x4 y;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) y[t] = round16<BF>(acc[4 * g + t] + rest[4 * g + t]);
+        *reinterpret_cast<f16x4*>(dst + 8 * g) = y;
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host.
+
+constexpr int kMaxBatch = 8184;
+
+// Waves side by side over heads: as many as the heads fill, so that a tile is
+// copied once for all of them.
+int waves_over_heads(int q_heads) { return q_heads <= 32 ? 1 : q_heads <= 64 ? 2 : 4; }
+
+struct Plan {
+  int head_groups;  // grid y
+  int groups;       // ranges of the stream: grid x
+  size_t q_lat, prefix, part_ml, part_o, bytes;
+};
+
+size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+Plan plan_for(int batch, int q_heads, int latent, int rope, int page_size, int table_stride,
+              int longest) {
+  Plan r;
+  const int nhg = waves_over_heads(q_heads);
+  r.head_groups = (q_heads + 32 * nhg - 1) / (32 * nhg);
+  const int64_t cap = (int64_t)page_size * table_stride;
+  const int64_t keys = std::max<int64_t>(1, std::min<int64_t>(longest, cap));
+  const int64_t tiles = (int64_t)batch * ((keys + kTileKeys - 1) / kTileKeys);
+  // A workgroup has a tile for each of its wave groups at least.
+  const int64_t most = std::max(1, kMaxGroups / r.head_groups);
+  r.groups = (int)std::max<int64_t>(1, std::min(most, (tiles + 4 / nhg - 1) / (4 / nhg)));
+  const size_t slots = (size_t)r.groups + batch;
+  size_t at = 0;
+  r.q_lat = at;
+  at = up256(at + (size_t)batch * q_heads * (latent + rope) * 2);
+  r.prefix = at;
+  at = up256(at + (size_t)(batch + 1) * 4);
+  r.part_ml = at;
+  at = up256(at + slots * q_heads * 8);
+  r.part_o = at;
+  r.bytes = up256(at + slots * q_heads * latent * 4);
+  return r;
+}
+
+template <int WP, int OB, bool BF>
+const void* decode_kernel(int nhg) {
+  switch (nhg) {
+    case 1: return (const void*)latent_decode_kernel<WP, OB, 1, BF>;
+    case 2: return (const void*)latent_decode_kernel<WP, OB, 2, BF>;
+    default: return (const void*)latent_decode_kernel<WP, OB, 4, BF>;
+  }
+}
+
+// The kernel of 256 latent dims (and 64 rotary ones) for rows that it holds.
+template <bool BF>
+const void* decode_kernel_for(int nhg, int latent) {
+  return latent <= 256 ? decode_kernel<10, 8, BF>(nhg) : decode_kernel<18, 16, BF>(nhg);
+}
+
+int check_decode(int32_t batch, int32_t q_heads, int32_t latent_dim, int32_t rope_dim,
+                 int32_t nope_dim, int32_t value_dim, int32_t page_size, int32_t table_stride) {
+  const int rc = check_shape(q_heads, latent_dim, rope_dim, nope_dim, value_dim);
+  if (rc != PDA_OK) return rc;
+  if (batch < 0 || batch > kMaxBatch || page_size <= 0 || table_stride <= 0)
+    return fail(PDA_ERR_INVALID_ARGUMENT, "batch=%d (at most %d) page_size=%d table_stride=%d",
+                batch, kMaxBatch, page_size, table_stride);
+  const int64_t keys = std::min<int64_t>((int64_t)page_size * table_stride, INT32_MAX);
+  if ((int64_t)batch * ((keys + kTileKeys - 1) / kTileKeys) > INT32_MAX)
+    return fail(PDA_ERR_TOO_LONG, "batch x keys exceeds the tile stream (2^31 tiles of %d keys)",
+                kTileKeys);
+  return PDA_OK;
+}
+
+int latent_append(const void* q, void* q_out, const void* latent, int64_t latent_stride,
+                  const void* k_rope, int64_t k_stride, const void* norm_weight, float eps,
+                  void* arena, const int32_t* positions, const int32_t* rows, int32_t n,
+                  int32_t q_heads, int32_t latent_dim, int32_t rope_dim, int32_t nope_dim,
+                  int64_t arena_rows, const float* inv_freq, bool bf, void* stream) {
+  const bool queries = q != nullptr || q_out != nullptr;
+  const int rc = check_shape(queries ? q_heads : 1, latent_dim, rope_dim, queries ? nope_dim : 8, 8);
+  if (rc != PDA_OK) return rc;
+  if (n < 0 || arena_rows < 0)
+    return fail(PDA_ERR_INVALID_ARGUMENT, "n=%d arena_rows=%lld", n, (long long)arena_rows);
+  if (n == 0) return ok();
+  if (queries && (!q || !q_out)) return fail(PDA_ERR_INVALID_ARGUMENT, "q and q_out go together");
+  const bool write = latent || arena || rows || (k_rope && rope_dim);
+  if (write && (!latent || !arena || !rows || (rope_dim && !k_rope)))
+    return fail(PDA_ERR_INVALID_ARGUMENT, "latent, k_rope, arena and rows go together");
+  if (!queries && !write) return fail(PDA_ERR_INVALID_ARGUMENT, "null buffer pointer");
+  if (inv_freq && !positions)
+    return fail(PDA_ERR_INVALID_ARGUMENT, "the rotation needs positions");
+  if (write && (latent_stride < latent_dim || latent_stride % 8 ||
+                (rope_dim && (k_stride < rope_dim || k_stride % 8))))
+    return fail(PDA_ERR_ALIGNMENT, "row strides must hold a row and be multiples of 8 elements");
+  if (norm_weight && !(eps >= 0.0f && eps < INFINITY))
+    return fail(PDA_ERR_INVALID_ARGUMENT, "eps must be finite and not negative");
+  const uintptr_t mis = (uintptr_t)q | (uintptr_t)q_out | (uintptr_t)latent |
+                        (rope_dim ? (uintptr_t)k_rope : 0) | (uintptr_t)arena |
+                        (uintptr_t)norm_weight;
+  if (mis & 15) return fail(PDA_ERR_ALIGNMENT, "16-bit buffers must be 16-byte aligned");
+  if (((uintptr_t)positions | (uintptr_t)rows | (uintptr_t)inv_freq) & 3)
+    return fail(PDA_ERR_ALIGNMENT, "positions, rows and inv_freq must be 4-byte aligned");
+  LatentAppendParams prm;
+  prm.q = static_cast<const f16*>(q);
+  prm.q_out = static_cast<f16*>(q_out);
+  prm.c = write ? static_cast<const f16*>(latent) : nullptr;
+  prm.k = static_cast<const f16*>(k_rope);
+  prm.norm = static_cast<const f16*>(norm_weight);
+  prm.arena = static_cast<f16*>(arena);
+  prm.positions = positions;
+  prm.rows = rows;
+  prm.inv_freq = rope_dim ? inv_freq : nullptr;
+  prm.c_stride = latent_stride;
+  prm.k_stride = k_stride;
+  prm.arena_rows = arena_rows;
+  prm.n = n;
+  prm.hq = q_heads;
+  prm.latent = latent_dim;
+  prm.rope = rope_dim;
+  prm.nope = nope_dim;
+  prm.head_groups = (q_heads + kAppendHeads - 1) / kAppendHeads;
+  prm.eps = eps;
+  const int64_t blocks =
+      (write ? ((int64_t)n + 3) / 4 : 0) + (queries ? (int64_t)n * prm.head_groups : 0);
+  if (blocks > INT32_MAX)
+    return fail(PDA_ERR_INVALID_ARGUMENT, "tokens x query heads exceeds 2^31 workgroups");
+  void* args[] = {&prm};
+  const hipError_t err =
+      hipLaunchKernel(bf ? (const void*)latent_append_kernel<true>
+                         : (const void*)latent_append_kernel<false>,
+                      dim3((unsigned)blocks), dim3(256), args, 0, static_cast<hipStream_t>(stream));
+  if (err != hipSuccess)
+    return fail(PDA_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(err));
+  return ok();
+}
+
+int latent_decode(const void* queries, const void* arena, const void* kv_b, const int32_t* tables,
+                  const int32_t* lengths, void* out, int32_t batch, int32_t q_heads,
+                  int32_t latent_dim, int32_t rope_dim, int32_t nope_dim, int32_t value_dim,
+                  int32_t page_size, int32_t table_stride, int64_t arena_rows, int32_t longest,
+                  float scale, bool bf, void* workspace, size_t workspace_bytes, void* stream) {
+  const int rc = check_decode(batch, q_heads, latent_dim, rope_dim, nope_dim, value_dim, page_size,
+                              table_stride);
+  if (rc != PDA_OK) return rc;
+  if (batch == 0) return ok();
+  if (!queries || !arena || !kv_b || !tables || !lengths || !out)
+    return fail(PDA_ERR_INVALID_ARGUMENT, "null buffer pointer");
+  if (arena_rows < page_size || arena_rows > INT32_MAX)
+    return fail(PDA_ERR_INVALID_ARGUMENT, "arena_rows %lld: a whole page at least, below 2^31",
+                (long long)arena_rows);
+  if (!(scale == scale) || isinf(scale))
+    return fail(PDA_ERR_INVALID_ARGUMENT, "scale must be finite");
+  if (((uintptr_t)queries | (uintptr_t)arena | (uintptr_t)kv_b | (uintptr_t)out) & 15)
+    return fail(PDA_ERR_ALIGNMENT, "16-bit buffers must be 16-byte aligned");
+  if (((uintptr_t)tables | (uintptr_t)lengths) & 3)
+    return fail(PDA_ERR_ALIGNMENT, "tables and lengths must be 4-byte aligned");
+  const Plan plan =
+      plan_for(batch, q_heads, latent_dim, rope_dim, page_size, table_stride, longest);
+  if (!workspace || workspace_bytes < plan.bytes)
+    return fail(PDA_ERR_WORKSPACE, "a workspace of %zu bytes is needed (got %zu)", plan.bytes,
+                workspace ? workspace_bytes : (size_t)0);
+  if ((uintptr_t)workspace & 255)
+    return fail(PDA_ERR_ALIGNMENT, "the workspace must be 256-byte aligned");
+  char* ws = static_cast<char*>(workspace);
+  const int nhg = waves_over_heads(q_heads);
+  LatentDecodeParams prm;
+  prm.q = static_cast<const f16*>(queries);
+  prm.kv_b = static_cast<const f16*>(kv_b);
+  prm.arena = static_cast<const f16*>(arena);
+  prm.tables = tables;
+  prm.lengths = lengths;
+  prm.out = static_cast<f16*>(out);
+  prm.q_lat = reinterpret_cast<f16*>(ws + plan.q_lat);
+  prm.prefix = reinterpret_cast<int32_t*>(ws + plan.prefix);
+  prm.part_ml = reinterpret_cast<float2*>(ws + plan.part_ml);
+  prm.part_o = reinterpret_cast<float*>(ws + plan.part_o);
+  prm.arena_pages = arena_rows / page_size;
+  prm.table_stride = table_stride;
+  prm.page_size = page_size;
+  prm.batch = batch;
+  prm.hq = q_heads;
+  prm.latent = latent_dim;
+  prm.rope = rope_dim;
+  prm.nope = nope_dim;
+  prm.value = value_dim;
+  prm.groups = plan.groups;
+  prm.scale_log2 = scale * kLog2e;
+  // Sequences a merge workgroup takes: fewer while the CUs are not all used.
+  prm.merge_batch = 32;
+  while (prm.merge_batch > 1 &&
+         (int64_t)q_heads * ((batch + prm.merge_batch - 1) / prm.merge_batch) < kMaxGroups)
+    prm.merge_batch /= 2;
+  void* args[] = {&prm};
+  const hipStream_t hs = static_cast<hipStream_t>(stream);
+  hipError_t err = hipLaunchKernel(
+      bf ? (const void*)latent_absorb_kernel<true> : (const void*)latent_absorb_kernel<false>,
+      dim3((latent_dim + 127) / 128, q_heads, (batch + 31) / 32), dim3(256), args, 0, hs);
+  if (err == hipSuccess)
+    err = hipLaunchKernel(bf ? decode_kernel_for<true>(nhg, latent_dim)
+                             : decode_kernel_for<false>(nhg, latent_dim),
+                          dim3(plan.groups, plan.head_groups), dim3(256), args, 0, hs);
+  if (err == hipSuccess)
+    err = hipLaunchKernel(
+        bf ? (const void*)latent_merge_kernel<true> : (const void*)latent_merge_kernel<false>,
+        dim3(q_heads, (batch + prm.merge_batch - 1) / prm.merge_batch), dim3(256), args, 0, hs);
+  if (err != hipSuccess)
+    return fail(PDA_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(err));
+  return ok();
+}
+
+}  // namespace
+
+extern "C" {
+
+int pda_latent_append(const void* q, void* q_out, const void* latent, int64_t latent_stride,
+                      const void* k_rope, int64_t k_stride, const void* norm_weight, float eps,
+                      void* arena, const int32_t* positions, const int32_t* rows, int32_t n,
+                      int32_t q_heads, int32_t latent_dim, int32_t rope_dim, int32_t nope_dim,
+                      int64_t arena_rows, const float* inv_freq, void* stream) {
+  return latent_append(q, q_out, latent, latent_stride, k_rope, k_stride, norm_weight, eps, arena,
+                       positions, rows, n, q_heads, latent_dim, rope_dim, nope_dim, arena_rows,
+                       inv_freq, false, stream);
+}
+
+int pda_latent_append_bf16(const void* q, void* q_out, const void* latent, int64_t latent_stride,
+                           const void* k_rope, int64_t k_stride, const void* norm_weight,
+                           float eps, void* arena, const int32_t* positions, const int32_t* rows,
+                           int32_t n, int32_t q_heads, int32_t latent_dim, int32_t rope_dim,
+                           int32_t nope_dim, int64_t arena_rows, const float* inv_freq,
+                           void* stream) {
+  return latent_append(q, q_out, latent, latent_stride, k_rope, k_stride, norm_weight, eps, arena,
+                       positions, rows, n, q_heads, latent_dim, rope_dim, nope_dim, arena_rows,
+                       inv_freq, true, stream);
+}
+
+int pda_latent_decode_workspace_bytes(int32_t batch, int32_t q_heads, int32_t latent_dim,
+                                      int32_t rope_dim, int32_t page_size, int32_t table_stride,
+                                      int32_t longest, size_t* bytes) {
+  const int rc = check_decode(batch, q_heads, latent_dim, rope_dim, 8, 8, page_size, table_stride);
+  if (rc != PDA_OK) return rc;
+  if (!bytes) return fail(PDA_ERR_INVALID_ARGUMENT, "null result pointer");
+  *bytes = batch == 0 ? 0
+                      : plan_for(batch, q_heads, latent_dim, rope_dim, page_size, table_stride,
+                                 longest)
+                            .bytes;
+  return ok();
+}
+
+int pda_latent_decode_attention(const void* queries, const void* arena, const void* kv_b,
+                                const int32_t* tables, const int32_t* lengths, void* out,
+                                int32_t batch, int32_t q_heads, int32_t latent_dim,
+                                int32_t rope_dim, int32_t nope_dim, int32_t value_dim,
+                                int32_t page_size, int32_t table_stride, int64_t arena_rows,
+                                int32_t longest, float scale, void* workspace,
+                                size_t workspace_bytes, void* stream) {
+  return latent_decode(queries, arena, kv_b, tables, lengths, out, batch, q_heads, latent_dim,
+                       rope_dim, nope_dim, value_dim, page_size, table_stride, arena_rows, longest,
+                       scale, false, workspace, workspace_bytes, stream);
+}
+
+int pda_latent_decode_attention_bf16(const void* queries, const void* arena, const void* kv_b,
+                                     const int32_t* tables, const int32_t* lengths, void* out,
+                                     int32_t batch, int32_t q_heads, int32_t latent_dim,
+                                     int32_t rope_dim, int32_t nope_dim, int32_t value_dim,
+                                     int32_t page_size, int32_t table_stride, int64_t arena_rows,
+                                     int32_t longest, float scale, void* workspace,
+                                     size_t workspace_bytes, void* stream) {
+  return latent_decode(queries, arena, kv_b, tables, lengths, out, batch, q_heads, latent_dim,
+                       rope_dim, nope_dim, value_dim, page_size, table_stride, arena_rows, longest,
+                       scale, true, workspace, workspace_bytes, stream);
+}
+
+}  // extern "C"

@@ -123,6 +123,17 @@ SIGNATURES["pda_decode_describe"] = (
     [c_int32] * 11 + [ctypes.POINTER(DecodeInfo)],
 )
 
+# Latent attention.
+_LATENT_APPEND_ARGS = ([c_void_p] * 3 + [c_int64, c_void_p, c_int64, c_void_p, c_float]
+                       + [c_void_p] * 3 + [c_int32] * 5 + [c_int64] + [c_void_p] * 2)
+_LATENT_DECODE_ARGS = ([c_void_p] * 6 + [c_int32] * 8
+                       + [c_int64, c_int32, c_float, c_void_p, c_size_t, c_void_p])
+for _suffix in ("", "_bf16"):
+    SIGNATURES["pda_latent_append" + _suffix] = (ctypes.c_int, _LATENT_APPEND_ARGS)
+    SIGNATURES["pda_latent_decode_attention" + _suffix] = (ctypes.c_int, _LATENT_DECODE_ARGS)
+SIGNATURES["pda_latent_decode_workspace_bytes"] = (
+    ctypes.c_int, [c_int32] * 7 + [ctypes.POINTER(c_size_t)])
+
 _lib: ctypes.CDLL | None = None
 
 
@@ -190,6 +201,15 @@ def plan(batch, q_heads, kv_heads, head_dim, page_size, table_stride, longest, w
                              longest, window, split_pages, ctypes.byref(pages),
                              ctypes.byref(splits)))
     return pages.value, splits.value
+
+
+def latent_decode_workspace_bytes(batch, q_heads, latent_dim, rope_dim, page_size, table_stride,
+                                  longest) -> int:
+    out = c_size_t(0)
+    check(library().pda_latent_decode_workspace_bytes(batch, q_heads, latent_dim, rope_dim,
+                                                      page_size, table_stride, longest,
+                                                      ctypes.byref(out)))
+    return out.value
 
 
 def describe(batch, q_heads, kv_heads, head_dim, page_size, table_stride, longest, window,
