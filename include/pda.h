@@ -641,6 +641,106 @@ int pda_latent_decode_attention_bf16(const void* queries, const void* arena,
                                      float scale, void* workspace,
                                      size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Eviction by accumulated attention weight. No counterpart in the reference
+ * (which bounds a cache by sliding windows, mlx_engine.py:349-372): every key
+ * is credited with the weights that each step's attention gave it, and a
+ * sequence past its bound keeps its heaviest keys, packed, per kv head. The
+ * credits belong to a sequence's logical positions (not to the arena's rows,
+ * which sequences may share): weights [batch, kv_heads, capacity] float32.
+ * ------------------------------------------------------------------------- */
+
+/* Bytes of workspace of the calls below: the step's unnormalised weights (4
+ * bytes a query head and position) and each 256-key chunk's maximum and sum. */
+int pda_attention_weights_workspace_bytes(int32_t batch, int32_t q_heads,
+                                          int32_t capacity, size_t* bytes);
+
+/* Credits a step's weights: for t < n = min(lengths[b], table_stride *
+ * page_size, capacity),
+ *   out[b, j, t] = (t < n - fresh ? weights[b, j, t] : 0)
+ *                  + sum over kv head j's query heads h of softmax(s_h)[t],
+ * s_h the scores of pda_paged_decode_attention on the same arguments (scale,
+ * softcap, window; hidden keys get 0); out may be weights. Entries from n on
+ * are left as they were. `fresh` (1 in a decode step) is how many of the newest
+ * positions have no credit yet; capacity (that of a prompt's first call) takes
+ * none from weights. Everything in float32, sums in a fixed order: repeated
+ * calls give the same bits. `longest` is a planning hint, as for the decode
+ * call. Keys and queries fp16, or bf16 (_bf16); int8 keys with fp16 scales
+ * under fp16 (_q8) or bf16 (_q8_bf16) queries. Two launches on `stream`; calls
+ * that share a workspace must not overlap. */
+int pda_attention_weights(const void* queries, const void* keys,
+                          const int32_t* tables, const int32_t* lengths,
+                          const float* weights, float* out, int32_t batch,
+                          int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                          int32_t page_size, int32_t table_stride,
+                          int64_t arena_rows, int32_t layout, int32_t capacity,
+                          int32_t longest, float scale, int32_t window,
+                          float softcap, int32_t fresh, void* workspace,
+                          size_t workspace_bytes, void* stream);
+int pda_attention_weights_bf16(const void* queries, const void* keys,
+                          const int32_t* tables, const int32_t* lengths,
+                          const float* weights, float* out, int32_t batch,
+                          int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                          int32_t page_size, int32_t table_stride,
+                          int64_t arena_rows, int32_t layout, int32_t capacity,
+                          int32_t longest, float scale, int32_t window,
+                          float softcap, int32_t fresh, void* workspace,
+                          size_t workspace_bytes, void* stream);
+int pda_attention_weights_q8(const void* queries, const void* keys,
+                          const void* key_scales,
+                          const int32_t* tables, const int32_t* lengths,
+                          const float* weights, float* out, int32_t batch,
+                          int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                          int32_t page_size, int32_t table_stride,
+                          int64_t arena_rows, int32_t layout, int32_t capacity,
+                          int32_t longest, float scale, int32_t window,
+                          float softcap, int32_t fresh, void* workspace,
+                          size_t workspace_bytes, void* stream);
+int pda_attention_weights_q8_bf16(const void* queries, const void* keys,
+                          const void* key_scales,
+                          const int32_t* tables, const int32_t* lengths,
+                          const float* weights, float* out, int32_t batch,
+                          int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                          int32_t page_size, int32_t table_stride,
+                          int64_t arena_rows, int32_t layout, int32_t capacity,
+                          int32_t longest, float scale, int32_t window,
+                          float softcap, int32_t fresh, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* Which positions to keep. Of a sequence's n = min(lengths[b], table_stride *
+ * page_size, capacity) positions those on a page that is negative or not in
+ * the arena are gone; of the others kv head j keeps the first `sinks` and the
+ * last `recent` positions of the n and then the heaviest by weights[b, j],
+ * `keep` in all (or all there are). Of two alike the lower position is kept;
+ * NaN counts as less than everything. Writes
+ *   kept        [batch, kv_heads, keep] the kept positions in order, then -1
+ *   new_lengths [batch] how many (the same for every kv head)
+ *   out_weights [batch, kv_heads, out_capacity] (may be NULL, or weights
+ *               itself): the kept positions' weights, in that order; the rest
+ *               is left as it was
+ * recent + sinks <= keep. One launch, no workspace. */
+int pda_evict_select(const float* weights, float* out_weights,
+                     const int32_t* tables, const int32_t* lengths, int32_t* kept,
+                     int32_t* new_lengths, int32_t batch, int32_t kv_heads,
+                     int32_t page_size, int32_t table_stride, int64_t arena_rows,
+                     int32_t capacity, int32_t out_capacity, int32_t keep,
+                     int32_t recent, int32_t sinks, void* stream);
+
+/* Packs the kept rows of one or two arenas of one shape (keys and values, or
+ * their scales; arena2 may be NULL): row kept[b, j, i] of a sequence and kv
+ * head goes to position i of out_tables. `width` is a row's bytes: head_dim
+ * elements, or 2 for a scale arena. out_tables is tables itself (the same
+ * pointer: the rows move to the front of their own pages) or names pages that
+ * no row is read from, except where a position stays where it is. A page that
+ * is written belongs to one sequence; rows whose place is not in the arena or
+ * past out_stride pages are dropped. One launch, no workspace. */
+int pda_evict_move(void* arena, void* arena2, int32_t width, const int32_t* kept,
+                   const int32_t* new_lengths, const int32_t* tables,
+                   const int32_t* out_tables, int32_t batch, int32_t kv_heads,
+                   int32_t page_size, int32_t table_stride, int32_t out_stride,
+                   int64_t arena_rows, int32_t layout, int32_t keep,
+                   void* stream);
+
 #ifdef __cplusplus
 }
 #endif

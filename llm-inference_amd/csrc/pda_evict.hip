@@ -1,0 +1,957 @@
+// Eviction from the paged K/V cache by accumulated attention weight for MI355X
+// (gfx950), C-ABI in pda.h (pda_attention_weights, pda_evict_select,
+// pda_evict_move). No reference counterpart: the reference bounds a cache by
+// sliding windows alone.
+//
+// After a step's attention every key of a sequence is credited with the
+// weights it was given, w[t] += sum over the query heads of a kv head of
+// softmax(score)[t]; when a sequence passes its bound the keys with the least
+// credit go and the rows of the others are packed, per kv head (a page tile's
+// rows of different heads need not hold the same positions). Credits are kept
+// per sequence and logical position, so sequences that share a prefix's pages
+// do not share them.
+
+#include <hip/hip_runtime.h>
+
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "pda.h"
+#include "pda_internal.h"
+
+namespace {
+
+using pda_internal::fail;
+using pda_internal::ok;
+
+typedef _Float16 f16;
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16;
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef signed char i8x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// Until the wave's loads have returned: before a barrier past which others
+// overwrite what was loaded.
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// ---------------------------------------------------------------------------
+// Weights.
+
+constexpr int kWaves = 4;        // waves of a score workgroup
+constexpr int kBlocks = 4;       // blocks of 16 keys a wave takes
+constexpr int kChunk = 16 * kBlocks * kWaves;  // keys per workgroup: 256
+constexpr int kSlots = 16;       // query heads per workgroup
+constexpr int kAddKeys = 1024;   // keys an adding workgroup takes
+constexpr int kMaxChunksX = 4096;
+
+struct WeightParams {
+  const f16* q;        // [batch, hq, D]
+  const void* k;       // arena: 16-bit, or int8 with scales
+  const f16* kscale;
+  const int32_t* tables;
+  const int32_t* lengths;
+  const float* weights;  // [batch, hkv, capacity]
+  float* out;
+  float* probs;        // [batch, hq, capacity] weights relative to their chunk's max
+  float2* stats;       // [batch, hq, chunks] (max, sum) of each chunk
+  int64_t arena_pages;
+  int64_t page_elems, scale_page;  // elements between pages,
+  int32_t head_elems, scale_head;  //   kv heads of a page,
+  int32_t row_elems, scale_row;    //   rows of a page and head
+  int32_t table_stride;
+  int32_t page_size;
+  int32_t hq;
+  int32_t hkv;
+  int32_t head_dim;
+  int32_t capacity;
+  int32_t chunks;      // ceil(capacity / kChunk)
+  int32_t window;
+  int32_t fresh;
+  float scale_log2;
+  float cap_in;        // 2 log2(e) scale / softcap
+  float cap_out;       // softcap log2(e); 0: no softcap
+};
+
+__device__ __forceinline__ int keys_of(const WeightParams& p, int b) {
+  const int64_t cap = min((int64_t)p.table_stride * p.page_size, (int64_t)p.capacity);
+  return (int)max((int64_t)0, min((int64_t)p.lengths[b], cap));
+}
+
+// 8 elements of a row from dim d on as 16-bit operands, zeros past the head
+// dim. VEC: head dims that are multiples of 8 (rows 8 elements aligned).
+template <bool Q8, bool BF, bool VEC>
+__device__ __forceinline__ f16x8 load8(const void* base, int64_t at, int d, int dim) {
+  f16x8 x = {};
+  if (d >= dim) return x;
+  if constexpr (Q8) {
+    const signed char* src = static_cast<const signed char*>(base) + at + d;
+    i8x8 y = {};
+    if constexpr (VEC) {
+      y = *reinterpret_cast<const i8x8*>(src);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (d + i < dim) y[i] = src[i];
+    }
+    // (Integers of 8 bits are exact in either type.)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (BF)
+        x[i] = __builtin_bit_cast(f16, (bf16)(float)y[i]);
+      else
+        x[i] = (f16)(float)y[i];
+    }
+  } else {
+    const f16* src = static_cast<const f16*>(base) + at + d;
+    if constexpr (VEC) {
+      x = *reinterpret_cast<const f16x8*>(src);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (d + i < dim) x[i] = src[i];
+    }
+  }
+  return x;
+}
+
+template <bool BF>
+__device__ __forceinline__ f32x4 mfma(const f16x8& a, const f16x8& b, const f32x4& c) {
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// Scores of 256 keys against up to 16 heads of one kv head, as weights relative
+// to the chunk's largest, with each head's largest and sum. K is read once,
+// straight into the matrix cores' operands (lane: key lane % 16, 8 dims), 64
+// bytes of a row per instruction, all loads of a wave's 64 keys under way
+// together where the head dim allows; a lane ends with 4 consecutive keys of one
+// head per block. Reads K and writes 4 bytes a head and key: the K bytes bound
+// it.
+template <int NC, bool Q8, bool BF, bool VEC>
+__global__ __launch_bounds__(64 * kWaves) void attention_scores_kernel(const WeightParams p) {
+  __shared__ float s_max[kWaves][kSlots], s_sum[kWaves][kSlots];
+  const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
+  const int n16 = lane & 15, g4 = lane >> 4;
+  const int group = p.hq / p.hkv, tiles = (group + kSlots - 1) / kSlots;
+  const int kvh = blockIdx.y / tiles, first = (blockIdx.y % tiles) * kSlots;
+  const int b = blockIdx.z;
+  const int slot = first + n16;
+  const bool live = slot < group;
+  const int h = kvh * group + slot;
+  const int keys = keys_of(p, b);
+  const int lo = p.window > 0 ? max(0, keys - p.window) : 0;
+  const uint32_t pages = (uint32_t)min(p.arena_pages, (int64_t)INT32_MAX);
+
+  f16x8 qf[NC];
+  const int64_t qat = ((int64_t)b * p.hq + (live ? h : 0)) * p.head_dim;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    qf[c] = load8<false, BF, VEC>(p.q, qat, 32 * c + 8 * g4, p.head_dim);
+    if (!live) qf[c] = f16x8{};
+  }
+  for (int chunk = lo / kChunk + blockIdx.x; chunk * (int64_t)kChunk < keys; chunk += gridDim.x) {
+    const int k0 = chunk * kChunk + w * (16 * kBlocks);
+    f32x4 s[kBlocks];
+    uint32_t seen = 0;  // bit i: this lane's key of block i has a row
+    int64_t at[kBlocks];
+    float ks[kBlocks];
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i) {
+      const int key = k0 + 16 * i + n16;
+      at[i] = 0;
+      ks[i] = 1.0f;
+      if (key >= lo && key < keys) {
+        const uint32_t pi = (uint32_t)key / (uint32_t)p.page_size;
+        const int r = key - (int)pi * p.page_size;
+        const uint32_t page = (uint32_t)p.tables[(int64_t)b * p.table_stride + pi];
+        if (page < pages) {
+          seen |= 1u << i;
+          at[i] = page * p.page_elems + (int64_t)kvh * p.head_elems + (int64_t)r * p.row_elems;
+          if constexpr (Q8)
+            ks[i] = (float)p.kscale[page * p.scale_page + (int64_t)kvh * p.scale_head +
+                                    (int64_t)r * p.scale_row];
+        }
+      }
+    }
+    f16x8 kf[kBlocks][NC <= 4 ? NC : 1];
+    if constexpr (NC <= 4) {
+#pragma unroll
+      for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+          kf[i][c] = load8<Q8, BF, VEC>(p.k, at[i], 32 * c + 8 * g4, p.head_dim);
+    }
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i) {
+      s[i] = f32x4{};
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        f16x8 a;
+        if constexpr (NC <= 4)
+          a = kf[i][c];
+        else
+          a = load8<Q8, BF, VEC>(p.k, at[i], 32 * c + 8 * g4, p.head_dim);
+        s[i] = mfma<BF>(a, qf[c], s[i]);
+      }
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i) {
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        // Key 4 g4 + v of the block: lane 4 g4 + v looked it up.
+        const int src = 4 * g4 + v;
+        const bool have = __shfl((int)(seen >> i & 1), src) != 0;
+        float x = s[i][v];
+        if constexpr (Q8) x *= __shfl(ks[i], src);
+        if (p.cap_out > 0.0f) {
+          const float e = __builtin_amdgcn_exp2f(x * p.cap_in);
+          x = (1.0f - 2.0f / (e + 1.0f)) * p.cap_out;
+        } else {
+          x *= p.scale_log2;
+        }
+        s[i][v] = have ? x : -INFINITY;
+        top = fmaxf(top, s[i][v]);
+      }
+    }
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    if (g4 == 0) s_max[w][n16] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) top = fmaxf(top, s_max[i][n16]);
+    const float mu = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i) {
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        s[i][v] = __builtin_amdgcn_exp2f(s[i][v] - mu);
+        sum += s[i][v];
+      }
+    }
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    if (g4 == 0) s_sum[w][n16] = sum;
+    __syncthreads();
+    if (live) {
+      const int64_t row = (int64_t)b * p.hq + h;
+      float* dst = p.probs + row * p.capacity;
+#pragma unroll
+      for (int i = 0; i < kBlocks; ++i) {
+        const int key = k0 + 16 * i + 4 * g4;
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+          if (key + v < keys) dst[key + v] = s[i][v];
+      }
+      if (w == 0 && g4 == 0) {
+        float all = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) all += s_sum[i][n16];
+        p.stats[row * p.chunks + chunk] = make_float2(top, all);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// out[t] = weights[t] (0 for the `fresh` newest) + the sum over the kv head's
+// query heads, in their order, of the normalised weights: the chunks' maxima and
+// sums give each head's, once a workgroup.
+__global__ __launch_bounds__(256) void attention_weights_kernel(const WeightParams p) {
+  constexpr int kHeads = 32;  // heads whose factors are held at once
+  constexpr int kParts = kAddKeys / kChunk;
+  __shared__ float s_f[kHeads][kParts];
+  const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
+  const int group = p.hq / p.hkv, kvh = blockIdx.y, b = blockIdx.z;
+  const int keys = keys_of(p, b);
+  const int lo = p.window > 0 ? max(0, keys - p.window) : 0;
+  const int c_lo = lo / kChunk, c_hi = (keys + kChunk - 1) / kChunk;
+  const int64_t base = ((int64_t)b * p.hkv + kvh) * p.capacity;
+  for (int64_t k0 = (int64_t)blockIdx.x * kAddKeys; k0 < keys; k0 += (int64_t)gridDim.x * kAddKeys) {
+    float acc[kAddKeys / 256] = {}, old[kAddKeys / 256];
+#pragma unroll
+    for (int i = 0; i < kAddKeys / 256; ++i) {
+      const int64_t t = k0 + 256 * i + tid;
+      old[i] = t < (int64_t)keys - p.fresh ? p.weights[base + t] : 0.0f;
+    }
+    for (int h0 = 0; h0 < group; h0 += kHeads) {
+      const int heads = min(kHeads, group - h0);
+      __syncthreads();
+      for (int i = w; i < heads; i += 4) {
+        const float2* st = p.stats + ((int64_t)b * p.hq + kvh * group + h0 + i) * p.chunks;
+        float top = -INFINITY, sum = 0.0f;
+        for (int c = c_lo + lane; c < c_hi; c += 64) {
+          const float2 x = st[c];
+          if (x.x == -INFINITY) continue;
+          if (x.x > top) {
+            sum *= top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - x.x);
+            top = x.x;
+          }
+          sum = fmaf(x.y, __builtin_amdgcn_exp2f(x.x - top), sum);
+        }
+#pragma unroll
+        for (int d = 32; d; d >>= 1) {
+          const float t2 = __shfl_xor(top, d), s2 = __shfl_xor(sum, d);
+          const float m = fmaxf(top, t2);
+          if (m != -INFINITY)
+            sum = sum * __builtin_amdgcn_exp2f(top - m) + s2 * __builtin_amdgcn_exp2f(t2 - m);
+          top = m;
+        }
+        if (lane < kParts) {
+          const int c = (int)(k0 / kChunk) + lane;
+          float f = 0.0f;
+          if (c >= c_lo && c < c_hi && sum > 0.0f) {
+            const float m = st[c].x;
+            if (m != -INFINITY) f = __builtin_amdgcn_exp2f(m - top) / sum;
+          }
+          if (sum != sum) f = sum;
+          s_f[i][lane] = f;
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kAddKeys / 256; ++i) {
+        const int64_t t = k0 + 256 * i + tid;
+        if (t >= lo / kChunk * kChunk && t < keys) {
+          const float* pr = p.probs + ((int64_t)b * p.hq + kvh * group + h0) * p.capacity + t;
+          for (int j = 0; j < heads; ++j)
+            acc[i] = fmaf(pr[(int64_t)j * p.capacity], s_f[j][(256 * i + tid) / kChunk], acc[i]);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kAddKeys / 256; ++i) {
+      const int64_t t = k0 + 256 * i + tid;
+      if (t < keys) p.out[base + t] = old[i] + acc[i];
+    }
+    __syncthreads();
+  }
+}
+
+template <bool Q8, bool BF>
+const void* scores_kernel(int dim) {
+  const int nc = (dim + 31) / 32;
+  if (dim % 8 == 0) {
+    if (nc <= 2) return (const void*)attention_scores_kernel<2, Q8, BF, true>;
+    if (nc <= 3) return (const void*)attention_scores_kernel<3, Q8, BF, true>;
+    if (nc <= 4) return (const void*)attention_scores_kernel<4, Q8, BF, true>;
+    if (nc <= 8) return (const void*)attention_scores_kernel<8, Q8, BF, true>;
+    return (const void*)attention_scores_kernel<16, Q8, BF, true>;
+  }
+  return nc <= 4 ? (const void*)attention_scores_kernel<4, Q8, BF, false>
+                 : (const void*)attention_scores_kernel<16, Q8, BF, false>;
+}
+
+size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+size_t weights_workspace(int batch, int q_heads, int capacity) {
+  const size_t rows = (size_t)batch * q_heads;
+  return up256(rows * ((capacity + kChunk - 1) / kChunk) * 8) + up256(rows * capacity * 4);
+}
+
+int attention_weights(const void* queries, const void* keys, const void* key_scales, bool q8,
+                      const int32_t* tables, const int32_t* lengths, const float* weights,
+                      float* out, int32_t batch, int32_t q_heads, int32_t kv_heads,
+                      int32_t head_dim, int32_t page_size, int32_t table_stride,
+                      int64_t arena_rows, int32_t layout, int32_t capacity, int32_t longest,
+                      float scale, int32_t window, float softcap, int32_t fresh, bool bf,
+                      void* workspace, size_t workspace_bytes, void* stream) {
+  if (batch < 0 || batch > 65535 || q_heads <= 0 || kv_heads <= 0 || page_size <= 0 ||
+      table_stride <= 0 || window < 0 || capacity <= 0 || fresh < 0)
+    return fail(PDA_ERR_INVALID_ARGUMENT,
+                "batch=%d q_heads=%d kv_heads=%d page_size=%d table_stride=%d window=%d "
+                "capacity=%d fresh=%d",
+                batch, q_heads, kv_heads, page_size, table_stride, window, capacity, fresh);
+  if (q_heads % kv_heads)
+    return fail(PDA_ERR_HEAD_RATIO, "query heads must be a multiple of kv heads");
+  if (head_dim <= 0 || head_dim > 512)
+    return fail(PDA_ERR_HEAD_DIM, "head_dim %d: 1..512", head_dim);
+  if (batch == 0) return ok();
+  if (!queries || !keys || !tables || !lengths || !weights || !out || (q8 && !key_scales))
+    return fail(PDA_ERR_INVALID_ARGUMENT, "null buffer pointer");
+  if (layout != PDA_LAYOUT_ROWS && layout != PDA_LAYOUT_PAGES)
+    return fail(PDA_ERR_INVALID_ARGUMENT, "unknown K/V layout %d", layout);
+  if ((int64_t)page_size * kv_heads * head_dim > INT32_MAX)
+    return fail(PDA_ERR_INVALID_ARGUMENT, "a page of one layer holds more than 2^31 elements");
+  if (arena_rows < page_size)
+    return fail(PDA_ERR_INVALID_ARGUMENT, "arena_rows %lld holds no whole page",
+                (long long)arena_rows);
+  if (!(scale == scale) || isinf(scale) || !(softcap >= 0.0f) || isinf(softcap))
+    return fail(PDA_ERR_INVALID_ARGUMENT, "scale must be finite and softcap >= 0");
+  if (capacity > INT32_MAX - 2 * kAddKeys)
+    return fail(PDA_ERR_TOO_LONG, "capacity %d next to 2^31", capacity);
+  if (((uintptr_t)queries | (uintptr_t)keys) & 15)
+    return fail(PDA_ERR_ALIGNMENT, "query and key buffers must be 16-byte aligned");
+  if (((uintptr_t)tables | (uintptr_t)lengths | (uintptr_t)weights | (uintptr_t)out) & 3)
+    return fail(PDA_ERR_ALIGNMENT, "tables, lengths and weights must be 4-byte aligned");
+  if (q8 && ((uintptr_t)key_scales & 1))
+    return fail(PDA_ERR_ALIGNMENT, "fp16 scale arenas must be 2-byte aligned");
+  const int group = q_heads / kv_heads;
+  const int64_t grid_y = (int64_t)kv_heads * ((group + kSlots - 1) / kSlots);
+  if (grid_y > 65535)
+    return fail(PDA_ERR_INVALID_ARGUMENT, "%d kv heads of %d query heads", kv_heads, group);
+  const size_t need = weights_workspace(batch, q_heads, capacity);
+  if (!workspace || workspace_bytes < need)
+    return fail(PDA_ERR_WORKSPACE, "a workspace of %zu bytes is needed (got %zu)", need,
+                workspace ? workspace_bytes : (size_t)0);
+  if ((uintptr_t)workspace & 255)
+    return fail(PDA_ERR_ALIGNMENT, "the workspace must be 256-byte aligned");
+  WeightParams prm;
+  prm.q = static_cast<const f16*>(queries);
+  prm.k = keys;
+  prm.kscale = static_cast<const f16*>(key_scales);
+  prm.tables = tables;
+  prm.lengths = lengths;
+  prm.weights = weights;
+  prm.out = out;
+  prm.chunks = (capacity + kChunk - 1) / kChunk;
+  prm.stats = static_cast<float2*>(workspace);
+  prm.probs = reinterpret_cast<float*>(static_cast<char*>(workspace) +
+                                       up256((size_t)batch * q_heads * prm.chunks * 8));
+  prm.arena_pages = arena_rows / page_size;
+  const bool rows = layout == PDA_LAYOUT_ROWS;
+  prm.page_elems = (int64_t)page_size * kv_heads * head_dim;
+  prm.head_elems = rows ? head_dim : page_size * head_dim;
+  prm.row_elems = rows ? kv_heads * head_dim : head_dim;
+  prm.scale_page = (int64_t)page_size * kv_heads;
+  prm.scale_head = rows ? 1 : page_size;
+  prm.scale_row = rows ? kv_heads : 1;
+  prm.table_stride = table_stride;
+  prm.page_size = page_size;
+  prm.hq = q_heads;
+  prm.hkv = kv_heads;
+  prm.head_dim = head_dim;
+  prm.capacity = capacity;
+  prm.window = window;
+  prm.fresh = fresh;
+  prm.scale_log2 = scale * kLog2e;
+  prm.cap_in = softcap > 0.0f ? 2.0f * kLog2e * scale / softcap : 0.0f;
+  prm.cap_out = softcap * kLog2e;
+  // The grid covers `longest` keys; workgroups go on to later ones if there are.
+  const int64_t span = std::max<int64_t>(1, std::min<int64_t>(longest, capacity));
+  const int64_t seen = window > 0 ? std::min<int64_t>(span, (int64_t)window + kChunk) : span;
+  const unsigned gx = (unsigned)std::min<int64_t>((seen + kChunk - 1) / kChunk, kMaxChunksX);
+  const unsigned ax = (unsigned)std::min<int64_t>((span + kAddKeys - 1) / kAddKeys, kMaxChunksX);
+  void* args[] = {&prm};
+  const hipStream_t hs = static_cast<hipStream_t>(stream);
+  const void* fn = q8 ? (bf ? scores_kernel<true, true>(head_dim)
+                            : scores_kernel<true, false>(head_dim))
+                      : (bf ? scores_kernel<false, true>(head_dim)
+                            : scores_kernel<false, false>(head_dim));
+  hipError_t err = hipLaunchKernel(fn, dim3(gx, (unsigned)grid_y, batch), dim3(64 * kWaves), args,
+                                   0, hs);
+  if (err == hipSuccess)
+    err = hipLaunchKernel((const void*)attention_weights_kernel, dim3(ax, kv_heads, batch),
+                          dim3(256), args, 0, hs);
+  if (err != hipSuccess)
+    return fail(PDA_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(err));
+  return ok();
+}
+
+// ---------------------------------------------------------------------------
+// Selection.
+
+constexpr int kSelectThreads = 1024;
+constexpr int kSelectWaves = kSelectThreads / 64;
+constexpr int kBins = 2048;
+
+struct SelectParams {
+  const float* weights;  // [batch, hkv, capacity]
+  float* out_weights;    // [batch, hkv, out_capacity]
+  const int32_t* tables;
+  const int32_t* lengths;
+  int32_t* kept;         // [batch, hkv, keep]
+  int32_t* new_lengths;  // [batch]
+  int64_t arena_pages;
+  int32_t table_stride;
+  int32_t page_size;
+  int32_t hkv;
+  int32_t capacity;
+  int32_t out_capacity;
+  int32_t keep;
+  int32_t recent;
+  int32_t sinks;
+};
+
+// Weights as unsigned integers of the same order; NaN lowest, -0 as 0.
+__device__ __forceinline__ uint32_t rank_of(float x) {
+  if (x != x) return 0;
+  const uint32_t u = __float_as_uint(x + 0.0f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// One workgroup a (sequence, kv head). The rank of the least kept weight is
+// found digit by digit from the top (11, 11 and 10 bits): a histogram of the
+// candidates that share the digits found so far, in LDS, and the bin in which
+// the count from above passes what is to be kept. Then every wave counts its
+// stretch of positions, the counts are summed over the waves before it, and the
+// wave writes its kept positions in order; of those at the last rank the lowest
+// positions are kept. Counts are integers, so their order does not matter. The
+// weights are read four times, the last three from L2.
+__global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const SelectParams p) {
+  __shared__ int s_hist[kBins];
+  __shared__ int s_part[kSelectWaves];
+  __shared__ int s_found[2];  // the digit's bin, what it has to give
+  __shared__ int s_above[kSelectWaves], s_equal[kSelectWaves];
+  const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
+  const int kvh = blockIdx.x, b = blockIdx.y;
+  const int64_t cap = min((int64_t)p.table_stride * p.page_size, (int64_t)p.capacity);
+  const int n = (int)max((int64_t)0, min((int64_t)p.lengths[b], cap));
+  const float* weights = p.weights + ((int64_t)b * p.hkv + kvh) * p.capacity;
+  const int32_t* table = p.tables + (int64_t)b * p.table_stride;
+  const uint32_t pages = (uint32_t)min(p.arena_pages, (int64_t)INT32_MAX);
+  auto held = [&](int t) { return (uint32_t)table[(uint32_t)t / (uint32_t)p.page_size] < pages; };
+  auto count = [](uint64_t lanes) { return (int)__popcll(lanes); };
+  auto guarded = [&](int t) { return t < p.sinks || t >= n - p.recent; };
+  auto block_sum = [&](int x) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
+    __syncthreads();
+    if (lane == 0) s_part[w] = x;
+    __syncthreads();
+    int sum = 0;
+    for (int i = 0; i < kSelectWaves; ++i) sum += s_part[i];
+    return sum;
+  };
+  int guards = 0, rest = 0;
+  for (int t = tid; t < n; t += kSelectThreads) {
+    if (!held(t)) continue;
+    if (guarded(t))
+      ++guards;
+    else
+      ++rest;
+  }
+  guards = block_sum(guards);
+  rest = block_sum(rest);
+  const int total = min(p.keep, guards + rest);
+  int want = max(0, p.keep - guards);  // candidates to keep
+  uint32_t least = 0;                  // rank of the least kept one
+  if (want == 0) {
+    least = 0xFFFFFFFFu;
+  } else if (want < rest) {
+    uint32_t mask = 0;
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+      const int bins = pass == 2 ? 1024 : 2048;
+      for (int i = tid; i < bins; i += kSelectThreads) s_hist[i] = 0;
+      __syncthreads();
+      for (int t = tid; t < n; t += kSelectThreads) {
+        if (guarded(t) || !held(t)) continue;
+        const uint32_t r = rank_of(weights[t]);
+        if ((r & mask) == least) atomicAdd(&s_hist[r >> shift & (bins - 1)], 1);
+      }
+      __syncthreads();
+      // Thread i takes the bins i * per .. from the top; the one in whose bins
+      // the running count passes `want` names the bin.
+      const int per = bins / kSelectThreads;
+      int mine = 0;
+      for (int i = 0; i < per; ++i) mine += s_hist[bins - 1 - (tid * per + i)];
+      int upto = mine;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int x = __shfl_up(upto, d);
+        if (lane >= d) upto += x;
+      }
+      if (lane == 63) s_part[w] = upto;
+      __syncthreads();
+      for (int i = 0; i < w; ++i) upto += s_part[i];
+      int above = upto - mine;
+      if (above < want && want <= upto) {
+        for (int i = 0; i < per; ++i) {
+          const int bin = bins - 1 - (tid * per + i);
+          if (above + s_hist[bin] >= want) {
+            s_found[0] = bin;
+            s_found[1] = want - above;
+            break;
+          }
+          above += s_hist[bin];
+        }
+      }
+      __syncthreads();
+      least |= (uint32_t)s_found[0] << shift;
+      want = s_found[1];
+      mask |= (uint32_t)(bins - 1) << shift;
+      __syncthreads();
+    }
+  }
+  // (All candidates kept: least 0, and want of them at rank 0 is enough for
+  // the NaN, which alone have it.)
+  const int stretch = ((n + kSelectWaves - 1) / kSelectWaves + 63) & ~63;
+  const int t0 = min(n, w * stretch), t1 = min(n, t0 + stretch);
+  auto classify = [&](int t, bool& over, bool& equal) {
+    over = equal = false;
+    if (t >= t1 || !held(t)) return;
+    if (guarded(t)) {
+      over = true;
+      return;
+    }
+    const uint32_t r = rank_of(weights[t]);
+    over = r > least;
+    equal = r == least;
+  };
+  int above = 0, equal = 0;
+  for (int t = t0; t < t1; t += 64) {
+    bool o, e;
+    classify(t + lane, o, e);
+    above += count(__ballot(o));
+    equal += count(__ballot(e));
+  }
+  if (lane == 0) {
+    s_above[w] = above;
+    s_equal[w] = equal;
+  }
+  __syncthreads();
+  int before_above = 0, before_equal = 0;
+  for (int i = 0; i < w; ++i) {
+    before_above += s_above[i];
+    before_equal += s_equal[i];
+  }
+  int32_t* kept = p.kept + ((int64_t)b * p.hkv + kvh) * p.keep;
+  int at = before_above + min(before_equal, want), left = max(0, want - before_equal);
+  const uint64_t lower = (1ull << lane) - 1;
+  for (int t = t0; t < t1; t += 64) {
+    bool o, e;
+    classify(t + lane, o, e);
+    const uint64_t eq = __ballot(e);
+    if (e && count(eq & lower) < left) o = true;
+    const uint64_t take = __ballot(o);
+    if (o) kept[at + count(take & lower)] = t + lane;
+    at += count(take);
+    left = max(0, left - count(eq));
+  }
+  for (int i = total + tid; i < p.keep; i += kSelectThreads) kept[i] = -1;
+  if (kvh == 0 && tid == 0) p.new_lengths[b] = total;
+  if (!p.out_weights) return;
+  // The kept positions' weights to the front, 1024 at a time: a later stretch's
+  // sources lie past every place written so far, so this also works in place.
+  __threadfence_block();
+  __syncthreads();
+  float* dst = p.out_weights + ((int64_t)b * p.hkv + kvh) * p.out_capacity;
+  for (int i0 = 0; i0 < total; i0 += kSelectThreads) {
+    const int i = i0 + tid;
+    float x = 0.0f;
+    if (i < total) x = weights[kept[i]];
+    wait_loads();
+    __syncthreads();
+    if (i < total) dst[i] = x;
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Packing.
+
+struct MoveParams {
+  char* arena[2];        // keys and values, or their scales; [1] may be null
+  const int32_t* kept;   // [batch, hkv, keep]
+  const int32_t* new_lengths;
+  const int32_t* tables;
+  const int32_t* out_tables;
+  int64_t arena_pages;
+  int64_t page_bytes;
+  int64_t head_bytes;
+  int64_t row_bytes;     // between rows of a page and head
+  int32_t width;         // bytes of a row
+  int32_t table_stride;
+  int32_t out_stride;
+  int32_t page_size;
+  int32_t hkv;
+  int32_t keep;
+};
+
+// Byte offset of position t's row, -1 if its page is not in the arena.
+__device__ __forceinline__ int64_t row_at(const MoveParams& p, const int32_t* table, int stride,
+                                          int t, int kvh) {
+  const uint32_t pi = (uint32_t)t / (uint32_t)p.page_size;
+  if (t < 0 || pi >= (uint32_t)stride) return -1;
+  const uint32_t page = (uint32_t)table[pi];
+  if ((int64_t)page >= min(p.arena_pages, (int64_t)INT32_MAX)) return -1;
+  return page * p.page_bytes + kvh * p.head_bytes +
+         (int64_t)(t - (int)pi * p.page_size) * p.row_bytes;
+}
+
+// Kept rows to other pages: every piece of V of every row by itself.
+template <class V>
+__global__ __launch_bounds__(256) void evict_copy_kernel(const MoveParams p) {
+  constexpr int kEach = 4;
+  const int kvh = blockIdx.y % p.hkv, b = blockIdx.z;
+  char* arena = p.arena[blockIdx.y / p.hkv];
+  const int pieces = p.width / (int)sizeof(V);
+  const int64_t total = (int64_t)p.new_lengths[b] * pieces;
+  const int32_t* kept = p.kept + ((int64_t)b * p.hkv + kvh) * p.keep;
+  const int32_t* from = p.tables + (int64_t)b * p.table_stride;
+  const int32_t* to = p.out_tables + (int64_t)b * p.out_stride;
+  for (int64_t i0 = (int64_t)blockIdx.x * (256 * kEach); i0 < total;
+       i0 += (int64_t)gridDim.x * (256 * kEach)) {
+    V x[kEach];
+    int64_t at[kEach];
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int64_t i = i0 + 256 * j + threadIdx.x;
+      at[j] = -1;
+      if (i < total) {
+        const int row = (int)(i / pieces), c = (int)(i - (int64_t)row * pieces);
+        const int64_t s = row_at(p, from, p.table_stride, kept[row], kvh);
+        const int64_t d = row_at(p, to, p.out_stride, row, kvh);
+        if (s >= 0 && d >= 0 && s != d) {
+          x[j] = *reinterpret_cast<const V*>(arena + s + c * sizeof(V));
+          at[j] = d + c * sizeof(V);
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+      if (at[j] >= 0) *reinterpret_cast<V*>(arena + at[j]) = x[j];
+  }
+}
+
+// Kept rows to the front of their own pages. A row's place lies at or before
+// it, and rows keep their order, so a workgroup that owns a slice of the rows
+// (kSlice bytes of every row of a sequence and kv head) may walk them in
+// stretches: a stretch's places hold no source of a later one. Within a stretch
+// all loads come before the first store.
+template <class V>
+__global__ __launch_bounds__(256) void evict_pack_kernel(const MoveParams p) {
+  constexpr int kSlice = sizeof(V) >= 4 ? 4 * sizeof(V) : sizeof(V);  // bytes
+  constexpr int kPieces = kSlice / (int)sizeof(V);
+  constexpr int kRows = 256 / kPieces;  // rows per pass
+  constexpr int kEach = 8;
+  const int slices = (p.width + kSlice - 1) / kSlice;
+  const int slice = blockIdx.x % slices;
+  char* arena = p.arena[blockIdx.x / slices];
+  const int kvh = blockIdx.y, b = blockIdx.z;
+  const int c = slice * kSlice + (threadIdx.x % kPieces) * (int)sizeof(V);
+  const bool mine = c < p.width;
+  const int total = p.new_lengths[b];
+  const int32_t* kept = p.kept + ((int64_t)b * p.hkv + kvh) * p.keep;
+  const int32_t* table = p.tables + (int64_t)b * p.table_stride;
+  for (int r0 = 0; r0 < total; r0 += kRows * kEach) {
+    V x[kEach];
+    int64_t at[kEach];
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int row = r0 + kRows * j + (int)threadIdx.x / kPieces;
+      at[j] = -1;
+      if (mine && row < total) {
+        const int from = kept[row];
+        if (from != row) {
+          const int64_t s = row_at(p, table, p.table_stride, from, kvh);
+          const int64_t d = row_at(p, table, p.table_stride, row, kvh);
+          if (s >= 0 && d >= 0) {
+            x[j] = *reinterpret_cast<const V*>(arena + s + c);
+            at[j] = d + c;
+          }
+        }
+      }
+    }
+    wait_loads();
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+      if (at[j] >= 0) *reinterpret_cast<V*>(arena + at[j]) = x[j];
+    __syncthreads();
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int pda_attention_weights_workspace_bytes(int32_t batch, int32_t q_heads, int32_t capacity,
+                                          size_t* bytes) {
+  if (batch < 0 || q_heads <= 0 || capacity <= 0 || !bytes)
+    return fail(PDA_ERR_INVALID_ARGUMENT, "batch=%d q_heads=%d capacity=%d", batch, q_heads,
+                capacity);
+  *bytes = weights_workspace(batch, q_heads, capacity);
+  return ok();
+}
+
+int pda_attention_weights(const void* queries, const void* keys, const int32_t* tables,
+                          const int32_t* lengths, const float* weights, float* out, int32_t batch,
+                          int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t page_size,
+                          int32_t table_stride, int64_t arena_rows, int32_t layout,
+                          int32_t capacity, int32_t longest, float scale, int32_t window,
+                          float softcap, int32_t fresh, void* workspace, size_t workspace_bytes,
+                          void* stream) {
+  return attention_weights(queries, keys, nullptr, false, tables, lengths, weights, out, batch,
+                           q_heads, kv_heads, head_dim, page_size, table_stride, arena_rows,
+                           layout, capacity, longest, scale, window, softcap, fresh, false,
+                           workspace, workspace_bytes, stream);
+}
+
+int pda_attention_weights_bf16(const void* queries, const void* keys, const int32_t* tables,
+                               const int32_t* lengths, const float* weights, float* out,
+                               int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                               int32_t page_size, int32_t table_stride, int64_t arena_rows,
+                               int32_t layout, int32_t capacity, int32_t longest, float scale,
+                               int32_t window, float softcap, int32_t fresh, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  return attention_weights(queries, keys, nullptr, false, tables, lengths, weights, out, batch,
+                           q_heads, kv_heads, head_dim, page_size, table_stride, arena_rows,
+                           layout, capacity, longest, scale, window, softcap, fresh, true,
+                           workspace, workspace_bytes, stream);
+}
+
+int pda_attention_weights_q8(const void* queries, const void* keys, const void* key_scales,
+                             const int32_t* tables, const int32_t* lengths, const float* weights,
+                             float* out, int32_t batch, int32_t q_heads, int32_t kv_heads,
+                             int32_t head_dim, int32_t page_size, int32_t table_stride,
+                             int64_t arena_rows, int32_t layout, int32_t capacity,
+                             int32_t longest, float scale, int32_t window, float softcap,
+                             int32_t fresh, void* workspace, size_t workspace_bytes,
+                             void* stream) {
+  return attention_weights(queries, keys, key_scales, true, tables, lengths, weights, out, batch,
+                           q_heads, kv_heads, head_dim, page_size, table_stride, arena_rows,
+                           layout, capacity, longest, scale, window, softcap, fresh, false,
+                           workspace, workspace_bytes, stream);
+}
+
+int pda_attention_weights_q8_bf16(const void* queries, const void* keys, const void* key_scales,
+                                  const int32_t* tables, const int32_t* lengths,
+                                  const float* weights, float* out, int32_t batch,
+                                  int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                                  int32_t page_size, int32_t table_stride, int64_t arena_rows,
+                                  int32_t layout, int32_t capacity, int32_t longest, float scale,
+                                  int32_t window, float softcap, int32_t fresh, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+  return attention_weights(queries, keys, key_scales, true, tables, lengths, weights, out, batch,
+                           q_heads, kv_heads, head_dim, page_size, table_stride, arena_rows,
+                           layout, capacity, longest, scale, window, softcap, fresh, true,
+                           workspace, workspace_bytes, stream);
+}
+
+int pda_evict_select(const float* weights, float* out_weights, const int32_t* tables,
+                     const int32_t* lengths, int32_t* kept, int32_t* new_lengths, int32_t batch,
+                     int32_t kv_heads, int32_t page_size, int32_t table_stride,
+                     int64_t arena_rows, int32_t capacity, int32_t out_capacity, int32_t keep,
+                     int32_t recent, int32_t sinks, void* stream) {
+  if (batch < 0 || batch > 65535 || kv_heads <= 0 || page_size <= 0 || table_stride <= 0 ||
+      capacity <= 0 || keep <= 0 || recent < 0 || sinks < 0)
+    return fail(PDA_ERR_INVALID_ARGUMENT,
+                "batch=%d kv_heads=%d page_size=%d table_stride=%d capacity=%d keep=%d recent=%d "
+                "sinks=%d",
+                batch, kv_heads, page_size, table_stride, capacity, keep, recent, sinks);
+  if ((int64_t)recent + sinks > keep)
+    return fail(PDA_ERR_INVALID_ARGUMENT, "recent %d and sinks %d exceed keep %d", recent, sinks,
+                keep);
+  if (batch == 0) return ok();
+  if (!weights || !tables || !lengths || !kept || !new_lengths)
+    return fail(PDA_ERR_INVALID_ARGUMENT, "null buffer pointer");
+  if (out_weights && out_capacity < std::min(keep, capacity))
+    return fail(PDA_ERR_INVALID_ARGUMENT, "out_capacity %d holds fewer than %d weights",
+                out_capacity, std::min(keep, capacity));
+  if (out_weights == weights && out_weights && out_capacity != capacity)
+    return fail(PDA_ERR_INVALID_ARGUMENT, "weights packed in place keep their capacity");
+  if (arena_rows < page_size)
+    return fail(PDA_ERR_INVALID_ARGUMENT, "arena_rows %lld holds no whole page",
+                (long long)arena_rows);
+  if (capacity > INT32_MAX - 4 * kSelectThreads)
+    return fail(PDA_ERR_TOO_LONG, "capacity %d next to 2^31", capacity);
+  if (((uintptr_t)weights | (uintptr_t)out_weights | (uintptr_t)tables | (uintptr_t)lengths |
+       (uintptr_t)kept | (uintptr_t)new_lengths) & 3)
+    return fail(PDA_ERR_ALIGNMENT, "all buffers must be 4-byte aligned");
+  SelectParams prm;
+  prm.weights = weights;
+  prm.out_weights = out_weights;
+  prm.tables = tables;
+  prm.lengths = lengths;
+  prm.kept = kept;
+  prm.new_lengths = new_lengths;
+  prm.arena_pages = arena_rows / page_size;
+  prm.table_stride = table_stride;
+  prm.page_size = page_size;
+  prm.hkv = kv_heads;
+  prm.capacity = capacity;
+  prm.out_capacity = out_capacity;
+  prm.keep = keep;
+  prm.recent = recent;
+  prm.sinks = sinks;
+  void* args[] = {&prm};
+  const hipError_t err =
+      hipLaunchKernel((const void*)evict_select_kernel, dim3(kv_heads, batch),
+                      dim3(kSelectThreads), args, 0, static_cast<hipStream_t>(stream));
+  if (err != hipSuccess)
+    return fail(PDA_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(err));
+  return ok();
+}
+
+int pda_evict_move(void* arena, void* arena2, int32_t width, const int32_t* kept,
+                   const int32_t* new_lengths, const int32_t* tables, const int32_t* out_tables,
+                   int32_t batch, int32_t kv_heads, int32_t page_size, int32_t table_stride,
+                   int32_t out_stride, int64_t arena_rows, int32_t layout, int32_t keep,
+                   void* stream) {
+  if (batch < 0 || batch > 65535 || kv_heads <= 0 || kv_heads > 32767 || page_size <= 0 ||
+      table_stride <= 0 || out_stride <= 0 || keep <= 0 || width <= 0)
+    return fail(PDA_ERR_INVALID_ARGUMENT,
+                "batch=%d kv_heads=%d page_size=%d table_stride=%d out_stride=%d keep=%d width=%d",
+                batch, kv_heads, page_size, table_stride, out_stride, keep, width);
+  if (batch == 0) return ok();
+  if (!arena || !kept || !new_lengths || !tables || !out_tables)
+    return fail(PDA_ERR_INVALID_ARGUMENT, "null buffer pointer");
+  if (layout != PDA_LAYOUT_ROWS && layout != PDA_LAYOUT_PAGES)
+    return fail(PDA_ERR_INVALID_ARGUMENT, "unknown K/V layout %d", layout);
+  if (arena_rows < page_size)
+    return fail(PDA_ERR_INVALID_ARGUMENT, "arena_rows %lld holds no whole page",
+                (long long)arena_rows);
+  if (((uintptr_t)kept | (uintptr_t)new_lengths | (uintptr_t)tables | (uintptr_t)out_tables) & 3)
+    return fail(PDA_ERR_ALIGNMENT, "index buffers must be 4-byte aligned");
+  MoveParams prm;
+  prm.arena[0] = static_cast<char*>(arena);
+  prm.arena[1] = static_cast<char*>(arena2);
+  prm.kept = kept;
+  prm.new_lengths = new_lengths;
+  prm.tables = tables;
+  prm.out_tables = out_tables;
+  prm.arena_pages = arena_rows / page_size;
+  prm.page_bytes = (int64_t)page_size * kv_heads * width;
+  const bool rows = layout == PDA_LAYOUT_ROWS;
+  prm.head_bytes = rows ? width : (int64_t)page_size * width;
+  prm.row_bytes = rows ? (int64_t)kv_heads * width : width;
+  prm.width = width;
+  prm.table_stride = table_stride;
+  prm.out_stride = out_stride;
+  prm.page_size = page_size;
+  prm.hkv = kv_heads;
+  prm.keep = keep;
+  // The widest piece that rows and buffers are aligned to.
+  const uintptr_t mis = (uintptr_t)arena | (uintptr_t)arena2 | (uintptr_t)width;
+  const int vec = mis % 16 == 0 ? 16 : mis % 4 == 0 ? 4 : mis % 2 == 0 ? 2 : 1;
+  const int arenas = arena2 ? 2 : 1;
+  void* args[] = {&prm};
+  const void* fn;
+  dim3 grid;
+  if (tables == out_tables) {
+    const int slice = vec >= 4 ? 4 * vec : vec;
+    const int64_t gx = (int64_t)arenas * ((width + slice - 1) / slice);
+    if (gx > INT32_MAX) return fail(PDA_ERR_INVALID_ARGUMENT, "width %d", width);
+    fn = vec == 16  ? (const void*)evict_pack_kernel<u32x4>
+         : vec == 4 ? (const void*)evict_pack_kernel<uint32_t>
+         : vec == 2 ? (const void*)evict_pack_kernel<uint16_t>
+                    : (const void*)evict_pack_kernel<uint8_t>;
+    grid = dim3((unsigned)gx, kv_heads, batch);
+  } else {
+    const int64_t per = ((int64_t)keep * (width / vec) + 1023) / 1024;
+    fn = vec == 16  ? (const void*)evict_copy_kernel<u32x4>
+         : vec == 4 ? (const void*)evict_copy_kernel<uint32_t>
+         : vec == 2 ? (const void*)evict_copy_kernel<uint16_t>
+                    : (const void*)evict_copy_kernel<uint8_t>;
+    grid = dim3((unsigned)std::min<int64_t>(per, 4096), arenas * kv_heads, batch);
+  }
+  const hipError_t err =
+      hipLaunchKernel(fn, grid, dim3(256), args, 0, static_cast<hipStream_t>(stream));
+  if (err != hipSuccess)
+    return fail(PDA_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(err));
+  return ok();
+}
+
+}  // extern "C"

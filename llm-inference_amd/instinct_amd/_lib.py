@@ -134,6 +134,21 @@ for _suffix in ("", "_bf16"):
 SIGNATURES["pda_latent_decode_workspace_bytes"] = (
     ctypes.c_int, [c_int32] * 7 + [ctypes.POINTER(c_size_t)])
 
+# Eviction by accumulated attention weight.
+_WEIGHTS_TAIL = ([c_void_p] * 4 + [c_int32] * 6 + [c_int64] + [c_int32] * 3
+                 + [c_float, c_int32, c_float, c_int32, c_void_p, c_size_t, c_void_p])
+for _suffix in ("", "_bf16"):
+    SIGNATURES["pda_attention_weights" + _suffix] = (ctypes.c_int, [c_void_p] * 2 + _WEIGHTS_TAIL)
+    SIGNATURES["pda_attention_weights_q8" + _suffix] = (ctypes.c_int,
+                                                        [c_void_p] * 3 + _WEIGHTS_TAIL)
+SIGNATURES["pda_attention_weights_workspace_bytes"] = (
+    ctypes.c_int, [c_int32] * 3 + [ctypes.POINTER(c_size_t)])
+SIGNATURES["pda_evict_select"] = (
+    ctypes.c_int, [c_void_p] * 6 + [c_int32] * 4 + [c_int64] + [c_int32] * 5 + [c_void_p])
+SIGNATURES["pda_evict_move"] = (
+    ctypes.c_int, [c_void_p] * 2 + [c_int32] + [c_void_p] * 4 + [c_int32] * 5
+    + [c_int64, c_int32, c_int32, c_void_p])
+
 _lib: ctypes.CDLL | None = None
 
 
@@ -209,6 +224,13 @@ def latent_decode_workspace_bytes(batch, q_heads, latent_dim, rope_dim, page_siz
     check(library().pda_latent_decode_workspace_bytes(batch, q_heads, latent_dim, rope_dim,
                                                       page_size, table_stride, longest,
                                                       ctypes.byref(out)))
+    return out.value
+
+
+def attention_weights_workspace_bytes(batch, q_heads, capacity) -> int:
+    out = c_size_t(0)
+    check(library().pda_attention_weights_workspace_bytes(batch, q_heads, capacity,
+                                                          ctypes.byref(out)))
     return out.value
 
 

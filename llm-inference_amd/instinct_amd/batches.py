@@ -22,6 +22,7 @@ from typing import Any
 import numpy as np
 import torch
 
+from .eviction import paged_attention_weights
 from .hip_kernels import (image_spans, paged_decode_attention, paged_prefill_attention, rope,
                           rope_append)
 from .paged_kv import KVCache
@@ -46,13 +47,23 @@ class DecodeBatch:
         *,
         positions: np.ndarray,
         tables: dict[str, list[np.ndarray]],
+        held: np.ndarray | None = None,
+        weights: dict[int, torch.Tensor] | None = None,
     ) -> None:
+        """``held``: the rows each sequence's cache holds before this token,
+        where rows were evicted (:meth:`KVCache.evict`) and it is no longer the
+        token's position. ``weights``: per layer float32 ``[batch, kv_heads,
+        capacity]``, to which the step's attention weights are added in place
+        (the new token's entry starts from them)."""
         device = cache.device
+        self.weights = weights or {}
         self.cache = cache
         self.tokens = tokens
         self.count = int(tokens.shape[0])
         positions = np.asarray(positions).astype(np.int64)
         self.offsets = torch.as_tensor(positions.astype(np.int32), device=device)
+        if held is not None:
+            positions = np.asarray(held).astype(np.int64)
         self.lengths = torch.as_tensor((positions + 1).astype(np.int32), device=device)
         self.longest = int(positions.max()) + 1
         page = cache.page_size
@@ -111,8 +122,15 @@ class DecodeBatch:
     def _attend_written(self, layer: int, q: torch.Tensor, *, scale: float,
                         softcap: float) -> torch.Tensor:
         group = self.cache.layer_group[layer]
+        q = q.to(self.cache.decode_dtype).contiguous()
+        if layer in self.weights:
+            paged_attention_weights(
+                q, self.cache.keys[layer], self._tables[group.name], self.lengths,
+                self.weights[layer], page_size=self.cache.page_size, longest=self.longest,
+                scale=scale, window=group.window, softcap=softcap,
+                scales=self.cache.scales(layer))
         out = paged_decode_attention(
-            q.to(self.cache.decode_dtype).contiguous(),
+            q,
             self.cache.keys[layer],
             self.cache.values[layer],
             self._tables[group.name],

@@ -321,6 +321,65 @@ class KVCache:
                 else:
                     arena[target, :, :count] = arena[source, :, :count]
 
+    def evict(self, name: str, tables: Sequence[np.ndarray], lengths: np.ndarray,
+              weights: dict[int, torch.Tensor], *, keep: int, recent: int = 0, sinks: int = 0
+              ) -> tuple[list[np.ndarray], np.ndarray]:
+        """Cut the sequences of a group that hold more than ``keep`` rows down to
+        ``keep``: in every layer and kv head the first ``sinks``, the last
+        ``recent`` and the heaviest other rows by ``weights[layer]`` (``[batch,
+        kv_heads, capacity]``, as ``DecodeBatch`` accumulates them), packed in
+        order at the front of the sequence's pages, the weights with them
+        (:func:`instinct_amd.eviction.evict_rows`). Pages no longer needed go
+        back to the pool. Where a cut sequence shares a page it would write
+        (a common prefix), the cut sequences move to fresh pages instead.
+        Returns the new page lists and lengths; the next token of a sequence
+        goes to row ``lengths[b]`` while its position counts on
+        (``DecodeBatch(held=...)``). No counterpart in the reference."""
+        from .eviction import evict_rows
+
+        group, pool = self.groups[name], self.pools[name]
+        if group.window:
+            raise ValueError("a windowed group releases its pages by position")
+        if keep <= 0 or recent < 0 or sinks < 0 or recent + sinks > keep:
+            raise ValueError("keep must be positive and hold recent and sinks")
+        lengths = np.asarray(lengths, dtype=np.int64)
+        tables = [np.asarray(t, dtype=np.int64) for t in tables]
+        need = [-(-int(n) // self.page_size) for n in lengths]
+        for table, pages in zip(tables, need):
+            if len(table) < pages or np.any(table[:pages] < 0):
+                raise RuntimeError("a sequence to evict from holds all its pages")
+        cut = [b for b, n in enumerate(lengths) if n > keep]
+        if not cut:
+            return tables, lengths
+        front = -(-keep // self.page_size)
+        packed = np.zeros((len(tables), max(need)), dtype=np.int32)
+        for b, pages in enumerate(need):
+            packed[b, :pages] = tables[b][:pages]
+        # Pages that more than one place of these tables, or another holder, has.
+        shared = any(pool.shared(int(page)) for b in cut for page in tables[b][:front])
+        out, fresh = None, {}
+        if shared:
+            taken = pool.allocate_many(front * len(cut), reserved=False).reshape(len(cut), front)
+            fresh = dict(zip(cut, taken))
+            out = np.zeros_like(packed)
+            for b, pages in enumerate(need):
+                new = fresh.get(b, tables[b][:pages])
+                out[b, :len(new)] = new
+        put = lambda a: torch.as_tensor(a.astype(np.int32), device=self.device)  # noqa: E731
+        dev_tables, dev_lengths = put(packed), put(lengths)
+        dev_out = None if out is None else put(out)
+        for layer in group.layers:
+            evict_rows(self.keys[layer], self.values[layer], weights[layer], dev_tables,
+                       dev_lengths, page_size=self.page_size, longest=int(lengths.max()),
+                       keep=keep, recent=recent, sinks=sinks, scales=self.scales(layer),
+                       out_tables=dev_out)
+        # (On this stream the rows are read before anything that follows writes
+        # the pages given back.)
+        for b in cut:
+            pool.release(tables[b] if shared else tables[b][front:])
+            tables[b] = np.asarray(fresh[b] if shared else tables[b][:front])
+        return tables, np.minimum(lengths, keep)
+
     def _split(self, rows: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         index = rows.long()
         return torch.div(index, self.page_size, rounding_mode="floor"), index % self.page_size
