@@ -641,6 +641,44 @@ int pda_latent_decode_attention_bf16(const void* queries, const void* arena,
                                      float scale, void* workspace,
                                      size_t workspace_bytes, void* stream);
 
+/* Bytes of workspace of a latent prefill call: the expanded keys and values of
+ * as many heads as fit in 1 GiB (one at least), the rotary keys beside them and,
+ * where key ranges are split, the ranges' partial results. */
+int pda_latent_prefill_workspace_bytes(int32_t start, int32_t count,
+                                       int32_t q_heads, int32_t rope_dim,
+                                       int32_t nope_dim, int32_t value_dim,
+                                       size_t* bytes);
+
+/* Prefill attention over latent rows for a chunk of one sequence's prompt, in
+ * the expanded form: every head's keys and values are projected out of the
+ * sequence's rows (rounded to the element type, into the workspace), then causal
+ * attention.
+ *   queries [count, q_heads, nope_dim + rope_dim] at positions start ..
+ *           start + count - 1, out [count, q_heads, value_dim]; table and its
+ *           masking as for pda_paged_prefill_attention (table_len >= 1); the
+ *           chunk's own rows are already written
+ * Query p sees the keys of positions 0 .. p that lie on a page of the arena; one
+ * that sees none gives zeros. Results are reproducible. A chunk of fewer than
+ * some 170 queries over a long prefix is cheaper as a
+ * pda_latent_decode_attention call with a batch row per token. Launches on
+ * `stream`; calls that share a workspace must not overlap. */
+int pda_latent_prefill_attention(const void* queries, const void* arena,
+                                 const void* kv_b, const int32_t* table,
+                                 int32_t table_len, int32_t start, int32_t count,
+                                 void* out, int32_t q_heads, int32_t latent_dim,
+                                 int32_t rope_dim, int32_t nope_dim,
+                                 int32_t value_dim, int32_t page_size,
+                                 int64_t arena_rows, float scale, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+int pda_latent_prefill_attention_bf16(const void* queries, const void* arena,
+                                 const void* kv_b, const int32_t* table,
+                                 int32_t table_len, int32_t start, int32_t count,
+                                 void* out, int32_t q_heads, int32_t latent_dim,
+                                 int32_t rope_dim, int32_t nope_dim,
+                                 int32_t value_dim, int32_t page_size,
+                                 int64_t arena_rows, float scale, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------------------
  * Eviction by accumulated attention weight. No counterpart in the reference
  * (which bounds a cache by sliding windows, mlx_engine.py:349-372): every key

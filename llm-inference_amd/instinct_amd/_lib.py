@@ -131,6 +131,11 @@ _LATENT_DECODE_ARGS = ([c_void_p] * 6 + [c_int32] * 8
 for _suffix in ("", "_bf16"):
     SIGNATURES["pda_latent_append" + _suffix] = (ctypes.c_int, _LATENT_APPEND_ARGS)
     SIGNATURES["pda_latent_decode_attention" + _suffix] = (ctypes.c_int, _LATENT_DECODE_ARGS)
+    SIGNATURES["pda_latent_prefill_attention" + _suffix] = (
+        ctypes.c_int, [c_void_p] * 4 + [c_int32] * 3 + [c_void_p] + [c_int32] * 6
+        + [c_int64, c_float, c_void_p, c_size_t, c_void_p])
+SIGNATURES["pda_latent_prefill_workspace_bytes"] = (
+    ctypes.c_int, [c_int32] * 6 + [ctypes.POINTER(c_size_t)])
 SIGNATURES["pda_latent_decode_workspace_bytes"] = (
     ctypes.c_int, [c_int32] * 7 + [ctypes.POINTER(c_size_t)])
 
@@ -224,6 +229,13 @@ def latent_decode_workspace_bytes(batch, q_heads, latent_dim, rope_dim, page_siz
     check(library().pda_latent_decode_workspace_bytes(batch, q_heads, latent_dim, rope_dim,
                                                       page_size, table_stride, longest,
                                                       ctypes.byref(out)))
+    return out.value
+
+
+def latent_prefill_workspace_bytes(start, count, q_heads, rope_dim, nope_dim, value_dim) -> int:
+    out = c_size_t(0)
+    check(library().pda_latent_prefill_workspace_bytes(start, count, q_heads, rope_dim, nope_dim,
+                                                       value_dim, ctypes.byref(out)))
     return out.value
 
 

@@ -9,11 +9,14 @@ share. The reference has no such layer; paging, tables, lengths and the order
 * :func:`latent_append`: normalise, rotate and write a step's or a chunk's rows
   and rotate the queries, in one launch;
 * :func:`latent_decode_attention`: one new token per sequence, absorbed form
-  (the queries are projected into the latent and attend over the rows).
+  (the queries are projected into the latent and attend over the rows);
+* :func:`latent_prefill_attention`: a chunk of one prompt, expanded form (every
+  head's keys and values are projected out, then causal attention).
 
 Head shapes: latents of 8..512 dims and nope and value dims of 8..128, in
 eights; rotary parts of 0..64 dims in sixteens; any number of heads; fp16 or
-bf16 throughout. The work happens in libpda.so (``csrc/pda_latent.hip``).
+bf16 throughout. The work happens in libpda.so (``csrc/pda_latent.hip``,
+``csrc/pda_latent_prefill.hip``).
 """
 
 from __future__ import annotations
@@ -187,5 +190,61 @@ def latent_decode_attention(queries: torch.Tensor, arena: torch.Tensor, kv_b: to
             lengths.data_ptr(), out.data_ptr(), batch, q_heads, latent, rope, nope, value,
             int(page_size), stride, int(arena.shape[0]), int(longest), float(scale),
             ws.data_ptr(), ws.numel(), stream)
+    _lib.check(rc)
+    return out
+
+
+def latent_prefill_workspace_bytes(start: int, queries_shape: tuple[int, int, int],
+                                   arena: torch.Tensor, kv_b: torch.Tensor) -> int:
+    """Bytes of workspace :func:`latent_prefill_attention` needs for this shape
+    (``pda_latent_prefill_workspace_bytes``)."""
+    count, q_heads, q_width = (int(x) for x in queries_shape)
+    _, _, rope, nope, value = _head_shape(q_width, arena, kv_b)
+    return _lib.latent_prefill_workspace_bytes(int(start), count, q_heads, rope, nope, value)
+
+
+def latent_prefill_attention(queries: torch.Tensor, arena: torch.Tensor, kv_b: torch.Tensor,
+                             table: torch.Tensor, *, start: int, page_size: int, scale: float,
+                             out: torch.Tensor | None = None,
+                             workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of one prompt chunk over its sequence's latent rows, in the
+    expanded form: ``queries`` ``[count, q_heads, nope + rope]`` (rotated) at
+    positions ``start ..``, each over the keys up to its own, the chunk's rows
+    already written; ``arena`` and ``kv_b`` as for
+    :func:`latent_decode_attention`, ``table`` the sequence's int32 pages.
+    Returns ``[count, q_heads, value]`` (zeros for a query with no key to see).
+    ``workspace``: a uint8 device tensor the caller owns (at least
+    :func:`latent_prefill_workspace_bytes`), else the stream's cached one."""
+    _check_16bit("queries", queries, 3, queries)
+    _check_16bit("arena", arena, 2, queries)
+    _check_16bit("kv_b", kv_b, 3, queries)
+    count, q_heads, q_width = (int(x) for x in queries.shape)
+    heads, latent, rope, nope, value = _head_shape(q_width, arena, kv_b)
+    if heads != q_heads:
+        raise ValueError("kv_b must have the queries' heads")
+    device = queries.device
+    if table.dtype != torch.int32 or table.dim() != 1 or table.device != device:
+        raise ValueError(f"table must be an int32 vector on {device}")
+    if int(table.shape[0]) == 0 and count > 0:
+        raise ValueError("the table holds no pages")
+    table = table.contiguous()
+    if out is None:
+        out = torch.empty((count, q_heads, value), dtype=queries.dtype, device=device)
+    _check_16bit("out", out, 3, queries)
+    if tuple(out.shape) != (count, q_heads, value):
+        raise ValueError("out must be [count, q_heads, value]")
+    if count == 0:
+        return out
+    need = _lib.latent_prefill_workspace_bytes(int(start), count, q_heads, rope, nope, value)
+    stream = int(torch.cuda.current_stream(device).cuda_stream)
+    ws = (stream_workspace(device, need, stream) if workspace is None
+          else _given_workspace(workspace, device, need))
+    entry = "pda_latent_prefill_attention" + ("_bf16" if queries.dtype == torch.bfloat16 else "")
+    with torch.cuda.device(device):
+        rc = getattr(_lib.library(), entry)(
+            queries.data_ptr(), arena.data_ptr(), kv_b.data_ptr(), table.data_ptr(),
+            int(table.shape[0]), int(start), count, out.data_ptr(), q_heads, latent, rope, nope,
+            value, int(page_size), int(arena.shape[0]), float(scale), ws.data_ptr(), ws.numel(),
+            stream)
     _lib.check(rc)
     return out

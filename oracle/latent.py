@@ -108,3 +108,52 @@ def append(q, latent, k_rope, arena, positions, rows, *, inv_freq, norm_weight, 
     if rope:
         q = torch.cat([q[..., :-rope], turn(q[..., -rope:])], dim=-1)
     return q, arena
+
+
+def prefill(q, arena, kv_b, table, *, start, page_size, scale):
+    """(out, bound) of the prefill call, [count, heads, value] float64.
+
+    The bound, with u half a step of the type: the output's rounding u |out|;
+    the weights' u p and the keys' (scores off by u A, A = scale * |q| . |key|),
+    to first order, each times |v - out|; the values' u p |v|; a fp16 weight
+    below the normal range by half its smallest step. 1.1, 2e-5 and 2^-24 a step
+    of the terms' size as for the decode call; the keys' and values' own sums
+    over 512 latent dims take 32 + 16 steps of the size of |U_h| |c|, |D_h| |c|."""
+    u = HALF_STEP[q.dtype]
+    heads, width, latent = kv_b.shape
+    count = q.shape[0]
+    rope = arena.shape[1] - latent
+    nope = q.shape[2] - rope
+    end = start + count
+    rows = rows_of(table, page_size, end, arena.shape[0])
+    good = torch.as_tensor(rows >= 0)
+    x = arena[torch.as_tensor(np.maximum(rows, 0))].double()
+    x[~good] = 0.0
+    c, k = x[:, :latent], x[:, latent:]
+    hidden = (torch.arange(end)[None] > start + torch.arange(count)[:, None]) | ~good[None]
+    none = hidden.all(-1)
+    out = torch.zeros((count, heads, width - nope), dtype=torch.float64)
+    bound = torch.zeros_like(out)
+    step = 48 * 2.0 ** -24
+    tiny = 2.0 ** -25 if q.dtype == torch.float16 else 0.0
+    for h in range(heads):
+        w = kv_b[h].double()
+        key, v = c @ w[:nope].t(), c @ w[nope:].t()
+        key_terms, v_terms = c.abs() @ w[:nope].abs().t(), c.abs() @ w[nope:].abs().t()
+        qh = q[:, h].double()
+        s = scale * (qh[:, :nope] @ key.t() + qh[:, nope:] @ k.t())
+        p = torch.softmax(s.masked_fill(hidden, -np.inf), dim=-1)
+        p[none] = 0.0
+        a = abs(scale) * (qh[:, :nope].abs() @ key.abs().t())
+        b = abs(scale) * (qh[:, :nope].abs() @ key_terms.t()) * step
+        o = p @ v
+        for i in range(count):
+            off = (v - o[i]).abs()
+            spread = (p[i] * (1 + a[i])) @ off
+            bound[i, h] = (1.1 * u * (o[i].abs() + spread + p[i] @ v.abs())
+                           + 1.1 * ((p[i] * b[i]) @ off) + step * (p[i] @ v_terms)
+                           + (end / 16 + 64) * 2.0 ** -24 * (p[i] @ v.abs())
+                           + tiny * (1 + (off * (~hidden[i])[:, None]).sum(0))
+                           + 2e-5 * (o[i].abs() + spread))
+        out[:, h] = o
+    return out, bound

@@ -27,6 +27,15 @@ def decode(**overrides):
     return _lib.library().pda_latent_decode_attention_bf16(*args.values())
 
 
+def prefill(**overrides):
+    args = dict(queries=FAKE, arena=FAKE, kv_b=FAKE, table=FAKE, table_len=64, start=100, count=50,
+                out=FAKE, q_heads=16, latent_dim=512, rope_dim=64, nope_dim=128, value_dim=128,
+                page_size=16, arena_rows=4096, scale=0.07, workspace=FAKE,
+                workspace_bytes=1 << 31, stream=None)
+    args.update(overrides)
+    return _lib.library().pda_latent_prefill_attention(*args.values())
+
+
 SHAPES = [
     (dict(q_heads=0), _lib.PDA_ERR_INVALID_ARGUMENT),
     (dict(q_heads=65536), _lib.PDA_ERR_INVALID_ARGUMENT),
@@ -86,7 +95,37 @@ def test_decode_rejects(overrides, code):
     assert _lib.library().pda_last_error().decode() != ""
 
 
+@pytest.mark.parametrize("overrides, code", SHAPES + [
+    (dict(value_dim=0), _lib.PDA_ERR_INVALID_ARGUMENT),
+    (dict(count=-1), _lib.PDA_ERR_INVALID_ARGUMENT),
+    (dict(start=-1), _lib.PDA_ERR_INVALID_ARGUMENT),
+    (dict(start=(1 << 31) - 60), _lib.PDA_ERR_TOO_LONG),
+    (dict(table_len=0), _lib.PDA_ERR_INVALID_ARGUMENT),
+    (dict(page_size=0), _lib.PDA_ERR_INVALID_ARGUMENT),
+    (dict(arena_rows=8), _lib.PDA_ERR_INVALID_ARGUMENT),
+    (dict(arena_rows=1 << 31), _lib.PDA_ERR_INVALID_ARGUMENT),
+    (dict(scale=float("nan")), _lib.PDA_ERR_INVALID_ARGUMENT),
+    (dict(table=None), _lib.PDA_ERR_INVALID_ARGUMENT),
+    (dict(table=FAKE + 2), _lib.PDA_ERR_ALIGNMENT),
+    (dict(workspace=None), _lib.PDA_ERR_WORKSPACE),
+    (dict(workspace_bytes=1024), _lib.PDA_ERR_WORKSPACE),
+    (dict(workspace=FAKE + 64), _lib.PDA_ERR_ALIGNMENT),
+])
+def test_prefill_rejects(overrides, code):
+    assert prefill(**overrides) == code
+    assert _lib.library().pda_last_error().decode() != ""
+
+
+def test_prefill_workspace_is_bounded():
+    """The expanded rows of as many heads as fit in 1 GiB, not of all."""
+    some = _lib.latent_prefill_workspace_bytes(0, 4096, 128, 64, 128, 128)
+    assert some >= 4096 * 128 * 256 * 2
+    far = _lib.latent_prefill_workspace_bytes(130000, 1024, 128, 64, 128, 128)
+    assert far < (1 << 30) + (1 << 29)
+
+
 def test_empty_calls_are_no_ops():
+    assert prefill(count=0) == _lib.PDA_OK
     assert append(n=0) == _lib.PDA_OK
     assert decode(batch=0, workspace=None, workspace_bytes=0) == _lib.PDA_OK
     assert _lib.latent_decode_workspace_bytes(0, 16, 512, 64, 16, 4, 1) == 0
