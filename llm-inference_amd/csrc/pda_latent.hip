@@ -237,7 +237,6 @@ __global__ __launch_bounds__(256) void latent_absorb_kernel(const LatentDecodePa
     }
   }
   const int d0 = (blockIdx.x * 4 + w) * 32;
-  if (d0 >= p.latent) return;
   // The wave's columns of U_h: rows of 64 bytes, zeros past either edge.
   const f16* u = p.kv_b + (int64_t)h * (p.nope + p.value) * p.latent;
   const int steps = (p.nope + 15) / 16;
@@ -277,15 +276,24 @@ __global__ __launch_bounds__(256) void latent_absorb_kernel(const LatentDecodePa
       if (i == j) q8 = qf[j];
     acc = mfma16<BF>(f16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}, q8, acc);
   }
-  if (!live) return;
-  f16* dst = p.q_lat + ((int64_t)(b0 + n) * p.hq + h) * width + d0 + 4 * hh;
+  // The workgroup's 32 x 128 results through LDS, written along the rows.
+  constexpr int kPitch = 136;
+  __syncthreads();
+  f16* so = s_u[0];
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
-    if (d0 + 8 * g >= p.latent) break;
     f16x4 y;
 #pragma unroll
     for (int t = 0; t < 4; ++t) y[t] = round16<BF>(acc[4 * g + t]);
-    *reinterpret_cast<f16x4*>(dst + 8 * g) = y;
+    *reinterpret_cast<f16x4*>(so + n * kPitch + 32 * w + 8 * g + 4 * hh) = y;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = tid; i < 32 * 16; i += 256) {
+    const int b = b0 + i / 16, d = blockIdx.x * 128 + 8 * (i % 16);
+    if (b < p.batch && d < p.latent)
+      *reinterpret_cast<f16x8*>(p.q_lat + ((int64_t)b * p.hq + h) * width + d) =
+          *reinterpret_cast<const f16x8*>(so + (i / 16) * kPitch + 8 * (i % 16));
   }
 }
 
@@ -372,10 +380,14 @@ __global__ __launch_bounds__(256, 1) void latent_decode_kernel(const LatentDecod
     const int keys = (int)keys_of(p, b);
     f16x8 qf[2 * WP];
     {
+      // (The pieces' places are computed here for every sequence: kept through
+      // the loop they were spilled, and 50 reloads in turn took 15 us.)
+      int part = 8 * hh;
+      asm volatile("" : "+v"(part));
       const f16* qp = p.q_lat + ((int64_t)b * p.hq + (live ? h : 0)) * width;
 #pragma unroll
       for (int c = 0; c < 2 * WP; ++c) {
-        const int d = 16 * c + 8 * hh;
+        const int d = 16 * c + part;
         const f16x8 x = *reinterpret_cast<const f16x8*>(qp + min(d, width - 8));
         qf[c] = live && d < width ? x : f16x8{};
       }
@@ -390,15 +402,23 @@ __global__ __launch_bounds__(256, 1) void latent_decode_kernel(const LatentDecod
       const int tiles = min(kChunkTiles, tb - c0);
       // Arena rows of the chunk's keys; -1: no such key, or no such page.
       __syncthreads();
-      for (int i = tid; i < tiles * kTileKeys; i += 256) {
-        const int key = c0 * kTileKeys + i;
-        int row = -1;
-        if (key < keys) {
-          const uint32_t pi = (uint32_t)key / (uint32_t)p.page_size;
-          const uint32_t page = (uint32_t)p.tables[(int64_t)b * p.table_stride + pi];
-          if (page < pages) row = (int)(page * (uint32_t)p.page_size + (key - pi * p.page_size));
+      {
+        constexpr int kEach = kChunkKeys / 256;
+        uint32_t page[kEach];
+        const int64_t table = (int64_t)b * p.table_stride;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+          const int key = c0 * kTileKeys + 256 * i + tid;
+          page[i] = ~0u;
+          if (256 * i < tiles * kTileKeys && key < keys)
+            page[i] = (uint32_t)p.tables[table + (uint32_t)key / (uint32_t)p.page_size];
         }
-        s_row[i] = row;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+          const int key = c0 * kTileKeys + 256 * i + tid;
+          const uint32_t r = (uint32_t)key % (uint32_t)p.page_size;
+          s_row[256 * i + tid] = page[i] < pages ? (int)(page[i] * (uint32_t)p.page_size + r) : -1;
+        }
       }
       __syncthreads();
       // Tile `tile` of the chunk into slot `slot` of the wave's ring: this
@@ -511,12 +531,27 @@ __global__ __launch_bounds__(256, 1) void latent_decode_kernel(const LatentDecod
       // have landed, everyone is past the round before, whose slot takes the
       // next copies.
       constexpr int kFirst = NHG > 1 ? NHG - 1 : 1;
+      // Copies of a tile that this wave issues: its planes, in two halves.
+      constexpr int kLess = 2 * (WP / NHG), kMore = 2 * ((WP + NHG - 1) / NHG);
+      constexpr int kTwo = NHG > 3 ? 2 : 0, kOne = NHG > 2 ? 1 : 0;
+      const bool more = hg < WP % NHG;
+      auto landed = [&](auto later) {  // all but those of `later` tiles
+        if (more)
+          wait_vmem<later.value * kMore>();
+        else
+          wait_vmem<later.value * kLess>();
+      };
       for (int r = 0; r < min(kFirst, rounds); ++r)
         if (r * kGroups + kg < tiles) copy(r * kGroups + kg, r % NHG);
       for (int r = 0; r < rounds; ++r) {
         const int tile = r * kGroups + kg;
         const bool here = tile < tiles;
-        wait_vmem<0>();
+        if (NHG > 3 && tile + 2 * kGroups < tiles)
+          landed(std::integral_constant<int, kTwo>{});
+        else if (NHG > 2 && tile + kGroups < tiles)
+          landed(std::integral_constant<int, kOne>{});
+        else
+          wait_vmem<0>();
         if (here) clean(tile, r % NHG);
         if constexpr (NHG > 1) {
           __syncthreads();
@@ -583,49 +618,104 @@ __global__ __launch_bounds__(256, 1) void latent_decode_kernel(const LatentDecod
 }
 
 // Joins the partials of each sequence and projects the result: out[b, h] = D_h
-// o / sum. A workgroup has one head and up to 32 sequences; the joined latents
-// go to LDS as two 16-bit numbers each (the value and what its rounding left),
-// so the product with D_h loses nothing that the output's rounding would show;
-// a wave takes 32 value dims at a time. D_h is read once a workgroup.
+// o / sum. A workgroup has one head and up to 32 sequences. D_h's rows, which
+// nothing before them decides, are loaded first and are under way while the
+// partials are joined: a wave has the rows of 32 value dims over half the latent.
+// A wave joins a whole row of partials (512 dims) of one sequence, several
+// waves share a sequence's partials where there are few sequences. The joined
+// latents go to LDS as two 16-bit numbers each (the value and what its rounding
+// left), so the product loses nothing that the output's rounding would show.
 template <bool BF>
-__global__ __launch_bounds__(256) void latent_merge_kernel(const LatentDecodeParams p) {
-  constexpr int kRow = kMaxLatent + 8;  // halves between sequences
+__global__ __launch_bounds__(512, 2) void latent_merge_kernel(const LatentDecodeParams p) {
+  constexpr int kWaves = 8;
+  constexpr int kRow = kMaxLatent + 8;        // halves between sequences
+  constexpr int kSteps = kMaxLatent / 16 / 2; // 16-dim steps of a half
   __shared__ __align__(16) f16 s_hi[32 * kRow];
   __shared__ __align__(16) f16 s_lo[32 * kRow];
+  __shared__ __align__(16) float s_part[kWaves][kMaxLatent];
   const int tid = threadIdx.x, w = uniform(tid >> 6), lane = tid & 63;
   const int n = lane & 31, hh = lane >> 5;
   const int h = blockIdx.x, b0 = blockIdx.y * p.merge_batch;
   const int count = min(p.merge_batch, p.batch - b0);
+  const int v0 = 32 * (w & 3), k0 = (w >> 2) * (kMaxLatent / 2);
+  f16x8 a[kSteps];
+  {
+    const f16* wp = p.kv_b + ((int64_t)h * (p.nope + p.value) + p.nope + min(v0 + n, p.value - 1)) *
+                                 p.latent;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      const int k = k0 + 16 * i + 8 * hh;
+      a[i] = f16x8{};
+      if (k < p.latent && v0 < p.value) a[i] = *reinterpret_cast<const f16x8*>(wp + k);
+    }
+  }
   const int total = p.prefix[p.batch];
   const int per = max(1, (int)(((int64_t)total + p.groups - 1) / p.groups));
-  for (int i = tid; i < count * (p.latent / 8); i += 256) {
-    const int r = i / (p.latent / 8), d = 8 * (i % (p.latent / 8));
-    const int b = b0 + r;
+  const int share = count >= 8 ? 1 : count >= 4 ? 2 : count >= 2 ? 4 : 8;  // waves a sequence
+  const int d = 8 * lane;
+  for (int r0 = 0; r0 < count; r0 += kWaves / share) {
+    const int r = r0 + w / share, part = w % share;
+    const bool have = r < count;
+    const int b = b0 + (have ? r : 0);
     const int seq0 = p.prefix[b], seq1 = p.prefix[b + 1];
-    const int g0 = seq0 / per, g1 = seq1 > seq0 ? (seq1 - 1) / per : g0 - 1;
-    float top = -INFINITY, sum = 0.0f;
-    for (int g = g0; g <= g1; ++g)
-      top = fmaxf(top, p.part_ml[((int64_t)g + b) * p.hq + h].x);
-    float acc[8] = {};
-    if (top != -INFINITY) {
-      for (int g = g0; g <= g1; ++g) {
-        const int64_t at = ((int64_t)g + b) * p.hq + h;
-        const float2 ml = p.part_ml[at];
-        if (ml.x == -INFINITY) continue;
-        const float f = __builtin_amdgcn_exp2f(ml.x - top);
-        sum = fmaf(ml.y, f, sum);
-        const float4* src = reinterpret_cast<const float4*>(p.part_o + at * p.latent + d);
-        const float4 x = src[0], y = src[1];
-        acc[0] = fmaf(x.x, f, acc[0]);
-        acc[1] = fmaf(x.y, f, acc[1]);
-        acc[2] = fmaf(x.z, f, acc[2]);
-        acc[3] = fmaf(x.w, f, acc[3]);
-        acc[4] = fmaf(y.x, f, acc[4]);
-        acc[5] = fmaf(y.y, f, acc[5]);
-        acc[6] = fmaf(y.z, f, acc[6]);
-        acc[7] = fmaf(y.w, f, acc[7]);
+    const int g0 = seq0 / per, slots = have && seq1 > seq0 ? (seq1 - 1) / per - g0 + 1 : 0;
+    const float2* ml = p.part_ml + ((int64_t)g0 + b) * p.hq + h;
+    const float* po = p.part_o + (((int64_t)g0 + b) * p.hq + h) * p.latent;
+    // A lane looks at every 64th partial's maximum and sum.
+    float top = -INFINITY;
+    for (int g = lane; g < slots; g += 64) top = fmaxf(top, ml[(int64_t)g * p.hq].x);
+#pragma unroll
+    for (int i = 32; i; i >>= 1) top = fmaxf(top, __shfl_xor(top, i));
+    float sum = 0.0f, acc[8] = {};
+    for (int base = 0; base < slots; base += 64) {
+      float f = 0.0f;
+      if (base + lane < slots && top != -INFINITY) {
+        const float2 x = ml[(int64_t)(base + lane) * p.hq];
+        f = x.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x.x - top);
+        sum = fmaf(x.y, f, sum);
+      }
+      const int end = min(64, slots - base);
+      constexpr int kEach = 4;  // rows under way
+      for (int g = part; g < end; g += share * kEach) {
+        float4 x[kEach][2];
+        float fg[kEach];
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+          const int at = g + share * j;
+          fg[j] = __shfl(f, min(at, 63));
+          if (at >= end || fg[j] == 0.0f || d >= p.latent) fg[j] = 0.0f;
+          const float4* src = reinterpret_cast<const float4*>(
+              po + (int64_t)(base + min(at, end - 1)) * p.hq * p.latent + min(d, p.latent - 8));
+          x[j][0] = src[0];
+          x[j][1] = src[1];
+        }
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+          // (A partial without a key holds zeros: nothing to leave out.)
+          acc[0] = fmaf(x[j][0].x, fg[j], acc[0]);
+          acc[1] = fmaf(x[j][0].y, fg[j], acc[1]);
+          acc[2] = fmaf(x[j][0].z, fg[j], acc[2]);
+          acc[3] = fmaf(x[j][0].w, fg[j], acc[3]);
+          acc[4] = fmaf(x[j][1].x, fg[j], acc[4]);
+          acc[5] = fmaf(x[j][1].y, fg[j], acc[5]);
+          acc[6] = fmaf(x[j][1].z, fg[j], acc[6]);
+          acc[7] = fmaf(x[j][1].w, fg[j], acc[7]);
+        }
       }
     }
+#pragma unroll
+    for (int i = 32; i; i >>= 1) sum += __shfl_xor(sum, i);
+    if (share > 1) {
+      if (r0) __syncthreads();
+      *reinterpret_cast<float4*>(&s_part[w][d]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      *reinterpret_cast<float4*>(&s_part[w][d + 4]) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+      __syncthreads();
+      if (part == 0)
+        for (int i = 1; i < share; ++i)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) acc[j] += s_part[w + i][d + j];
+    }
+    if (part || !have || d >= p.latent) continue;
     const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
     f16x8 hi, lo;
 #pragma unroll
@@ -639,34 +729,36 @@ __global__ __launch_bounds__(256) void latent_merge_kernel(const LatentDecodePar
   }
   __syncthreads();
   const bool have = n < count;
-  const f16* down = p.kv_b + ((int64_t)h * (p.nope + p.value) + p.nope) * p.latent;
-  for (int v0 = 32 * w; v0 < p.value; v0 += 128) {
-    const int vr = v0 + n;
-    const f16* wp = down + (int64_t)min(vr, p.value - 1) * p.latent + 8 * hh;
-    f32x16 acc = {}, rest = {};
-    for (int k = 0; k < p.latent; k += 16) {
-      f16x8 a = {}, hi = {}, lo = {};
-      if (k + 8 * hh < p.latent) {
-        a = *reinterpret_cast<const f16x8*>(wp + k);
-        if (have) {
-          hi = *reinterpret_cast<const f16x8*>(&s_hi[n * kRow + k + 8 * hh]);
-          lo = *reinterpret_cast<const f16x8*>(&s_lo[n * kRow + k + 8 * hh]);
-        }
-      }
-      acc = mfma16<BF>(a, hi, acc);
-      rest = mfma16<BF>(a, lo, rest);
-    }
-    if (have) {
-      f16* dst = p.out + ((int64_t)(b0 + n) * p.hq + h) * p.value + v0 + 4 * hh;
+  f32x16 acc = {}, rest = {};
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        if (v0 + 8 * g >= p.value) break;
-        f16x4 y;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) y[t] = round16<BF>(acc[4 * g + t] + rest[4 * g + t]);
-        *reinterpret_cast<f16x4*>(dst + 8 * g) = y;
-      }
+  for (int i = 0; i < kSteps; ++i) {
+    const int k = k0 + 16 * i + 8 * hh;
+    f16x8 hi = {}, lo = {};
+    if (have && k < p.latent) {
+      hi = *reinterpret_cast<const f16x8*>(&s_hi[n * kRow + k]);
+      lo = *reinterpret_cast<const f16x8*>(&s_lo[n * kRow + k]);
     }
+    acc = mfma16<BF>(a[i], hi, acc);
+    rest = mfma16<BF>(a[i], lo, rest);
+  }
+  // The two halves of the latent.
+  float* join = &s_part[0][0];
+  __syncthreads();
+  if (w >= 4) {
+#pragma unroll
+    for (int v = 0; v < 16; ++v) join[((w - 4) * 16 + v) * 64 + lane] = acc[v] + rest[v];
+  }
+  __syncthreads();
+  if (w >= 4 || !have) return;
+  f16* dst = p.out + ((int64_t)(b0 + n) * p.hq + h) * p.value + v0 + 4 * hh;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    if (v0 + 8 * g >= p.value) break;
+    f16x4 y;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+      y[t] = round16<BF>(acc[4 * g + t] + rest[4 * g + t] + join[(w * 16 + 4 * g + t) * 64 + lane]);
+    *reinterpret_cast<f16x4*>(dst + 8 * g) = y;
   }
 }
 
@@ -871,7 +963,7 @@ int latent_decode(const void* queries, const void* arena, const void* kv_b, cons
   if (err == hipSuccess)
     err = hipLaunchKernel(
         bf ? (const void*)latent_merge_kernel<true> : (const void*)latent_merge_kernel<false>,
-        dim3(q_heads, (batch + prm.merge_batch - 1) / prm.merge_batch), dim3(256), args, 0, hs);
+        dim3(q_heads, (batch + prm.merge_batch - 1) / prm.merge_batch), dim3(512), args, 0, hs);
   if (err != hipSuccess)
     return fail(PDA_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(err));
   return ok();
