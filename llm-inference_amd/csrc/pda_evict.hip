@@ -151,6 +151,7 @@ __global__ __launch_bounds__(64 * kWaves) void attention_scores_kernel(const Wei
   const int lo = p.window > 0 ? max(0, keys - p.window) : 0;
   const uint32_t pages = (uint32_t)min(p.arena_pages, (int64_t)INT32_MAX);
 
+  const int32_t* table = p.tables + (int64_t)b * p.table_stride;
   f16x8 qf[NC];
   const int64_t qat = ((int64_t)b * p.hq + (live ? h : 0)) * p.head_dim;
 #pragma unroll
@@ -164,23 +165,27 @@ __global__ __launch_bounds__(64 * kWaves) void attention_scores_kernel(const Wei
     uint32_t seen = 0;  // bit i: this lane's key of block i has a row
     int64_t at[kBlocks];
     float ks[kBlocks];
+    // (All table entries first, then all rows: with a branch per key the
+    // lookups waited for each other.)
+    uint32_t page[kBlocks], row[kBlocks];
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i) {
+      const uint32_t key = (uint32_t)min(k0 + 16 * i + n16, keys - 1);
+      const uint32_t pi = key / (uint32_t)p.page_size;
+      row[i] = key - pi * (uint32_t)p.page_size;
+      page[i] = (uint32_t)table[pi];
+    }
 #pragma unroll
     for (int i = 0; i < kBlocks; ++i) {
       const int key = k0 + 16 * i + n16;
-      at[i] = 0;
+      const bool have = key >= lo && key < keys && page[i] < pages;
+      seen |= have ? 1u << i : 0u;
+      page[i] = have ? page[i] : 0u;
+      at[i] = page[i] * p.page_elems + (int64_t)kvh * p.head_elems + (int64_t)row[i] * p.row_elems;
       ks[i] = 1.0f;
-      if (key >= lo && key < keys) {
-        const uint32_t pi = (uint32_t)key / (uint32_t)p.page_size;
-        const int r = key - (int)pi * p.page_size;
-        const uint32_t page = (uint32_t)p.tables[(int64_t)b * p.table_stride + pi];
-        if (page < pages) {
-          seen |= 1u << i;
-          at[i] = page * p.page_elems + (int64_t)kvh * p.head_elems + (int64_t)r * p.row_elems;
-          if constexpr (Q8)
-            ks[i] = (float)p.kscale[page * p.scale_page + (int64_t)kvh * p.scale_head +
-                                    (int64_t)r * p.scale_row];
-        }
-      }
+      if constexpr (Q8)
+        ks[i] = (float)p.kscale[page[i] * p.scale_page + (int64_t)kvh * p.scale_head +
+                                (int64_t)row[i] * p.scale_row];
     }
     f16x8 kf[kBlocks][NC <= 4 ? NC : 1];
     if constexpr (NC <= 4) {
@@ -266,10 +271,12 @@ __global__ __launch_bounds__(64 * kWaves) void attention_scores_kernel(const Wei
 
 // out[t] = weights[t] (0 for the `fresh` newest) + the sum over the kv head's
 // query heads, in their order, of the normalised weights: the chunks' maxima and
-// sums give each head's, once a workgroup.
+// sums give each head's, once a workgroup, while the weights themselves are
+// already under way. Reads 4 bytes a head and key, from the caches that the
+// launch before left them in.
 __global__ __launch_bounds__(256) void attention_weights_kernel(const WeightParams p) {
-  constexpr int kHeads = 32;  // heads whose factors are held at once
-  constexpr int kParts = kAddKeys / kChunk;
+  constexpr int kHeads = 8;  // heads at once: two a wave for the statistics
+  constexpr int kParts = kAddKeys / kChunk, kEach = kAddKeys / 256;
   __shared__ float s_f[kHeads][kParts];
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
   const int group = p.hq / p.hkv, kvh = blockIdx.y, b = blockIdx.z;
@@ -278,59 +285,66 @@ __global__ __launch_bounds__(256) void attention_weights_kernel(const WeightPara
   const int c_lo = lo / kChunk, c_hi = (keys + kChunk - 1) / kChunk;
   const int64_t base = ((int64_t)b * p.hkv + kvh) * p.capacity;
   for (int64_t k0 = (int64_t)blockIdx.x * kAddKeys; k0 < keys; k0 += (int64_t)gridDim.x * kAddKeys) {
-    float acc[kAddKeys / 256] = {}, old[kAddKeys / 256];
+    float acc[kEach] = {}, old[kEach];
 #pragma unroll
-    for (int i = 0; i < kAddKeys / 256; ++i) {
+    for (int i = 0; i < kEach; ++i) {
       const int64_t t = k0 + 256 * i + tid;
       old[i] = t < (int64_t)keys - p.fresh ? p.weights[base + t] : 0.0f;
     }
     for (int h0 = 0; h0 < group; h0 += kHeads) {
       const int heads = min(kHeads, group - h0);
+      const int64_t row = (int64_t)b * p.hq + kvh * group + h0;
+      float x[kHeads][kEach];
+#pragma unroll
+      for (int j = 0; j < kHeads; ++j)
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+          const int64_t t = k0 + 256 * i + tid;
+          x[j][i] = 0.0f;
+          if (j < heads && t >= (int64_t)c_lo * kChunk && t < keys)
+            x[j][i] = p.probs[(row + j) * p.capacity + t];
+        }
       __syncthreads();
       for (int i = w; i < heads; i += 4) {
-        const float2* st = p.stats + ((int64_t)b * p.hq + kvh * group + h0 + i) * p.chunks;
+        const float2* st = p.stats + (row + i) * p.chunks;
+        const int mine = (int)(k0 / kChunk) + lane;
+        const bool part = lane < kParts && mine >= c_lo && mine < c_hi;
+        const float m = part ? st[mine].x : -INFINITY;
         float top = -INFINITY, sum = 0.0f;
         for (int c = c_lo + lane; c < c_hi; c += 64) {
-          const float2 x = st[c];
-          if (x.x == -INFINITY) continue;
-          if (x.x > top) {
-            sum *= top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - x.x);
-            top = x.x;
+          const float2 y = st[c];
+          if (y.x == -INFINITY) {
+            sum += y.y;  // (0, or NaN where all scores were)
+            continue;
           }
-          sum = fmaf(x.y, __builtin_amdgcn_exp2f(x.x - top), sum);
+          if (y.x > top) {
+            sum *= top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - y.x);
+            top = y.x;
+          }
+          sum = fmaf(y.y, __builtin_amdgcn_exp2f(y.x - top), sum);
         }
 #pragma unroll
         for (int d = 32; d; d >>= 1) {
           const float t2 = __shfl_xor(top, d), s2 = __shfl_xor(sum, d);
-          const float m = fmaxf(top, t2);
-          if (m != -INFINITY)
-            sum = sum * __builtin_amdgcn_exp2f(top - m) + s2 * __builtin_amdgcn_exp2f(t2 - m);
-          top = m;
+          const float both = fmaxf(top, t2);
+          if (both != -INFINITY)
+            sum = sum * __builtin_amdgcn_exp2f(top - both) + s2 * __builtin_amdgcn_exp2f(t2 - both);
+          else
+            sum += s2;
+          top = both;
         }
-        if (lane < kParts) {
-          const int c = (int)(k0 / kChunk) + lane;
-          float f = 0.0f;
-          if (c >= c_lo && c < c_hi && sum > 0.0f) {
-            const float m = st[c].x;
-            if (m != -INFINITY) f = __builtin_amdgcn_exp2f(m - top) / sum;
-          }
-          if (sum != sum) f = sum;
-          s_f[i][lane] = f;
-        }
+        if (lane < kParts)
+          s_f[i][lane] = sum != sum ? sum : m != -INFINITY ? __builtin_amdgcn_exp2f(m - top) / sum : 0.0f;
       }
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < kAddKeys / 256; ++i) {
-        const int64_t t = k0 + 256 * i + tid;
-        if (t >= lo / kChunk * kChunk && t < keys) {
-          const float* pr = p.probs + ((int64_t)b * p.hq + kvh * group + h0) * p.capacity + t;
-          for (int j = 0; j < heads; ++j)
-            acc[i] = fmaf(pr[(int64_t)j * p.capacity], s_f[j][(256 * i + tid) / kChunk], acc[i]);
-        }
-      }
+      for (int j = 0; j < kHeads; ++j)
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+          if (j < heads) acc[i] = fmaf(x[j][i], s_f[j][(256 * i + tid) / kChunk], acc[i]);
     }
 #pragma unroll
-    for (int i = 0; i < kAddKeys / 256; ++i) {
+    for (int i = 0; i < kEach; ++i) {
       const int64_t t = k0 + 256 * i + tid;
       if (t < keys) p.out[base + t] = old[i] + acc[i];
     }
@@ -490,19 +504,22 @@ __device__ __forceinline__ uint32_t rank_of(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// One workgroup a (sequence, kv head). The rank of the least kept weight is
-// found digit by digit from the top (11, 11 and 10 bits): a histogram of the
-// candidates that share the digits found so far, in LDS, and the bin in which
-// the count from above passes what is to be kept. Then every wave counts its
-// stretch of positions, the counts are summed over the waves before it, and the
-// wave writes its kept positions in order; of those at the last rank the lowest
-// positions are kept. Counts are integers, so their order does not matter. The
-// weights are read four times, the last three from L2.
+// One workgroup a (sequence, kv head), a block of 8192 positions at a time, 8 a
+// thread in registers (one block is read once). The rank of the least kept
+// weight is found digit by digit from the top (11, 11 and 10 bits): a histogram
+// of the candidates that share the digits found so far, in LDS, and the bin in
+// which the count from above passes what is to be kept. Then each 64 positions
+// (a wave's ballot) are counted, the counts are summed over those before, and
+// the kept positions written in order; of those at the last rank the lowest
+// positions are kept. Counts are integers, so their order does not matter.
 __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const SelectParams p) {
+  constexpr int kEach = 8, kBlock = kEach * kSelectThreads;
+  constexpr int kGroups = kEach * kSelectWaves;  // ballots of a block
   __shared__ int s_hist[kBins];
   __shared__ int s_part[kSelectWaves];
   __shared__ int s_found[2];  // the digit's bin, what it has to give
-  __shared__ int s_above[kSelectWaves], s_equal[kSelectWaves];
+  __shared__ int s_over[kGroups], s_equal[kGroups];
+  __shared__ int s_total[2];
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
   const int kvh = blockIdx.x, b = blockIdx.y;
   const int64_t cap = min((int64_t)p.table_stride * p.page_size, (int64_t)p.capacity);
@@ -510,9 +527,7 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Sele
   const float* weights = p.weights + ((int64_t)b * p.hkv + kvh) * p.capacity;
   const int32_t* table = p.tables + (int64_t)b * p.table_stride;
   const uint32_t pages = (uint32_t)min(p.arena_pages, (int64_t)INT32_MAX);
-  auto held = [&](int t) { return (uint32_t)table[(uint32_t)t / (uint32_t)p.page_size] < pages; };
   auto count = [](uint64_t lanes) { return (int)__popcll(lanes); };
-  auto guarded = [&](int t) { return t < p.sinks || t >= n - p.recent; };
   auto block_sum = [&](int x) {
 #pragma unroll
     for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
@@ -523,13 +538,37 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Sele
     for (int i = 0; i < kSelectWaves; ++i) sum += s_part[i];
     return sum;
   };
+  // This thread's positions t0 + 1024 i + tid of a block: ranks, and bits of
+  // those that are guarded and of those that stand for selection.
+  uint32_t rank[kEach], guarded = 0, open = 0;
+  const int blocks = (n + kBlock - 1) / kBlock;
+  auto load = [&](int block) {
+    guarded = open = 0;
+    uint32_t page[kEach];
+    float x[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int t = min(block * kBlock + i * kSelectThreads + tid, n - 1);
+      page[i] = (uint32_t)table[(uint32_t)t / (uint32_t)p.page_size];
+      x[i] = weights[t];
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int t = block * kBlock + i * kSelectThreads + tid;
+      rank[i] = rank_of(x[i]);
+      if (t < n && page[i] < pages) {
+        if (t < p.sinks || t >= n - p.recent)
+          guarded |= 1u << i;
+        else
+          open |= 1u << i;
+      }
+    }
+  };
   int guards = 0, rest = 0;
-  for (int t = tid; t < n; t += kSelectThreads) {
-    if (!held(t)) continue;
-    if (guarded(t))
-      ++guards;
-    else
-      ++rest;
+  for (int block = 0; block < blocks; ++block) {
+    load(block);
+    guards += __popc(guarded);
+    rest += __popc(open);
   }
   guards = block_sum(guards);
   rest = block_sum(rest);
@@ -545,10 +584,12 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Sele
       const int bins = pass == 2 ? 1024 : 2048;
       for (int i = tid; i < bins; i += kSelectThreads) s_hist[i] = 0;
       __syncthreads();
-      for (int t = tid; t < n; t += kSelectThreads) {
-        if (guarded(t) || !held(t)) continue;
-        const uint32_t r = rank_of(weights[t]);
-        if ((r & mask) == least) atomicAdd(&s_hist[r >> shift & (bins - 1)], 1);
+      for (int block = 0; block < blocks; ++block) {
+        if (blocks > 1) load(block);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+          if ((open >> i & 1) && (rank[i] & mask) == least)
+            atomicAdd(&s_hist[rank[i] >> shift & (bins - 1)], 1);
       }
       __syncthreads();
       // Thread i takes the bins i * per .. from the top; the one in whose bins
@@ -586,48 +627,52 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Sele
   }
   // (All candidates kept: least 0, and want of them at rank 0 is enough for
   // the NaN, which alone have it.)
-  const int stretch = ((n + kSelectWaves - 1) / kSelectWaves + 63) & ~63;
-  const int t0 = min(n, w * stretch), t1 = min(n, t0 + stretch);
-  auto classify = [&](int t, bool& over, bool& equal) {
-    over = equal = false;
-    if (t >= t1 || !held(t)) return;
-    if (guarded(t)) {
-      over = true;
-      return;
-    }
-    const uint32_t r = rank_of(weights[t]);
-    over = r > least;
-    equal = r == least;
-  };
-  int above = 0, equal = 0;
-  for (int t = t0; t < t1; t += 64) {
-    bool o, e;
-    classify(t + lane, o, e);
-    above += count(__ballot(o));
-    equal += count(__ballot(e));
-  }
-  if (lane == 0) {
-    s_above[w] = above;
-    s_equal[w] = equal;
-  }
-  __syncthreads();
-  int before_above = 0, before_equal = 0;
-  for (int i = 0; i < w; ++i) {
-    before_above += s_above[i];
-    before_equal += s_equal[i];
-  }
   int32_t* kept = p.kept + ((int64_t)b * p.hkv + kvh) * p.keep;
-  int at = before_above + min(before_equal, want), left = max(0, want - before_equal);
   const uint64_t lower = (1ull << lane) - 1;
-  for (int t = t0; t < t1; t += 64) {
-    bool o, e;
-    classify(t + lane, o, e);
-    const uint64_t eq = __ballot(e);
-    if (e && count(eq & lower) < left) o = true;
-    const uint64_t take = __ballot(o);
-    if (o) kept[at + count(take & lower)] = t + lane;
-    at += count(take);
-    left = max(0, left - count(eq));
+  int done = 0, equals = 0;  // kept, and met at the last rank, in the blocks before
+  for (int block = 0; block < blocks; ++block) {
+    if (blocks > 1) load(block);
+    uint32_t over = guarded, equal = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      if ((open >> i & 1) && rank[i] > least) over |= 1u << i;
+      if ((open >> i & 1) && rank[i] == least) equal |= 1u << i;
+      const uint64_t o = __ballot(over >> i & 1), e = __ballot(equal >> i & 1);
+      if (lane == 0) {
+        s_over[i * kSelectWaves + w] = count(o);
+        s_equal[i * kSelectWaves + w] = count(e);
+      }
+    }
+    __syncthreads();
+    if (w < 2) {  // exclusive sums: one wave each, two groups a lane
+      int* c = w ? s_equal : s_over;
+      const int a = c[2 * lane], z = c[2 * lane + 1];
+      int upto = a + z;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int x = __shfl_up(upto, d);
+        if (lane >= d) upto += x;
+      }
+      c[2 * lane] = upto - a - z;
+      c[2 * lane + 1] = upto - z;
+      if (lane == 63) s_total[w] = upto;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const uint64_t o = __ballot(over >> i & 1), e = __ballot(equal >> i & 1);
+      const int group = i * kSelectWaves + w;
+      const int before = equals + s_equal[group];  // at the last rank, lower positions
+      const int at = done + s_over[group] + min(before, want) - min(equals, want);
+      const int ties = before + count(e & lower);
+      const bool take = (over >> i & 1) || ((equal >> i & 1) && ties < want);
+      if (take)
+        kept[at + count(o & lower) + min(ties, want) - min(before, want)] =
+            block * kBlock + i * kSelectThreads + tid;
+    }
+    done += s_total[0] + min(equals + s_total[1], want) - min(equals, want);
+    equals += s_total[1];
+    __syncthreads();
   }
   for (int i = total + tid; i < p.keep; i += kSelectThreads) kept[i] = -1;
   if (kvh == 0 && tid == 0) p.new_lengths[b] = total;
@@ -669,49 +714,57 @@ struct MoveParams {
   int32_t keep;
 };
 
-// Byte offset of position t's row, -1 if its page is not in the arena.
+// Byte offset of position t's row, -1 if its page is not in the arena (or t is
+// negative).
 __device__ __forceinline__ int64_t row_at(const MoveParams& p, const int32_t* table, int stride,
                                           int t, int kvh) {
   const uint32_t pi = (uint32_t)t / (uint32_t)p.page_size;
-  if (t < 0 || pi >= (uint32_t)stride) return -1;
-  const uint32_t page = (uint32_t)table[pi];
-  if ((int64_t)page >= min(p.arena_pages, (int64_t)INT32_MAX)) return -1;
+  const uint32_t page = (uint32_t)table[min(pi, (uint32_t)stride - 1)];
+  if (t < 0 || pi >= (uint32_t)stride || page >= (uint32_t)min(p.arena_pages, (int64_t)INT32_MAX))
+    return -1;
   return page * p.page_bytes + kvh * p.head_bytes +
          (int64_t)(t - (int)pi * p.page_size) * p.row_bytes;
 }
 
-// Kept rows to other pages: every piece of V of every row by itself.
+// Kept rows to other pages: a thread moves one piece of V of kEach rows, their
+// positions, places and then the rows looked up together.
 template <class V>
 __global__ __launch_bounds__(256) void evict_copy_kernel(const MoveParams p) {
-  constexpr int kEach = 4;
+  constexpr int kEach = 8;
   const int kvh = blockIdx.y % p.hkv, b = blockIdx.z;
   char* arena = p.arena[blockIdx.y / p.hkv];
   const int pieces = p.width / (int)sizeof(V);
-  const int64_t total = (int64_t)p.new_lengths[b] * pieces;
+  const int across = min(pieces, 256), rows = 256 / across;  // threads a row, rows a pass
+  const int total = p.new_lengths[b];
   const int32_t* kept = p.kept + ((int64_t)b * p.hkv + kvh) * p.keep;
   const int32_t* from = p.tables + (int64_t)b * p.table_stride;
   const int32_t* to = p.out_tables + (int64_t)b * p.out_stride;
-  for (int64_t i0 = (int64_t)blockIdx.x * (256 * kEach); i0 < total;
-       i0 += (int64_t)gridDim.x * (256 * kEach)) {
-    V x[kEach];
-    int64_t at[kEach];
+  const int mine = (int)threadIdx.x / across, first = (int)threadIdx.x % across;
+  if (mine >= rows) return;
+  for (int64_t r0 = (int64_t)blockIdx.x * (rows * kEach); r0 < total;
+       r0 += (int64_t)gridDim.x * (rows * kEach)) {
+    int64_t s[kEach], d[kEach];
+    int pos[kEach];
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
-      const int64_t i = i0 + 256 * j + threadIdx.x;
-      at[j] = -1;
-      if (i < total) {
-        const int row = (int)(i / pieces), c = (int)(i - (int64_t)row * pieces);
-        const int64_t s = row_at(p, from, p.table_stride, kept[row], kvh);
-        const int64_t d = row_at(p, to, p.out_stride, row, kvh);
-        if (s >= 0 && d >= 0 && s != d) {
-          x[j] = *reinterpret_cast<const V*>(arena + s + c * sizeof(V));
-          at[j] = d + c * sizeof(V);
-        }
-      }
+      const int64_t row = r0 + rows * j + mine;
+      pos[j] = row < total ? kept[row] : -1;
     }
 #pragma unroll
-    for (int j = 0; j < kEach; ++j)
-      if (at[j] >= 0) *reinterpret_cast<V*>(arena + at[j]) = x[j];
+    for (int j = 0; j < kEach; ++j) {
+      s[j] = row_at(p, from, p.table_stride, pos[j], kvh);
+      d[j] = row_at(p, to, p.out_stride, (int)(r0 + rows * j + mine), kvh);
+      if (pos[j] < 0 || d[j] < 0 || d[j] == s[j]) s[j] = -1;
+    }
+    for (int c = first; c < pieces; c += across) {
+      V x[kEach];
+#pragma unroll
+      for (int j = 0; j < kEach; ++j)
+        if (s[j] >= 0) x[j] = *reinterpret_cast<const V*>(arena + s[j] + c * (int64_t)sizeof(V));
+#pragma unroll
+      for (int j = 0; j < kEach; ++j)
+        if (s[j] >= 0) *reinterpret_cast<V*>(arena + d[j] + c * (int64_t)sizeof(V)) = x[j];
+    }
   }
 }
 
@@ -940,7 +993,8 @@ int pda_evict_move(void* arena, void* arena2, int32_t width, const int32_t* kept
                     : (const void*)evict_pack_kernel<uint8_t>;
     grid = dim3((unsigned)gx, kv_heads, batch);
   } else {
-    const int64_t per = ((int64_t)keep * (width / vec) + 1023) / 1024;
+    const int rows = 256 / std::min(width / vec, 256);
+    const int64_t per = ((int64_t)keep + 8 * rows - 1) / (8 * rows);
     fn = vec == 16  ? (const void*)evict_copy_kernel<u32x4>
          : vec == 4 ? (const void*)evict_copy_kernel<uint32_t>
          : vec == 2 ? (const void*)evict_copy_kernel<uint16_t>
