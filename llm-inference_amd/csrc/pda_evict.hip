@@ -17,6 +17,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "pda.h"
 #include "pda_internal.h"
@@ -31,7 +32,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16;
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef signed char i8x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -44,11 +45,18 @@ __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)"
 // Weights.
 
 constexpr int kWaves = 4;        // waves of a score workgroup
-constexpr int kBlocks = 4;       // blocks of 16 keys a wave takes
-constexpr int kChunk = 16 * kBlocks * kWaves;  // keys per workgroup: 256
 constexpr int kSlots = 16;       // query heads per workgroup
 constexpr int kAddKeys = 1024;   // keys an adding workgroup takes
 constexpr int kMaxChunksX = 4096;
+constexpr int kScoreGroups = 1024;  // score workgroups to fill an MI355X
+
+// 32-dim planes of a head that the score kernels hold, and the blocks of 16 keys
+// a wave takes at once: 64 registers of K.
+constexpr int planes_for(int dim) {
+  return dim <= 64 ? 2 : dim <= 96 ? 3 : dim <= 128 ? 4 : dim <= 256 ? 8 : 16;
+}
+constexpr int blocks_for(int planes) { return planes <= 4 ? 4 : 16 / planes; }
+constexpr int chunk_for(int planes) { return 16 * kWaves * blocks_for(planes); }
 
 struct WeightParams {
   const f16* q;        // [batch, hq, D]
@@ -58,7 +66,7 @@ struct WeightParams {
   const int32_t* lengths;
   const float* weights;  // [batch, hkv, capacity]
   float* out;
-  float* probs;        // [batch, hq, capacity] weights relative to their chunk's max
+  float* probs;        // [batch, hq, pitch] weights relative to their chunk's max
   float2* stats;       // [batch, hq, chunks] (max, sum) of each chunk
   int64_t arena_pages;
   int64_t page_elems, scale_page;  // elements between pages,
@@ -70,7 +78,9 @@ struct WeightParams {
   int32_t hkv;
   int32_t head_dim;
   int32_t capacity;
-  int32_t chunks;      // ceil(capacity / kChunk)
+  int32_t pitch;       // capacity, up to a multiple of 4
+  int32_t chunk;       // keys per chunk
+  int32_t chunks;      // ceil(capacity / chunk)
   int32_t window;
   int32_t fresh;
   float scale_log2;
@@ -83,39 +93,39 @@ __device__ __forceinline__ int keys_of(const WeightParams& p, int b) {
   return (int)max((int64_t)0, min((int64_t)p.lengths[b], cap));
 }
 
-// 8 elements of a row from dim d on as 16-bit operands, zeros past the head
-// dim. VEC: head dims that are multiples of 8 (rows 8 elements aligned).
-template <bool Q8, bool BF, bool VEC>
-__device__ __forceinline__ f16x8 load8(const void* base, int64_t at, int d, int dim) {
-  f16x8 x = {};
-  if (d >= dim) return x;
-  if constexpr (Q8) {
-    const signed char* src = static_cast<const signed char*>(base) + at + d;
-    i8x8 y = {};
-    if constexpr (VEC) {
-      y = *reinterpret_cast<const i8x8*>(src);
-    } else {
+// 8 elements of a row from dim d on, as they are stored. VEC: head dims that are
+// multiples of 8; past the head dim the row's last elements again (the queries
+// are zeros there). Else element by element, zeros past the head dim.
+template <class E, class V, bool VEC>
+__device__ __forceinline__ V load8(const void* base, int64_t at, int d, int dim) {
+  const E* src = static_cast<const E*>(base) + at;
+  if constexpr (VEC) return *reinterpret_cast<const V*>(src + min(d, dim - 8));
+  V x = {};
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (d + i < dim) y[i] = src[i];
-    }
-    // (Integers of 8 bits are exact in either type.)
+  for (int i = 0; i < 8; ++i) {
+    if (d + i >= dim) break;
+    if constexpr (sizeof(E) == 1)
+      x[i / 4] |= (uint32_t)(uint8_t)src[d + i] << (8 * (i % 4));
+    else
+      x[i] = src[d + i];
+  }
+  return x;
+}
+
+// Them as operands: integers of 8 bits are exact in either type. (They are held
+// as two dwords: a vector of bytes would take a register each.)
+template <bool BF>
+__device__ __forceinline__ f16x8 operand(const f16x8& x) { return x; }
+template <bool BF>
+__device__ __forceinline__ f16x8 operand(const u32x2& y) {
+  f16x8 x;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if constexpr (BF)
-        x[i] = __builtin_bit_cast(f16, (bf16)(float)y[i]);
-      else
-        x[i] = (f16)(float)y[i];
-    }
-  } else {
-    const f16* src = static_cast<const f16*>(base) + at + d;
-    if constexpr (VEC) {
-      x = *reinterpret_cast<const f16x8*>(src);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (d + i < dim) x[i] = src[i];
-    }
+  for (int i = 0; i < 8; ++i) {
+    const float f = (float)(int)__builtin_amdgcn_sbfe((int)y[i / 4], 8 * (i % 4), 8);
+    if constexpr (BF)
+      x[i] = __builtin_bit_cast(f16, (bf16)f);
+    else
+      x[i] = (f16)f;
   }
   return x;
 }
@@ -129,16 +139,20 @@ __device__ __forceinline__ f32x4 mfma(const f16x8& a, const f16x8& b, const f32x
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// Scores of 256 keys against up to 16 heads of one kv head, as weights relative
-// to the chunk's largest, with each head's largest and sum. K is read once,
-// straight into the matrix cores' operands (lane: key lane % 16, 8 dims), 64
-// bytes of a row per instruction, all loads of a wave's 64 keys under way
-// together where the head dim allows; a lane ends with 4 consecutive keys of one
-// head per block. Reads K and writes 4 bytes a head and key: the K bytes bound
-// it.
+// Scores of a chunk of keys against up to 16 heads of one kv head, as weights
+// relative to the chunk's largest, with each head's largest and sum. K is read
+// once, straight into the matrix cores' operands (lane: key lane % 16, 8 dims),
+// 64 bytes of a row per instruction; a lane ends with 4 consecutive keys of one
+// head per block. A workgroup goes over its chunks with the next one's rows, and
+// the page numbers of the one after that, under way. Reads K and writes 4 bytes a
+// head and key: the K bytes bound it.
 template <int NC, bool Q8, bool BF, bool VEC>
-__global__ __launch_bounds__(64 * kWaves) void attention_scores_kernel(const WeightParams p) {
-  __shared__ float s_max[kWaves][kSlots], s_sum[kWaves][kSlots];
+__global__ __launch_bounds__(64 * kWaves, NC == 16 && !Q8 ? 1 : 2) void attention_scores_kernel(const WeightParams p) {
+  typedef std::conditional_t<Q8, signed char, f16> Elem;
+  typedef std::conditional_t<Q8, u32x2, f16x8> Elem8;
+  constexpr int kBlocks = blocks_for(NC);
+  constexpr int kChunk = chunk_for(NC);
+  __shared__ float s_max[2][kWaves][kSlots], s_sum[2][kWaves][kSlots];
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
   const int n16 = lane & 15, g4 = lane >> 4;
   const int group = p.hq / p.hkv, tiles = (group + kSlots - 1) / kSlots;
@@ -150,90 +164,103 @@ __global__ __launch_bounds__(64 * kWaves) void attention_scores_kernel(const Wei
   const int keys = keys_of(p, b);
   const int lo = p.window > 0 ? max(0, keys - p.window) : 0;
   const uint32_t pages = (uint32_t)min(p.arena_pages, (int64_t)INT32_MAX);
-
   const int32_t* table = p.tables + (int64_t)b * p.table_stride;
+  const int stride = gridDim.x;
+  const int c_end = (keys + kChunk - 1) / kChunk;
+  const int c_first = lo / kChunk + blockIdx.x;
+  if (c_first >= c_end) return;
+
   f16x8 qf[NC];
   const int64_t qat = ((int64_t)b * p.hq + (live ? h : 0)) * p.head_dim;
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    qf[c] = load8<false, BF, VEC>(p.q, qat, 32 * c + 8 * g4, p.head_dim);
-    if (!live) qf[c] = f16x8{};
+    const int d = 32 * c + 8 * g4;
+    qf[c] = load8<f16, f16x8, VEC>(p.q, qat, d, p.head_dim);
+    if (!live || d >= p.head_dim) qf[c] = f16x8{};
   }
-  for (int chunk = lo / kChunk + blockIdx.x; chunk * (int64_t)kChunk < keys; chunk += gridDim.x) {
-    const int k0 = chunk * kChunk + w * (16 * kBlocks);
-    f32x4 s[kBlocks];
-    uint32_t seen = 0;  // bit i: this lane's key of block i has a row
-    int64_t at[kBlocks];
-    float ks[kBlocks];
-    // (All table entries first, then all rows: with a branch per key the
-    // lookups waited for each other.)
-    uint32_t page[kBlocks], row[kBlocks];
+  // The keys of a chunk that this lane looks up: 16 i + n16 of the wave's.
+  struct Rows {
+    uint32_t page[kBlocks];
+  };
+  struct Keys {
+    Elem8 k[kBlocks][NC];
+    f16 scale[kBlocks];
+    uint32_t seen;  // bit i: this lane's key of block i has a row
+  };
+  auto key_at = [&](int chunk, int i) {
+    return chunk * (int64_t)kChunk + w * (16 * kBlocks) + 16 * i + n16;
+  };
+  auto look_up = [&](int chunk, Rows& r) {
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i)
+      r.page[i] = (uint32_t)table[(uint32_t)min(key_at(chunk, i), (int64_t)keys - 1) /
+                                  (uint32_t)p.page_size];
+  };
+  auto fetch = [&](int chunk, const Rows& r, Keys& x) {
+    x.seen = 0;
 #pragma unroll
     for (int i = 0; i < kBlocks; ++i) {
-      const uint32_t key = (uint32_t)min(k0 + 16 * i + n16, keys - 1);
-      const uint32_t pi = key / (uint32_t)p.page_size;
-      row[i] = key - pi * (uint32_t)p.page_size;
-      page[i] = (uint32_t)table[pi];
-    }
+      const int64_t key = key_at(chunk, i);
+      const bool have = key >= lo && key < keys && r.page[i] < pages;
+      x.seen |= have ? 1u << i : 0u;
+      const uint32_t row = (uint32_t)min(key, (int64_t)keys - 1) % (uint32_t)p.page_size;
+      const uint32_t page = have ? r.page[i] : 0u;
+      const int64_t at =
+          page * p.page_elems + (int64_t)kvh * p.head_elems + (int64_t)row * p.row_elems;
 #pragma unroll
-    for (int i = 0; i < kBlocks; ++i) {
-      const int key = k0 + 16 * i + n16;
-      const bool have = key >= lo && key < keys && page[i] < pages;
-      seen |= have ? 1u << i : 0u;
-      page[i] = have ? page[i] : 0u;
-      at[i] = page[i] * p.page_elems + (int64_t)kvh * p.head_elems + (int64_t)row[i] * p.row_elems;
-      ks[i] = 1.0f;
+      for (int c = 0; c < NC; ++c)
+        x.k[i][c] = load8<Elem, Elem8, VEC>(p.k, at, 32 * c + 8 * g4, p.head_dim);
+      x.scale[i] = (f16)1.0f;
       if constexpr (Q8)
-        ks[i] = (float)p.kscale[page[i] * p.scale_page + (int64_t)kvh * p.scale_head +
-                                (int64_t)row[i] * p.scale_row];
+        x.scale[i] = p.kscale[page * p.scale_page + (int64_t)kvh * p.scale_head +
+                                     (int64_t)row * p.scale_row];
     }
-    f16x8 kf[kBlocks][NC <= 4 ? NC : 1];
-    if constexpr (NC <= 4) {
+  };
+  auto weigh = [&](int chunk, const Keys& x, int buf) {
+    f32x4 s[kBlocks];
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i) s[i] = f32x4{};
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int i = 0; i < kBlocks; ++i) s[i] = mfma<BF>(operand<BF>(x.k[i][c]), qf[c], s[i]);
+    if constexpr (Q8) {
 #pragma unroll
       for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
-          kf[i][c] = load8<Q8, BF, VEC>(p.k, at[i], 32 * c + 8 * g4, p.head_dim);
+        for (int v = 0; v < 4; ++v) s[i][v] *= __shfl((float)x.scale[i], 4 * g4 + v);
     }
+    if (p.cap_out > 0.0f) {
 #pragma unroll
-    for (int i = 0; i < kBlocks; ++i) {
-      s[i] = f32x4{};
+      for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        f16x8 a;
-        if constexpr (NC <= 4)
-          a = kf[i][c];
-        else
-          a = load8<Q8, BF, VEC>(p.k, at[i], 32 * c + 8 * g4, p.head_dim);
-        s[i] = mfma<BF>(a, qf[c], s[i]);
-      }
+        for (int v = 0; v < 4; ++v) {
+          const float e = __builtin_amdgcn_exp2f(s[i][v] * p.cap_in);
+          s[i][v] = (1.0f - 2.0f / (e + 1.0f)) * p.cap_out;
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) s[i][v] *= p.scale_log2;
     }
+    // Key 4 g4 + v of a block was looked up by lane 4 g4 + v.
     float top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < kBlocks; ++i) {
+      const uint32_t have = (uint32_t)__ballot(x.seen >> i & 1) >> (4 * g4);
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
-        // Key 4 g4 + v of the block: lane 4 g4 + v looked it up.
-        const int src = 4 * g4 + v;
-        const bool have = __shfl((int)(seen >> i & 1), src) != 0;
-        float x = s[i][v];
-        if constexpr (Q8) x *= __shfl(ks[i], src);
-        if (p.cap_out > 0.0f) {
-          const float e = __builtin_amdgcn_exp2f(x * p.cap_in);
-          x = (1.0f - 2.0f / (e + 1.0f)) * p.cap_out;
-        } else {
-          x *= p.scale_log2;
-        }
-        s[i][v] = have ? x : -INFINITY;
+        if (!(have >> v & 1)) s[i][v] = -INFINITY;
         top = fmaxf(top, s[i][v]);
       }
     }
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
-    if (g4 == 0) s_max[w][n16] = top;
+    if (g4 == 0) s_max[buf][w][n16] = top;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) top = fmaxf(top, s_max[i][n16]);
+    for (int i = 0; i < kWaves; ++i) top = fmaxf(top, s_max[buf][i][n16]);
     const float mu = top == -INFINITY ? 0.0f : top;
     float sum = 0.0f;
 #pragma unroll
@@ -246,26 +273,40 @@ __global__ __launch_bounds__(64 * kWaves) void attention_scores_kernel(const Wei
     }
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
-    if (g4 == 0) s_sum[w][n16] = sum;
-    __syncthreads();
+    if (g4 == 0) s_sum[buf][w][n16] = sum;
+    const int64_t row = (int64_t)b * p.hq + h;
     if (live) {
-      const int64_t row = (int64_t)b * p.hq + h;
-      float* dst = p.probs + row * p.capacity;
+      float* dst = p.probs + row * p.pitch;
 #pragma unroll
       for (int i = 0; i < kBlocks; ++i) {
-        const int key = k0 + 16 * i + 4 * g4;
-#pragma unroll
-        for (int v = 0; v < 4; ++v)
-          if (key + v < keys) dst[key + v] = s[i][v];
-      }
-      if (w == 0 && g4 == 0) {
-        float all = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kWaves; ++i) all += s_sum[i][n16];
-        p.stats[row * p.chunks + chunk] = make_float2(top, all);
+        const int64_t key = chunk * (int64_t)kChunk + w * (16 * kBlocks) + 16 * i + 4 * g4;
+        if (key < keys) *reinterpret_cast<f32x4*>(dst + key) = s[i];
       }
     }
     __syncthreads();
+    if (live && w == 0 && g4 == 0) {
+      float all = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) all += s_sum[buf][i][n16];
+      p.stats[row * p.chunks + chunk] = make_float2(top, all);
+    }
+  };
+  Rows rows;
+  Keys even, odd;
+  look_up(c_first, rows);
+  fetch(c_first, rows, even);
+  if (c_first + stride < c_end) look_up(c_first + stride, rows);
+  for (int c = c_first;; c += 2 * stride) {
+    // (Both statistics buffers: a chunk's are read past its second barrier.)
+    Rows next;
+    if (c + 2 * stride < c_end) look_up(c + 2 * stride, next);
+    if (c + stride < c_end) fetch(c + stride, rows, odd);
+    weigh(c, even, 0);
+    if (c + stride >= c_end) break;
+    if (c + 3 * (int64_t)stride < c_end) look_up(c + 3 * stride, rows);
+    if (c + 2 * stride < c_end) fetch(c + 2 * stride, next, even);
+    weigh(c + stride, odd, 1);
+    if (c + 2 * stride >= c_end) break;
   }
 }
 
@@ -276,13 +317,14 @@ __global__ __launch_bounds__(64 * kWaves) void attention_scores_kernel(const Wei
 // launch before left them in.
 __global__ __launch_bounds__(256) void attention_weights_kernel(const WeightParams p) {
   constexpr int kHeads = 8;  // heads at once: two a wave for the statistics
-  constexpr int kParts = kAddKeys / kChunk, kEach = kAddKeys / 256;
-  __shared__ float s_f[kHeads][kParts];
+  constexpr int kMaxParts = kAddKeys / chunk_for(16), kEach = kAddKeys / 256;
+  __shared__ float s_f[kHeads][kMaxParts];
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
   const int group = p.hq / p.hkv, kvh = blockIdx.y, b = blockIdx.z;
   const int keys = keys_of(p, b);
   const int lo = p.window > 0 ? max(0, keys - p.window) : 0;
-  const int c_lo = lo / kChunk, c_hi = (keys + kChunk - 1) / kChunk;
+  const int chunk = p.chunk, parts = kAddKeys / chunk;
+  const int c_lo = lo / chunk, c_hi = (keys + chunk - 1) / chunk;
   const int64_t base = ((int64_t)b * p.hkv + kvh) * p.capacity;
   for (int64_t k0 = (int64_t)blockIdx.x * kAddKeys; k0 < keys; k0 += (int64_t)gridDim.x * kAddKeys) {
     float acc[kEach] = {}, old[kEach];
@@ -301,14 +343,14 @@ __global__ __launch_bounds__(256) void attention_weights_kernel(const WeightPara
         for (int i = 0; i < kEach; ++i) {
           const int64_t t = k0 + 256 * i + tid;
           x[j][i] = 0.0f;
-          if (j < heads && t >= (int64_t)c_lo * kChunk && t < keys)
-            x[j][i] = p.probs[(row + j) * p.capacity + t];
+          if (j < heads && t >= (int64_t)c_lo * chunk && t < keys)
+            x[j][i] = p.probs[(row + j) * p.pitch + t];
         }
       __syncthreads();
       for (int i = w; i < heads; i += 4) {
         const float2* st = p.stats + (row + i) * p.chunks;
-        const int mine = (int)(k0 / kChunk) + lane;
-        const bool part = lane < kParts && mine >= c_lo && mine < c_hi;
+        const int mine = (int)(k0 / chunk) + lane;
+        const bool part = lane < parts && mine >= c_lo && mine < c_hi;
         const float m = part ? st[mine].x : -INFINITY;
         float top = -INFINITY, sum = 0.0f;
         for (int c = c_lo + lane; c < c_hi; c += 64) {
@@ -333,7 +375,7 @@ __global__ __launch_bounds__(256) void attention_weights_kernel(const WeightPara
             sum += s2;
           top = both;
         }
-        if (lane < kParts)
+        if (lane < parts)
           s_f[i][lane] = sum != sum ? sum : m != -INFINITY ? __builtin_amdgcn_exp2f(m - top) / sum : 0.0f;
       }
       __syncthreads();
@@ -341,7 +383,7 @@ __global__ __launch_bounds__(256) void attention_weights_kernel(const WeightPara
       for (int j = 0; j < kHeads; ++j)
 #pragma unroll
         for (int i = 0; i < kEach; ++i)
-          if (j < heads) acc[i] = fmaf(x[j][i], s_f[j][(256 * i + tid) / kChunk], acc[i]);
+          if (j < heads) acc[i] = fmaf(x[j][i], s_f[j][(256 * i + tid) / chunk], acc[i]);
     }
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
@@ -354,23 +396,37 @@ __global__ __launch_bounds__(256) void attention_weights_kernel(const WeightPara
 
 template <bool Q8, bool BF>
 const void* scores_kernel(int dim) {
-  const int nc = (dim + 31) / 32;
+  const int nc = planes_for(dim);
   if (dim % 8 == 0) {
-    if (nc <= 2) return (const void*)attention_scores_kernel<2, Q8, BF, true>;
-    if (nc <= 3) return (const void*)attention_scores_kernel<3, Q8, BF, true>;
-    if (nc <= 4) return (const void*)attention_scores_kernel<4, Q8, BF, true>;
-    if (nc <= 8) return (const void*)attention_scores_kernel<8, Q8, BF, true>;
-    return (const void*)attention_scores_kernel<16, Q8, BF, true>;
+    switch (nc) {
+      case 2: return (const void*)attention_scores_kernel<2, Q8, BF, true>;
+      case 3: return (const void*)attention_scores_kernel<3, Q8, BF, true>;
+      case 4: return (const void*)attention_scores_kernel<4, Q8, BF, true>;
+      case 8: return (const void*)attention_scores_kernel<8, Q8, BF, true>;
+      default: return (const void*)attention_scores_kernel<16, Q8, BF, true>;
+    }
   }
   return nc <= 4 ? (const void*)attention_scores_kernel<4, Q8, BF, false>
                  : (const void*)attention_scores_kernel<16, Q8, BF, false>;
 }
 
+// Planes of the kernel that scores_kernel picks.
+int planes_run(int dim) {
+  const int nc = planes_for(dim);
+  return dim % 8 == 0 ? nc : nc <= 4 ? 4 : 16;
+}
+
 size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
+// (The chunks of the widest heads, the smallest, whatever the head dim.)
+size_t stats_bytes(int batch, int q_heads, int capacity) {
+  const int chunk = chunk_for(16);
+  return up256((size_t)batch * q_heads * (((size_t)capacity + chunk - 1) / chunk) * 8);
+}
+
 size_t weights_workspace(int batch, int q_heads, int capacity) {
-  const size_t rows = (size_t)batch * q_heads;
-  return up256(rows * ((capacity + kChunk - 1) / kChunk) * 8) + up256(rows * capacity * 4);
+  return stats_bytes(batch, q_heads, capacity) +
+         up256((size_t)batch * q_heads * (((size_t)capacity + 3) & ~(size_t)3) * 4);
 }
 
 int attention_weights(const void* queries, const void* keys, const void* key_scales, bool q8,
@@ -428,10 +484,12 @@ int attention_weights(const void* queries, const void* keys, const void* key_sca
   prm.lengths = lengths;
   prm.weights = weights;
   prm.out = out;
-  prm.chunks = (capacity + kChunk - 1) / kChunk;
+  prm.pitch = (capacity + 3) & ~3;
+  prm.chunk = chunk_for(planes_run(head_dim));
+  prm.chunks = (capacity + prm.chunk - 1) / prm.chunk;
   prm.stats = static_cast<float2*>(workspace);
   prm.probs = reinterpret_cast<float*>(static_cast<char*>(workspace) +
-                                       up256((size_t)batch * q_heads * prm.chunks * 8));
+                                       stats_bytes(batch, q_heads, capacity));
   prm.arena_pages = arena_rows / page_size;
   const bool rows = layout == PDA_LAYOUT_ROWS;
   prm.page_elems = (int64_t)page_size * kv_heads * head_dim;
@@ -451,10 +509,16 @@ int attention_weights(const void* queries, const void* keys, const void* key_sca
   prm.scale_log2 = scale * kLog2e;
   prm.cap_in = softcap > 0.0f ? 2.0f * kLog2e * scale / softcap : 0.0f;
   prm.cap_out = softcap * kLog2e;
-  // The grid covers `longest` keys; workgroups go on to later ones if there are.
+  // The grid covers `longest` keys (workgroups go on to later ones if there
+  // are): a workgroup a chunk while the GPU holds them all at once, else up to
+  // four chunks each, whose loads then overlap.
   const int64_t span = std::max<int64_t>(1, std::min<int64_t>(longest, capacity));
-  const int64_t seen = window > 0 ? std::min<int64_t>(span, (int64_t)window + kChunk) : span;
-  const unsigned gx = (unsigned)std::min<int64_t>((seen + kChunk - 1) / kChunk, kMaxChunksX);
+  const int64_t seen =
+      window > 0 ? std::min<int64_t>(span, (int64_t)window + prm.chunk) : span;
+  const int64_t chunks = (seen + prm.chunk - 1) / prm.chunk;
+  const int64_t one = std::max<int64_t>(1, kScoreGroups / (grid_y * batch));
+  const unsigned gx = (unsigned)std::min<int64_t>(
+      std::max(std::min(chunks, one), (chunks + 3) / 4), kMaxChunksX);
   const unsigned ax = (unsigned)std::min<int64_t>((span + kAddKeys - 1) / kAddKeys, kMaxChunksX);
   void* args[] = {&prm};
   const hipStream_t hs = static_cast<hipStream_t>(stream);
@@ -528,14 +592,11 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Sele
   const int32_t* table = p.tables + (int64_t)b * p.table_stride;
   const uint32_t pages = (uint32_t)min(p.arena_pages, (int64_t)INT32_MAX);
   auto count = [](uint64_t lanes) { return (int)__popcll(lanes); };
-  auto block_sum = [&](int x) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
-    __syncthreads();
-    if (lane == 0) s_part[w] = x;
-    __syncthreads();
+  // Sums of s_part below the wave's entry.
+  auto below = [&]() {
     int sum = 0;
-    for (int i = 0; i < kSelectWaves; ++i) sum += s_part[i];
+#pragma unroll
+    for (int i = 0; i < kSelectWaves; ++i) sum += i < w ? s_part[i] : 0;
     return sum;
   };
   // This thread's positions t0 + 1024 i + tid of a block: ranks, and bits of
@@ -570,8 +631,22 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Sele
     guards += __popc(guarded);
     rest += __popc(open);
   }
-  guards = block_sum(guards);
-  rest = block_sum(rest);
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    guards += __shfl_xor(guards, d);
+    rest += __shfl_xor(rest, d);
+  }
+  if (lane == 0) {
+    s_over[w] = guards;
+    s_equal[w] = rest;
+  }
+  __syncthreads();
+  guards = rest = 0;
+#pragma unroll
+  for (int i = 0; i < kSelectWaves; ++i) {
+    guards += s_over[i];
+    rest += s_equal[i];
+  }
   const int total = min(p.keep, guards + rest);
   int want = max(0, p.keep - guards);  // candidates to keep
   uint32_t least = 0;                  // rank of the least kept one
@@ -605,7 +680,7 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Sele
       }
       if (lane == 63) s_part[w] = upto;
       __syncthreads();
-      for (int i = 0; i < w; ++i) upto += s_part[i];
+      upto += below();
       int above = upto - mine;
       if (above < want && want <= upto) {
         for (int i = 0; i < per; ++i) {
@@ -628,6 +703,9 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Sele
   // (All candidates kept: least 0, and want of them at rank 0 is enough for
   // the NaN, which alone have it.)
   int32_t* kept = p.kept + ((int64_t)b * p.hkv + kvh) * p.keep;
+  float* dst = p.out_weights + ((int64_t)b * p.hkv + kvh) * p.out_capacity;
+  const bool apart = p.out_weights && p.out_weights != p.weights;
+  __syncthreads();
   const uint64_t lower = (1ull << lane) - 1;
   int done = 0, equals = 0;  // kept, and met at the last rank, in the blocks before
   for (int block = 0; block < blocks; ++block) {
@@ -666,9 +744,12 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Sele
       const int at = done + s_over[group] + min(before, want) - min(equals, want);
       const int ties = before + count(e & lower);
       const bool take = (over >> i & 1) || ((equal >> i & 1) && ties < want);
-      if (take)
-        kept[at + count(o & lower) + min(ties, want) - min(before, want)] =
-            block * kBlock + i * kSelectThreads + tid;
+      if (take) {
+        const int t = block * kBlock + i * kSelectThreads + tid;
+        const int to = at + count(o & lower) + min(ties, want) - min(before, want);
+        kept[to] = t;
+        if (apart) dst[to] = weights[t];
+      }
     }
     done += s_total[0] + min(equals + s_total[1], want) - min(equals, want);
     equals += s_total[1];
@@ -676,12 +757,11 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Sele
   }
   for (int i = total + tid; i < p.keep; i += kSelectThreads) kept[i] = -1;
   if (kvh == 0 && tid == 0) p.new_lengths[b] = total;
-  if (!p.out_weights) return;
-  // The kept positions' weights to the front, 1024 at a time: a later stretch's
-  // sources lie past every place written so far, so this also works in place.
+  if (!p.out_weights || apart) return;
+  // In place the kept positions' weights go to the front 1024 at a time: a later
+  // stretch's sources lie past every place written so far.
   __threadfence_block();
   __syncthreads();
-  float* dst = p.out_weights + ((int64_t)b * p.hkv + kvh) * p.out_capacity;
   for (int i0 = 0; i0 < total; i0 += kSelectThreads) {
     const int i = i0 + tid;
     float x = 0.0f;
