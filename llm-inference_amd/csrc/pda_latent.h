@@ -36,6 +36,19 @@ constexpr int kMaxHead = 128;    // nope dims and value dims of a head
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
+// A value at a wave-uniform place, through the scalar cache (nothing in the
+// launch writes it).
+template <class T>
+__device__ __forceinline__ T scalar_load(const T* p, int64_t i) {
+  return *(const __attribute__((address_space(4))) T*)(uintptr_t)(p + i);
+}
+
+// The larger of a lane's value and that of the lane 32 on.
+__device__ __forceinline__ float max_halves(float x) {
+  const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+}
+
 // A 16-lane group's transposed LDS read: 4 rows x 16 columns of 16-bit
 // elements, lane s given the address of row s / 4, columns 4 (s % 4) ..; it
 // receives the 4 rows of column s.

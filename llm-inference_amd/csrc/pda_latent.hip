@@ -158,6 +158,9 @@ constexpr int kChunkTiles = 64;   // tiles whose rows are looked up at once
 constexpr int kChunkKeys = kTileKeys * kChunkTiles;
 constexpr int kMaxGroups = 256;   // workgroups of a launch: one per CU of an MI355X
 constexpr float kSlack = 8.0f;    // scores may pass the running max by 2^8
+// What a workgroup spends on a sequence besides its tiles (queries, rows, the
+// partial), in tiles: the cuts of the stream count it.
+constexpr int kSequenceTiles = 8;
 
 struct LatentDecodeParams {
   const f16* q;          // [batch, hq, nope + rope]
@@ -167,7 +170,7 @@ struct LatentDecodeParams {
   const int32_t* lengths;
   f16* out;              // [batch, hq, value]
   f16* q_lat;            // [batch, hq, latent + rope]: absorbed queries
-  int32_t* prefix;       // [batch + 1] tiles before each sequence
+  int32_t* prefix;       // [batch + 1] tiles, kSequenceTiles a sequence, before each
   float* part_o;         // [groups + batch, hq, latent] unnormalised partial sums
   float2* part_ml;       // [groups + batch, hq] (running max, sum)
   int64_t arena_pages;
@@ -189,6 +192,12 @@ __device__ __forceinline__ int64_t keys_of(const LatentDecodeParams& p, int b) {
   return max((int64_t)0, min((int64_t)p.lengths[b], cap));
 }
 
+// Units of the stream that sequence b takes.
+__device__ __forceinline__ int units_of(const LatentDecodeParams& p, int b) {
+  const int tiles = (int)((keys_of(p, b) + kTileKeys - 1) / kTileKeys);
+  return tiles ? tiles + kSequenceTiles : 0;
+}
+
 // Queries into the latent: q_lat[b, h] = [U_h^T q_nope | q_rope], rounded to
 // the element type (the matrix cores take 16-bit operands; the products and
 // their sum are float32). As products: (U_h^T) (32 latent dims x nope) by
@@ -207,7 +216,7 @@ __global__ __launch_bounds__(256) void latent_absorb_kernel(const LatentDecodePa
     const int each = (p.batch + 255) / 256, first = min(tid * each, p.batch);
     const int end = min(first + each, p.batch);
     int sum = 0;
-    for (int b = first; b < end; ++b) sum += (int)((keys_of(p, b) + kTileKeys - 1) / kTileKeys);
+    for (int b = first; b < end; ++b) sum += units_of(p, b);
     s_scan[tid] = sum;
     __syncthreads();
     for (int d = 1; d < 256; d <<= 1) {
@@ -219,7 +228,7 @@ __global__ __launch_bounds__(256) void latent_absorb_kernel(const LatentDecodePa
     int at = s_scan[tid] - sum;
     for (int b = first; b < end; ++b) {
       p.prefix[b] = at;
-      at += (int)((keys_of(p, b) + kTileKeys - 1) / kTileKeys);
+      at += units_of(p, b);
     }
     if (tid == 255) p.prefix[p.batch] = s_scan[255];
   }
@@ -317,7 +326,8 @@ __global__ __launch_bounds__(256, 1) void latent_decode_kernel(const LatentDecod
   constexpr int kGroups = 4 / NHG;           // tiles under way side by side
   constexpr int kPlane = kTileKeys * 32;     // halves of a 64-byte column plane
   constexpr int kTile = WP * kPlane;
-  constexpr int kPitch = 132;                // floats of a head's 128 dims
+  constexpr int kJoin = OB > 8 ? 256 : 128;  // dims joined at once
+  constexpr int kPitch = kJoin + 4;          // floats of a head's
   constexpr int kAhead = 4;                  // operands read early
   __shared__ __align__(1024) f16 s_t[4][kTile];
   __shared__ int s_row[kChunkKeys];
@@ -334,12 +344,12 @@ __global__ __launch_bounds__(256, 1) void latent_decode_kernel(const LatentDecod
   const bool live = h < p.hq;
   const int width = p.latent + p.rope;
 
-  const int total = p.prefix[p.batch];
+  const int total = scalar_load(p.prefix, p.batch);
   const int per = (int)(((int64_t)total + p.groups - 1) / p.groups);
   const int64_t from = (int64_t)blockIdx.x * per;
   if (from >= total) return;
   const int t0 = (int)from, t1 = (int)min((int64_t)total, from + per);
-  // The sequence that holds tile t0: those that end at or before it lie before it.
+  // The sequence that holds unit t0: those that end at or before it lie before it.
   int before = 0;
   for (int i = tid; i < p.batch; i += 256) before += p.prefix[i + 1] <= t0 ? 1 : 0;
 #pragma unroll
@@ -368,16 +378,42 @@ __global__ __launch_bounds__(256, 1) void latent_decode_kernel(const LatentDecod
   const uint32_t lds = uniform(lds_address(&s_t[0][0]));
   const uint32_t pages = (uint32_t)min(p.arena_pages, (int64_t)INT32_MAX);
 
-  while (b < p.batch) {
-    const int seq0 = uniform(p.prefix[b]);
+  // A positive scale is applied with the maximum's subtraction, another one to
+  // the scores.
+  const bool direct = p.scale_log2 > 0.0f;
+  const float c = direct ? p.scale_log2 : 1.0f;
+
+  for (; b < p.batch; ++b) {
+    const int seq0 = scalar_load(p.prefix, b), seq1 = scalar_load(p.prefix, b + 1);
+    const int keys =
+        (int)max((int64_t)0, min((int64_t)scalar_load(p.lengths, b),
+                                 (int64_t)p.table_stride * p.page_size));
     if (seq0 >= t1) break;
-    const int seq1 = uniform(p.prefix[b + 1]);
-    const int ta = max(t0, seq0) - seq0, tb = min(t1, seq1) - seq0;
-    if (ta >= tb) {  // an empty sequence
-      ++b;
-      continue;
-    }
-    const int keys = (int)keys_of(p, b);
+    const int tb = min(t1, seq1) - seq0 - kSequenceTiles;
+    const int ta = max(0, t0 - seq0 - kSequenceTiles);
+    if (ta >= tb) continue;  // none of the sequence's tiles
+
+    // Arena rows of a chunk's keys; -1: no such key, or no such page.
+    constexpr int kEach = kChunkKeys / 256;
+    uint32_t page[kEach];
+    auto look_up = [&](int c0) {
+      const int64_t table = (int64_t)b * p.table_stride;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const uint32_t key = (uint32_t)c0 * kTileKeys + 256 * i + tid;  // (may pass 2^31)
+        page[i] = ~0u;
+        if (256 * i < min(tb - c0, kChunkTiles) * kTileKeys && key < (uint32_t)keys)
+          page[i] = (uint32_t)p.tables[table + key / (uint32_t)p.page_size];
+      }
+    };
+    auto put_rows = [&](int c0) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const uint32_t r = ((uint32_t)c0 * kTileKeys + 256 * i + tid) % (uint32_t)p.page_size;
+        s_row[256 * i + tid] = page[i] < pages ? (int)(page[i] * (uint32_t)p.page_size + r) : -1;
+      }
+    };
+    look_up(ta);
     f16x8 qf[2 * WP];
     {
       // (The pieces' places are computed here for every sequence: kept through
@@ -386,10 +422,10 @@ __global__ __launch_bounds__(256, 1) void latent_decode_kernel(const LatentDecod
       asm volatile("" : "+v"(part));
       const f16* qp = p.q_lat + ((int64_t)b * p.hq + (live ? h : 0)) * width;
 #pragma unroll
-      for (int c = 0; c < 2 * WP; ++c) {
-        const int d = 16 * c + part;
+      for (int i = 0; i < 2 * WP; ++i) {
+        const int d = 16 * i + part;
         const f16x8 x = *reinterpret_cast<const f16x8*>(qp + min(d, width - 8));
-        qf[c] = live && d < width ? x : f16x8{};
+        qf[i] = live && d < width ? x : f16x8{};
       }
     }
     f32x16 o[OB];
@@ -400,35 +436,19 @@ __global__ __launch_bounds__(256, 1) void latent_decode_kernel(const LatentDecod
 
     for (int c0 = ta; c0 < tb; c0 += kChunkTiles) {
       const int tiles = min(kChunkTiles, tb - c0);
-      // Arena rows of the chunk's keys; -1: no such key, or no such page.
-      __syncthreads();
-      {
-        constexpr int kEach = kChunkKeys / 256;
-        uint32_t page[kEach];
-        const int64_t table = (int64_t)b * p.table_stride;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-          const int key = c0 * kTileKeys + 256 * i + tid;
-          page[i] = ~0u;
-          if (256 * i < tiles * kTileKeys && key < keys)
-            page[i] = (uint32_t)p.tables[table + (uint32_t)key / (uint32_t)p.page_size];
-        }
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-          const int key = c0 * kTileKeys + 256 * i + tid;
-          const uint32_t r = (uint32_t)key % (uint32_t)p.page_size;
-          s_row[256 * i + tid] = page[i] < pages ? (int)(page[i] * (uint32_t)p.page_size + r) : -1;
-        }
+      if (c0 > ta) {
+        look_up(c0);
+        __syncthreads();  // (everyone is past the chunk before)
       }
+      put_rows(c0);
       __syncthreads();
       // Tile `tile` of the chunk into slot `slot` of the wave's ring: this
-      // wave's planes.
-      auto copy = [&](int tile, int slot) {
+      // wave's planes of the rows `row` (lane / 4 of either half).
+      auto copy = [&](const int (&row)[2], int slot) {
         const uint32_t dst = lds + (kg * NHG + slot) * (2 * kTile) + hg * (2 * kPlane);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int row = s_row[tile * kTileKeys + 16 * i + (lane >> 2)];
-          const f16* src = p.arena + (int64_t)max(row, 0) * width;
+          const f16* src = p.arena + (int64_t)max(row[i], 0) * width;
           if (whole) {
             each_plane([&](auto j) {
               if (NHG * j.value + hg < WP)
@@ -443,36 +463,38 @@ __global__ __launch_bounds__(256, 1) void latent_decode_kernel(const LatentDecod
           }
         }
       };
+      auto rows_of = [&](int tile, int (&row)[2]) {
+        row[0] = s_row[tile * kTileKeys + (lane >> 2)];
+        row[1] = s_row[tile * kTileKeys + 16 + (lane >> 2)];
+      };
       // Rows of no key become zeros once they have landed (their weight is 0;
       // zero rows keep 0 * V finite whatever the arena holds).
-      auto clean = [&](int tile, int slot) {
+      auto clean = [&](uint32_t okm, int slot) {
         f16* t = s_t[kg * NHG + slot] + hg * kPlane;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          if (s_row[tile * kTileKeys + 16 * i + (lane >> 2)] >= 0) continue;
+          if (okm >> (16 * i + (lane >> 2)) & 1) continue;
           for (int j = 0; NHG * j + hg < WP; ++j)
             *reinterpret_cast<f16x8*>(t + j * (NHG * kPlane) + 512 * i + 8 * lane) = f16x8{};
         }
       };
-      auto math = [&](int tile, int slot) {
+      auto math = [&](uint32_t okm, int slot) {
         const f16* t = s_t[kg * NHG + slot];
-        const uint32_t okm =
-            (uint32_t)__ballot(s_row[tile * kTileKeys + n] >= 0);
         // Operands are read kAhead products early (the reads and products
         // would else wait for each other in turn).
         f32x16 s = {};
         f16x8 a[2 * WP];
-        auto read_k = [&](int c) {
-          a[c] = *reinterpret_cast<const f16x8*>(t + (c & 1 ? k_lane1 : k_lane0) +
-                                                 kPlane * (c >> 1));
+        auto read_k = [&](int i) {
+          a[i] = *reinterpret_cast<const f16x8*>(t + (i & 1 ? k_lane1 : k_lane0) +
+                                                 kPlane * (i >> 1));
         };
 #pragma unroll
-        for (int c = 0; c < kAhead; ++c) read_k(c);
+        for (int i = 0; i < kAhead; ++i) read_k(i);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int c = 0; c < 2 * WP; ++c) {
-          s = mfma16<BF>(a[c], qf[c], s);
-          if (c + kAhead < 2 * WP) read_k(c + kAhead);
+        for (int i = 0; i < 2 * WP; ++i) {
+          s = mfma16<BF>(a[i], qf[i], s);
+          if (i + kAhead < 2 * WP) read_k(i + kAhead);
           __builtin_amdgcn_sched_barrier(0);
         }
         f16x8 va[2 * OB];
@@ -483,8 +505,10 @@ __global__ __launch_bounds__(256, 1) void latent_decode_kernel(const LatentDecod
         };
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) read_v(j);
+        if (!direct) {
 #pragma unroll
-        for (int v = 0; v < 16; ++v) s[v] *= p.scale_log2;
+          for (int v = 0; v < 16; ++v) s[v] *= p.scale_log2;
+        }
         if (okm != 0xFFFFFFFFu) {
           const uint32_t see = okm >> (4 * hh);
 #pragma unroll
@@ -494,27 +518,30 @@ __global__ __launch_bounds__(256, 1) void latent_decode_kernel(const LatentDecod
         float top = s[0];
 #pragma unroll
         for (int v = 1; v < 16; ++v) top = fmaxf(top, s[v]);
-        top = fmaxf(top, __shfl_xor(top, 32));
-        if (__ballot(top > m + kSlack)) {
-          float f = 1.0f;
-          if (top > m + kSlack) {
-            f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-            m = top;
-            l *= f;
-          }
-          outputs_settle(o);
+        top = max_halves(top) * c;
+        const bool grow = top > m + kSlack;
+        if (__ballot(grow)) {
+          // (Sums of a lane that has seen no key are zeros: a sequence's first
+          // tile scales nothing.)
+          const bool seen = __ballot(grow && m != -INFINITY) != 0;
+          const float f = grow ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
+          m = grow ? top : m;
+          l *= f;
+          if (seen) {
+            outputs_settle(o);
 #pragma unroll
-          for (int i = 0; i < OB; ++i) {
+            for (int i = 0; i < OB; ++i) {
 #pragma unroll
-            for (int v = 0; v < 16; ++v) o[i][v] *= f;
-            asm volatile("" : "+a"(o[i]));
+              for (int v = 0; v < 16; ++v) o[i][v] *= f;
+              asm volatile("" : "+a"(o[i]));
+            }
           }
         }
         const float mu = m == -INFINITY ? 0.0f : m;
         f16x8 pb[2];
 #pragma unroll
         for (int v = 0; v < 16; ++v)
-          pb[v / 8][v % 8] = round16<BF>(__builtin_amdgcn_exp2f(s[v] - mu));
+          pb[v / 8][v % 8] = round16<BF>(__builtin_amdgcn_exp2f(fmaf(s[v], c, -mu)));
 #pragma unroll
         for (int v = 0; v < 16; v += 2) l = add_pair<BF>(pb[v / 8][v % 8], pb[v / 8][v % 8 + 1], l);
         operands_settle(pb);
@@ -529,7 +556,8 @@ __global__ __launch_bounds__(256, 1) void latent_decode_kernel(const LatentDecod
       const int rounds = (tiles + kGroups - 1) / kGroups;
       // Copies of the first ring - 1 rounds; then per round: this round's rows
       // have landed, everyone is past the round before, whose slot takes the
-      // next copies.
+      // next copies. The rows of those copies and this tile's mask were read a
+      // round before.
       constexpr int kFirst = NHG > 1 ? NHG - 1 : 1;
       // Copies of a tile that this wave issues: its planes, in two halves.
       constexpr int kLess = 2 * (WP / NHG), kMore = 2 * ((WP + NHG - 1) / NHG);
@@ -541,32 +569,46 @@ __global__ __launch_bounds__(256, 1) void latent_decode_kernel(const LatentDecod
         else
           wait_vmem<later.value * kLess>();
       };
+      int row[2];
       for (int r = 0; r < min(kFirst, rounds); ++r)
-        if (r * kGroups + kg < tiles) copy(r * kGroups + kg, r % NHG);
+        if (r * kGroups + kg < tiles) {
+          rows_of(r * kGroups + kg, row);
+          copy(row, r % NHG);
+        }
+      // (Reads past the last tile stay in the chunk's rows; what they give is
+      // not used.)
+      constexpr int kLast = kChunkTiles - 1;
+      rows_of(min(kFirst * kGroups + kg, kLast), row);
+      int key_row = s_row[min(kg, kLast) * kTileKeys + n];
       for (int r = 0; r < rounds; ++r) {
         const int tile = r * kGroups + kg;
         const bool here = tile < tiles;
+        const int next = tile + kFirst * kGroups;
+        const uint32_t okm = (uint32_t)__ballot(key_row >= 0);
         if (NHG > 3 && tile + 2 * kGroups < tiles)
           landed(std::integral_constant<int, kTwo>{});
         else if (NHG > 2 && tile + kGroups < tiles)
           landed(std::integral_constant<int, kOne>{});
         else
           wait_vmem<0>();
-        if (here) clean(tile, r % NHG);
+        if (here && okm != 0xFFFFFFFFu) clean(okm, r % NHG);
         if constexpr (NHG > 1) {
           __syncthreads();
-          const int next = tile + kFirst * kGroups;
-          if (next < tiles) copy(next, (r + kFirst) % NHG);
+          if (next < tiles) copy(row, (r + kFirst) % NHG);
         }
-        if (here) math(tile, r % NHG);
+        key_row = s_row[min(tile + kGroups, kLast) * kTileKeys + n];
+        if constexpr (NHG > 1) rows_of(min(next + kGroups, kLast), row);
+        if (here) math(okm, r % NHG);
         wait_lds();
-        if constexpr (NHG == 1)
-          if (tile + kGroups < tiles) copy(tile + kGroups, 0);
+        if constexpr (NHG == 1) {
+          if (next < tiles) copy(row, 0);
+          rows_of(min(next + kGroups, kLast), row);
+        }
       }
     }
 
     // One partial of the wave groups' sums: each scaled to their common max,
-    // 128 dims a round through LDS, added and written along the rows.
+    // kJoin dims a round through LDS, added and written along the rows.
     outputs_settle(o);
     l += __shfl_xor(l, 32);
     if (hh == 0) s_ml[w][n] = make_float2(m, l);
@@ -584,13 +626,13 @@ __global__ __launch_bounds__(256, 1) void latent_decode_kernel(const LatentDecod
     if (kg == 0 && hh == 0 && live) p.part_ml[slot * p.hq + h] = make_float2(mm, ll);
     float* join = reinterpret_cast<float*>(&s_t[0][0]);
 #pragma unroll
-    for (int q = 0; q < OB / 4; ++q) {
-      const int d0 = 128 * q;
+    for (int q = 0; q < 32 * OB / kJoin; ++q) {
+      const int d0 = kJoin * q;
       if (d0 >= p.latent) break;
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        f32x16& x = o[4 * q + i];
+      for (int i = 0; i < kJoin / 32; ++i) {
+        f32x16& x = o[kJoin / 32 * q + i];
         asm volatile("" : "+a"(x));
         float* at = join + (32 * w + n) * kPitch + 32 * i + 4 * hh;
 #pragma unroll
@@ -599,8 +641,10 @@ __global__ __launch_bounds__(256, 1) void latent_decode_kernel(const LatentDecod
               make_float4(x[4 * g] * f, x[4 * g + 1] * f, x[4 * g + 2] * f, x[4 * g + 3] * f);
       }
       __syncthreads();
-      for (int i = tid; i < 32 * NHG * 32; i += 256) {
-        const int hd = i / 32, d = 4 * (i % 32);
+      constexpr int kWide = kJoin / 4;  // threads along a row
+#pragma unroll 4
+      for (int i = 0; i < 32 * NHG * kWide / 256; ++i) {
+        const int hd = i * (256 / kWide) + tid / kWide, d = 4 * (tid % kWide);
         float4 x = *reinterpret_cast<const float4*>(join + hd * kPitch + d);
 #pragma unroll
         for (int g = 1; g < kGroups; ++g) {
@@ -613,7 +657,6 @@ __global__ __launch_bounds__(256, 1) void latent_decode_kernel(const LatentDecod
       }
     }
     __syncthreads();
-    ++b;
   }
 }
 
@@ -658,7 +701,8 @@ __global__ __launch_bounds__(512, 2) void latent_merge_kernel(const LatentDecode
     const bool have = r < count;
     const int b = b0 + (have ? r : 0);
     const int seq0 = p.prefix[b], seq1 = p.prefix[b + 1];
-    const int g0 = seq0 / per, slots = have && seq1 > seq0 ? (seq1 - 1) / per - g0 + 1 : 0;
+    const int g0 = (seq0 + kSequenceTiles) / per;
+    const int slots = have && seq1 > seq0 ? (seq1 - 1) / per - g0 + 1 : 0;
     const float2* ml = p.part_ml + ((int64_t)g0 + b) * p.hq + h;
     const float* po = p.part_o + (((int64_t)g0 + b) * p.hq + h) * p.latent;
     // A lane looks at every 64th partial's maximum and sum.
@@ -786,7 +830,7 @@ Plan plan_for(int batch, int q_heads, int latent, int rope, int page_size, int t
   r.head_groups = (q_heads + 32 * nhg - 1) / (32 * nhg);
   const int64_t cap = (int64_t)page_size * table_stride;
   const int64_t keys = std::max<int64_t>(1, std::min<int64_t>(longest, cap));
-  const int64_t tiles = (int64_t)batch * ((keys + kTileKeys - 1) / kTileKeys);
+  const int64_t tiles = (int64_t)batch * ((keys + kTileKeys - 1) / kTileKeys + kSequenceTiles);
   // A workgroup has a tile for each of its wave groups at least.
   const int64_t most = std::max(1, kMaxGroups / r.head_groups);
   r.groups = (int)std::max<int64_t>(1, std::min(most, (tiles + 4 / nhg - 1) / (4 / nhg)));
@@ -826,7 +870,7 @@ int check_decode(int32_t batch, int32_t q_heads, int32_t latent_dim, int32_t rop
     return fail(PDA_ERR_INVALID_ARGUMENT, "batch=%d (at most %d) page_size=%d table_stride=%d",
                 batch, kMaxBatch, page_size, table_stride);
   const int64_t keys = std::min<int64_t>((int64_t)page_size * table_stride, INT32_MAX);
-  if ((int64_t)batch * ((keys + kTileKeys - 1) / kTileKeys) > INT32_MAX)
+  if ((int64_t)batch * ((keys + kTileKeys - 1) / kTileKeys + kSequenceTiles) > INT32_MAX)
     return fail(PDA_ERR_TOO_LONG, "batch x keys exceeds the tile stream (2^31 tiles of %d keys)",
                 kTileKeys);
   return PDA_OK;
