@@ -208,6 +208,7 @@ __device__ __forceinline__ int units_of(const LatentDecodeParams& p, int b) {
 template <bool BF>
 __global__ __launch_bounds__(256) void latent_absorb_kernel(const LatentDecodeParams p) {
   __shared__ __align__(1024) f16 s_u[4][kMaxHead * 32];
+  __shared__ __align__(16) f16 s_q[32 * (kMaxHead + 8)];
   __shared__ int s_scan[256];
   const int tid = threadIdx.x, w = uniform(tid >> 6), lane = tid & 63;
   const int n = lane & 31, hh = lane >> 5;
@@ -248,7 +249,6 @@ __global__ __launch_bounds__(256) void latent_absorb_kernel(const LatentDecodePa
   const int d0 = (blockIdx.x * 4 + w) * 32;
   // The wave's columns of U_h: rows of 64 bytes, zeros past either edge.
   const f16* u = p.kv_b + (int64_t)h * (p.nope + p.value) * p.latent;
-  const int steps = (p.nope + 15) / 16;
   const int col = d0 + 8 * (lane & 3);
   f16x8 rows[kMaxHead / 16];
 #pragma unroll
@@ -258,32 +258,33 @@ __global__ __launch_bounds__(256) void latent_absorb_kernel(const LatentDecodePa
     if (r < p.nope && col < p.latent)
       rows[i] = *reinterpret_cast<const f16x8*>(u + (int64_t)r * p.latent + col);
   }
-  const bool live = b0 + n < p.batch;
-  const f16* qp = p.q + ((int64_t)(live ? b0 + n : 0) * p.hq + h) * qwidth + 4 * hh;
-  f16x8 qf[kMaxHead / 16];
+  // The queries of 32 sequences, by rows, zeros past either edge.
+  constexpr int kQPitch = kMaxHead + 8;
 #pragma unroll
-  for (int i = 0; i < kMaxHead / 16; ++i) {
-    f16x4 lo = {}, hi = {};
-    if (live && 16 * i < p.nope) lo = *reinterpret_cast<const f16x4*>(qp + 16 * i);
-    if (live && 16 * i + 8 < p.nope) hi = *reinterpret_cast<const f16x4*>(qp + 16 * i + 8);
-    qf[i] = f16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  for (int i = tid; i < 32 * (kMaxHead / 8); i += 256) {
+    const int r = i / (kMaxHead / 8), d = 8 * (i % (kMaxHead / 8));
+    f16x8 x = {};
+    if (b0 + r < p.batch && d < p.nope)
+      x = *reinterpret_cast<const f16x8*>(p.q + ((int64_t)(b0 + r) * p.hq + h) * qwidth + d);
+    *reinterpret_cast<f16x8*>(s_q + r * kQPitch + d) = x;
   }
   f16* su = s_u[w];
 #pragma unroll
   for (int i = 0; i < kMaxHead / 16; ++i)
     *reinterpret_cast<f16x8*>(su + (16 * i + (lane >> 2)) * 32 + 8 * (lane & 3)) = rows[i];
-  // (The wave's own rows: its LDS writes are done before its reads.)
+  __syncthreads();
   const int g16 = lane >> 4, s16 = lane & 15;
   const f16* vp = su + (4 * (g16 >> 1) + (s16 >> 2)) * 32 + 16 * (g16 & 1) + 4 * (s16 & 3);
+  const f16* qp = s_q + n * kQPitch + 4 * hh;
   f32x16 acc = {};
-  for (int i = 0; i < kMaxHead / 16; ++i) {
-    if (i >= steps) break;
-    const f16x4 lo = read_tr(vp + 512 * i), hi = read_tr(vp + 512 * i + 256);
-    f16x8 q8 = qf[0];
 #pragma unroll
-    for (int j = 1; j < kMaxHead / 16; ++j)
-      if (i == j) q8 = qf[j];
-    acc = mfma16<BF>(f16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}, q8, acc);
+  for (int i = 0; i < kMaxHead / 16; ++i) {
+    if (16 * i >= p.nope) break;
+    const f16x4 lo = read_tr(vp + 512 * i), hi = read_tr(vp + 512 * i + 256);
+    const f16x4 ql = *reinterpret_cast<const f16x4*>(qp + 16 * i);
+    const f16x4 qh = *reinterpret_cast<const f16x4*>(qp + 16 * i + 8);
+    acc = mfma16<BF>(f16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]},
+                     f16x8{ql[0], ql[1], ql[2], ql[3], qh[0], qh[1], qh[2], qh[3]}, acc);
   }
   // The workgroup's 32 x 128 results through LDS, written along the rows.
   constexpr int kPitch = 136;
