@@ -123,6 +123,11 @@ __device__ __forceinline__ float add_pair(f16 a, f16 b, float s) {
     return __builtin_amdgcn_fdot2(x, f16x2{(f16)1.0f, (f16)1.0f}, s, false);
 }
 
+// Rows of 64 16-bit elements in LDS keep their 16-byte pieces at place piece ^
+// swizzle(row): 16 lanes that read one piece of 16 rows, and the 32 that read 64
+// bytes of 4 rows transposed, then fall on all 64 banks once.
+__device__ __forceinline__ int swizzle(int row) { return (row & 2) * 2 + (row >> 2 & 3); }
+
 // LDS byte address of a shared object.
 __device__ __forceinline__ uint32_t lds_address(const void* at) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)at;

@@ -318,18 +318,23 @@ __global__ __launch_bounds__(256) void latent_absorb_kernel(const LatentDecodePa
 // from the scores' registers to the next product without LDS: scores S^T = K
 // Q^T leave a lane 16 keys of one head, which are the B operand of O^T += V^T
 // P^T when V's rows are read in that order (two transposed reads). K and V are
-// the same rows: one copy in LDS serves both, swizzled in 16-byte pieces by
-// the row's group of four, which both reads undo.
+// the same rows: one copy in LDS serves both, in planes of 64 dims whose 16-byte
+// pieces are swizzled so that neither read meets a bank twice (swizzle). A copy
+// instruction moves 128 bytes of 8 rows: at 64 bytes of 16 rows the L2 was asked
+// twice as often, and its requests bound the launch.
 // NHG: waves side by side over heads, sharing a tile; 4 / NHG groups of waves
 // take tiles in turn. The LDS holds four tiles: a ring of NHG per group.
 template <int WP, int OB, int NHG, bool BF>
 __global__ __launch_bounds__(256, 1) void latent_decode_kernel(const LatentDecodeParams p) {
   constexpr int kGroups = 4 / NHG;           // tiles under way side by side
-  constexpr int kPlane = kTileKeys * 32;     // halves of a 64-byte column plane
+  constexpr int kPlane = kTileKeys * 64;     // halves of a 64-dim plane of a tile
   constexpr int kTile = WP * kPlane;
+  constexpr int kChunks = 4 * WP;            // 16-dim steps of a row
+  constexpr int kRows = 4 / NHG;             // 8-row parts of a tile a wave copies
   constexpr int kJoin = OB > 8 ? 256 : 128;  // dims joined at once
   constexpr int kPitch = kJoin + 4;          // floats of a head's
-  constexpr int kAhead = 4;                  // operands read early
+  // Operands read early: as many as the registers hold beside the queries.
+  constexpr int kAhead = NHG == 1 ? 2 : NHG == 2 ? 3 : 4;
   __shared__ __align__(1024) f16 s_t[4][kTile];
   __shared__ int s_row[kChunkKeys];
   __shared__ float2 s_ml[4][32];
@@ -359,23 +364,24 @@ __global__ __launch_bounds__(256, 1) void latent_decode_kernel(const LatentDecod
   __syncthreads();
   int b = uniform(s_at[0] + s_at[1] + s_at[2] + s_at[3]);
 
-  const int ksw = (n >> 2) & 3;
-  const int k_lane0 = 32 * n + 8 * (hh ^ ksw);
-  const int k_lane1 = 32 * n + 8 * ((2 + hh) ^ ksw);
+  // A lane's places in a tile's plane for the two reads: steps of 16 dims, and 8
+  // rows or 32 dims on, differ in bits of the swizzled place.
   const int g16 = lane >> 4, s16 = lane & 15;
-  const int vc = 2 * (g16 & 1) + ((s16 & 3) >> 1);  // 16-byte piece of the plane's row
+  const int k_place = 64 * n + 8 * (hh ^ swizzle(n));
   const int v_row = 4 * hh + (s16 >> 2);
-  const int v_lo = 32 * v_row + 8 * (vc ^ hh) + 4 * (s16 & 1);
-  const int v_hi = 32 * (v_row + 8) + 8 * (vc ^ (2 + hh)) + 4 * (s16 & 1);
-  // The copies: lane i of an instruction moves row i / 4 (of 16), one 16-byte
-  // piece; pieces past the row's end (widths below the kernel's) are another
-  // piece of the row, whose query elements are zeros.
-  const int piece = (lane & 3) ^ ((lane >> 4) & 3);
+  const int v_place = 64 * v_row + 4 * (s16 & 1) +
+                      8 * ((2 * (g16 & 1) + ((s16 & 3) >> 1)) ^ swizzle(v_row));
+  // The copies: lane i of an instruction moves a 16-byte piece of row i / 8 (of
+  // 8); pieces past the row's end (widths below the kernel's) are another
+  // piece of the row, whose query elements are zeros. The wave has the rows of
+  // parts hg, hg + NHG, ..
   const int last_piece = width / 8 - 1;
-  const bool whole = width == 32 * WP;
-  auto each_plane = [&](auto f) {
-    each(f, std::make_integer_sequence<int, (WP + NHG - 1) / NHG>{});
-  };
+  const bool whole = width == 64 * WP;
+  auto each_plane = [&](auto f) { each(f, std::make_integer_sequence<int, WP>{}); };
+  const int row0 = 8 * hg + (lane >> 3), piece0 = (lane & 7) ^ swizzle(row0);
+  // Row 8 (hg + NHG i) + lane / 8 and its piece's place.
+  auto part_row = [&](int i) { return row0 + 8 * NHG * i; };
+  auto piece = [&](int i) { return piece0 ^ 2 * (NHG * i & 1); };
   const uint32_t lds = uniform(lds_address(&s_t[0][0]));
   const uint32_t pages = (uint32_t)min(p.arena_pages, (int64_t)INT32_MAX);
 
@@ -415,7 +421,7 @@ __global__ __launch_bounds__(256, 1) void latent_decode_kernel(const LatentDecod
       }
     };
     look_up(ta);
-    f16x8 qf[2 * WP];
+    f16x8 qf[kChunks];
     {
       // (The pieces' places are computed here for every sequence: kept through
       // the loop they were spilled, and 50 reloads in turn took 15 us.)
@@ -423,7 +429,7 @@ __global__ __launch_bounds__(256, 1) void latent_decode_kernel(const LatentDecod
       asm volatile("" : "+v"(part));
       const f16* qp = p.q_lat + ((int64_t)b * p.hq + (live ? h : 0)) * width;
 #pragma unroll
-      for (int i = 0; i < 2 * WP; ++i) {
+      for (int i = 0; i < kChunks; ++i) {
         const int d = 16 * i + part;
         const f16x8 x = *reinterpret_cast<const f16x8*>(qp + min(d, width - 8));
         qf[i] = live && d < width ? x : f16x8{};
@@ -444,64 +450,65 @@ __global__ __launch_bounds__(256, 1) void latent_decode_kernel(const LatentDecod
       put_rows(c0);
       __syncthreads();
       // Tile `tile` of the chunk into slot `slot` of the wave's ring: this
-      // wave's planes of the rows `row` (lane / 4 of either half).
-      auto copy = [&](const int (&row)[2], int slot) {
-        const uint32_t dst = lds + (kg * NHG + slot) * (2 * kTile) + hg * (2 * kPlane);
+      // wave's parts, their arena rows in `row`.
+      auto copy = [&](const int (&row)[kRows], int slot) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < kRows; ++i) {
+          const uint32_t dst =
+              lds + (kg * NHG + slot) * (2 * kTile) + 1024 * (hg + NHG * i);
           const f16* src = p.arena + (int64_t)max(row[i], 0) * width;
           if (whole) {
             each_plane([&](auto j) {
-              if (NHG * j.value + hg < WP)
-                copy_to_lds<64 * NHG * j.value, (2 * kPlane - 64) * NHG * j.value>(
-                    src + 32 * hg + 8 * piece, dst + 1024 * i);
+              copy_to_lds<128 * j.value, (2 * kPlane - 128) * j.value>(src + 8 * piece(i), dst);
             });
           } else {
 #pragma unroll 1
-            for (int j = 0; NHG * j + hg < WP; ++j)
-              copy_to_lds<0, 0>(src + 8 * min(4 * (NHG * j + hg) + piece, last_piece),
-                                dst + j * (NHG * 2 * kPlane) + 1024 * i);
+            for (int j = 0; j < WP; ++j)
+              copy_to_lds<0, 0>(src + 8 * min(8 * j + piece(i), last_piece), dst + j * (2 * kPlane));
           }
         }
       };
-      auto rows_of = [&](int tile, int (&row)[2]) {
-        row[0] = s_row[tile * kTileKeys + (lane >> 2)];
-        row[1] = s_row[tile * kTileKeys + 16 + (lane >> 2)];
+      auto rows_of = [&](int tile, int (&row)[kRows]) {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) row[i] = s_row[tile * kTileKeys + part_row(i)];
       };
       // Rows of no key become zeros once they have landed (their weight is 0;
       // zero rows keep 0 * V finite whatever the arena holds).
       auto clean = [&](uint32_t okm, int slot) {
-        f16* t = s_t[kg * NHG + slot] + hg * kPlane;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (okm >> (16 * i + (lane >> 2)) & 1) continue;
-          for (int j = 0; NHG * j + hg < WP; ++j)
-            *reinterpret_cast<f16x8*>(t + j * (NHG * kPlane) + 512 * i + 8 * lane) = f16x8{};
+        for (int i = 0; i < kRows; ++i) {
+          if (okm >> part_row(i) & 1) continue;
+          f16* t = s_t[kg * NHG + slot] + 64 * part_row(i) + 8 * (lane & 7);
+          for (int j = 0; j < WP; ++j) *reinterpret_cast<f16x8*>(t + j * kPlane) = f16x8{};
         }
       };
       auto math = [&](uint32_t okm, int slot) {
         const f16* t = s_t[kg * NHG + slot];
         // Operands are read kAhead products early (the reads and products
         // would else wait for each other in turn).
+        // (The places are formed per tile: kept, they cost 8 registers of the
+        // few left beside the queries, and what was spilled for them 8 us.)
+        int k0 = k_place, v0 = v_place;
+        asm volatile("" : "+v"(k0), "+v"(v0));
         f32x16 s = {};
-        f16x8 a[2 * WP];
+        f16x8 a[kChunks];
         auto read_k = [&](int i) {
-          a[i] = *reinterpret_cast<const f16x8*>(t + (i & 1 ? k_lane1 : k_lane0) +
-                                                 kPlane * (i >> 1));
+          a[i] = *reinterpret_cast<const f16x8*>(t + (k0 ^ 16 * (i & 3)) + kPlane * (i >> 2));
         };
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) read_k(i);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < 2 * WP; ++i) {
+        for (int i = 0; i < kChunks; ++i) {
           s = mfma16<BF>(a[i], qf[i], s);
-          if (i + kAhead < 2 * WP) read_k(i + kAhead);
+          if (i + kAhead < kChunks) read_k(i + kAhead);
           __builtin_amdgcn_sched_barrier(0);
         }
         f16x8 va[2 * OB];
         auto read_v = [&](int j) {
-          const f16* vp = t + kPlane * (j % OB) + 512 * (j / OB);
-          const f16x4 lo = read_tr(vp + v_lo), hi = read_tr(vp + v_hi);
+          const f16* vp = t + kPlane * (j % OB / 2) + 1024 * (j / OB);
+          const f16x4 lo = read_tr(vp + (v0 ^ 32 * (j & 1)));
+          const f16x4 hi = read_tr(vp + (v0 ^ (16 + 32 * (j & 1))) + 512);
           va[j] = f16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
         };
 #pragma unroll
@@ -560,17 +567,10 @@ __global__ __launch_bounds__(256, 1) void latent_decode_kernel(const LatentDecod
       // next copies. The rows of those copies and this tile's mask were read a
       // round before.
       constexpr int kFirst = NHG > 1 ? NHG - 1 : 1;
-      // Copies of a tile that this wave issues: its planes, in two halves.
-      constexpr int kLess = 2 * (WP / NHG), kMore = 2 * ((WP + NHG - 1) / NHG);
+      auto landed = [&](auto later) { wait_vmem<later.value * kRows * WP>(); };  // all but
+      // those of `later` tiles
       constexpr int kTwo = NHG > 3 ? 2 : 0, kOne = NHG > 2 ? 1 : 0;
-      const bool more = hg < WP % NHG;
-      auto landed = [&](auto later) {  // all but those of `later` tiles
-        if (more)
-          wait_vmem<later.value * kMore>();
-        else
-          wait_vmem<later.value * kLess>();
-      };
-      int row[2];
+      int row[kRows];
       for (int r = 0; r < min(kFirst, rounds); ++r)
         if (r * kGroups + kg < tiles) {
           rows_of(r * kGroups + kg, row);
@@ -860,7 +860,7 @@ const void* decode_kernel(int nhg) {
 // The kernel of 256 latent dims (and 64 rotary ones) for rows that it holds.
 template <bool BF>
 const void* decode_kernel_for(int nhg, int latent) {
-  return latent <= 256 ? decode_kernel<10, 8, BF>(nhg) : decode_kernel<18, 16, BF>(nhg);
+  return latent <= 256 ? decode_kernel<5, 8, BF>(nhg) : decode_kernel<9, 16, BF>(nhg);
 }
 
 int check_decode(int32_t batch, int32_t q_heads, int32_t latent_dim, int32_t rope_dim,

@@ -27,6 +27,7 @@ constexpr int kKeys = 64;       // keys per tile
 constexpr int kMaxSplits = 64;
 constexpr float kSlack = 8.0f;
 constexpr int kXcds = 8;
+constexpr int kCus = 256;
 
 struct PrefillParams {
   const f16* q;         // [count, hq, nope + rope]
@@ -62,29 +63,35 @@ struct PrefillParams {
 // ---------------------------------------------------------------------------
 // Expansion.
 
-constexpr int kRowsM = 128;   // tokens of a workgroup
-constexpr int kColsN = 128;   // projected dims of a workgroup
-
 // keys[h, t] = U_h c_t, values[h, t] = D_h c_t, rounded to the element type: a
-// matrix product of 128 tokens by 128 dims of one head over the latent, 64
-// latent dims at a time through two LDS buffers, a wave 64 by 64. Tokens
-// without a row become zeros. The workgroups of the group's first dims also
-// gather the rotary keys and the mask of keys that have a row.
-template <bool BF>
-__global__ __launch_bounds__(256, 2) void latent_expand_kernel(const PrefillParams p) {
-  constexpr int kPlane = 128 * 32;  // halves of a 32-dim plane of 128 rows
-  __shared__ __align__(1024) f16 s_w[2][2 * kPlane];
-  __shared__ __align__(1024) f16 s_c[2][2 * kPlane];
-  __shared__ int s_row[kRowsM];
+// matrix product in which the tokens stay and the projections stream. A wave
+// keeps 32 TB tokens' whole latents as operands (TB x 128 registers at 512 dims,
+// gathered from the pages once); the workgroup walks the projected dims of its
+// heads 32 at a time through a ring of LDS blocks, each read once by every wave
+// for TB products: with two token blocks the matrix cores and not the LDS bound
+// it. Results are stored a block late, so that no wait for a copy waits for a
+// store. Tokens without a row are zeros from the start. The workgroups of the
+// group's first heads also gather the rotary keys and the mask of keys that have
+// a row.
+template <int TB, bool BF>
+__global__ __launch_bounds__(256, TB == 2 ? 1 : 2) void latent_expand_kernel(const PrefillParams p) {
+  constexpr int kRing = TB == 2 ? 4 : 2;
+  constexpr int kPlane = 32 * 64;  // halves of 64 latent dims of a block
+  constexpr int kPlanes = kMaxLatent / 64;
+  constexpr int kChunks = 4 * kPlanes;
+  constexpr int kTokens = 128 * TB;
+  constexpr int kCopies = kPlanes;  // a wave's, a block
+  constexpr int kPitch = 40;        // halves of a token's 32 results
+  __shared__ __align__(1024) f16 s_w[kRing][kPlanes * kPlane];
+  __shared__ __align__(16) f16 s_out[4][32 * TB * kPitch];
+  __shared__ int s_row[kTokens];
   const int tid = threadIdx.x, w = uniform(tid >> 6), lane = tid & 63;
   const int n = lane & 31, hh = lane >> 5;
   const int outs = p.nope + p.value;
-  const int cols = (outs + kColsN - 1) / kColsN;
-  const int t0 = blockIdx.x * kRowsM;
-  const int hl = blockIdx.y / cols, j0 = (blockIdx.y % cols) * kColsN;
+  const int t0 = blockIdx.y * kTokens;
   const int width = p.latent + p.rope;
-  if (tid < kRowsM) {
-    const int t = t0 + tid;
+  for (int i = tid; i < kTokens; i += 256) {
+    const int t = t0 + i;
     int row = -1;
     if (t < p.start + p.count) {
       const uint32_t pi = (uint32_t)t / (uint32_t)p.page_size;
@@ -94,16 +101,61 @@ __global__ __launch_bounds__(256, 2) void latent_expand_kernel(const PrefillPara
           row = (int)(page * (uint32_t)p.page_size + (t - pi * p.page_size));
       }
     }
-    s_row[tid] = row;
-    if (blockIdx.y == 0) {
+    s_row[i] = row;
+    if (blockIdx.x == 0) {
       const uint64_t have = __ballot(row >= 0);
       if ((tid & 63) == 0 && t < p.span) p.seen[t / 64] = have;
     }
   }
   __syncthreads();
-  if (blockIdx.y == 0) {
+  // The group's blocks of 32 projected dims (a head's nope dims, then its value
+  // dims, each to a whole block), shared out evenly.
+  const int nope_blocks = (p.nope + 31) / 32, each_head = nope_blocks + (p.value + 31) / 32;
+  const int64_t every = (int64_t)p.heads * each_head;
+  const int b0 = uniform((int)(every * blockIdx.x / gridDim.x));
+  const int b1 = uniform((int)(every * (blockIdx.x + 1) / gridDim.x));
+
+  // Copies: an instruction moves 128 bytes of 8 projection rows, the wave's. Past
+  // the latent's end they repeat its last piece (the tokens are zeros there),
+  // past a head's part its last row (not used).
+  const int my_row = 8 * w + (lane >> 3);
+  const int piece = (lane & 7) ^ swizzle(my_row);
+  const int last_piece = p.latent / 8 - 1;
+  const uint32_t lds = uniform(lds_address(&s_w[0][0]));
+  auto copy = [&](int block) {
+    const int h = block / each_head, part = block - h * each_head;
+    const bool value = part >= nope_blocks;
+    const int d0 = 32 * (value ? part - nope_blocks : part);
+    const int size = value ? p.value : p.nope;
+    const f16* src =
+        p.kv_b + ((int64_t)(p.head0 + h) * outs + (value ? p.nope : 0) + min(d0 + my_row, size - 1)) *
+                     p.latent;
+    const uint32_t dst = lds + ((block - b0) % kRing) * (2 * kPlanes * kPlane) + 1024 * w;
+#pragma unroll
+    for (int j = 0; j < kPlanes; ++j)
+      copy_to_lds<0, 0>(src + 8 * min(8 * j + piece, last_piece), dst + j * (2 * kPlane));
+  };
+  if (b0 < b1) copy(b0);
+  if constexpr (kRing > 2) {
+    if (b0 + 1 < b1) copy(b0 + 1);
+    if (b0 + 2 < b1) copy(b0 + 2);
+  }
+  // The wave's tokens.
+  f16x8 tok[TB][kChunks];
+#pragma unroll
+  for (int j = 0; j < TB; ++j) {
+    const int row = s_row[32 * (TB * w + j) + n];
+    const f16* src = p.arena + (int64_t)max(row, 0) * width;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+      const int d = 16 * c + 8 * hh;
+      const f16x8 x = *reinterpret_cast<const f16x8*>(src + min(d, p.latent - 8));
+      tok[j][c] = row >= 0 && d < p.latent ? x : f16x8{};
+    }
+  }
+  if (blockIdx.x == 0) {
     const int pieces = p.rdim / 8;
-    for (int i = tid; i < kRowsM * pieces; i += 256) {
+    for (int i = tid; i < kTokens * pieces; i += 256) {
       const int r = i / pieces, j = i - r * pieces;
       if (t0 + r >= p.span) break;
       f16x8 x = {};
@@ -112,93 +164,87 @@ __global__ __launch_bounds__(256, 2) void latent_expand_kernel(const PrefillPara
       *reinterpret_cast<f16x8*>(p.rope_keys + (int64_t)(t0 + r) * p.rdim + 8 * j) = x;
     }
   }
-  // Copies: a wave moves 32 rows of each operand, 16 rows and 64 bytes an
-  // instruction, the 16-byte pieces swizzled by the row's group of four.
-  const int piece = (lane & 3) ^ ((lane >> 4) & 3);
-  const int last_piece = p.latent / 8 - 1;
-  const f16* src_w[2];
-  const f16* src_c[2];
+  // A block's results (32 dims of the wave's tokens), by rows from the wave's
+  // part of LDS: 64 bytes a row. The expanded rows hold whole blocks, so every
+  // dim of it is stored, also those past the head's part (keys are zeros there,
+  // which the queries' zeros meet).
+  f16* so = s_out[w];
+  auto store = [&](int block) {
+    const int h = block / each_head, part = block - h * each_head;
+    const bool value = part >= nope_blocks;
+    const int d0 = 32 * (value ? part - nope_blocks : part);
+    f16* base = value ? p.values + (int64_t)h * p.span * p.vdim
+                      : p.keys + (int64_t)h * p.span * p.kdim;
+    const int pitch = value ? p.vdim : p.kdim;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = 32 * w + 16 * i + (lane >> 2);
-    src_w[i] = p.kv_b + ((int64_t)(p.head0 + hl) * outs + min(j0 + r, outs - 1)) * p.latent;
-    src_c[i] = p.arena + (int64_t)max(s_row[r], 0) * width;
-  }
-  const uint32_t w_dst = uniform(lds_address(&s_w[0][0]) + 2048 * w);
-  const uint32_t c_dst = uniform(lds_address(&s_c[0][0]) + 2048 * w);
-  const int steps = (p.latent + 63) / 64;
-  auto copy = [&](int k, int buf) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int at = 8 * min(8 * k + 4 * j + piece, last_piece);
-        const uint32_t off = buf * (4 * kPlane) + j * (2 * kPlane) + 1024 * i;
-        copy_to_lds<0, 0>(src_w[i] + at, w_dst + off);
-        copy_to_lds<0, 0>(src_c[i] + at, c_dst + off);
-      }
+    for (int j = 0; j < 2 * TB; ++j) {
+      const int r = 16 * j + (lane >> 2);
+      const int64_t t = t0 + 32 * TB * w + r;
+      if (t >= p.span) continue;
+      *reinterpret_cast<f16x8*>(base + t * pitch + d0 + 8 * (lane & 3)) =
+          *reinterpret_cast<const f16x8*>(so + r * kPitch + 8 * (lane & 3));
+      // (Planes of the keys that no block fills.)
+      if (part == nope_blocks - 1 && (lane & 3) == 0)
+        for (int d = 32 * nope_blocks; d < p.kdim; d += 8)
+          *reinterpret_cast<f16x8*>(base + t * pitch + d) = f16x8{};
+    }
   };
-  const int ksw = (n >> 2) & 3;
-  const int lane0 = 32 * n + 8 * (hh ^ ksw), lane1 = 32 * n + 8 * ((2 + hh) ^ ksw);
-  const int wo = w & 1, wt = w >> 1;
-  f32x16 acc[2][2] = {};
-  copy(0, 0);
-  for (int k = 0; k < steps; ++k) {
-    const int buf = k & 1;
-    wait_vmem<0>();
+  int w_lane[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w_lane[i] = 64 * n + 8 * ((2 * i + hh) ^ swizzle(n));
+  const int steps = (p.latent + 15) / 16;
+  for (int b = b0; b < b1; ++b) {
+    // (Operations end in order: of the last 2 kCopies, a block's stores may be
+    // among them.)
+    if (kRing > 2 && b + 2 < b1)
+      wait_vmem<2 * kCopies>();
+    else if (kRing > 2 && b + 1 < b1)
+      wait_vmem<kCopies>();
+    else
+      wait_vmem<0>();
     __syncthreads();
-    if (k + 1 < steps) copy(k + 1, buf ^ 1);
-    if (64 * (k + 1) > p.latent) {
-      // The pieces past the latent repeat its last: zeros on one side.
-      const int have = p.latent / 8 - 8 * k;
-      for (int i = tid; i < 128 * 8; i += 256) {
-        const int r = i >> 3, c = i & 7;
-        if (c >= have)
-          *reinterpret_cast<f16x8*>(&s_w[buf][(c >> 2) * kPlane + 32 * r +
-                                              8 * ((c & 3) ^ ((r >> 2) & 3))]) = f16x8{};
+    if (b > b0) store(b - 1);
+    constexpr int kNext = kRing > 2 ? 3 : 1;
+    if (b + kNext < b1) copy(b + kNext);
+    const f16* wp = s_w[(b - b0) % kRing];
+    f32x16 acc[TB];
+#pragma unroll
+    for (int j = 0; j < TB; ++j) acc[j] = f32x16{};
+    constexpr int kAhead = 4;
+    f16x8 a[kChunks];
+    auto read = [&](int c) {
+      a[c] = *reinterpret_cast<const f16x8*>(wp + (c >> 2) * kPlane + w_lane[c & 3]);
+    };
+    auto products = [&](auto count) {
+#pragma unroll
+      for (int c = 0; c < kAhead; ++c) read(c);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int c = 0; c < count.value; ++c) {
+#pragma unroll
+        for (int j = 0; j < TB; ++j) acc[j] = mfma16<BF>(a[c], tok[j][c], acc[j]);
+        if (c + kAhead < count.value) read(c + kAhead);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      __syncthreads();
-    }
-    const f16* wp = s_w[buf] + 64 * 32 * wo;
-    const f16* cp = s_c[buf] + 64 * 32 * wt;
+    };
+    if (steps <= kChunks / 2)
+      products(std::integral_constant<int, kChunks / 2>{});
+    else
+      products(std::integral_constant<int, kChunks>{});
+    const int part = b % each_head;
+    const int left = part >= nope_blocks ? 32 : p.nope - 32 * part;  // keys' dims of the block
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      f16x8 a[2], b[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int at = (c >> 1) * kPlane + 1024 * i + (c & 1 ? lane1 : lane0);
-        a[i] = *reinterpret_cast<const f16x8*>(wp + at);
-        b[i] = *reinterpret_cast<const f16x8*>(cp + at);
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = mfma16<BF>(a[i], b[j], acc[i][j]);
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int r = 64 * wt + 32 * j + n;
-    const int64_t t = t0 + r;
-    if (t >= p.span) continue;
-    const bool have = s_row[r] >= 0;
-    f16* krow = p.keys + ((int64_t)hl * p.span + t) * p.kdim;
-    f16* vrow = p.values + ((int64_t)hl * p.span + t) * p.vdim;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < TB; ++j)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const int d = j0 + 64 * wo + 32 * i + 8 * g + 4 * hh;
-        if (d >= outs) continue;
         f16x4 y;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) y[v] = have ? round16<BF>(acc[i][j][4 * g + v]) : (f16)0.0f;
-        *reinterpret_cast<f16x4*>(d < p.nope ? krow + d : vrow + (d - p.nope)) = y;
+        for (int v = 0; v < 4; ++v)
+          y[v] = 8 * g < left ? round16<BF>(acc[j][4 * g + v]) : (f16)0.0f;
+        *reinterpret_cast<f16x4*>(so + (32 * j + n) * kPitch + 8 * g + 4 * hh) = y;
       }
-    // (The queries are zeros past the nope dims; the keys have to be finite.)
-    if (j0 == 0 && wo == 0 && hh == 0)
-      for (int d = p.nope; d < p.kdim; d += 8) *reinterpret_cast<f16x8*>(krow + d) = f16x8{};
   }
+  if (b0 < b1) store(b1 - 1);
 }
 
 // ---------------------------------------------------------------------------
@@ -211,12 +257,13 @@ __global__ __launch_bounds__(256, 2) void latent_expand_kernel(const PrefillPara
 // transposed in the order the scores hold the keys). Two workgroups a CU, so
 // that one's products run beside the other's weights. The query tiles of a head
 // are dispatched to one XCD, whose L2 then serves the head's keys and values.
-// NP, RP, VP: planes of 32 dims of the nope part, the rotary part and the
+// NP, RP, VP: planes of 64 dims of the nope part, the rotary part and the
 // values.
 template <int NP, int RP, int VP, bool BF>
 __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(const PrefillParams p) {
-  constexpr int kPlane = kKeys * 32;
+  constexpr int kPlane = kKeys * 64;  // halves of a 64-dim plane of a tile
   constexpr int KP = NP + RP;
+  constexpr int OB = 2 * VP;          // 32-dim blocks of the output
   __shared__ __align__(1024) f16 s_k[2][KP * kPlane];
   __shared__ __align__(1024) f16 s_v[2][VP * kPlane];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -246,16 +293,16 @@ __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(const PrefillPar
   const bool q_live = qi < p.count;
   const int wfirst = p.start + wq0, wlast = p.start + min(wq0 + 31, p.count - 1);
 
-  f16x8 qf[2 * KP];
+  f16x8 qf[4 * KP];
   {
     const f16* qp = p.q + ((int64_t)(q_live ? qi : 0) * p.hq + h) * (p.nope + p.rope);
 #pragma unroll
-    for (int c = 0; c < 2 * KP; ++c) {
-      const int d = (c < 2 * NP ? 16 * c : 16 * (c - 2 * NP)) + 8 * hh;
-      const int lim = c < 2 * NP ? p.nope : p.rope;
-      qf[c] = f16x8{};
+    for (int i = 0; i < 4 * KP; ++i) {
+      const int d = (i < 4 * NP ? 16 * i : 16 * (i - 4 * NP)) + 8 * hh;
+      const int lim = i < 4 * NP ? p.nope : p.rope;
+      qf[i] = f16x8{};
       if (q_live && d < lim)
-        qf[c] = *reinterpret_cast<const f16x8*>(qp + (c < 2 * NP ? 0 : p.nope) + d);
+        qf[i] = *reinterpret_cast<const f16x8*>(qp + (i < 4 * NP ? 0 : p.nope) + d);
     }
   }
   const int ntile = (p.start + q1 - 1) / kKeys + 1;
@@ -263,41 +310,59 @@ __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(const PrefillPar
   const int t_end = (int)((int64_t)ntile * (split + 1) / p.splits);
   const int wave_end = wq0 < p.count ? min(t_end, wlast / kKeys + 1) : t_begin;
 
-  // Copies: a wave moves 16 keys of a tile, 64 bytes of a row an instruction;
-  // the keys' 16-byte pieces are swizzled.
-  const int gk = 16 * w + (lane >> 2);
-  const f16* src_k = p.keys + ((int64_t)hl * p.span + gk) * (32 * NP) + 8 * ((lane & 3) ^ ((lane >> 4) & 3));
-  const f16* src_r = p.rope_keys + (int64_t)gk * (32 * RP) + 8 * ((lane & 3) ^ ((lane >> 4) & 3));
-  const f16* src_v = p.values + ((int64_t)hl * p.span + gk) * (32 * VP) + 8 * (lane & 3);
-  const uint32_t k_dst = uniform(lds_address(&s_k[0][0]) + 1024 * w);
-  const uint32_t v_dst = uniform(lds_address(&s_v[0][0]) + 1024 * w);
+  // Copies: a wave moves 16 keys of a tile, 128 bytes of 8 rows an instruction,
+  // their 16-byte pieces swizzled.
+  const f16 *src_k[2], *src_r[2], *src_v[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int key = 16 * w + 8 * i + (lane >> 3);
+    const int piece = 8 * ((lane & 7) ^ swizzle(key));
+    src_k[i] = p.keys + ((int64_t)hl * p.span + key) * (64 * NP) + piece;
+    src_r[i] = p.rope_keys + (int64_t)key * (64 * RP) + piece;
+    src_v[i] = p.values + ((int64_t)hl * p.span + key) * (64 * VP) + piece;
+  }
+  const uint32_t k_dst = uniform(lds_address(&s_k[0][0]) + 2048 * w);
+  const uint32_t v_dst = uniform(lds_address(&s_v[0][0]) + 2048 * w);
   auto copy = [&](int t, int buf) {
     const int64_t k0 = (int64_t)t * kKeys;
-    const f16* sk = src_k + k0 * (32 * NP);
-    const f16* sv = src_v + k0 * (32 * VP);
-    const f16* sr = src_r + k0 * (32 * RP);
-    const uint32_t kd = k_dst + buf * (2 * KP * kPlane), vd = v_dst + buf * (2 * VP * kPlane);
-    auto nope = [&](auto i) { copy_to_lds<64 * i.value, (2 * kPlane - 64) * i.value>(sk, kd); };
-    auto rope = [&](auto i) {
-      copy_to_lds<64 * i.value, (2 * kPlane - 64) * i.value + 2 * NP * kPlane>(sr, kd);
-    };
-    auto vals = [&](auto i) { copy_to_lds<64 * i.value, (2 * kPlane - 64) * i.value>(sv, vd); };
-    each(nope, std::make_integer_sequence<int, NP>{});
-    each(rope, std::make_integer_sequence<int, RP>{});
-    each(vals, std::make_integer_sequence<int, VP>{});
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const f16* sk = src_k[i] + k0 * (64 * NP);
+      const f16* sv = src_v[i] + k0 * (64 * VP);
+      const f16* sr = src_r[i] + k0 * (64 * RP);
+      const uint32_t kd = k_dst + buf * (2 * KP * kPlane) + 1024 * i;
+      const uint32_t vd = v_dst + buf * (2 * VP * kPlane) + 1024 * i;
+      auto nope = [&](auto j) { copy_to_lds<128 * j.value, (2 * kPlane - 128) * j.value>(sk, kd); };
+      auto rope = [&](auto j) {
+        copy_to_lds<128 * j.value, (2 * kPlane - 128) * j.value + 2 * NP * kPlane>(sr, kd);
+      };
+      auto vals = [&](auto j) { copy_to_lds<128 * j.value, (2 * kPlane - 128) * j.value>(sv, vd); };
+      each(nope, std::make_integer_sequence<int, NP>{});
+      each(rope, std::make_integer_sequence<int, RP>{});
+      each(vals, std::make_integer_sequence<int, VP>{});
+    }
   };
-  const int ksw = (n >> 2) & 3;
-  const int k_lane0 = 32 * n + 8 * (hh ^ ksw), k_lane1 = 32 * n + 8 * ((2 + hh) ^ ksw);
+  int k_lane[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) k_lane[i] = 64 * n + 8 * ((2 * i + hh) ^ swizzle(n));
   const int g16 = lane >> 4, s16 = lane & 15;
-  const int v_lane = (4 * (g16 >> 1) + (s16 >> 2)) * 32 + 16 * (g16 & 1) + 4 * (s16 & 3);
+  int v_lane[2][2];  // [rows 8 on][odd 32 dims of a plane]
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int r = 8 * i + 4 * hh + (s16 >> 2);
+      v_lane[i][j] = 64 * r + 4 * (s16 & 1) +
+                     8 * ((4 * j + 2 * (g16 & 1) + ((s16 & 3) >> 1)) ^ swizzle(r));
+    }
   // A positive scale is applied with the maximum's subtraction, another one to
   // the scores.
   const bool direct = p.scale_log2 > 0.0f;
   const float c = direct ? p.scale_log2 : 1.0f;
 
-  f32x16 o[VP];
+  f32x16 o[OB];
 #pragma unroll
-  for (int i = 0; i < VP; ++i) o[i] = f32x16{};
+  for (int i = 0; i < OB; ++i) o[i] = f32x16{};
   float m = -INFINITY, l = 0.0f;
   uint64_t ok_next = 0;
   if (t_begin < t_end) {
@@ -319,11 +384,11 @@ __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(const PrefillPar
     const int k0 = t * kKeys;
     f32x16 s[2] = {};
 #pragma unroll
-    for (int cc = 0; cc < 2 * KP; ++cc) {
-      const f16* kp = kt + (cc & 1 ? k_lane1 : k_lane0) + kPlane * (cc >> 1);
+    for (int cc = 0; cc < 4 * KP; ++cc) {
+      const f16* kp = kt + k_lane[cc & 3] + kPlane * (cc >> 2);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        s[i] = mfma16<BF>(*reinterpret_cast<const f16x8*>(kp + 1024 * i), qf[cc], s[i]);
+        s[i] = mfma16<BF>(*reinterpret_cast<const f16x8*>(kp + 2048 * i), qf[cc], s[i]);
     }
     if (!direct) {
 #pragma unroll
@@ -354,7 +419,7 @@ __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(const PrefillPar
         m = top;
         l *= f;
 #pragma unroll
-        for (int i = 0; i < VP; ++i)
+        for (int i = 0; i < OB; ++i)
 #pragma unroll
           for (int v = 0; v < 16; ++v) o[i][v] *= f;
       }
@@ -375,9 +440,9 @@ __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(const PrefillPar
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-        for (int b = 0; b < VP; ++b) {
-          const f16* vp = vt + v_lane + kPlane * b + 1024 * i + 512 * ks;
-          const f16x4 lo = read_tr(vp), hi = read_tr(vp + 256);
+        for (int b = 0; b < OB; ++b) {
+          const f16* vp = vt + kPlane * (b / 2) + 2048 * i + 1024 * ks;
+          const f16x4 lo = read_tr(vp + v_lane[0][b & 1]), hi = read_tr(vp + v_lane[1][b & 1]);
           o[b] = mfma16<BF>(f16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]},
                             pb[i][ks], o[b]);
         }
@@ -390,7 +455,7 @@ __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(const PrefillPar
     const int64_t pair = (int64_t)split * p.count * p.hq + at;
     float* dst = p.part_o + pair * p.value + 4 * hh;
 #pragma unroll
-    for (int b = 0; b < VP; ++b)
+    for (int b = 0; b < OB; ++b)
 #pragma unroll
       for (int g = 0; g < 4; ++g)
         if (32 * b + 8 * g < p.value)
@@ -402,7 +467,7 @@ __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(const PrefillPar
   const float inv = l > 0.0f ? 1.0f / l : 0.0f;
   f16* dst = p.out + at * p.value + 4 * hh;
 #pragma unroll
-  for (int b = 0; b < VP; ++b)
+  for (int b = 0; b < OB; ++b)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       if (32 * b + 8 * g >= p.value) continue;
@@ -455,7 +520,7 @@ constexpr size_t kExpandBytes = (size_t)1 << 30;  // expanded keys and values at
 constexpr int kSlots = 512;                       // workgroups resident on an MI355X
 
 struct PrefillPlan {
-  bool small;   // planes of 64 + 32 and 64 dims, else 128 + 64 and 128
+  bool small;   // planes of 64 + 64 and 64 dims, else 128 + 64 and 128
   int kdim, vdim, rdim;
   int span, tiles, splits, heads;  // heads per group
   size_t keys, values, rope, seen, part_o, part_ml, bytes;
@@ -463,10 +528,10 @@ struct PrefillPlan {
 
 PrefillPlan plan_for(int start, int count, int q_heads, int rope, int nope, int value) {
   PrefillPlan r;
-  r.small = nope <= 64 && rope <= 32 && value <= 64;
+  r.small = nope <= 64 && value <= 64;
   r.kdim = r.small ? 64 : 128;
   r.vdim = r.kdim;
-  r.rdim = r.small ? 32 : 64;
+  r.rdim = 64;
   r.span = (start + count + kKeys - 1) / kKeys * kKeys;
   r.tiles = (count + kQueries - 1) / kQueries;
   const size_t head_bytes = (size_t)r.span * (r.kdim + r.vdim) * 2;
@@ -503,15 +568,15 @@ int check_prefill(int32_t start, int32_t count, int32_t q_heads, int32_t latent_
   if (rc != PDA_OK) return rc;
   if (start < 0 || count < 0)
     return fail(PDA_ERR_INVALID_ARGUMENT, "start=%d count=%d", start, count);
-  if ((int64_t)start + count > INT32_MAX - 2 * kRowsM)
+  if ((int64_t)start + count > INT32_MAX - 512)
     return fail(PDA_ERR_TOO_LONG, "start + count next to 2^31");
   return PDA_OK;
 }
 
 template <bool BF>
 const void* prefill_kernel(bool small) {
-  return small ? (const void*)latent_prefill_kernel<2, 1, 2, BF>
-               : (const void*)latent_prefill_kernel<4, 2, 4, BF>;
+  return small ? (const void*)latent_prefill_kernel<1, 1, 1, BF>
+               : (const void*)latent_prefill_kernel<2, 1, 2, BF>;
 }
 
 int latent_prefill(const void* queries, const void* arena, const void* kv_b, const int32_t* table,
@@ -539,10 +604,8 @@ int latent_prefill(const void* queries, const void* arena, const void* kv_b, con
   if ((uintptr_t)table & 3) return fail(PDA_ERR_ALIGNMENT, "the table must be 4-byte aligned");
   const PrefillPlan plan = plan_for(start, count, q_heads, rope_dim, nope_dim, value_dim);
   const int64_t grid = (int64_t)plan.tiles * plan.splits * plan.heads;
-  const int outs = nope_dim + value_dim;
-  const int64_t cols = (int64_t)plan.heads * ((outs + kColsN - 1) / kColsN);
   const int64_t join = ((int64_t)count * q_heads * (value_dim / 4) + 255) / 256;
-  if (grid > INT32_MAX || cols > 65535 || join > INT32_MAX)
+  if (grid > INT32_MAX || join > INT32_MAX)
     return fail(PDA_ERR_INVALID_ARGUMENT, "queries x heads beyond one launch's workgroups");
   if (!workspace || workspace_bytes < plan.bytes)
     return fail(PDA_ERR_WORKSPACE, "a workspace of %zu bytes is needed (got %zu)", plan.bytes,
@@ -581,17 +644,26 @@ int latent_prefill(const void* queries, const void* arena, const void* kv_b, con
   prm.scale_log2 = scale * kLog2e;
   void* args[] = {&prm};
   const hipStream_t hs = static_cast<hipStream_t>(stream);
-  const void* expand =
-      bf ? (const void*)latent_expand_kernel<true> : (const void*)latent_expand_kernel<false>;
+  // Two token blocks a wave where that still fills the CUs (one workgroup
+  // each), one where it would not (two workgroups each).
+  const int64_t wide = ((int64_t)plan.span + 255) / 256 * plan.heads;
+  const bool two = wide >= kCus;
+  const void* expand = two ? (bf ? (const void*)latent_expand_kernel<2, true>
+                                 : (const void*)latent_expand_kernel<2, false>)
+                           : (bf ? (const void*)latent_expand_kernel<1, true>
+                                 : (const void*)latent_expand_kernel<1, false>);
+  const int tokens = two ? 256 : 128;
+  const int token_tiles = (plan.span + tokens - 1) / tokens;
   const void* attend = bf ? prefill_kernel<true>(plan.small) : prefill_kernel<false>(plan.small);
   hipError_t err = hipSuccess;
   for (int h0 = 0; h0 < q_heads && err == hipSuccess; h0 += plan.heads) {
     prm.head0 = h0;
     prm.heads = std::min(plan.heads, q_heads - h0);
-    err = hipLaunchKernel(expand,
-                          dim3((plan.span + kRowsM - 1) / kRowsM,
-                               prm.heads * ((outs + kColsN - 1) / kColsN)),
-                          dim3(256), args, 0, hs);
+    // The projected dims shared out so that the workgroups just fill the GPU.
+    const int every = prm.heads * ((nope_dim + 31) / 32 + (value_dim + 31) / 32);
+    int shares = std::min(every, std::max(1, (two ? kCus : 2 * kCus) / token_tiles));
+    if (shares > kXcds) shares = shares / kXcds * kXcds;
+    err = hipLaunchKernel(expand, dim3(shares, token_tiles), dim3(256), args, 0, hs);
     if (err == hipSuccess)
       err = hipLaunchKernel(attend, dim3(plan.tiles * plan.splits * prm.heads), dim3(256), args, 0,
                             hs);
