@@ -56,6 +56,7 @@ struct PrefillParams {
   int32_t value;
   int32_t kdim, vdim, rdim;  // widths of the expanded rows (planes of 32)
   int32_t tiles;        // query tiles
+  int32_t paired;       // two query tiles of a head a workgroup
   int32_t splits;
   float scale_log2;
 };
@@ -72,12 +73,12 @@ struct PrefillParams {
 // it. Results are stored a block late, so that no wait for a copy waits for a
 // store. Tokens without a row are zeros from the start. The workgroups of the
 // group's first heads also gather the rotary keys and the mask of keys that have
-// a row.
-template <int TB, bool BF>
+// a row. PL: planes of 64 latent dims.
+template <int TB, int PL, bool BF>
 __global__ __launch_bounds__(256, TB == 2 ? 1 : 2) void latent_expand_kernel(const PrefillParams p) {
   constexpr int kRing = TB == 2 ? 4 : 2;
   constexpr int kPlane = 32 * 64;  // halves of 64 latent dims of a block
-  constexpr int kPlanes = kMaxLatent / 64;
+  constexpr int kPlanes = PL;
   constexpr int kChunks = 4 * kPlanes;
   constexpr int kTokens = 128 * TB;
   constexpr int kCopies = kPlanes;  // a wave's, a block
@@ -192,7 +193,6 @@ __global__ __launch_bounds__(256, TB == 2 ? 1 : 2) void latent_expand_kernel(con
   int w_lane[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) w_lane[i] = 64 * n + 8 * ((2 * i + hh) ^ swizzle(n));
-  const int steps = (p.latent + 15) / 16;
   for (int b = b0; b < b1; ++b) {
     // (Operations end in order: of the last 2 kCopies, a block's stores may be
     // among them.)
@@ -215,22 +215,16 @@ __global__ __launch_bounds__(256, TB == 2 ? 1 : 2) void latent_expand_kernel(con
     auto read = [&](int c) {
       a[c] = *reinterpret_cast<const f16x8*>(wp + (c >> 2) * kPlane + w_lane[c & 3]);
     };
-    auto products = [&](auto count) {
 #pragma unroll
-      for (int c = 0; c < kAhead; ++c) read(c);
+    for (int c = 0; c < kAhead; ++c) read(c);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+#pragma unroll
+      for (int j = 0; j < TB; ++j) acc[j] = mfma16<BF>(a[c], tok[j][c], acc[j]);
+      if (c + kAhead < kChunks) read(c + kAhead);
       __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int c = 0; c < count.value; ++c) {
-#pragma unroll
-        for (int j = 0; j < TB; ++j) acc[j] = mfma16<BF>(a[c], tok[j][c], acc[j]);
-        if (c + kAhead < count.value) read(c + kAhead);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    };
-    if (steps <= kChunks / 2)
-      products(std::integral_constant<int, kChunks / 2>{});
-    else
-      products(std::integral_constant<int, kChunks>{});
+    }
     const int part = b % each_head;
     const int left = part >= nope_blocks ? 32 : p.nope - 32 * part;  // keys' dims of the block
 #pragma unroll
@@ -257,12 +251,13 @@ __global__ __launch_bounds__(256, TB == 2 ? 1 : 2) void latent_expand_kernel(con
 // transposed in the order the scores hold the keys). Two workgroups a CU, so
 // that one's products run beside the other's weights. The query tiles of a head
 // are dispatched to one XCD, whose L2 then serves the head's keys and values.
-// NP, RP, VP: planes of 64 dims of the nope part, the rotary part and the
-// values.
-template <int NP, int RP, int VP, bool BF>
+// NP, VP: planes of 64 dims of the nope part and of the values; RS: 16-dim steps
+// of the rotary plane that are computed.
+template <int NP, int RS, int VP, bool BF>
 __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(const PrefillParams p) {
   constexpr int kPlane = kKeys * 64;  // halves of a 64-dim plane of a tile
-  constexpr int KP = NP + RP;
+  constexpr int RP = 1, KP = NP + RP;
+  constexpr int kSteps = 4 * NP + RS;  // 16-dim steps of a score
   constexpr int OB = 2 * VP;          // 32-dim blocks of the output
   __shared__ __align__(1024) f16 s_k[2][KP * kPlane];
   __shared__ __align__(1024) f16 s_v[2][VP * kPlane];
@@ -293,11 +288,11 @@ __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(const PrefillPar
   const bool q_live = qi < p.count;
   const int wfirst = p.start + wq0, wlast = p.start + min(wq0 + 31, p.count - 1);
 
-  f16x8 qf[4 * KP];
+  f16x8 qf[kSteps];
   {
     const f16* qp = p.q + ((int64_t)(q_live ? qi : 0) * p.hq + h) * (p.nope + p.rope);
 #pragma unroll
-    for (int i = 0; i < 4 * KP; ++i) {
+    for (int i = 0; i < kSteps; ++i) {
       const int d = (i < 4 * NP ? 16 * i : 16 * (i - 4 * NP)) + 8 * hh;
       const int lim = i < 4 * NP ? p.nope : p.rope;
       qf[i] = f16x8{};
@@ -384,7 +379,7 @@ __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(const PrefillPar
     const int k0 = t * kKeys;
     f32x16 s[2] = {};
 #pragma unroll
-    for (int cc = 0; cc < 4 * KP; ++cc) {
+    for (int cc = 0; cc < kSteps; ++cc) {
       const f16* kp = kt + k_lane[cc & 3] + kPlane * (cc >> 2);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -478,6 +473,434 @@ __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(const PrefillPar
     }
 }
 
+// The same attention with two blocks of 32 queries a wave (256 queries a
+// workgroup, one workgroup a CU), for rows of two nope planes, a rotary plane and
+// two value planes. A fragment read from LDS serves both blocks, which halves the
+// LDS reads that bound the kernel above, and with one wave a SIMD the weights are
+// taken beside the products by a schedule: while the scores of one 32-key block
+// are summed up and the values of another are weighed in, alternating, the weights
+// of the block between them are formed, a few instructions after each product. A
+// tile's V is used an iteration after its K. The outputs (2 x 32 x 128, 128
+// registers a lane) and the queries live in accumulator registers.
+// What takes the running maximum past 2^8 is found from the weights' sum after
+// the fact and weighed again (settle).
+template <bool BF>
+__global__ __launch_bounds__(256, 1) void latent_prefill_pipe_kernel(const PrefillParams p) {
+  constexpr int NP = 2, RP = 1, VP = 2, KP = NP + RP, OB = 2 * VP, QB = 2;
+  constexpr int kPlane = kKeys * 64;
+  constexpr int kSteps = 4 * KP;  // 16-dim steps of a score
+  constexpr int kWide = 128 * QB; // queries of a workgroup
+  __shared__ __align__(1024) f16 s_k[2][KP * kPlane];
+  __shared__ __align__(1024) f16 s_v[2][VP * kPlane];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = uniform(tid >> 6);
+  const int n = lane & 31, hh = lane >> 5;
+
+  const int units = p.paired ? (p.tiles + 1) / 2 : p.tiles;
+  const int per = units * p.splits;
+  int item = blockIdx.x, hl;
+  const int whole = p.heads / kXcds * kXcds;
+  if (item < whole * per) {
+    const int x = item % kXcds, j = item / kXcds;
+    hl = j / per * kXcds + x;
+    item = j % per;
+  } else {
+    item -= whole * per;
+    const int rest = p.heads - whole;
+    hl = whole + item % rest;
+    item /= rest;
+  }
+  const int split = item % p.splits, unit = item / p.splits;
+  const int h = p.head0 + hl;
+  // Paired: the longest query tile left and then the shortest, so that every
+  // workgroup has the same number of keys to go over.
+  const int last_tile = p.paired ? unit : p.tiles - 1 - unit;
+#pragma unroll 1
+  for (int tile = p.tiles - 1 - unit; tile >= last_tile;
+       tile = tile > last_tile ? last_tile : last_tile - 1) {
+  const int q0 = tile * kWide, q1 = min(q0 + kWide, p.count);
+  const int wq0 = q0 + 32 * QB * w, qi = wq0 + n;
+  const int qpos = p.start + qi;
+  const int wfirst = p.start + wq0, wlast = p.start + min(wq0 + 32 * QB - 1, p.count - 1);
+  const int ntile = (p.start + q1 - 1) / kKeys + 1;
+  const int t_begin = (int)((int64_t)ntile * split / p.splits);
+  const int t_end = (int)((int64_t)ntile * (split + 1) / p.splits);
+  // The tiles that this wave's queries see.
+  const int wb = uniform(wq0 < p.count ? min(t_end, wlast / kKeys + 1) : t_begin);
+
+  // Copies, as above.
+  const f16 *src_k[2], *src_r[2], *src_v[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int key = 16 * w + 8 * i + (lane >> 3);
+    const int piece = 8 * ((lane & 7) ^ swizzle(key));
+    const int64_t at = (int64_t)t_begin * kKeys + key;
+    src_k[i] = p.keys + ((int64_t)hl * p.span + at) * (64 * NP) + piece;
+    src_r[i] = p.rope_keys + at * (64 * RP) + piece;
+    src_v[i] = p.values + ((int64_t)hl * p.span + at) * (64 * VP) + piece;
+  }
+  const uint32_t k_dst = uniform(lds_address(&s_k[0][0]) + 2048 * w);
+  const uint32_t v_dst = uniform(lds_address(&s_v[0][0]) + 2048 * w);
+  // Copy i of a tile's K (two rows' parts, NP nope planes and the rotary ones
+  // each) and of its V, whose sources move on a tile at a time.
+  auto copy_k = [&](auto i, int buf) __attribute__((always_inline)) {
+    constexpr int half = i.value / KP, j = i.value % KP;
+    const uint32_t kd = k_dst + buf * (2 * KP * kPlane) + 1024 * half;
+    if constexpr (j < NP)
+      copy_to_lds<128 * j, (2 * kPlane - 128) * j>(src_k[half], kd);
+    else
+      copy_to_lds<128 * (j - NP), (2 * kPlane - 128) * (j - NP) + 2 * NP * kPlane>(src_r[half], kd);
+  };
+  auto copy_v = [&](auto i, int buf) __attribute__((always_inline)) {
+    constexpr int half = i.value / VP, j = i.value % VP;
+    copy_to_lds<128 * j, (2 * kPlane - 128) * j>(src_v[half],
+                                                 v_dst + buf * (2 * VP * kPlane) + 1024 * half);
+  };
+  auto next_k = [&]() {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      src_k[i] += kKeys * 64 * NP;
+      src_r[i] += kKeys * 64 * RP;
+    }
+  };
+  auto next_v = [&]() {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) src_v[i] += kKeys * 64 * VP;
+  };
+  auto all_k = [&](int buf) {
+    auto one = [&](auto i) { copy_k(i, buf); };
+    each(one, std::make_integer_sequence<int, 2 * KP>{});
+  };
+  auto all_v = [&](int buf) {
+    auto one = [&](auto i) { copy_v(i, buf); };
+    each(one, std::make_integer_sequence<int, 2 * VP>{});
+    next_v();
+  };
+  uint64_t ok_now = t_begin < t_end ? p.seen[t_begin] : 0;
+  if (t_begin < t_end) all_k(0);
+  if (t_begin + 1 < t_end) next_k();
+
+  f16x8 qf[QB][kSteps];
+#pragma unroll
+  for (int j = 0; j < QB; ++j) {
+    const bool live = qi + 32 * j < p.count;
+    const f16* qp = p.q + ((int64_t)(live ? qi + 32 * j : 0) * p.hq + h) * (p.nope + p.rope);
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      const int d = (i < 4 * NP ? 16 * i : 16 * (i - 4 * NP)) + 8 * hh;
+      const int lim = i < 4 * NP ? p.nope : p.rope;
+      const f16x8 x = *reinterpret_cast<const f16x8*>(qp + (d < lim ? (i < 4 * NP ? 0 : p.nope) + d : 0));
+      qf[j][i] = live && d < lim ? x : f16x8{};
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < QB; ++j)
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) asm volatile("" : "+a"(qf[j][i]));
+
+  const int g16 = lane >> 4, s16 = lane & 15;
+  const int k_place = 64 * n + 8 * (hh ^ swizzle(n));
+  const int v_row = 4 * hh + (s16 >> 2);
+  const int v_place =
+      64 * v_row + 4 * (s16 & 1) + 8 * ((2 * (g16 & 1) + ((s16 & 3) >> 1)) ^ swizzle(v_row));
+  const bool direct = p.scale_log2 > 0.0f;
+  const float c = direct ? p.scale_log2 : 1.0f;
+
+  f32x16 o[QB * OB];
+#pragma unroll
+  for (int i = 0; i < QB * OB; ++i) o[i] = f32x16{};
+  outputs_settle(o);
+  float m[QB], l[QB], lb[QB];
+#pragma unroll
+  for (int j = 0; j < QB; ++j) {
+    m[j] = -INFINITY;
+    l[j] = 0.0f;
+  }
+  f32x16 s0[QB] = {}, s1[QB] = {};        // scores of the even and the odd 32-key block
+  f16x8 p0[2 * QB] = {}, p1[2 * QB] = {};  // and their weights
+
+  auto read_k = [&](const f16* kt, int i) {
+    return *reinterpret_cast<const f16x8*>(kt + (k_place ^ 16 * (i & 3)) + kPlane * (i >> 2));
+  };
+  auto read_v = [&](const f16* vt, int i) {  // product i: dims 32 (i % OB), keys 16 (i / OB)
+    const f16* vp = vt + kPlane * (i % OB / 2) + 1024 * (i / OB);
+    const f16x4 lo = read_tr(vp + (v_place ^ 32 * (i & 1)));
+    const f16x4 hi = read_tr(vp + (v_place ^ (16 + 32 * (i & 1))) + 512);
+    return f16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  };
+  // Scores of a block in place: a scale that is not positive, and the masks
+  // where the block has any.
+  auto shape = [&](f32x16 (&x)[QB], int k0, uint32_t okm) __attribute__((always_inline)) {
+    if (!direct) {
+#pragma unroll
+      for (int j = 0; j < QB; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) x[j][v] *= p.scale_log2;
+    }
+    if (k0 + 31 <= wfirst && okm == 0xFFFFFFFFu) return;
+#pragma unroll
+    for (int j = 0; j < QB; ++j) {
+      const int hi = qpos + 32 * j - k0;  // the last visible key of the block
+      uint32_t see = hi >= 31 ? 0xFFFFFFFFu : hi < 0 ? 0u : (2u << hi) - 1u;
+      see = (see & okm) >> (4 * hh);
+#pragma unroll
+      for (int v = 0; v < 16; ++v)
+        if (!(see >> (8 * (v / 4) + v % 4) & 1)) x[j][v] = -INFINITY;
+    }
+  };
+  auto plain = [&](int k0, uint32_t okm) {
+    return direct && k0 + 31 <= wfirst && okm == 0xFFFFFFFFu;
+  };
+  auto put_pair = [&](f16x8 (&pb)[2 * QB], int j, int i, float e0, float e1) __attribute__((always_inline)) {
+    pb[2 * j + i / 4][2 * (i % 4)] = round16<BF>(e0);
+    pb[2 * j + i / 4][2 * (i % 4) + 1] = round16<BF>(e1);
+  };
+  auto total = [&](const f16x8 (&pb)[2 * QB], int j, float start) __attribute__((always_inline)) {
+    float sum[2] = {start, 0.0f};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      sum[i & 1] = add_pair<BF>(pb[2 * j + i / 4][2 * (i % 4)], pb[2 * j + i / 4][2 * (i % 4) + 1],
+                                sum[i & 1]);
+    return sum[0] + sum[1];
+  };
+  auto scores = [&](f32x16 (&x)[QB], const f16* kt) __attribute__((always_inline)) {
+    f16x8 a[kSteps];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = read_k(kt, i);
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+#pragma unroll
+      for (int j = 0; j < QB; ++j) x[j] = mfma16<BF>(a[i], qf[j][i], i == 0 ? f32x16{} : x[j]);
+      if (i + 4 < kSteps) a[i + 4] = read_k(kt, i + 4);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  auto accumulate = [&](const f16x8 (&pb)[2 * QB], const f16* vt) __attribute__((always_inline)) {
+    f16x8 a[2 * OB];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = read_v(vt, i);
+#pragma unroll
+    for (int i = 0; i < 2 * OB; ++i) {
+#pragma unroll
+      for (int j = 0; j < QB; ++j) mfma_acc<BF>(a[i], pb[2 * j + i / OB], o[j * OB + i % OB]);
+      if (i + 4 < 2 * OB) a[i + 4] = read_v(vt, i + 4);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // The weights of a block were taken against the running maximum and summed in
+  // lb. A weight past 2^8 makes lb pass it; only then, or while no key was
+  // visible (lb then is infinite), the maximum is taken and the block weighed
+  // again.
+  auto settle = [&](const f32x16 (&x)[QB], f16x8 (&pb)[2 * QB]) __attribute__((always_inline)) {
+    bool again = false;
+#pragma unroll
+    for (int j = 0; j < QB; ++j) again |= !(lb[j] <= 256.0f);
+    if (__ballot(again) != 0) {
+      bool seen = false;
+      float f[QB];
+#pragma unroll
+      for (int j = 0; j < QB; ++j) {
+        float top = x[j][0];
+#pragma unroll
+        for (int v = 1; v < 16; ++v) top = fmaxf(top, x[j][v]);
+        top = max_halves(top) * c;
+        const bool grow = top > m[j] + kSlack;
+        seen |= grow && m[j] != -INFINITY;
+        f[j] = grow ? __builtin_amdgcn_exp2f(m[j] - top) : 1.0f;
+        m[j] = grow ? top : m[j];
+        l[j] *= f[j];
+        const float mu = m[j] == -INFINITY ? 0.0f : m[j];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          put_pair(pb, j, i, __builtin_amdgcn_exp2f(fmaf(x[j][2 * i], c, -mu)),
+                   __builtin_amdgcn_exp2f(fmaf(x[j][2 * i + 1], c, -mu)));
+        lb[j] = total(pb, j, 0.0f);
+      }
+      // (Sums of a lane that has seen no key are zeros.)
+      if (__ballot(seen) != 0) {
+        outputs_settle(o);
+#pragma unroll
+        for (int i = 0; i < QB * OB; ++i) {
+#pragma unroll
+          for (int v = 0; v < 16; ++v) o[i][v] *= f[i / OB];
+          asm volatile("" : "+a"(o[i]));
+        }
+      }
+      operands_settle(pb);
+    }
+#pragma unroll
+    for (int j = 0; j < QB; ++j) l[j] += lb[j];
+  };
+  // One step: of every five fragments three are K's (scores of a later block, xn)
+  // and two V's (weights pv), each for both query blocks; beside them the
+  // weights of the block between (x, into pb, summed into lb).
+  auto step = [&](const f32x16 (&x)[QB], f16x8 (&pb)[2 * QB], const f16x8 (&pv)[2 * QB],
+                  f32x16 (&xn)[QB], const f16* kt, const f16* vt,
+                  auto beside) __attribute__((always_inline)) {
+    constexpr int kOps = kSteps + 2 * OB, kSlots = QB * kOps, kAhead = 4;
+    constexpr int kScores = 16 * QB;
+    static_assert(kSteps % 3 == 0 && 2 * kSteps == 3 * 2 * OB, "three K to two V");
+    float mu[QB], e[kScores];
+#pragma unroll
+    for (int j = 0; j < QB; ++j) {
+      mu[j] = m[j] == -INFINITY ? 0.0f : m[j];
+      lb[j] = m[j] == -INFINITY ? INFINITY : 0.0f;
+    }
+    f16x8 a[kOps];
+    auto read = [&](int i) {
+      a[i] = i % 5 & 1 ? read_v(vt, i / 5 * 2 + i % 5 / 2) : read_k(kt, i / 5 * 3 + i % 5 / 2);
+    };
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) read(i);
+    e[0] = fmaf(x[0][0], c, -mu[0]);
+    __builtin_amdgcn_sched_barrier(0);
+    auto slot = [&](auto sc) __attribute__((always_inline)) {
+      constexpr int i = sc.value / QB, j = sc.value % QB;
+      if constexpr (i % 5 & 1) {
+        constexpr int v = i / 5 * 2 + i % 5 / 2;
+        mfma_acc<BF>(a[i], pv[2 * j + v / OB], o[j * OB + v % OB]);
+      } else {
+        constexpr int k = i / 5 * 3 + i % 5 / 2;
+        xn[j] = mfma16<BF>(a[i], qf[j][k], k == 0 ? f32x16{} : xn[j]);
+      }
+      if constexpr (j == QB - 1 && i + kAhead < kOps) read(i + kAhead);
+      if constexpr (j == 0) beside(std::integral_constant<int, i>{});
+      constexpr int v0 = kScores * sc.value / (kSlots - 2);
+      constexpr int v1 = kScores * (sc.value + 1) / (kSlots - 2);
+#pragma unroll
+      for (int v = v0 < kScores ? v0 : kScores; v < (v1 < kScores ? v1 : kScores); ++v) {
+        // The argument of the next exp, this exp, the pair before.
+        if (v + 1 < kScores) e[v + 1] = fmaf(x[(v + 1) / 16][(v + 1) % 16], c, -mu[(v + 1) / 16]);
+        e[v] = __builtin_amdgcn_exp2f(e[v]);
+        if ((v & 1) && v >= 3) put_pair(pb, (v - 3) / 16, (v - 3) % 16 / 2, e[v - 3], e[v - 2]);
+      }
+      if constexpr (sc.value == kSlots - 2)
+        put_pair(pb, QB - 1, 7, e[kScores - 2], e[kScores - 1]);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    each(slot, std::make_integer_sequence<int, kSlots>{});
+#pragma unroll
+    for (int j = 0; j < QB; ++j) lb[j] = total(pb, j, lb[j]);
+    // Keeps the step's products in it (they would sink past settle's branch).
+#pragma unroll
+    for (int j = 0; j < QB; ++j)
+      asm volatile("" : "+v"(xn[j]), "+v"(pb[2 * j]), "+v"(pb[2 * j + 1]), "+v"(lb[j]));
+  };
+  // Iteration t: V of tile t and K of the next (of the last one again) are copied
+  // beside the wave's math, and published by the barrier at its end. (The phases in a row, each
+  // with a loop of its own: where paths met in one loop the outputs were copied.
+  // In the steps a copy goes out every other fragment: issued together they
+  // waited for each other, 600 of 4900 cycles a tile.)
+  uint64_t ok_prev = 0;
+  auto open = [&](int t) {
+    const int buf = (t - t_begin) & 1;
+    all_v(buf);
+    all_k(buf ^ 1);
+    if (t + 2 < t_end) next_k();
+  };
+  auto close = [&](int t) {
+    ok_prev = ok_now;
+    if (t + 1 < t_end) ok_now = p.seen[t + 1];
+    wait_vmem<0>();
+    __syncthreads();
+  };
+  wait_vmem<0>();
+  __syncthreads();
+  int t = t_begin;
+  if (t < wb) {
+    // First tile: scores of both blocks, weights of the first.
+    open(t);
+    scores(s0, s_k[0]);
+    shape(s0, t * kKeys, (uint32_t)ok_now);
+    scores(s1, s_k[0] + 2048);
+#pragma unroll
+    for (int j = 0; j < QB; ++j) lb[j] = INFINITY;
+    settle(s0, p0);
+    close(t);
+    for (++t; t < wb; ++t) {
+      const int buf = (t - t_begin) & 1;
+      const int k0 = t * kKeys;
+      const f16* kt = s_k[buf];
+      const f16* vt = s_v[buf ^ 1];
+      const uint32_t odd = (uint32_t)(ok_prev >> 32), even = (uint32_t)ok_now;
+      if (!plain(k0 - 32, odd)) shape(s1, k0 - 32, odd);
+      step(s1, p1, p0, s0, kt, vt, [&](auto i) __attribute__((always_inline)) {
+        if constexpr (i.value % 2 == 0) {
+          constexpr int c = i.value / 2;
+          if constexpr (c < 2 * VP) {
+            copy_v(std::integral_constant<int, c>{}, buf);
+          } else if constexpr (c < 2 * VP + 2 * KP) {
+            copy_k(std::integral_constant<int, c - 2 * VP>{}, buf ^ 1);
+          }
+        }
+      });
+      next_v();
+      if (t + 2 < t_end) next_k();
+      settle(s1, p1);
+      if (!plain(k0, even)) shape(s0, k0, even);
+      step(s0, p0, p1, s1, kt + 2048, vt + 2048, [](auto) {});
+      settle(s0, p0);
+      close(t);
+    }
+    // The products of the wave's last tile.
+    if (t < t_end) open(t);
+    const f16* vt = s_v[(t - 1 - t_begin) & 1];
+    shape(s1, (t - 1) * kKeys + 32, (uint32_t)(ok_prev >> 32));
+    accumulate(p0, vt);
+#pragma unroll
+    for (int j = 0; j < QB; ++j) lb[j] = INFINITY;
+    settle(s1, p1);
+    accumulate(p1, vt + 2048);
+    outputs_settle(o);
+    if (t < t_end) {
+      close(t);
+      ++t;
+    }
+  }
+  for (; t < t_end; ++t) {
+    open(t);
+    close(t);
+  }
+#pragma unroll
+  for (int j = 0; j < QB; ++j) {
+    if (qi + 32 * j >= p.count) continue;
+    const float all = l[j] + __shfl_xor(l[j], 32);
+    const int64_t at = (int64_t)(qi + 32 * j) * p.hq + h;
+    if (p.splits > 1) {
+      const int64_t pair = (int64_t)split * p.count * p.hq + at;
+      float* dst = p.part_o + pair * p.value + 4 * hh;
+#pragma unroll
+      for (int b = 0; b < OB; ++b) {
+        const f32x16& x = o[j * OB + b];
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          if (32 * b + 8 * g < p.value)
+            *reinterpret_cast<float4*>(dst + 32 * b + 8 * g) =
+                make_float4(x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]);
+      }
+      if (hh == 0) p.part_ml[pair] = make_float2(m[j], all);
+      continue;
+    }
+    const float inv = all > 0.0f ? 1.0f / all : 0.0f;
+    f16* dst = p.out + at * p.value + 4 * hh;
+#pragma unroll
+    for (int b = 0; b < OB; ++b) {
+      const f32x16& x = o[j * OB + b];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        if (32 * b + 8 * g >= p.value) continue;
+        f16x4 y;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) y[v] = round16<BF>(x[4 * g + v] * inv);
+        *reinterpret_cast<f16x4*>(dst + 32 * b + 8 * g) = y;
+      }
+    }
+  }
+  __syncthreads();  // (the tiles' LDS is the next one's)
+  }
+}
+
 // Joins the key ranges of a split call: a thread has 4 value dims of one query
 // and head.
 template <bool BF>
@@ -518,9 +941,17 @@ size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 constexpr size_t kExpandBytes = (size_t)1 << 30;  // expanded keys and values at once
 constexpr int kSlots = 512;                       // workgroups resident on an MI355X
+// Two query blocks a wave from whole workgroups of queries and as many keys on
+// that their longer start is paid for (us a call, one block / two: 16 heads of
+// 128 + 64, 512 tokens at 0 36 / 44, 256 at 7777 103 / 106, 512 at 30000 360 /
+// 343; 128 heads, 512 at 0 62 / 64, 1024 at 0 130 / 118, 4096 at 0 910 / 843).
+constexpr int kPipeQueries = 256;
+constexpr int kPipeKeys = 1024;
 
 struct PrefillPlan {
   bool small;   // planes of 64 + 64 and 64 dims, else 128 + 64 and 128
+  bool pipe;    // two query blocks a wave
+  bool paired;  // two query tiles a workgroup
   int kdim, vdim, rdim;
   int span, tiles, splits, heads;  // heads per group
   size_t keys, values, rope, seen, part_o, part_ml, bytes;
@@ -533,7 +964,9 @@ PrefillPlan plan_for(int start, int count, int q_heads, int rope, int nope, int 
   r.vdim = r.kdim;
   r.rdim = 64;
   r.span = (start + count + kKeys - 1) / kKeys * kKeys;
-  r.tiles = (count + kQueries - 1) / kQueries;
+  r.pipe = !r.small && count >= kPipeQueries && start + count >= kPipeKeys;
+  const int queries = r.pipe ? 2 * kQueries : kQueries;
+  r.tiles = (count + queries - 1) / queries;
   const size_t head_bytes = (size_t)r.span * (r.kdim + r.vdim) * 2;
   // Heads in groups whose expanded rows fit the bound, whole rounds of XCDs
   // where that many do.
@@ -544,7 +977,9 @@ PrefillPlan plan_for(int start, int count, int q_heads, int rope, int nope, int 
   // of keys at least.
   const int64_t items = (int64_t)r.tiles * r.heads;
   const int64_t most = std::min<int64_t>(kMaxSplits, std::max(1, r.span / kKeys / 4));
-  r.splits = (int)std::max<int64_t>(1, std::min(most, kSlots / items));
+  r.splits = (int)std::max<int64_t>(1, std::min(most, (r.pipe ? kCus : kSlots) / items));
+  // Paired tiles level the causal work where workgroups come in several rounds.
+  r.paired = r.pipe && r.splits == 1 && items >= 2 * kCus;
   size_t at = 0;
   r.keys = at;
   at = up256(at + (size_t)r.heads * r.span * r.kdim * 2);
@@ -574,9 +1009,19 @@ int check_prefill(int32_t start, int32_t count, int32_t q_heads, int32_t latent_
 }
 
 template <bool BF>
-const void* prefill_kernel(bool small) {
-  return small ? (const void*)latent_prefill_kernel<1, 1, 1, BF>
-               : (const void*)latent_prefill_kernel<2, 1, 2, BF>;
+const void* expand_kernel(bool two, int latent) {
+  if (latent <= 256)
+    return two ? (const void*)latent_expand_kernel<2, 4, BF>
+               : (const void*)latent_expand_kernel<1, 4, BF>;
+  return two ? (const void*)latent_expand_kernel<2, 8, BF>
+             : (const void*)latent_expand_kernel<1, 8, BF>;
+}
+
+template <bool BF>
+const void* prefill_kernel(bool small, int rope) {
+  if (!small) return (const void*)latent_prefill_kernel<2, 4, 2, BF>;
+  return rope <= 32 ? (const void*)latent_prefill_kernel<1, 2, 1, BF>
+                    : (const void*)latent_prefill_kernel<1, 4, 1, BF>;
 }
 
 int latent_prefill(const void* queries, const void* arena, const void* kv_b, const int32_t* table,
@@ -640,6 +1085,7 @@ int latent_prefill(const void* queries, const void* arena, const void* kv_b, con
   prm.vdim = plan.vdim;
   prm.rdim = plan.rdim;
   prm.tiles = plan.tiles;
+  prm.paired = plan.paired;
   prm.splits = plan.splits;
   prm.scale_log2 = scale * kLog2e;
   void* args[] = {&prm};
@@ -648,13 +1094,14 @@ int latent_prefill(const void* queries, const void* arena, const void* kv_b, con
   // each), one where it would not (two workgroups each).
   const int64_t wide = ((int64_t)plan.span + 255) / 256 * plan.heads;
   const bool two = wide >= kCus;
-  const void* expand = two ? (bf ? (const void*)latent_expand_kernel<2, true>
-                                 : (const void*)latent_expand_kernel<2, false>)
-                           : (bf ? (const void*)latent_expand_kernel<1, true>
-                                 : (const void*)latent_expand_kernel<1, false>);
+  const void* expand = bf ? expand_kernel<true>(two, latent_dim) : expand_kernel<false>(two, latent_dim);
   const int tokens = two ? 256 : 128;
   const int token_tiles = (plan.span + tokens - 1) / tokens;
-  const void* attend = bf ? prefill_kernel<true>(plan.small) : prefill_kernel<false>(plan.small);
+  const void* attend =
+      plan.pipe ? (bf ? (const void*)latent_prefill_pipe_kernel<true>
+                      : (const void*)latent_prefill_pipe_kernel<false>)
+                : (bf ? prefill_kernel<true>(plan.small, rope_dim)
+                      : prefill_kernel<false>(plan.small, rope_dim));
   hipError_t err = hipSuccess;
   for (int h0 = 0; h0 < q_heads && err == hipSuccess; h0 += plan.heads) {
     prm.head0 = h0;
@@ -665,8 +1112,10 @@ int latent_prefill(const void* queries, const void* arena, const void* kv_b, con
     if (shares > kXcds) shares = shares / kXcds * kXcds;
     err = hipLaunchKernel(expand, dim3(shares, token_tiles), dim3(256), args, 0, hs);
     if (err == hipSuccess)
-      err = hipLaunchKernel(attend, dim3(plan.tiles * plan.splits * prm.heads), dim3(256), args, 0,
-                            hs);
+      err = hipLaunchKernel(
+          attend,
+          dim3((plan.paired ? (plan.tiles + 1) / 2 : plan.tiles) * plan.splits * prm.heads),
+          dim3(256), args, 0, hs);
   }
   if (err == hipSuccess && plan.splits > 1)
     err = hipLaunchKernel(

@@ -147,13 +147,16 @@ def prefill(q, arena, kv_b, table, *, start, page_size, scale):
         a = abs(scale) * (qh[:, :nope].abs() @ key.abs().t())
         b = abs(scale) * (qh[:, :nope].abs() @ key_terms.t()) * step
         o = p @ v
-        for i in range(count):
-            off = (v - o[i]).abs()
-            spread = (p[i] * (1 + a[i])) @ off
-            bound[i, h] = (1.1 * u * (o[i].abs() + spread + p[i] @ v.abs())
-                           + 1.1 * ((p[i] * b[i]) @ off) + step * (p[i] @ v_terms)
-                           + (end / 16 + 64) * 2.0 ** -24 * (p[i] @ v.abs())
-                           + tiny * (1 + (off * (~hidden[i])[:, None]).sum(0))
-                           + 2e-5 * (o[i].abs() + spread))
+        part = max(1, (1 << 24) // (end * (width - nope)))
+        for i in range(0, count, part):
+            z = slice(i, min(i + part, count))
+            off = (v[None] - o[z, None]).abs()  # [queries, keys, value]
+            weigh = lambda x, off=off: torch.matmul(x[:, None], off)[:, 0]  # noqa: E731
+            spread = weigh(p[z] * (1 + a[z]))
+            bound[z, h] = (1.1 * u * (o[z].abs() + spread + p[z] @ v.abs())
+                           + 1.1 * weigh(p[z] * b[z]) + step * (p[z] @ v_terms)
+                           + (end / 16 + 64) * 2.0 ** -24 * (p[z] @ v.abs())
+                           + tiny * (1 + weigh((~hidden[z]).double()))
+                           + 2e-5 * (o[z].abs() + spread))
         out[:, h] = o
     return out, bound

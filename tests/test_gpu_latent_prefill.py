@@ -57,6 +57,43 @@ def test_split_key_ranges(gpu):
     check(gpu, WIDE, 1, 1500, 20, dtype=torch.float16)
 
 
+# The kernel of two query blocks a wave: wide heads, 256 queries and 1024 keys at
+# least.
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape, heads, start, count", [
+    (WIDE, 2, 0, 1100), (WIDE, 1, 767, 257), (UNEVEN, 9, 801, 256), ((512, 0, 72, 128), 2, 300, 800)])
+def test_two_blocks(gpu, shape, heads, start, count, dtype):
+    check(gpu, shape, heads, start, count, dtype=dtype)
+
+
+def test_two_blocks_split(gpu):
+    """Key ranges that no query of a wave sees, and ones that some do."""
+    check(gpu, WIDE, 1, 4000, 300, dtype=torch.float16)
+
+
+@pytest.mark.parametrize("count", [1030, 1300])
+def test_two_blocks_paired(gpu, count):
+    """Two query tiles a workgroup, an odd number of tiles and an even one."""
+    check(gpu, (8, 16, 72, 8), 130, 0, count, page=64)
+
+
+def test_two_blocks_masked(gpu):
+    def change(arena, table):
+        arena[:16] = float("inf")  # page 0, that -1 must not lead to
+        table[table == 0] = -1
+        table[0], table[1], table[30], table[40] = -1, 1 << 20, -9, 1 << 30
+        table[-2] = -1
+
+    got = check(gpu, (64, 16, 96, 40), 2, 0, 1100, change=change)
+    assert bool((got[:32] == 0).all())
+
+
+@pytest.mark.parametrize("scale", [-0.05, 0.6])
+def test_two_blocks_scales(gpu, scale):
+    """A negative scale, and scores that move the running maximum."""
+    check(gpu, (256, 32, 128, 72), 2, 500, 530, scale=scale, dtype=torch.float16)
+
+
 def test_head_groups(gpu):
     """More heads than fit the bound on expanded rows: groups of heads in turn."""
     from instinct_amd import _lib

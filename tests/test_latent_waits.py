@@ -10,7 +10,8 @@ from test_mfma_waits import OBJDUMP, faults, parse
 
 from instinct_amd import _lib
 
-KERNELS = {"latent_decode_kernel": 12}  # two widths, 1, 2 or 4 waves over heads, two types
+# Two widths, 1, 2 or 4 waves over heads, two types; two types.
+KERNELS = {"latent_decode_kernel": 12, "latent_prefill_pipe_kernel": 2}
 
 
 @pytest.mark.skipif(OBJDUMP is None, reason="no llvm-objdump")
@@ -21,7 +22,8 @@ def test_built_kernels(tmp_path):
                    stdout=subprocess.DEVNULL)
     seen = dict.fromkeys(KERNELS, 0)
     for image in sorted(tmp_path.glob("*gfx950*")):
-        if b"latent_decode_kernel" not in image.read_bytes():
+        code = image.read_bytes()
+        if not any(kernel.encode() in code for kernel in KERNELS):
             continue
         text = subprocess.run([OBJDUMP, "-d", image.name], cwd=tmp_path, check=True,
                               capture_output=True, text=True).stdout
