@@ -485,7 +485,7 @@ __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(const PrefillPar
 // What takes the running maximum past 2^8 is found from the weights' sum after
 // the fact and weighed again (settle).
 template <bool BF>
-__global__ __launch_bounds__(256, 1) void latent_prefill_pipe_kernel(const PrefillParams p) {
+__global__ __launch_bounds__(256, 1) void latent_prefill_wide_kernel(const PrefillParams p) {
   constexpr int NP = 2, RP = 1, VP = 2, KP = NP + RP, OB = 2 * VP, QB = 2;
   constexpr int kPlane = kKeys * 64;
   constexpr int kSteps = 4 * KP;  // 16-dim steps of a score
@@ -1098,8 +1098,8 @@ int latent_prefill(const void* queries, const void* arena, const void* kv_b, con
   const int tokens = two ? 256 : 128;
   const int token_tiles = (plan.span + tokens - 1) / tokens;
   const void* attend =
-      plan.pipe ? (bf ? (const void*)latent_prefill_pipe_kernel<true>
-                      : (const void*)latent_prefill_pipe_kernel<false>)
+      plan.pipe ? (bf ? (const void*)latent_prefill_wide_kernel<true>
+                      : (const void*)latent_prefill_wide_kernel<false>)
                 : (bf ? prefill_kernel<true>(plan.small, rope_dim)
                       : prefill_kernel<false>(plan.small, rope_dim));
   hipError_t err = hipSuccess;

@@ -11,7 +11,7 @@ from test_mfma_waits import OBJDUMP, faults, parse
 from instinct_amd import _lib
 
 # Two widths, 1, 2 or 4 waves over heads, two types; two types.
-KERNELS = {"latent_decode_kernel": 12, "latent_prefill_pipe_kernel": 2}
+KERNELS = {"latent_decode_kernel": 12, "latent_prefill_wide_kernel": 2}
 
 
 @pytest.mark.skipif(OBJDUMP is None, reason="no llvm-objdump")
