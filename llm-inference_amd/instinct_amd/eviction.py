@@ -20,7 +20,7 @@ from typing import Any
 import torch
 
 from . import _lib
-from .hip_kernels import _arena_geometry, _given_workspace, stream_workspace
+from .hip_kernels import _arena_geometry, _given_workspace, on_device, stream_workspace
 
 
 def _check_index(name: str, t: torch.Tensor, shape: tuple, device: torch.device) -> torch.Tensor:
@@ -109,7 +109,7 @@ def paged_attention_weights(queries: torch.Tensor, keys: torch.Tensor, tables: t
           else _given_workspace(workspace, device, need))
     entry = ("pda_attention_weights" + ("_q8" if q8 else "")
              + ("_bf16" if queries.dtype == torch.bfloat16 else ""))
-    with torch.cuda.device(device):
+    with on_device(device):
         rc = getattr(_lib.library(), entry)(
             queries.data_ptr(), keys.data_ptr(), *((scales[0].data_ptr(),) if q8 else ()),
             tables.data_ptr(), lengths.data_ptr(), weights.data_ptr(), out.data_ptr(), batch,
@@ -178,7 +178,7 @@ def evict_rows(keys: torch.Tensor, values: torch.Tensor | None, weights: torch.T
     lib = _lib.library()
     stride = int(tables.shape[1])
     stream = int(torch.cuda.current_stream(device).cuda_stream)
-    with torch.cuda.device(device):
+    with on_device(device):
         _lib.check(lib.pda_evict_select(
             weights.data_ptr(), out_weights.data_ptr(), tables.data_ptr(), lengths.data_ptr(),
             kept.data_ptr(), new_lengths.data_ptr(), batch, kv_heads, int(page_size), stride,

@@ -26,6 +26,7 @@ the split workspace, and passes device pointers and the current stream.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from collections import OrderedDict
@@ -41,6 +42,17 @@ from . import _lib
 # streams keep one; the least recently used one is dropped past that.
 _workspaces: "OrderedDict[tuple[int, int], torch.Tensor]" = OrderedDict()
 _WORKSPACE_STREAMS = 4
+
+
+_CURRENT = contextlib.nullcontext()
+
+
+def on_device(device: torch.device) -> Any:
+    """A context in which ``device`` is the current one: nothing to enter or
+    leave where it is already (a switch there and back costs a call 2 us)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _CURRENT
+    return torch.cuda.device(device)
 
 
 def new_workspace(nbytes: int, device: torch.device) -> torch.Tensor:

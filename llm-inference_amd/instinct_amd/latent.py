@@ -26,7 +26,8 @@ from typing import Any
 import torch
 
 from . import _lib
-from .hip_kernels import _given_workspace, _int32_vector, rope_inv_freq, stream_workspace
+from .hip_kernels import (_given_workspace, _int32_vector, on_device, rope_inv_freq,
+                          stream_workspace)
 
 
 def _check_16bit(name: str, t: torch.Tensor, dims: int, like: torch.Tensor,
@@ -119,7 +120,7 @@ def latent_append(q: torch.Tensor | None, latent: torch.Tensor, k_rope: torch.Te
     # (One row has no distance to a next one, whatever its stride says.)
     stride = lambda t, w: w if n == 1 else t.stride(0)  # noqa: E731
     entry = "pda_latent_append" + ("_bf16" if arena.dtype == torch.bfloat16 else "")
-    with torch.cuda.device(arena.device):
+    with on_device(arena.device):
         rc = getattr(_lib.library(), entry)(
             ptr(q), ptr(q_out), ptr(latent), stride(latent, width), ptr(k_rope) if rope else None,
             stride(k_rope, rope), ptr(norm_weight), float(eps), ptr(arena),
@@ -184,7 +185,7 @@ def latent_decode_attention(queries: torch.Tensor, arena: torch.Tensor, kv_b: to
     ws = (stream_workspace(device, need, stream) if workspace is None
           else _given_workspace(workspace, device, need))
     entry = "pda_latent_decode_attention" + ("_bf16" if queries.dtype == torch.bfloat16 else "")
-    with torch.cuda.device(device):
+    with on_device(device):
         rc = getattr(_lib.library(), entry)(
             queries.data_ptr(), arena.data_ptr(), kv_b.data_ptr(), tables.data_ptr(),
             lengths.data_ptr(), out.data_ptr(), batch, q_heads, latent, rope, nope, value,
@@ -240,7 +241,7 @@ def latent_prefill_attention(queries: torch.Tensor, arena: torch.Tensor, kv_b: t
     ws = (stream_workspace(device, need, stream) if workspace is None
           else _given_workspace(workspace, device, need))
     entry = "pda_latent_prefill_attention" + ("_bf16" if queries.dtype == torch.bfloat16 else "")
-    with torch.cuda.device(device):
+    with on_device(device):
         rc = getattr(_lib.library(), entry)(
             queries.data_ptr(), arena.data_ptr(), kv_b.data_ptr(), table.data_ptr(),
             int(table.shape[0]), int(start), count, out.data_ptr(), q_heads, latent, rope, nope,
