@@ -66,7 +66,7 @@ struct WeightParams {
   const int32_t* lengths;
   const float* weights;  // [batch, hkv, capacity]
   float* out;
-  float* probs;        // [batch, hq, pitch] weights relative to their chunk's max
+  float* scores;       // [batch, hq, pitch] times log2 e
   float2* stats;       // [batch, hq, chunks] (max, sum) of each chunk
   int64_t arena_pages;
   int64_t page_elems, scale_page;  // elements between pages,
@@ -139,20 +139,29 @@ __device__ __forceinline__ f32x4 mfma(const f16x8& a, const f16x8& b, const f32x
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// Scores of a chunk of keys against up to 16 heads of one kv head, as weights
-// relative to the chunk's largest, with each head's largest and sum. K is read
-// once, straight into the matrix cores' operands (lane: key lane % 16, 8 dims),
-// 64 bytes of a row per instruction; a lane ends with 4 consecutive keys of one
-// head per block. A workgroup goes over its chunks with the next one's rows, and
-// the page numbers of the one after that, under way. Reads K and writes 4 bytes a
-// head and key: the K bytes bound it.
+// (largest, sum relative to it) of two sets of scores together.
+__device__ __forceinline__ float2 join(const float2& a, const float2& b) {
+  const float m = fmaxf(a.x, b.x), mu = m == -INFINITY ? 0.0f : m;
+  return make_float2(m, a.y * __builtin_amdgcn_exp2f(a.x - mu) +
+                            b.y * __builtin_amdgcn_exp2f(b.x - mu));
+}
+
+// Scores (times log2 e) of a sequence's keys against up to 16 heads of one kv
+// head, with each head's largest and sum of exp2(score - largest) per chunk of
+// keys. K is read once, straight into the matrix cores' operands (lane: key
+// lane % 16, 8 dims), 64 bytes of a row per instruction; a lane ends with 4
+// consecutive keys of one head per block. The scores are stored as they are, so
+// the waves of a chunk meet only for its statistics. A workgroup goes over its
+// chunks with the next one's rows, and the page numbers of the one after that,
+// under way. Reads K and writes 4 bytes a head and key: the K bytes bound it
+// (at the shape below 316 MB in 75 us, 4.2 TB/s).
 template <int NC, bool Q8, bool BF, bool VEC>
 __global__ __launch_bounds__(64 * kWaves, NC == 16 && !Q8 ? 1 : 2) void attention_scores_kernel(const WeightParams p) {
   typedef std::conditional_t<Q8, signed char, f16> Elem;
   typedef std::conditional_t<Q8, u32x2, f16x8> Elem8;
   constexpr int kBlocks = blocks_for(NC);
   constexpr int kChunk = chunk_for(NC);
-  __shared__ float s_max[2][kWaves][kSlots], s_sum[2][kWaves][kSlots];
+  __shared__ float2 s_stats[2][kWaves][kSlots];
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
   const int n16 = lane & 15, g4 = lane >> 4;
   const int group = p.hq / p.hkv, tiles = (group + kSlots - 1) / kSlots;
@@ -216,6 +225,7 @@ __global__ __launch_bounds__(64 * kWaves, NC == 16 && !Q8 ? 1 : 2) void attentio
                                      (int64_t)row * p.scale_row];
     }
   };
+  float* dst = p.scores + ((int64_t)b * p.hq + h) * p.pitch;
   auto weigh = [&](int chunk, const Keys& x, int buf) {
     f32x4 s[kBlocks];
 #pragma unroll
@@ -245,50 +255,38 @@ __global__ __launch_bounds__(64 * kWaves, NC == 16 && !Q8 ? 1 : 2) void attentio
         for (int v = 0; v < 4; ++v) s[i][v] *= p.scale_log2;
     }
     // Key 4 g4 + v of a block was looked up by lane 4 g4 + v.
-    float top = -INFINITY;
+    float2 all = make_float2(-INFINITY, 0.0f);
 #pragma unroll
     for (int i = 0; i < kBlocks; ++i) {
       const uint32_t have = (uint32_t)__ballot(x.seen >> i & 1) >> (4 * g4);
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         if (!(have >> v & 1)) s[i][v] = -INFINITY;
-        top = fmaxf(top, s[i][v]);
+        all.x = fmaxf(all.x, s[i][v]);
       }
     }
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
-    if (g4 == 0) s_max[buf][w][n16] = top;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) top = fmaxf(top, s_max[buf][i][n16]);
-    const float mu = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kBlocks; ++i) {
-#pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        s[i][v] = __builtin_amdgcn_exp2f(s[i][v] - mu);
-        sum += s[i][v];
-      }
-    }
-    sum += __shfl_xor(sum, 16);
-    sum += __shfl_xor(sum, 32);
-    if (g4 == 0) s_sum[buf][w][n16] = sum;
-    const int64_t row = (int64_t)b * p.hq + h;
     if (live) {
-      float* dst = p.probs + row * p.pitch;
 #pragma unroll
       for (int i = 0; i < kBlocks; ++i) {
-        const int64_t key = chunk * (int64_t)kChunk + w * (16 * kBlocks) + 16 * i + 4 * g4;
+        const int64_t key = key_at(chunk, i) - n16 + 4 * g4;
         if (key < keys) *reinterpret_cast<f32x4*>(dst + key) = s[i];
       }
     }
+    const float mu = all.x == -INFINITY ? 0.0f : all.x;
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) all.y += __builtin_amdgcn_exp2f(s[i][v] - mu);
+    // The lanes', then the waves' statistics of a head. (Two buffers: a chunk's are
+    // read before the next one's barrier.)
+    all = join(all, make_float2(__shfl_xor(all.x, 16), __shfl_xor(all.y, 16)));
+    all = join(all, make_float2(__shfl_xor(all.x, 32), __shfl_xor(all.y, 32)));
+    if (g4 == 0) s_stats[buf][w][n16] = all;
     __syncthreads();
     if (live && w == 0 && g4 == 0) {
-      float all = 0.0f;
 #pragma unroll
-      for (int i = 0; i < kWaves; ++i) all += s_sum[buf][i][n16];
-      p.stats[row * p.chunks + chunk] = make_float2(top, all);
+      for (int i = 1; i < kWaves; ++i) all = join(all, s_stats[buf][i][n16]);
+      p.stats[((int64_t)b * p.hq + h) * p.chunks + chunk] = all;
     }
   };
   Rows rows;
@@ -297,7 +295,6 @@ __global__ __launch_bounds__(64 * kWaves, NC == 16 && !Q8 ? 1 : 2) void attentio
   fetch(c_first, rows, even);
   if (c_first + stride < c_end) look_up(c_first + stride, rows);
   for (int c = c_first;; c += 2 * stride) {
-    // (Both statistics buffers: a chunk's are read past its second barrier.)
     Rows next;
     if (c + 2 * stride < c_end) look_up(c + 2 * stride, next);
     if (c + stride < c_end) fetch(c + stride, rows, odd);
@@ -311,20 +308,19 @@ __global__ __launch_bounds__(64 * kWaves, NC == 16 && !Q8 ? 1 : 2) void attentio
 }
 
 // out[t] = weights[t] (0 for the `fresh` newest) + the sum over the kv head's
-// query heads, in their order, of the normalised weights: the chunks' maxima and
-// sums give each head's, once a workgroup, while the weights themselves are
-// already under way. Reads 4 bytes a head and key, from the caches that the
+// query heads, in their order, of exp2(score - the head's largest) / its sum, the
+// two joined from the chunks' once a workgroup, while the scores themselves
+// are already under way. Reads 4 bytes a head and key, from the caches that the
 // launch before left them in.
 __global__ __launch_bounds__(256) void attention_weights_kernel(const WeightParams p) {
   constexpr int kHeads = 8;  // heads at once: two a wave for the statistics
-  constexpr int kMaxParts = kAddKeys / chunk_for(16), kEach = kAddKeys / 256;
-  __shared__ float s_f[kHeads][kMaxParts];
+  constexpr int kEach = kAddKeys / 256;
+  __shared__ float2 s_stats[kHeads];
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
   const int group = p.hq / p.hkv, kvh = blockIdx.y, b = blockIdx.z;
   const int keys = keys_of(p, b);
   const int lo = p.window > 0 ? max(0, keys - p.window) : 0;
-  const int chunk = p.chunk, parts = kAddKeys / chunk;
-  const int c_lo = lo / chunk, c_hi = (keys + chunk - 1) / chunk;
+  const int c_lo = lo / p.chunk, c_hi = (keys + p.chunk - 1) / p.chunk;
   const int64_t base = ((int64_t)b * p.hkv + kvh) * p.capacity;
   for (int64_t k0 = (int64_t)blockIdx.x * kAddKeys; k0 < keys; k0 += (int64_t)gridDim.x * kAddKeys) {
     float acc[kEach] = {}, old[kEach];
@@ -342,55 +338,37 @@ __global__ __launch_bounds__(256) void attention_weights_kernel(const WeightPara
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
           const int64_t t = k0 + 256 * i + tid;
-          x[j][i] = 0.0f;
-          if (j < heads && t >= (int64_t)c_lo * chunk && t < keys)
-            x[j][i] = p.probs[(row + j) * p.pitch + t];
+          x[j][i] = -INFINITY;
+          if (j < heads && t >= lo && t < keys) x[j][i] = p.scores[(row + j) * p.pitch + t];
         }
       __syncthreads();
       for (int i = w; i < heads; i += 4) {
         const float2* st = p.stats + (row + i) * p.chunks;
-        const int mine = (int)(k0 / chunk) + lane;
-        const bool part = lane < parts && mine >= c_lo && mine < c_hi;
-        const float m = part ? st[mine].x : -INFINITY;
-        float top = -INFINITY, sum = 0.0f;
-        for (int c = c_lo + lane; c < c_hi; c += 64) {
-          const float2 y = st[c];
-          if (y.x == -INFINITY) {
-            sum += y.y;  // (0, or NaN where all scores were)
-            continue;
-          }
-          if (y.x > top) {
-            sum *= top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - y.x);
-            top = y.x;
-          }
-          sum = fmaf(y.y, __builtin_amdgcn_exp2f(y.x - top), sum);
-        }
+        float2 all = make_float2(-INFINITY, 0.0f);
+        for (int c = c_lo + lane; c < c_hi; c += 64) all = join(all, st[c]);
 #pragma unroll
-        for (int d = 32; d; d >>= 1) {
-          const float t2 = __shfl_xor(top, d), s2 = __shfl_xor(sum, d);
-          const float both = fmaxf(top, t2);
-          if (both != -INFINITY)
-            sum = sum * __builtin_amdgcn_exp2f(top - both) + s2 * __builtin_amdgcn_exp2f(t2 - both);
-          else
-            sum += s2;
-          top = both;
-        }
-        if (lane < parts)
-          s_f[i][lane] = sum != sum ? sum : m != -INFINITY ? __builtin_amdgcn_exp2f(m - top) / sum : 0.0f;
+        for (int d = 32; d; d >>= 1)
+          all = join(all, make_float2(__shfl_xor(all.x, d), __shfl_xor(all.y, d)));
+        // (A head that sees no key gives nothing; its sum is 0, or NaN.)
+        if (lane == 0)
+          s_stats[i] = make_float2(all.x == -INFINITY ? 0.0f : all.x,
+                                   all.y == 0.0f ? 0.0f : 1.0f / all.y);
       }
       __syncthreads();
 #pragma unroll
-      for (int j = 0; j < kHeads; ++j)
+      for (int j = 0; j < kHeads; ++j) {
+        if (j >= heads) break;
+        const float2 st = s_stats[j];
 #pragma unroll
         for (int i = 0; i < kEach; ++i)
-          if (j < heads) acc[i] = fmaf(x[j][i], s_f[j][(256 * i + tid) / chunk], acc[i]);
+          acc[i] = fmaf(__builtin_amdgcn_exp2f(x[j][i] - st.x), st.y, acc[i]);
+      }
     }
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       const int64_t t = k0 + 256 * i + tid;
       if (t < keys) p.out[base + t] = old[i] + acc[i];
     }
-    __syncthreads();
   }
 }
 
@@ -488,7 +466,7 @@ int attention_weights(const void* queries, const void* keys, const void* key_sca
   prm.chunk = chunk_for(planes_run(head_dim));
   prm.chunks = (capacity + prm.chunk - 1) / prm.chunk;
   prm.stats = static_cast<float2*>(workspace);
-  prm.probs = reinterpret_cast<float*>(static_cast<char*>(workspace) +
+  prm.scores = reinterpret_cast<float*>(static_cast<char*>(workspace) +
                                        stats_bytes(batch, q_heads, capacity));
   prm.arena_pages = arena_rows / page_size;
   const bool rows = layout == PDA_LAYOUT_ROWS;
@@ -511,15 +489,20 @@ int attention_weights(const void* queries, const void* keys, const void* key_sca
   prm.cap_out = softcap * kLog2e;
   // The grid covers `longest` keys (workgroups go on to later ones if there
   // are): a workgroup a chunk while the GPU holds them all at once, else up to
-  // four chunks each, whose loads then overlap.
+  // four chunks each, whose loads then overlap. An odd number per sequence:
+  // workgroups go to the 8 XCDs in turn, and with 8 a sequence the first XCD has
+  // a share of every sequence and the last only of the longest (64 sequences of
+  // 512 to 8192 keys, 28 over 4 heads of 128 dims: scores 81 us with 8 and 82
+  // with 16, 75 with 9 and 73 with 17).
   const int64_t span = std::max<int64_t>(1, std::min<int64_t>(longest, capacity));
   const int64_t seen =
       window > 0 ? std::min<int64_t>(span, (int64_t)window + prm.chunk) : span;
   const int64_t chunks = (seen + prm.chunk - 1) / prm.chunk;
   const int64_t one = std::max<int64_t>(1, kScoreGroups / (grid_y * batch));
   const unsigned gx = (unsigned)std::min<int64_t>(
-      std::max(std::min(chunks, one), (chunks + 3) / 4), kMaxChunksX);
-  const unsigned ax = (unsigned)std::min<int64_t>((span + kAddKeys - 1) / kAddKeys, kMaxChunksX);
+      std::max(std::min(chunks, one), (chunks + 3) / 4), kMaxChunksX) | 1;
+  const unsigned ax =
+      (unsigned)std::min<int64_t>((span + kAddKeys - 1) / kAddKeys, kMaxChunksX) | 1;
   void* args[] = {&prm};
   const hipStream_t hs = static_cast<hipStream_t>(stream);
   const void* fn = q8 ? (bf ? scores_kernel<true, true>(head_dim)
