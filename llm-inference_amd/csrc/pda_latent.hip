@@ -351,7 +351,7 @@ __global__ __launch_bounds__(256, 1) void latent_decode_kernel(const LatentDecod
   const int width = p.latent + p.rope;
 
   const int total = scalar_load(p.prefix, p.batch);
-  const int per = (int)(((int64_t)total + p.groups - 1) / p.groups);
+  const int per = (int)(((uint32_t)total + p.groups - 1) / (uint32_t)p.groups);
   const int64_t from = (int64_t)blockIdx.x * per;
   if (from >= total) return;
   const int t0 = (int)from, t1 = (int)min((int64_t)total, from + per);
@@ -662,9 +662,9 @@ __global__ __launch_bounds__(256, 1) void latent_decode_kernel(const LatentDecod
 }
 
 // Joins the partials of each sequence and projects the result: out[b, h] = D_h
-// o / sum. A workgroup has one head and up to 32 sequences. D_h's rows, which
-// nothing before them decides, are loaded first and are under way while the
-// partials are joined: a wave has the rows of 32 value dims over half the latent.
+// o / sum. A workgroup has one head and up to 32 sequences. D_h's rows are
+// under way while the partials are joined: a wave has the rows of 32 value dims
+// over half the latent.
 // A wave joins a whole row of partials (512 dims) of one sequence, several
 // waves share a sequence's partials where there are few sequences. The joined
 // latents go to LDS as two 16-bit numbers each (the value and what its rounding
@@ -673,80 +673,105 @@ template <bool BF>
 __global__ __launch_bounds__(512, 2) void latent_merge_kernel(const LatentDecodeParams p) {
   constexpr int kWaves = 8;
   constexpr int kRow = kMaxLatent + 8;        // halves between sequences
-  constexpr int kSteps = kMaxLatent / 16 / 2; // 16-dim steps of a half
+  constexpr int kSlices = 8;                  // loads of 4 rows for a wave's 32
   __shared__ __align__(16) f16 s_hi[32 * kRow];
   __shared__ __align__(16) f16 s_lo[32 * kRow];
   __shared__ __align__(16) float s_part[kWaves][kMaxLatent];
+  __shared__ __align__(1024) f16 s_d[kWaves][32 * 128];
   const int tid = threadIdx.x, w = uniform(tid >> 6), lane = tid & 63;
   const int n = lane & 31, hh = lane >> 5;
   const int h = blockIdx.x, b0 = blockIdx.y * p.merge_batch;
   const int count = min(p.merge_batch, p.batch - b0);
   const int v0 = 32 * (w & 3), k0 = (w >> 2) * (kMaxLatent / 2);
-  f16x8 a[kSteps];
-  {
-    const f16* wp = p.kv_b + ((int64_t)h * (p.nope + p.value) + p.nope + min(v0 + n, p.value - 1)) *
-                                 p.latent;
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      const int k = k0 + 16 * i + 8 * hh;
-      a[i] = f16x8{};
-      if (k < p.latent && v0 < p.value) a[i] = *reinterpret_cast<const f16x8*>(wp + k);
-    }
-  }
-  const int total = p.prefix[p.batch];
-  const int per = max(1, (int)(((int64_t)total + p.groups - 1) / p.groups));
+  // Lane i: the stream's place before sequence b0 + i, the ranges of its units
+  // on either side.
+  const uint32_t place = (uint32_t)p.prefix[b0 + min(lane, count)];
+  const uint32_t per =
+      max(1u, ((uint32_t)scalar_load(p.prefix, p.batch) + p.groups - 1) / (uint32_t)p.groups);
+  const int range_in = (int)((place + kSequenceTiles) / per), range_end = (int)((place - 1) / per);
   const int share = count >= 8 ? 1 : count >= 4 ? 2 : count >= 2 ? 4 : 8;  // waves a sequence
   const int d = 8 * lane;
+  // A wave's slice of D_h: rows v0 .. v0 + 31, dims k0 .. k0 + 255, in two halves
+  // of 128. A load moves 256 bytes of 4 rows (lanes side by side read 16 bytes
+  // side by side: a product's operand straight from memory, 32 rows an
+  // instruction, takes the cache 4 times as long); row r has piece p at place
+  // p ^ (r % 16).
+  auto weights_at = [&](int i, int from) {
+    const int r = 4 * i + (lane >> 4), piece = (lane & 15) ^ (r & 15);
+    return reinterpret_cast<const f16x8*>(
+        p.kv_b +
+        ((int64_t)h * (p.nope + p.value) + p.nope + min(v0 + r, p.value - 1)) * p.latent +
+        min(k0 + from + 8 * piece, p.latent - 8));
+  };
+  const uint32_t lds = uniform(lds_address(&s_d[w][0]));
+  f16x8 a[kSlices];
   for (int r0 = 0; r0 < count; r0 += kWaves / share) {
     const int r = r0 + w / share, part = w % share;
     const bool have = r < count;
     const int b = b0 + (have ? r : 0);
-    const int seq0 = p.prefix[b], seq1 = p.prefix[b + 1];
-    const int g0 = (seq0 + kSequenceTiles) / per;
-    const int slots = have && seq1 > seq0 ? (seq1 - 1) / per - g0 + 1 : 0;
+    const int at = have ? r : 0;
+    const bool some = __builtin_amdgcn_readlane(place, at + 1) !=
+                      __builtin_amdgcn_readlane(place, at);  // it has keys
+    const int g0 = __builtin_amdgcn_readlane(range_in, at);
+    const int slots = have && some ? __builtin_amdgcn_readlane(range_end, at + 1) - g0 + 1 : 0;
     const float2* ml = p.part_ml + ((int64_t)g0 + b) * p.hq + h;
     const float* po = p.part_o + (((int64_t)g0 + b) * p.hq + h) * p.latent;
-    // A lane looks at every 64th partial's maximum and sum.
-    float top = -INFINITY;
-    for (int g = lane; g < slots; g += 64) top = fmaxf(top, ml[(int64_t)g * p.hq].x);
+    // This wave's partials part + share i, kEach of them under way, the first
+    // before what they weigh is known.
+    constexpr int kEach = 8;
+    float4 x[kEach][2];
+    auto load = [&](int g) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 32; i; i >>= 1) top = fmaxf(top, __shfl_xor(top, i));
-    float sum = 0.0f, acc[8] = {};
-    for (int base = 0; base < slots; base += 64) {
-      float f = 0.0f;
-      if (base + lane < slots && top != -INFINITY) {
-        const float2 x = ml[(int64_t)(base + lane) * p.hq];
-        f = x.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x.x - top);
-        sum = fmaf(x.y, f, sum);
-      }
-      const int end = min(64, slots - base);
-      constexpr int kEach = 4;  // rows under way
-      for (int g = part; g < end; g += share * kEach) {
-        float4 x[kEach][2];
-        float fg[kEach];
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-          const int at = g + share * j;
-          fg[j] = __shfl(f, min(at, 63));
-          if (at >= end || fg[j] == 0.0f || d >= p.latent) fg[j] = 0.0f;
-          const float4* src = reinterpret_cast<const float4*>(
-              po + (int64_t)(base + min(at, end - 1)) * p.hq * p.latent + min(d, p.latent - 8));
+      for (int j = 0; j < kEach; ++j) {
+        x[j][0] = x[j][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (g + share * j < slots && d < p.latent) {
+          const float4* src =
+              reinterpret_cast<const float4*>(po + (int64_t)(g + share * j) * p.hq * p.latent + d);
           x[j][0] = src[0];
           x[j][1] = src[1];
         }
+      }
+    };
+    // A lane looks at every 64th partial's maximum and sum.
+    float2 mine = make_float2(-INFINITY, 0.0f);
+    if (lane < slots) mine = ml[(int64_t)lane * p.hq];
+    load(part);
+    if (r0 == 0) {  // (loads return in their order: behind the first partials)
+      auto copy = [&](auto i) __attribute__((always_inline)) {
+        copy_to_lds<0, decltype(i)::value * 1024>(weights_at(i, 0), lds);
+      };
+      each(copy, std::make_integer_sequence<int, kSlices>{});
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-          // (A partial without a key holds zeros: nothing to leave out.)
-          acc[0] = fmaf(x[j][0].x, fg[j], acc[0]);
-          acc[1] = fmaf(x[j][0].y, fg[j], acc[1]);
-          acc[2] = fmaf(x[j][0].z, fg[j], acc[2]);
-          acc[3] = fmaf(x[j][0].w, fg[j], acc[3]);
-          acc[4] = fmaf(x[j][1].x, fg[j], acc[4]);
-          acc[5] = fmaf(x[j][1].y, fg[j], acc[5]);
-          acc[6] = fmaf(x[j][1].z, fg[j], acc[6]);
-          acc[7] = fmaf(x[j][1].w, fg[j], acc[7]);
+      for (int i = 0; i < kSlices; ++i) a[i] = *weights_at(i, 128);
+    }
+    float top = mine.x;
+    for (int g = lane + 64; g < slots; g += 64) top = fmaxf(top, ml[(int64_t)g * p.hq].x);
+#pragma unroll
+    for (int i = 32; i; i >>= 1) top = fmaxf(top, __shfl_xor(top, i));
+    float sum = 0.0f, f = 0.0f, acc[8] = {};
+    for (int base = 0; base < slots; base += share * kEach) {
+      if (base % 64 == 0) {  // (share * kEach divides 64)
+        f = 0.0f;
+        if (base + lane < slots && top != -INFINITY) {
+          const float2 y = base ? ml[(int64_t)(base + lane) * p.hq] : mine;
+          f = y.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(y.x - top);
+          sum = fmaf(y.y, f, sum);
         }
       }
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        // (A partial without a key holds zeros: nothing to leave out.)
+        const float fg = __shfl(f, (base + part + share * j) % 64);
+        acc[0] = fmaf(x[j][0].x, fg, acc[0]);
+        acc[1] = fmaf(x[j][0].y, fg, acc[1]);
+        acc[2] = fmaf(x[j][0].z, fg, acc[2]);
+        acc[3] = fmaf(x[j][0].w, fg, acc[3]);
+        acc[4] = fmaf(x[j][1].x, fg, acc[4]);
+        acc[5] = fmaf(x[j][1].y, fg, acc[5]);
+        acc[6] = fmaf(x[j][1].z, fg, acc[6]);
+        acc[7] = fmaf(x[j][1].w, fg, acc[7]);
+      }
+      if (base + share * kEach < slots) load(base + share * kEach + part);
     }
 #pragma unroll
     for (int i = 32; i; i >>= 1) sum += __shfl_xor(sum, i);
@@ -756,9 +781,12 @@ __global__ __launch_bounds__(512, 2) void latent_merge_kernel(const LatentDecode
       *reinterpret_cast<float4*>(&s_part[w][d + 4]) = make_float4(acc[4], acc[5], acc[6], acc[7]);
       __syncthreads();
       if (part == 0)
-        for (int i = 1; i < share; ++i)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) acc[j] += s_part[w + i][d + j];
+        for (int i = 1; i < share; ++i) {
+          const float4 y = *reinterpret_cast<const float4*>(&s_part[w + i][d]);
+          const float4 z = *reinterpret_cast<const float4*>(&s_part[w + i][d + 4]);
+          acc[0] += y.x, acc[1] += y.y, acc[2] += y.z, acc[3] += y.w;
+          acc[4] += z.x, acc[5] += z.y, acc[6] += z.z, acc[7] += z.w;
+        }
     }
     if (part || !have || d >= p.latent) continue;
     const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
@@ -772,19 +800,27 @@ __global__ __launch_bounds__(512, 2) void latent_merge_kernel(const LatentDecode
     *reinterpret_cast<f16x8*>(&s_hi[r * kRow + d]) = hi;
     *reinterpret_cast<f16x8*>(&s_lo[r * kRow + d]) = lo;
   }
+  wait_vmem<0>();
   __syncthreads();
-  const bool have = n < count;
+  const bool have = n < count;  // (other columns hold anything)
   f32x16 acc = {}, rest = {};
 #pragma unroll
-  for (int i = 0; i < kSteps; ++i) {
-    const int k = k0 + 16 * i + 8 * hh;
-    f16x8 hi = {}, lo = {};
-    if (have && k < p.latent) {
-      hi = *reinterpret_cast<const f16x8*>(&s_hi[n * kRow + k]);
-      lo = *reinterpret_cast<const f16x8*>(&s_lo[n * kRow + k]);
+  for (int half = 0; half < 2; ++half) {
+    if (half) {  // (a wave's own reads and writes of LDS keep their order)
+#pragma unroll
+      for (int i = 0; i < kSlices; ++i)
+        *reinterpret_cast<f16x8*>(&s_d[w][512 * i + 8 * lane]) = a[i];
     }
-    acc = mfma16<BF>(a[i], hi, acc);
-    rest = mfma16<BF>(a[i], lo, rest);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int k = k0 + 128 * half + 16 * i + 8 * hh, at = n * kRow + min(k, p.latent - 8);
+      f16x8 x = *reinterpret_cast<const f16x8*>(&s_d[w][128 * n + 8 * ((2 * i + hh) ^ (n & 15))]);
+      f16x8 hi = *reinterpret_cast<const f16x8*>(&s_hi[at]);
+      f16x8 lo = *reinterpret_cast<const f16x8*>(&s_lo[at]);
+      if (k >= p.latent) x = hi = lo = f16x8{};
+      acc = mfma16<BF>(x, hi, acc);
+      rest = mfma16<BF>(x, lo, rest);
+    }
   }
   // The two halves of the latent.
   float* join = &s_part[0][0];
