@@ -24,10 +24,12 @@ using pda_internal::ok;
 
 constexpr int kQueries = 128;   // queries per workgroup
 constexpr int kKeys = 64;       // keys per tile
+constexpr int kTokenTile = 128; // tokens an expanding workgroup keeps
 constexpr int kMaxSplits = 64;
 constexpr float kSlack = 8.0f;
 constexpr int kXcds = 8;
 constexpr int kCus = 256;
+constexpr int kSlots = 2 * kCus;  // workgroups resident on an MI355X, two a CU
 
 struct PrefillParams {
   const f16* q;         // [count, hq, nope + rope]
@@ -66,32 +68,34 @@ struct PrefillParams {
 
 // keys[h, t] = U_h c_t, values[h, t] = D_h c_t, rounded to the element type: a
 // matrix product in which the tokens stay and the projections stream. A wave
-// keeps 32 TB tokens' whole latents as operands (TB x 128 registers at 512 dims,
-// gathered from the pages once); the workgroup walks the projected dims of its
-// heads 32 at a time through a ring of LDS blocks, each read once by every wave
-// for TB products: with two token blocks the matrix cores and not the LDS bound
-// it. Results are stored a block late, so that no wait for a copy waits for a
-// store. Tokens without a row are zeros from the start. The workgroups of the
-// group's first heads also gather the rotary keys and the mask of keys that have
-// a row. PL: planes of 64 latent dims.
-template <int TB, int PL, bool BF>
-__global__ __launch_bounds__(256, TB == 2 ? 1 : 2) void latent_expand_kernel(const PrefillParams p) {
-  constexpr int kRing = TB == 2 ? 4 : 2;
+// keeps 32 tokens' whole latents as operands (128 registers at 512 dims, gathered
+// from the pages once); the workgroup walks the projected dims of its heads 32 at
+// a time through two LDS blocks, each read once by every wave. Two workgroups a
+// CU, so that one's products run beside the other's waits. (Two token blocks a
+// wave, which halve the LDS reads, and one workgroup a CU were slower: 128 heads,
+// 512 tokens 63 us a call against 59, 16 heads, 256 at 30000 272 against 257.)
+// The next block's copies and the last one's stores go out among the products:
+// issued together they held the wave for as long as the products. 16 heads of
+// 128 + 128 dims, 8289 tokens 48 us, 128 heads, 4096 tokens 159 us (860 TFLOP/s);
+// the products and the copies' rate into LDS bound it about alike.
+// Results are stored a block late. Tokens without a row are zeros from the start.
+// The workgroups of the group's first heads also gather the rotary keys and the
+// mask of keys that have a row. PL: planes of 64 latent dims.
+template <int PL, bool BF>
+__global__ __launch_bounds__(256, 2) void latent_expand_kernel(const PrefillParams p) {
   constexpr int kPlane = 32 * 64;  // halves of 64 latent dims of a block
   constexpr int kPlanes = PL;
   constexpr int kChunks = 4 * kPlanes;
-  constexpr int kTokens = 128 * TB;
-  constexpr int kCopies = kPlanes;  // a wave's, a block
   constexpr int kPitch = 40;        // halves of a token's 32 results
-  __shared__ __align__(1024) f16 s_w[kRing][kPlanes * kPlane];
-  __shared__ __align__(16) f16 s_out[4][32 * TB * kPitch];
-  __shared__ int s_row[kTokens];
+  __shared__ __align__(1024) f16 s_w[2][kPlanes * kPlane];
+  __shared__ __align__(16) f16 s_out[4][32 * kPitch];
+  __shared__ int s_row[kTokenTile];
   const int tid = threadIdx.x, w = uniform(tid >> 6), lane = tid & 63;
   const int n = lane & 31, hh = lane >> 5;
   const int outs = p.nope + p.value;
-  const int t0 = blockIdx.y * kTokens;
+  const int t0 = blockIdx.y * kTokenTile;
   const int width = p.latent + p.rope;
-  for (int i = tid; i < kTokens; i += 256) {
+  for (int i = tid; i < kTokenTile; i += 256) {
     const int t = t0 + i;
     int row = -1;
     if (t < p.start + p.count) {
@@ -123,40 +127,66 @@ __global__ __launch_bounds__(256, TB == 2 ? 1 : 2) void latent_expand_kernel(con
   const int piece = (lane & 7) ^ swizzle(my_row);
   const int last_piece = p.latent / 8 - 1;
   const uint32_t lds = uniform(lds_address(&s_w[0][0]));
-  auto copy = [&](int block) {
-    const int h = block / each_head, part = block - h * each_head;
-    const bool value = part >= nope_blocks;
-    const int d0 = 32 * (value ? part - nope_blocks : part);
-    const int size = value ? p.value : p.nope;
-    const f16* src =
-        p.kv_b + ((int64_t)(p.head0 + h) * outs + (value ? p.nope : 0) + min(d0 + my_row, size - 1)) *
-                     p.latent;
-    const uint32_t dst = lds + ((block - b0) % kRing) * (2 * kPlanes * kPlane) + 1024 * w;
-#pragma unroll
-    for (int j = 0; j < kPlanes; ++j)
-      copy_to_lds<0, 0>(src + 8 * min(8 * j + piece, last_piece), dst + j * (2 * kPlane));
+  struct Block {
+    int h, part;
   };
-  if (b0 < b1) copy(b0);
-  if constexpr (kRing > 2) {
-    if (b0 + 1 < b1) copy(b0 + 1);
-    if (b0 + 2 < b1) copy(b0 + 2);
-  }
-  // The wave's tokens.
-  f16x8 tok[TB][kChunks];
+  auto after = [&](Block x) {
+    return x.part + 1 < each_head ? Block{x.h, x.part + 1} : Block{x.h + 1, 0};
+  };
+  auto is_value = [&](Block x) { return x.part >= nope_blocks; };
+  auto dim_of = [&](Block x) { return 32 * (is_value(x) ? x.part - nope_blocks : x.part); };
+  auto source = [&](Block x) {
+    const int size = is_value(x) ? p.value : p.nope;
+    return p.kv_b + ((int64_t)(p.head0 + x.h) * outs + (is_value(x) ? p.nope : 0) +
+                     min(dim_of(x) + my_row, size - 1)) *
+                        p.latent;
+  };
+  auto copy = [&](const f16* src, int to, int j) __attribute__((always_inline)) {
+    copy_to_lds<0, 0>(src + 8 * min(8 * j + piece, last_piece),
+                      lds + to * (2 * kPlanes * kPlane) + 1024 * w + j * (2 * kPlane));
+  };
+  int w_lane[4];
 #pragma unroll
-  for (int j = 0; j < TB; ++j) {
-    const int row = s_row[32 * (TB * w + j) + n];
-    const f16* src = p.arena + (int64_t)max(row, 0) * width;
+  for (int i = 0; i < 4; ++i) w_lane[i] = 64 * n + 8 * ((2 * i + hh) ^ swizzle(n));
+  // The wave's tokens, half the planes at a time by way of its quarter of the
+  // ring: as for the projections an instruction moves 128 bytes of 8 rows.
+  // (Fragments straight from memory, 16 bytes of a row a lane, take the cache 4
+  // times as long: 16 thousand cycles a CU at 512 dims.)
+  constexpr int kHalf = kPlanes / 2;
+  f16x8 tok[kChunks];
+  const bool have = s_row[32 * w + n] >= 0;
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-      const int d = 16 * c + 8 * hh;
-      const f16x8 x = *reinterpret_cast<const f16x8*>(src + min(d, p.latent - 8));
-      tok[j][c] = row >= 0 && d < p.latent ? x : f16x8{};
+  for (int half = 0; half < 2; ++half) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 8 * i + (lane >> 3), at = (lane & 7) ^ swizzle(r);
+      const f16* src = p.arena + (int64_t)max(s_row[32 * w + r], 0) * width;
+#pragma unroll
+      for (int j = 0; j < kHalf; ++j)
+        copy_to_lds<0, 0>(src + 8 * min(8 * (kHalf * half + j) + at, last_piece),
+                          lds + (w * kHalf + j) * (2 * kPlane) + 1024 * i);
     }
+    wait_vmem<0>();
+    asm volatile("" ::: "memory");  // (no barrier: the wave's own copies and reads)
+#pragma unroll
+    for (int c = 0; c < kChunks / 2; ++c) {
+      const int k = 16 * (kChunks / 2 * half + c) + 8 * hh;
+      const f16x8 x = *reinterpret_cast<const f16x8*>(
+          &s_w[0][0] + (w * kHalf + (c >> 2)) * kPlane + w_lane[c & 3]);
+      tok[kChunks / 2 * half + c] = have && k < p.latent ? x : f16x8{};
+    }
+    wait_lds();
+  }
+  __syncthreads();
+  Block now = {b0 / each_head, b0 % each_head};
+  if (b0 < b1) {
+    const f16* src = source(now);
+#pragma unroll
+    for (int j = 0; j < kPlanes; ++j) copy(src, 0, j);
   }
   if (blockIdx.x == 0) {
     const int pieces = p.rdim / 8;
-    for (int i = tid; i < kTokens * pieces; i += 256) {
+    for (int i = tid; i < kTokenTile * pieces; i += 256) {
       const int r = i / pieces, j = i - r * pieces;
       if (t0 + r >= p.span) break;
       f16x8 x = {};
@@ -170,46 +200,30 @@ __global__ __launch_bounds__(256, TB == 2 ? 1 : 2) void latent_expand_kernel(con
   // dim of it is stored, also those past the head's part (keys are zeros there,
   // which the queries' zeros meet).
   f16* so = s_out[w];
-  auto store = [&](int block) {
-    const int h = block / each_head, part = block - h * each_head;
-    const bool value = part >= nope_blocks;
-    const int d0 = 32 * (value ? part - nope_blocks : part);
-    f16* base = value ? p.values + (int64_t)h * p.span * p.vdim
-                      : p.keys + (int64_t)h * p.span * p.kdim;
-    const int pitch = value ? p.vdim : p.kdim;
-#pragma unroll
-    for (int j = 0; j < 2 * TB; ++j) {
-      const int r = 16 * j + (lane >> 2);
-      const int64_t t = t0 + 32 * TB * w + r;
-      if (t >= p.span) continue;
-      *reinterpret_cast<f16x8*>(base + t * pitch + d0 + 8 * (lane & 3)) =
-          *reinterpret_cast<const f16x8*>(so + r * kPitch + 8 * (lane & 3));
-      // (Planes of the keys that no block fills.)
-      if (part == nope_blocks - 1 && (lane & 3) == 0)
-        for (int d = 32 * nope_blocks; d < p.kdim; d += 8)
-          *reinterpret_cast<f16x8*>(base + t * pitch + d) = f16x8{};
-    }
+  auto load_out = [&](int j) {
+    return *reinterpret_cast<const f16x8*>(so + (16 * j + (lane >> 2)) * kPitch + 8 * (lane & 3));
   };
-  int w_lane[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w_lane[i] = 64 * n + 8 * ((2 * i + hh) ^ swizzle(n));
-  for (int b = b0; b < b1; ++b) {
-    // (Operations end in order: of the last 2 kCopies, a block's stores may be
-    // among them.)
-    if (kRing > 2 && b + 2 < b1)
-      wait_vmem<2 * kCopies>();
-    else if (kRing > 2 && b + 1 < b1)
-      wait_vmem<kCopies>();
-    else
-      wait_vmem<0>();
+  auto store = [&](Block x, int j, const f16x8& y) __attribute__((always_inline)) {
+    f16* base = is_value(x) ? p.values + (int64_t)x.h * p.span * p.vdim
+                            : p.keys + (int64_t)x.h * p.span * p.kdim;
+    const int pitch = is_value(x) ? p.vdim : p.kdim;
+    const int64_t t = t0 + 32 * w + 16 * j + (lane >> 2);
+    if (t >= p.span) return;
+    *reinterpret_cast<f16x8*>(base + t * pitch + dim_of(x) + 8 * (lane & 3)) = y;
+    // (Planes of the keys that no block fills.)
+    if (x.part == nope_blocks - 1 && (lane & 3) == 0)
+      for (int d = 32 * nope_blocks; d < p.kdim; d += 8)
+        *reinterpret_cast<f16x8*>(base + t * pitch + d) = f16x8{};
+  };
+  Block last = now;
+  for (int b = b0; b < b1; ++b, last = now, now = after(now)) {
+    wait_vmem<0>();
     __syncthreads();
-    if (b > b0) store(b - 1);
-    constexpr int kNext = kRing > 2 ? 3 : 1;
-    if (b + kNext < b1) copy(b + kNext);
-    const f16* wp = s_w[(b - b0) % kRing];
-    f32x16 acc[TB];
-#pragma unroll
-    for (int j = 0; j < TB; ++j) acc[j] = f32x16{};
+    const bool more = b + 1 < b1;
+    const f16* src = source(more ? after(now) : now);
+    const f16x8 y0 = load_out(0), y1 = load_out(1);  // (of the block before)
+    const f16* wp = s_w[(b - b0) & 1];
+    f32x16 acc = {};
     constexpr int kAhead = 4;
     f16x8 a[kChunks];
     auto read = [&](int c) {
@@ -220,25 +234,26 @@ __global__ __launch_bounds__(256, TB == 2 ? 1 : 2) void latent_expand_kernel(con
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
-#pragma unroll
-      for (int j = 0; j < TB; ++j) acc[j] = mfma16<BF>(a[c], tok[j][c], acc[j]);
+      acc = mfma16<BF>(a[c], tok[c], acc);
       if (c + kAhead < kChunks) read(c + kAhead);
+      if (c == 1 && b > b0) store(last, 0, y0);
+      if (c == 3 && b > b0) store(last, 1, y1);
+      if (c % 2 == 0 && c < 2 * kPlanes && more) copy(src, (b - b0 + 1) & 1, c / 2);
       __builtin_amdgcn_sched_barrier(0);
     }
-    const int part = b % each_head;
-    const int left = part >= nope_blocks ? 32 : p.nope - 32 * part;  // keys' dims of the block
+    const int left = is_value(now) ? 32 : p.nope - dim_of(now);  // keys' dims of the block
 #pragma unroll
-    for (int j = 0; j < TB; ++j)
+    for (int g = 0; g < 4; ++g) {
+      f16x4 y;
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        f16x4 y;
-#pragma unroll
-        for (int v = 0; v < 4; ++v)
-          y[v] = 8 * g < left ? round16<BF>(acc[j][4 * g + v]) : (f16)0.0f;
-        *reinterpret_cast<f16x4*>(so + (32 * j + n) * kPitch + 8 * g + 4 * hh) = y;
-      }
+      for (int v = 0; v < 4; ++v) y[v] = 8 * g < left ? round16<BF>(acc[4 * g + v]) : (f16)0.0f;
+      *reinterpret_cast<f16x4*>(so + n * kPitch + 8 * g + 4 * hh) = y;
+    }
   }
-  if (b0 < b1) store(b1 - 1);
+  if (b0 < b1) {
+    store(last, 0, load_out(0));
+    store(last, 1, load_out(1));
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -940,7 +955,6 @@ __global__ __launch_bounds__(256) void latent_join_kernel(const PrefillParams p)
 size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 constexpr size_t kExpandBytes = (size_t)1 << 30;  // expanded keys and values at once
-constexpr int kSlots = 512;                       // workgroups resident on an MI355X
 // Two query blocks a wave from whole workgroups of queries and as many keys on
 // that their longer start is paid for (us a call, one block / two: 16 heads of
 // 128 + 64, 512 tokens at 0 36 / 44, 256 at 7777 103 / 106, 512 at 30000 360 /
@@ -1006,15 +1020,6 @@ int check_prefill(int32_t start, int32_t count, int32_t q_heads, int32_t latent_
   if ((int64_t)start + count > INT32_MAX - 512)
     return fail(PDA_ERR_TOO_LONG, "start + count next to 2^31");
   return PDA_OK;
-}
-
-template <bool BF>
-const void* expand_kernel(bool two, int latent) {
-  if (latent <= 256)
-    return two ? (const void*)latent_expand_kernel<2, 4, BF>
-               : (const void*)latent_expand_kernel<1, 4, BF>;
-  return two ? (const void*)latent_expand_kernel<2, 8, BF>
-             : (const void*)latent_expand_kernel<1, 8, BF>;
 }
 
 template <bool BF>
@@ -1090,13 +1095,11 @@ int latent_prefill(const void* queries, const void* arena, const void* kv_b, con
   prm.scale_log2 = scale * kLog2e;
   void* args[] = {&prm};
   const hipStream_t hs = static_cast<hipStream_t>(stream);
-  // Two token blocks a wave where that still fills the CUs (one workgroup
-  // each), one where it would not (two workgroups each).
-  const int64_t wide = ((int64_t)plan.span + 255) / 256 * plan.heads;
-  const bool two = wide >= kCus;
-  const void* expand = bf ? expand_kernel<true>(two, latent_dim) : expand_kernel<false>(two, latent_dim);
-  const int tokens = two ? 256 : 128;
-  const int token_tiles = (plan.span + tokens - 1) / tokens;
+  const void* expand = latent_dim <= 256 ? (bf ? (const void*)latent_expand_kernel<4, true>
+                                               : (const void*)latent_expand_kernel<4, false>)
+                                         : (bf ? (const void*)latent_expand_kernel<8, true>
+                                               : (const void*)latent_expand_kernel<8, false>);
+  const int token_tiles = (plan.span + kTokenTile - 1) / kTokenTile;
   const void* attend =
       plan.pipe ? (bf ? (const void*)latent_prefill_wide_kernel<true>
                       : (const void*)latent_prefill_wide_kernel<false>)
@@ -1108,7 +1111,7 @@ int latent_prefill(const void* queries, const void* arena, const void* kv_b, con
     prm.heads = std::min(plan.heads, q_heads - h0);
     // The projected dims shared out so that the workgroups just fill the GPU.
     const int every = prm.heads * ((nope_dim + 31) / 32 + (value_dim + 31) / 32);
-    int shares = std::min(every, std::max(1, (two ? kCus : 2 * kCus) / token_tiles));
+    int shares = std::min(every, std::max(1, kSlots / token_tiles));
     if (shares > kXcds) shares = shares / kXcds * kXcds;
     err = hipLaunchKernel(expand, dim3(shares, token_tiles), dim3(256), args, 0, hs);
     if (err == hipSuccess)
