@@ -66,8 +66,10 @@ struct PrefillParams {
 // ---------------------------------------------------------------------------
 // Expansion.
 
-// keys[h, t] = U_h c_t, values[h, t] = D_h c_t, rounded to the element type: a
-// matrix product in which the tokens stay and the projections stream. A wave
+// keys[h, t] = U_h c_t, values[h, t] = D_h c_t, rounded to the element type, as a
+// cache of keys and values per head would hold them (in bf16 that moves the result
+// by 1.0e-3 and 1.2e-3 of its 2-norm, beside 1.7e-3 for its own rounding): a matrix
+// product in which the tokens stay and the projections stream. A wave
 // keeps 32 tokens' whole latents as operands (128 registers at 512 dims, gathered
 // from the pages once); the workgroup walks the projected dims of its heads 32 at
 // a time through two LDS blocks, each read once by every wave. Two workgroups a
@@ -266,8 +268,12 @@ __global__ __launch_bounds__(256, 2) void latent_expand_kernel(const PrefillPara
 // transposed in the order the scores hold the keys). Two workgroups a CU, so
 // that one's products run beside the other's weights. The query tiles of a head
 // are dispatched to one XCD, whose L2 then serves the head's keys and values.
+// The weights are rounded to 16 bits for the second product (in bf16 1.2e-3 of the
+// result's 2-norm), and the sum that divides it is of the rounded ones.
 // NP, VP: planes of 64 dims of the nope part and of the values; RS: 16-dim steps
-// of the rotary plane that are computed.
+// of the rotary plane that are computed. 14 heads of 64 + 32 and 64 dims, 1531
+// queries after 389 keys 23 us: 168 workgroups of up to 30 tiles, whose length
+// bounds it.
 template <int NP, int RS, int VP, bool BF>
 __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(const PrefillParams p) {
   constexpr int kPlane = kKeys * 64;  // halves of a 64-dim plane of a tile
@@ -498,7 +504,9 @@ __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(const PrefillPar
 // tile's V is used an iteration after its K. The outputs (2 x 32 x 128, 128
 // registers a lane) and the queries live in accumulator registers.
 // What takes the running maximum past 2^8 is found from the weights' sum after
-// the fact and weighed again (settle).
+// the fact and weighed again (settle). Rounded as above. 128 heads, 4096 tokens 780 to
+// 830 us for 687 GFLOP (0.83 to 0.88 PFLOP/s), 16 heads, 512 at 7777 56 us for 42
+// GFLOP; the matrix cores bound it at the clock that their load leaves.
 template <bool BF>
 __global__ __launch_bounds__(256, 1) void latent_prefill_wide_kernel(const PrefillParams p) {
   constexpr int NP = 2, RP = 1, VP = 2, KP = NP + RP, OB = 2 * VP, QB = 2;
@@ -803,8 +811,9 @@ __global__ __launch_bounds__(256, 1) void latent_prefill_wide_kernel(const Prefi
       asm volatile("" : "+v"(xn[j]), "+v"(pb[2 * j]), "+v"(pb[2 * j + 1]), "+v"(lb[j]));
   };
   // Iteration t: V of tile t and K of the next (of the last one again) are copied
-  // beside the wave's math, and published by the barrier at its end. (The phases in a row, each
-  // with a loop of its own: where paths met in one loop the outputs were copied.
+  // beside the wave's math, and published by the barrier at its end. (The phases in
+  // a row, each with a loop of its own: where paths met in one loop the outputs
+  // were copied.
   // In the steps a copy goes out every other fragment: issued together they
   // waited for each other, 600 of 4900 cycles a tile.)
   uint64_t ok_prev = 0;
@@ -917,7 +926,8 @@ __global__ __launch_bounds__(256, 1) void latent_prefill_wide_kernel(const Prefi
 }
 
 // Joins the key ranges of a split call: a thread has 4 value dims of one query
-// and head.
+// and head. Reads each partial once, which bounds it (16 heads, 512 tokens in 8
+// ranges: 36 MB in 10 us).
 template <bool BF>
 __global__ __launch_bounds__(256) void latent_join_kernel(const PrefillParams p) {
   const int64_t pairs = (int64_t)p.count * p.hq;
@@ -957,14 +967,17 @@ size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 constexpr size_t kExpandBytes = (size_t)1 << 30;  // expanded keys and values at once
 // Two query blocks a wave from whole workgroups of queries and as many keys on
 // that their longer start is paid for (us a call, one block / two: 16 heads of
-// 128 + 64, 512 tokens at 0 36 / 44, 256 at 7777 103 / 106, 512 at 30000 360 /
-// 343; 128 heads, 512 at 0 62 / 64, 1024 at 0 130 / 118, 4096 at 0 910 / 843).
-constexpr int kPipeQueries = 256;
-constexpr int kPipeKeys = 1024;
+// 128 + 64, 512 tokens at 0 30 / 37, 256 at 7777 104 / 105, 512 at 30000 338 /
+// 324; 128 heads, 512 at 0 55 / 56, 1024 at 0 123 / 108, 4096 at 0 921 / 861).
+constexpr int kWideQueries = 256;
+constexpr int kWideKeys = 1024;
 
 struct PrefillPlan {
-  bool small;   // planes of 64 + 64 and 64 dims, else 128 + 64 and 128
-  bool pipe;    // two query blocks a wave
+  // Planes of 64 + 64 and 64 dims, else 128 + 64 and 128 (64 + 32 and 64 dims, us a
+  // call with the small and the large planes: 14 heads, 1531 tokens at 389 40 and
+  // 51, 32 heads, 4096 at 0 167 and 185).
+  bool small;
+  bool wide;    // two query blocks a wave
   bool paired;  // two query tiles a workgroup
   int kdim, vdim, rdim;
   int span, tiles, splits, heads;  // heads per group
@@ -978,8 +991,8 @@ PrefillPlan plan_for(int start, int count, int q_heads, int rope, int nope, int 
   r.vdim = r.kdim;
   r.rdim = 64;
   r.span = (start + count + kKeys - 1) / kKeys * kKeys;
-  r.pipe = !r.small && count >= kPipeQueries && start + count >= kPipeKeys;
-  const int queries = r.pipe ? 2 * kQueries : kQueries;
+  r.wide = !r.small && count >= kWideQueries && start + count >= kWideKeys;
+  const int queries = r.wide ? 2 * kQueries : kQueries;
   r.tiles = (count + queries - 1) / queries;
   const size_t head_bytes = (size_t)r.span * (r.kdim + r.vdim) * 2;
   // Heads in groups whose expanded rows fit the bound, whole rounds of XCDs
@@ -988,12 +1001,14 @@ PrefillPlan plan_for(int start, int count, int q_heads, int rope, int nope, int 
   if (heads >= kXcds) heads = heads / kXcds * kXcds;
   r.heads = (int)std::min<int64_t>(heads, q_heads);
   // Key ranges: enough for the workgroups to fill the GPU, each of four tiles
-  // of keys at least.
+  // of keys at least. (us a call with 2, 4 and 8: 16 heads, 512 tokens at 0 35, 33,
+  // 31; one at 1000 31, 31, 35; 512 at 7777 130, 121, 128.)
   const int64_t items = (int64_t)r.tiles * r.heads;
   const int64_t most = std::min<int64_t>(kMaxSplits, std::max(1, r.span / kKeys / 4));
-  r.splits = (int)std::max<int64_t>(1, std::min(most, (r.pipe ? kCus : kSlots) / items));
-  // Paired tiles level the causal work where workgroups come in several rounds.
-  r.paired = r.pipe && r.splits == 1 && items >= 2 * kCus;
+  r.splits = (int)std::max<int64_t>(1, std::min(most, (r.wide ? kCus : kSlots) / items));
+  // Paired tiles level the causal work where workgroups come in several rounds
+  // (128 heads, 4096 tokens at 0: 873 us a call, 938 unpaired).
+  r.paired = r.wide && r.splits == 1 && items >= 2 * kCus;
   size_t at = 0;
   r.keys = at;
   at = up256(at + (size_t)r.heads * r.span * r.kdim * 2);
@@ -1025,6 +1040,8 @@ int check_prefill(int32_t start, int32_t count, int32_t q_heads, int32_t latent_
 template <bool BF>
 const void* prefill_kernel(bool small, int rope) {
   if (!small) return (const void*)latent_prefill_kernel<2, 4, 2, BF>;
+  // (32 rotary dims, us a call with 2 and 4 steps: 32 heads, 4096 tokens at 0 159 and
+  // 171.)
   return rope <= 32 ? (const void*)latent_prefill_kernel<1, 2, 1, BF>
                     : (const void*)latent_prefill_kernel<1, 4, 1, BF>;
 }
@@ -1095,13 +1112,15 @@ int latent_prefill(const void* queries, const void* arena, const void* kv_b, con
   prm.scale_log2 = scale * kLog2e;
   void* args[] = {&prm};
   const hipStream_t hs = static_cast<hipStream_t>(stream);
+  // (256 latent dims, us a call with 4 and 8 planes: 14 heads, 1531 tokens at 389 38
+  // and 44, 16 heads, 512 at 8000 67 and 74.)
   const void* expand = latent_dim <= 256 ? (bf ? (const void*)latent_expand_kernel<4, true>
                                                : (const void*)latent_expand_kernel<4, false>)
                                          : (bf ? (const void*)latent_expand_kernel<8, true>
                                                : (const void*)latent_expand_kernel<8, false>);
   const int token_tiles = (plan.span + kTokenTile - 1) / kTokenTile;
   const void* attend =
-      plan.pipe ? (bf ? (const void*)latent_prefill_wide_kernel<true>
+      plan.wide ? (bf ? (const void*)latent_prefill_wide_kernel<true>
                       : (const void*)latent_prefill_wide_kernel<false>)
                 : (bf ? prefill_kernel<true>(plan.small, rope_dim)
                       : prefill_kernel<false>(plan.small, rope_dim));
