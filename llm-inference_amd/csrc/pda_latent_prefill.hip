@@ -60,6 +60,7 @@ struct PrefillParams {
   int32_t tiles;        // query tiles
   int32_t paired;       // two query tiles of a head a workgroup
   int32_t splits;
+  int32_t shares;       // workgroups that share a token tile's projected dims
   float scale_log2;
 };
 
@@ -95,7 +96,8 @@ __global__ __launch_bounds__(256, 2) void latent_expand_kernel(const PrefillPara
   const int tid = threadIdx.x, w = uniform(tid >> 6), lane = tid & 63;
   const int n = lane & 31, hh = lane >> 5;
   const int outs = p.nope + p.value;
-  const int t0 = blockIdx.y * kTokenTile;
+  const int share = blockIdx.x % p.shares;
+  const int t0 = (int)(blockIdx.x / p.shares) * kTokenTile;
   const int width = p.latent + p.rope;
   for (int i = tid; i < kTokenTile; i += 256) {
     const int t = t0 + i;
@@ -109,7 +111,7 @@ __global__ __launch_bounds__(256, 2) void latent_expand_kernel(const PrefillPara
       }
     }
     s_row[i] = row;
-    if (blockIdx.x == 0) {
+    if (share == 0) {
       const uint64_t have = __ballot(row >= 0);
       if ((tid & 63) == 0 && t < p.span) p.seen[t / 64] = have;
     }
@@ -119,8 +121,8 @@ __global__ __launch_bounds__(256, 2) void latent_expand_kernel(const PrefillPara
   // dims, each to a whole block), shared out evenly.
   const int nope_blocks = (p.nope + 31) / 32, each_head = nope_blocks + (p.value + 31) / 32;
   const int64_t every = (int64_t)p.heads * each_head;
-  const int b0 = uniform((int)(every * blockIdx.x / gridDim.x));
-  const int b1 = uniform((int)(every * (blockIdx.x + 1) / gridDim.x));
+  const int b0 = uniform((int)(every * share / p.shares));
+  const int b1 = uniform((int)(every * (share + 1) / p.shares));
 
   // Copies: an instruction moves 128 bytes of 8 projection rows, the wave's. Past
   // the latent's end they repeat its last piece (the tokens are zeros there),
@@ -186,7 +188,7 @@ __global__ __launch_bounds__(256, 2) void latent_expand_kernel(const PrefillPara
 #pragma unroll
     for (int j = 0; j < kPlanes; ++j) copy(src, 0, j);
   }
-  if (blockIdx.x == 0) {
+  if (share == 0) {
     const int pieces = p.rdim / 8;
     for (int i = tid; i < kTokenTile * pieces; i += 256) {
       const int r = i / pieces, j = i - r * pieces;
@@ -1132,7 +1134,8 @@ int latent_prefill(const void* queries, const void* arena, const void* kv_b, con
     const int every = prm.heads * ((nope_dim + 31) / 32 + (value_dim + 31) / 32);
     int shares = std::min(every, std::max(1, kSlots / token_tiles));
     if (shares > kXcds) shares = shares / kXcds * kXcds;
-    err = hipLaunchKernel(expand, dim3(shares, token_tiles), dim3(256), args, 0, hs);
+    prm.shares = shares;
+    err = hipLaunchKernel(expand, dim3((unsigned)(shares * token_tiles)), dim3(256), args, 0, hs);
     if (err == hipSuccess)
       err = hipLaunchKernel(
           attend,

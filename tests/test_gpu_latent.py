@@ -77,6 +77,24 @@ def test_decode_long(gpu, heads):
     check_decode(gpu, SMALL, heads, [4500, 3, 2048, 2049], 16, torch.float16)
 
 
+@pytest.mark.parametrize("heads", [3, 256])
+@pytest.mark.parametrize("batch", [1, 2, 3, 4, 5, 7, 8, 9, 31, 33, 70])
+def test_decode_batches(gpu, batch, heads):
+    """Any number of sequences in the join, one to 32 of them a workgroup, empty
+    ones first, last and between."""
+    g = torch.Generator().manual_seed(batch)
+    lengths = torch.randint(0, 180, (batch,), generator=g).tolist()
+    lengths[0] = 0 if batch > 2 else 77
+    lengths[-1] = 0 if batch > 3 else 130
+    lengths[batch // 2] = 0 if batch > 4 else lengths[batch // 2]
+    check_decode(gpu, (32, 16, 24, 40), heads, lengths, 16, torch.float16)
+
+
+def test_decode_many_parts(gpu):
+    """A sequence in more parts than a wave has lanes."""
+    check_decode(gpu, (72, 16, 16, 128), 5, [21000, 40], 64, torch.bfloat16)
+
+
 def test_decode_one_key_is_its_value(gpu):
     check_decode(gpu, WIDE, 16, [1], 16, torch.float16)
 

@@ -105,6 +105,23 @@ def test_head_groups(gpu):
     check(gpu, THIN, heads, start, count)
 
 
+def test_far_prefix(gpu):
+    """More tiles of tokens than a launch's second dimension holds, most of them
+    on released pages: the same as the pages that are left alone."""
+    from instinct_amd.latent import latent_prefill_attention
+
+    page, start, count = 64, 65536 * 128 + 100, 3
+    arena, kv_b, g = layer(THIN, 2, 4 * page, torch.float16)
+    table = torch.full((-(-(start + count) // page),), -1, dtype=torch.int32)
+    table[0], table[1000], table[-1] = 2, 0, 3
+    q = torch.randn((count, 2, 8), generator=g).to(torch.float16)
+    got = latent_prefill_attention(q.to(gpu), arena.to(gpu), kv_b.to(gpu), table.to(gpu),
+                                   start=start, page_size=page, scale=0.35)
+    want, bound = oracle.prefill(q, arena, kv_b, torch.tensor([2, 0, 3]),
+                                 start=2 * page + start % page, page_size=page, scale=0.35)
+    assert bool(((got.cpu().double() - want).abs() <= bound).all())
+
+
 def test_masked_pages(gpu):
     """Released and unknown pages hide their keys whatever the rows hold;
     queries with nothing left give zeros."""
