@@ -26,7 +26,7 @@ from .hip_kernels import _arena_geometry, _given_workspace, on_device, stream_wo
 def _check_index(name: str, t: torch.Tensor, shape: tuple, device: torch.device) -> torch.Tensor:
     if t.dtype != torch.int32:
         raise TypeError(f"{name} must be int32")
-    if t.dim() != len(shape) or any(w is not None and int(s) != w for s, w in zip(t.shape, shape)):
+    if t.dim() != len(shape) or t.shape[0] != shape[0]:  # (a second one may be anything)
         raise ValueError(f"{name} must be {list(shape)}")
     if t.device != device:
         raise ValueError(f"{name} must be on {device}")
@@ -37,11 +37,11 @@ def _check_weights(name: str, t: torch.Tensor, batch: int, kv_heads: int,
                    device: torch.device) -> int:
     if t.dtype != torch.float32:
         raise TypeError(f"{name} must be float32")
-    if t.dim() != 3 or tuple(t.shape[:2]) != (batch, kv_heads) or int(t.shape[2]) == 0:
+    if t.dim() != 3 or t.shape[0] != batch or t.shape[1] != kv_heads or t.shape[2] == 0:
         raise ValueError(f"{name} must be [batch, kv_heads, capacity]")
     if t.device != device or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous and on {device}")
-    return int(t.shape[2])
+    return t.shape[2]
 
 
 def _check_arena(name: str, t: torch.Tensor, keys: torch.Tensor, dtype: torch.dtype) -> None:
@@ -78,7 +78,7 @@ def paged_attention_weights(queries: torch.Tensor, keys: torch.Tensor, tables: t
     q8 = scales is not None
     if queries.dim() != 3 or queries.dtype not in (torch.float16, torch.bfloat16):
         raise TypeError("queries must be [batch, q_heads, head_dim] float16 or bfloat16")
-    batch, q_heads, head_dim = (int(x) for x in queries.shape)
+    batch, q_heads, head_dim = queries.shape
     layout, arena_rows, kv_heads, a_dim = _arena_geometry(keys, page_size)
     if not queries.is_cuda or not queries.is_contiguous():
         raise ValueError("queries must be a contiguous GPU tensor")

@@ -288,7 +288,7 @@ def rope_inv_freq(dims: int, *, base: float | None = None, freqs: Any = None,
             raise ValueError("freqs must hold dims // 2 entries")
         key = ("freqs", dims, freqs[:half].tobytes())
     device = torch.device(device)
-    key = key + (str(device),)
+    key = key + (device,)
     table = _inv_freq_cache.get(key)
     if table is None:
         if freqs is None:

@@ -34,6 +34,9 @@ def _check_16bit(name: str, t: torch.Tensor, dims: int, like: torch.Tensor,
                  rows_only: bool = False) -> None:
     """A GPU tensor of ``like``'s device and 16-bit type; contiguous, or with
     ``rows_only`` of contiguous rows any distance apart."""
+    if (t is not like and t.dtype is like.dtype and t.dim() == dims and t.device == like.device
+            and t.is_contiguous()):
+        return  # (most tensors of most calls; `like` is checked itself)
     if t.dtype not in (torch.float16, torch.bfloat16) or t.dtype != like.dtype:
         raise TypeError(f"{name} must be {like.dtype} (float16 or bfloat16), got {t.dtype}")
     if not t.is_cuda or t.device != like.device:
@@ -56,8 +59,8 @@ def _int32_on(name: str, t: torch.Tensor, n: int, device: torch.device) -> torch
 
 def _head_shape(q_width: int, arena: torch.Tensor, kv_b: torch.Tensor) -> tuple[int, ...]:
     """(q_heads, latent, rope, nope, value) of a layer from its tensors."""
-    q_heads, out, latent = (int(x) for x in kv_b.shape)
-    rope = int(arena.shape[1]) - latent
+    q_heads, out, latent = kv_b.shape
+    rope = arena.shape[1] - latent
     nope = q_width - rope
     if rope < 0 or nope <= 0 or out - nope <= 0:
         raise ValueError("queries [.., q_heads, nope + rope], arena [rows, latent + rope] and "
@@ -86,28 +89,29 @@ def latent_append(q: torch.Tensor | None, latent: torch.Tensor, k_rope: torch.Te
     _check_16bit("arena", arena, 2, arena)
     _check_16bit("latent", latent, 2, arena, rows_only=True)
     _check_16bit("k_rope", k_rope, 2, arena, rows_only=True)
-    n, width = (int(x) for x in latent.shape)
-    rope = int(k_rope.shape[1])
-    if int(k_rope.shape[0]) != n or width + rope != int(arena.shape[1]):
+    n, width = latent.shape
+    rope = k_rope.shape[1]
+    if k_rope.shape[0] != n or width + rope != arena.shape[1]:
         raise ValueError("latent and k_rope must be the arena's columns of n rows")
     if dims not in (0, rope):
         raise ValueError("dims must be 0 or the rotary width")
     q_heads = nope = 0
     if q is not None:
         _check_16bit("q", q, 3, arena)
-        q_heads, nope = int(q.shape[1]), int(q.shape[2]) - rope
-        if int(q.shape[0]) != n or nope <= 0 or q_heads == 0:
+        q_heads, nope = q.shape[1], q.shape[2] - rope
+        if q.shape[0] != n or nope <= 0 or q_heads == 0:
             raise ValueError("q must be [n, q_heads, nope + rope]")
         if q_out is None:
             q_out = torch.empty_like(q)
-        _check_16bit("q_out", q_out, 3, arena)
-        if q_out.shape != q.shape:
-            raise ValueError("q_out must have q's shape")
+        else:
+            _check_16bit("q_out", q_out, 3, arena)
+            if q_out.shape != q.shape:
+                raise ValueError("q_out must have q's shape")
     elif q_out is not None:
         raise ValueError("q_out needs q")
     if norm_weight is not None:
         _check_16bit("norm_weight", norm_weight, 1, arena)
-        if int(norm_weight.shape[0]) != width:
+        if norm_weight.shape[0] != width:
             raise ValueError("norm_weight must be [latent]")
     rows = _int32_on("rows", rows, n, arena.device)
     if n == 0:
@@ -125,7 +129,7 @@ def latent_append(q: torch.Tensor | None, latent: torch.Tensor, k_rope: torch.Te
             ptr(q), ptr(q_out), ptr(latent), stride(latent, width), ptr(k_rope) if rope else None,
             stride(k_rope, rope), ptr(norm_weight), float(eps), ptr(arena),
             ptr(positions) if dims else None, ptr(rows), n, q_heads, width, rope, nope,
-            int(arena.shape[0]), ptr(table), torch.cuda.current_stream(arena.device).cuda_stream)
+            arena.shape[0], ptr(table), torch.cuda.current_stream(arena.device).cuda_stream)
     _lib.check(rc)
     return q_out
 
@@ -159,13 +163,13 @@ def latent_decode_attention(queries: torch.Tensor, arena: torch.Tensor, kv_b: to
     _check_16bit("queries", queries, 3, queries)
     _check_16bit("arena", arena, 2, queries)
     _check_16bit("kv_b", kv_b, 3, queries)
-    batch, q_heads, q_width = (int(x) for x in queries.shape)
+    batch, q_heads, q_width = queries.shape
     heads, latent, rope, nope, value = _head_shape(q_width, arena, kv_b)
     if heads != q_heads:
         raise ValueError("kv_b must have the queries' heads")
     if tables.dtype != torch.int32 or lengths.dtype != torch.int32:
         raise TypeError("tables and lengths must be int32")
-    if tables.dim() != 2 or int(tables.shape[0]) != batch or tuple(lengths.shape) != (batch,):
+    if tables.dim() != 2 or tables.shape[0] != batch or lengths.shape != (batch,):
         raise ValueError("tables must be [batch, width] and lengths [batch]")
     device = queries.device
     if tables.device != device or lengths.device != device:
@@ -173,12 +177,13 @@ def latent_decode_attention(queries: torch.Tensor, arena: torch.Tensor, kv_b: to
     tables, lengths = tables.contiguous(), lengths.contiguous()
     if out is None:
         out = torch.empty((batch, q_heads, value), dtype=queries.dtype, device=device)
-    _check_16bit("out", out, 3, queries)
-    if tuple(out.shape) != (batch, q_heads, value):
-        raise ValueError("out must be [batch, q_heads, value]")
+    else:
+        _check_16bit("out", out, 3, queries)
+        if out.shape != (batch, q_heads, value):
+            raise ValueError("out must be [batch, q_heads, value]")
     if batch == 0:
         return out
-    stride = int(tables.shape[1])
+    stride = tables.shape[1]
     need = _lib.latent_decode_workspace_bytes(batch, q_heads, latent, rope, int(page_size), stride,
                                               int(longest))
     stream = int(torch.cuda.current_stream(device).cuda_stream)
@@ -189,7 +194,7 @@ def latent_decode_attention(queries: torch.Tensor, arena: torch.Tensor, kv_b: to
         rc = getattr(_lib.library(), entry)(
             queries.data_ptr(), arena.data_ptr(), kv_b.data_ptr(), tables.data_ptr(),
             lengths.data_ptr(), out.data_ptr(), batch, q_heads, latent, rope, nope, value,
-            int(page_size), stride, int(arena.shape[0]), int(longest), float(scale),
+            int(page_size), stride, arena.shape[0], int(longest), float(scale),
             ws.data_ptr(), ws.numel(), stream)
     _lib.check(rc)
     return out
@@ -219,7 +224,7 @@ def latent_prefill_attention(queries: torch.Tensor, arena: torch.Tensor, kv_b: t
     _check_16bit("queries", queries, 3, queries)
     _check_16bit("arena", arena, 2, queries)
     _check_16bit("kv_b", kv_b, 3, queries)
-    count, q_heads, q_width = (int(x) for x in queries.shape)
+    count, q_heads, q_width = queries.shape
     heads, latent, rope, nope, value = _head_shape(q_width, arena, kv_b)
     if heads != q_heads:
         raise ValueError("kv_b must have the queries' heads")
@@ -231,9 +236,10 @@ def latent_prefill_attention(queries: torch.Tensor, arena: torch.Tensor, kv_b: t
     table = table.contiguous()
     if out is None:
         out = torch.empty((count, q_heads, value), dtype=queries.dtype, device=device)
-    _check_16bit("out", out, 3, queries)
-    if tuple(out.shape) != (count, q_heads, value):
-        raise ValueError("out must be [count, q_heads, value]")
+    else:
+        _check_16bit("out", out, 3, queries)
+        if out.shape != (count, q_heads, value):
+            raise ValueError("out must be [count, q_heads, value]")
     if count == 0:
         return out
     need = _lib.latent_prefill_workspace_bytes(int(start), count, q_heads, rope, nope, value)
