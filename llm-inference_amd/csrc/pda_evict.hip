@@ -584,12 +584,12 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Sele
   };
   // This thread's positions t0 + 1024 i + tid of a block: ranks, and bits of
   // those that are guarded and of those that stand for selection.
+  float x[kEach];
   uint32_t rank[kEach], guarded = 0, open = 0;
   const int blocks = (n + kBlock - 1) / kBlock;
   auto load = [&](int block) {
     guarded = open = 0;
     uint32_t page[kEach];
-    float x[kEach];
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       const int t = min(block * kBlock + i * kSelectThreads + tid, n - 1);
@@ -687,7 +687,8 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Sele
   // the NaN, which alone have it.)
   int32_t* kept = p.kept + ((int64_t)b * p.hkv + kvh) * p.keep;
   float* dst = p.out_weights + ((int64_t)b * p.hkv + kvh) * p.out_capacity;
-  const bool apart = p.out_weights && p.out_weights != p.weights;
+  // (One block's weights have all been read: they may be overwritten at once.)
+  const bool at_once = p.out_weights && (p.out_weights != p.weights || blocks == 1);
   __syncthreads();
   const uint64_t lower = (1ull << lane) - 1;
   int done = 0, equals = 0;  // kept, and met at the last rank, in the blocks before
@@ -731,7 +732,7 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Sele
         const int t = block * kBlock + i * kSelectThreads + tid;
         const int to = at + count(o & lower) + min(ties, want) - min(before, want);
         kept[to] = t;
-        if (apart) dst[to] = weights[t];
+        if (at_once) dst[to] = x[i];
       }
     }
     done += s_total[0] + min(equals + s_total[1], want) - min(equals, want);
@@ -740,18 +741,18 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Sele
   }
   for (int i = total + tid; i < p.keep; i += kSelectThreads) kept[i] = -1;
   if (kvh == 0 && tid == 0) p.new_lengths[b] = total;
-  if (!p.out_weights || apart) return;
+  if (!p.out_weights || at_once) return;
   // In place the kept positions' weights go to the front 1024 at a time: a later
   // stretch's sources lie past every place written so far.
   __threadfence_block();
   __syncthreads();
   for (int i0 = 0; i0 < total; i0 += kSelectThreads) {
     const int i = i0 + tid;
-    float x = 0.0f;
-    if (i < total) x = weights[kept[i]];
+    float y = 0.0f;
+    if (i < total) y = weights[kept[i]];
     wait_loads();
     __syncthreads();
-    if (i < total) dst[i] = x;
+    if (i < total) dst[i] = y;
     __syncthreads();
   }
 }
