@@ -688,8 +688,8 @@ int pda_latent_prefill_attention_bf16(const void* queries, const void* arena,
  * which sequences may share): weights [batch, kv_heads, capacity] float32.
  * ------------------------------------------------------------------------- */
 
-/* Bytes of workspace of the calls below: the step's unnormalised weights (4
- * bytes a query head and position) and each 256-key chunk's maximum and sum. */
+/* Bytes of workspace of the calls below: the step's scores (4 bytes a query head
+ * and position) and each chunk's maximum and sum. */
 int pda_attention_weights_workspace_bytes(int32_t batch, int32_t q_heads,
                                           int32_t capacity, size_t* bytes);
 

@@ -331,9 +331,9 @@ __global__ __launch_bounds__(256) void latent_absorb_kernel(const LatentDecodePa
 // divides it is of the rounded ones; in bf16 that moves the result by 1.2e-3 of its
 // 2-norm. (Two 16-bit numbers a weight would take that to nothing and a third
 // more time: 64 x 128 heads 132 us for 101, and the result from 2.5e-3 to 2.3e-3.)
-// 64 sequences of 512 to 8192 keys, 128 heads: 101 us for 82 GFLOP and 339 MB of
+// 64 sequences of 512 to 8192 keys, 128 heads: 102 us for 82 GFLOP and 339 MB of
 // rows, the products and the rows about alike; 32 heads, two sequences of 228
-// thousand keys together 61 us (263 MB, 4.3 TB/s: the rows).
+// thousand keys together 60 us (263 MB, 4.4 TB/s: the rows).
 // NHG: waves side by side over heads, sharing a tile; 4 / NHG groups of waves
 // take tiles in turn. The LDS holds four tiles: a ring of NHG per group.
 template <int WP, int OB, int NHG, bool BF>

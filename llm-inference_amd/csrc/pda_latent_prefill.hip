@@ -507,7 +507,7 @@ __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(const PrefillPar
 // registers a lane) and the queries live in accumulator registers.
 // What takes the running maximum past 2^8 is found from the weights' sum after
 // the fact and weighed again (settle). Rounded as above. 128 heads, 4096 tokens 780 to
-// 830 us for 687 GFLOP (0.83 to 0.88 PFLOP/s), 16 heads, 512 at 7777 56 us for 42
+// 830 us for 687 GFLOP (0.83 to 0.88 PFLOP/s), 16 heads, 512 at 7777 54 us for 42
 // GFLOP; the matrix cores bound it at the clock that their load leaves.
 template <bool BF>
 __global__ __launch_bounds__(256, 1) void latent_prefill_wide_kernel(const PrefillParams p) {
