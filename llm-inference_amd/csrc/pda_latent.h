@@ -136,14 +136,22 @@ __device__ __forceinline__ uint32_t lds_address(const void* at) {
 // 16 bytes per lane from global memory straight into LDS: lane i's, from src +
 // kOff bytes, to dst + kOff + kPlus + 16 i (dst: wave-uniform; the
 // instruction adds its offset to both addresses). The caller waits
-// (wait_vmem) before the barrier that publishes them.
-template <int kOff, int kPlus>
+// (wait_vmem) before the barrier that publishes them. kOnce: data that nothing
+// reads again soon, which is not to displace what the caches hold.
+template <int kOff, int kPlus, bool kOnce = false>
 __device__ __forceinline__ void copy_to_lds(const void* src, uint32_t dst) {
   static_assert(kOff < 4096, "the instruction's offset has 12 bits");
-  asm volatile("s_add_u32 m0, %0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off offset:%3" ::"s"(
-                   dst),
-               "v"(src), "n"(kPlus), "n"(kOff)
-               : "memory", "m0", "scc");
+  if constexpr (kOnce)
+    asm volatile(
+        "s_add_u32 m0, %0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off offset:%3 nt" ::"s"(
+            dst),
+        "v"(src), "n"(kPlus), "n"(kOff)
+        : "memory", "m0", "scc");
+  else
+    asm volatile("s_add_u32 m0, %0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off offset:%3" ::"s"(
+                     dst),
+                 "v"(src), "n"(kPlus), "n"(kOff)
+                 : "memory", "m0", "scc");
 }
 
 // f(0), f(1), ... with compile-time arguments.

@@ -187,6 +187,7 @@ struct LatentDecodeParams {
   int32_t value;
   int32_t groups;        // workgroups the stream of tiles is cut over
   int32_t merge_batch;   // sequences a merge workgroup takes
+  int32_t once;          // rows past the caches
   float scale_log2;
 };
 
@@ -333,7 +334,7 @@ __global__ __launch_bounds__(256) void latent_absorb_kernel(const LatentDecodePa
 // more time: 64 x 128 heads 132 us for 101, and the result from 2.5e-3 to 2.3e-3.)
 // 64 sequences of 512 to 8192 keys, 128 heads: 102 us for 82 GFLOP and 339 MB of
 // rows, the products and the rows about alike; 32 heads, two sequences of 228
-// thousand keys together 60 us (263 MB, 4.4 TB/s: the rows).
+// thousand keys together 56 us (263 MB, 4.7 TB/s: the rows).
 // NHG: waves side by side over heads, sharing a tile; 4 / NHG groups of waves
 // take tiles in turn. The LDS holds four tiles: a ring of NHG per group.
 template <int WP, int OB, int NHG, bool BF>
@@ -489,10 +490,14 @@ __global__ __launch_bounds__(256, 1) void latent_decode_kernel(const LatentDecod
           const uint32_t dst =
               lds + (kg * NHG + slot) * (2 * kTile) + 1024 * (hg + NHG * i);
           const f16* src = p.arena + (int64_t)max(row[i], 0) * width;
-          if (whole) {
-            each_plane([&](auto j) {
-              copy_to_lds<128 * j.value, (2 * kPlane - 128) * j.value>(src + 8 * piece(i), dst);
-            });
+          auto plane = [&](auto j, auto once) {
+            copy_to_lds<128 * j.value, (2 * kPlane - 128) * j.value, once.value>(
+                src + 8 * piece(i), dst);
+          };
+          if (whole && p.once) {
+            each_plane([&](auto j) { plane(j, std::true_type{}); });
+          } else if (whole) {
+            each_plane([&](auto j) { plane(j, std::false_type{}); });
           } else {
 #pragma unroll 1
             for (int j = 0; j < WP; ++j)
@@ -881,6 +886,12 @@ __global__ __launch_bounds__(512, 2) void latent_merge_kernel(const LatentDecode
 // Host.
 
 constexpr int kMaxBatch = 8184;
+// Rows of so many bytes go past the caches: a quarter of what an MI355X's last
+// cache holds, so that from four layers on it would not have them at the next step.
+// (32 sequences of 4000 keys, 147 MB a layer, us a call kept and past: 8 layers in
+// turn, 16 heads 57 and 53, 64 heads 67 and 61; one layer again and again 55 and 57,
+// 63 and 67. Widths below the kernel's gain nothing and stay.)
+constexpr int64_t kOnceBytes = (int64_t)64 << 20;
 
 // Waves side by side over heads: as many as the heads fill, so that a tile is
 // copied once for all of them. (64 sequences of 512 to 8192 keys, us a call with 1,
@@ -1066,6 +1077,7 @@ int latent_decode(const void* queries, const void* arena, const void* kv_b, cons
   prm.groups = plan.groups;
   prm.scale_log2 = scale * kLog2e;
   // Sequences a merge workgroup takes: fewer while the CUs are not all used.
+  prm.once = (int64_t)batch * longest * (latent_dim + rope_dim) * 2 > kOnceBytes;
   // As many sequences a merging workgroup as leave one for each CU, 32 at most, the
   // columns of a product. (64 sequences, us a call with 8, with 32 and by the rule: 16
   // heads 78, 83, 78; 128 heads 147, 129, 129.)
