@@ -153,6 +153,23 @@ def test_decode_repeats_and_hint(gpu):
         assert bool(((a.cpu().double() - want).abs() <= bound).all())
 
 
+@pytest.mark.parametrize("heads", [16, 64, 128])
+def test_decode_past_the_caches(gpu, heads):
+    """A `longest` whose rows would pass what the caches hold: their rows are
+    copied the other way, over chunks of rows and in the middle of one."""
+    from instinct_amd.latent import latent_decode_attention
+
+    lengths, page = [2500, 1, 0, 130], 16
+    arena, kv_b, g = layer(WIDE, heads, 200 * page, torch.float16)
+    tables = pack(lengths, page, 200, g)
+    q = torch.randn((4, heads, 192), generator=g).to(torch.float16)
+    got = latent_decode_attention(*(x.to(gpu) for x in (q, arena, kv_b, tables)),
+                                  torch.tensor(lengths, dtype=torch.int32, device=gpu),
+                                  page_size=page, longest=1 << 17, scale=0.07)
+    want, bound = oracle.decode(q, arena, kv_b, tables, lengths, page_size=page, scale=0.07)
+    assert bool(((got.cpu().double() - want).abs() <= bound).all())
+
+
 def test_decode_far_rows(gpu):
     """Rows whose element offset passes 2^31."""
     latent, rope, nope, value = WIDE
