@@ -47,14 +47,17 @@ class DecodeBatch:
         *,
         positions: np.ndarray,
         tables: dict[str, list[np.ndarray]],
-        held: np.ndarray | None = None,
+        held: np.ndarray | dict[str, np.ndarray] | None = None,
         weights: dict[int, torch.Tensor] | None = None,
     ) -> None:
         """``held``: the rows each sequence's cache holds before this token,
         where rows were evicted (:meth:`KVCache.evict`) and it is no longer the
-        token's position. ``weights``: per layer float32 ``[batch, kv_heads,
-        capacity]``, to which the step's attention weights are added in place
-        (the new token's entry starts from them)."""
+        token's position; by group name in a cache of several groups, of which
+        those not named hold a row for every position. ``weights``: per layer
+        float32 ``[batch, kv_heads, capacity]``, to which the step's attention
+        weights are added in place (the new token's entry starts from them).
+        ``lengths`` and ``longest`` are those of the groups without evictions, or
+        of the only group."""
         device = cache.device
         self.weights = weights or {}
         self.cache = cache
@@ -62,19 +65,43 @@ class DecodeBatch:
         self.count = int(tokens.shape[0])
         positions = np.asarray(positions).astype(np.int64)
         self.offsets = torch.as_tensor(positions.astype(np.int32), device=device)
-        if held is not None:
-            positions = np.asarray(held).astype(np.int64)
-        self.lengths = torch.as_tensor((positions + 1).astype(np.int32), device=device)
+        by_group = self._held_rows(held)
+        if len(cache.groups) == 1:
+            positions = by_group.get(next(iter(cache.groups)), positions)
+        put = lambda n: torch.as_tensor((n + 1).astype(np.int32), device=device)  # noqa: E731
+        self.lengths = put(positions)
         self.longest = int(positions.max()) + 1
         page = cache.page_size
+        self._lengths: dict[str, torch.Tensor] = {}
+        self._longest: dict[str, int] = {}
         self._write: dict[str, torch.Tensor] = {}
         self._tables: dict[str, torch.Tensor] = {}
         for name in cache.groups:
+            at = by_group.get(name, positions)
+            self._lengths[name] = self.lengths if at is positions else put(at)
+            self._longest[name] = int(at.max()) + 1
             packed = pack_tables(tables[name], self.count)
-            pages = packed[np.arange(self.count), positions // page]
-            rows = (pages.astype(np.int64) * page + positions % page).astype(np.int32)
+            pages = packed[np.arange(self.count), at // page]
+            rows = (pages.astype(np.int64) * page + at % page).astype(np.int32)
             self._write[name] = torch.as_tensor(rows, device=device)
             self._tables[name] = torch.as_tensor(packed, device=device)
+
+    def _held_rows(self, held: np.ndarray | dict[str, np.ndarray] | None) -> dict[str, np.ndarray]:
+        """``held`` by group name, int64."""
+        groups = self.cache.groups
+        if held is None:
+            return {}
+        if not isinstance(held, dict):
+            if len(groups) > 1:
+                raise ValueError("held must name its groups in a cache of several")
+            held = dict.fromkeys(groups, held)
+        rows = {name: np.asarray(n).astype(np.int64) for name, n in held.items()}
+        for name, n in rows.items():
+            if name not in groups:
+                raise ValueError(f"held names no group {name!r}")
+            if n.shape != (self.count,) or np.any(n < 0):
+                raise ValueError("held must be the rows of each sequence")
+        return rows
 
     @property
     def positions(self) -> torch.Tensor:
@@ -125,18 +152,19 @@ class DecodeBatch:
         q = q.to(self.cache.decode_dtype).contiguous()
         if layer in self.weights:
             paged_attention_weights(
-                q, self.cache.keys[layer], self._tables[group.name], self.lengths,
-                self.weights[layer], page_size=self.cache.page_size, longest=self.longest,
-                scale=scale, window=group.window, softcap=softcap,
+                q, self.cache.keys[layer], self._tables[group.name], self._lengths[group.name],
+                self.weights[layer], page_size=self.cache.page_size,
+                longest=self._longest[group.name], scale=scale, window=group.window,
+                softcap=softcap,
                 scales=self.cache.scales(layer))
         out = paged_decode_attention(
             q,
             self.cache.keys[layer],
             self.cache.values[layer],
             self._tables[group.name],
-            self.lengths,
+            self._lengths[group.name],
             page_size=self.cache.page_size,
-            longest=self.longest,
+            longest=self._longest[group.name],
             scale=scale,
             window=group.window,
             softcap=softcap,
