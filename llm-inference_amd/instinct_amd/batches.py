@@ -78,6 +78,10 @@ class DecodeBatch:
         self._tables: dict[str, torch.Tensor] = {}
         for name in cache.groups:
             at = by_group.get(name, positions)
+            past = at // page >= np.array([len(table) for table in tables[name]])
+            if np.any(past):
+                b = int(np.argmax(past))
+                raise ValueError(f"group {name!r}: no page for row {at[b]} of sequence {b}")
             self._lengths[name] = self.lengths if at is positions else put(at)
             self._longest[name] = int(at.max()) + 1
             packed = pack_tables(tables[name], self.count)

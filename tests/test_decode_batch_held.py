@@ -65,3 +65,13 @@ def test_nothing_held_apart():
     b = batch(store, {"full": full, "local": LOCAL})
     assert rows(b, "full") == ([8 * PAGE + 5, 2 * PAGE + 4], [38, 21], 38)
     assert rows(b, "local")[1:] == ([38, 21], 38)
+
+
+@pytest.mark.parametrize("held", [None, {"full": np.array([16, 20])}])
+def test_a_row_needs_its_page(held):
+    """The packed tables are padded with page 0, another sequence's: a sequence
+    whose new row lies past its own pages (as after an eviction down to whole
+    pages) is refused."""
+    positions = (16, 20) if held is None else (37, 20)
+    with pytest.raises(ValueError, match="no page for row 16"):
+        batch(cache(("full", 0)), {"full": FULL}, positions=positions, held=held)
