@@ -55,7 +55,8 @@ class DecodeBatch:
         token's position; by group name in a cache of several groups, of which
         those not named hold a row for every position. ``weights``: per layer
         float32 ``[batch, kv_heads, capacity]``, to which the step's attention
-        weights are added in place (the new token's entry starts from them).
+        weights are added in place (the new token's entry starts from them);
+        the capacity holds every sequence with its new token.
         ``lengths`` and ``longest`` are those of the groups without evictions, or
         of the only group."""
         device = cache.device
@@ -89,6 +90,10 @@ class DecodeBatch:
             rows = (pages.astype(np.int64) * page + at % page).astype(np.int32)
             self._write[name] = torch.as_tensor(rows, device=device)
             self._tables[name] = torch.as_tensor(packed, device=device)
+        for layer, w in self.weights.items():
+            group = cache.layer_group.get(layer)
+            if group is None or w.shape[-1] < self._longest[group.name]:
+                raise ValueError(f"weights of layer {layer} must hold its longest sequence")
 
     def _held_rows(self, held: np.ndarray | dict[str, np.ndarray] | None) -> dict[str, np.ndarray]:
         """``held`` by group name, int64."""

@@ -139,7 +139,8 @@ def evict_rows(keys: torch.Tensor, values: torch.Tensor | None, weights: torch.T
     without it the rows move to the front of their own pages, which then must
     not be shared with another sequence. ``out_weights`` (``weights`` itself
     unless given) receives the kept positions' weights; its other entries are
-    left. ``longest`` is the host-side largest length. Returns (new lengths int32
+    left. ``longest`` is the host-side largest length, which tables and weights
+    must hold: rows past either could not be kept. Returns (new lengths int32
     ``[batch]``, kept positions int32 ``[batch, kv_heads, keep]``, -1 past a
     sequence's last)."""
     layout, arena_rows, kv_heads, head_dim = _arena_geometry(keys, page_size)
@@ -163,6 +164,10 @@ def evict_rows(keys: torch.Tensor, values: torch.Tensor | None, weights: torch.T
     capacity = _check_weights("weights", weights, batch, kv_heads, device)
     tables = _check_index("tables", tables, (batch, None), device)
     lengths = _check_index("lengths", lengths, (batch,), device)
+    if int(longest) > capacity:
+        raise ValueError(f"weights of {capacity} positions for a sequence of {int(longest)}")
+    if int(longest) > tables.shape[1] * page_size:
+        raise ValueError(f"tables of {tables.shape[1]} pages for a sequence of {int(longest)}")
     keep = int(keep)
     if out_tables is None:
         to = tables

@@ -75,3 +75,18 @@ def test_a_row_needs_its_page(held):
     positions = (16, 20) if held is None else (37, 20)
     with pytest.raises(ValueError, match="no page for row 16"):
         batch(cache(("full", 0)), {"full": FULL}, positions=positions, held=held)
+
+
+def test_weights_hold_every_sequence():
+    """A shorter capacity would cut a sequence's newest keys from its softmax."""
+    store = cache(("full", 0), ("local", 16))
+    tables = {"full": FULL, "local": LOCAL}
+    held = {"full": np.array([8, 20])}
+    fits = {0: torch.zeros((2, 1, 21)), 1: torch.zeros((2, 1, 38))}
+    assert batch(store, tables, held=held, weights=fits).weights is fits
+    for layer, capacity in ((0, 20), (1, 37)):
+        with pytest.raises(ValueError, match=f"layer {layer}"):
+            batch(store, tables, held=held,
+                  weights={**fits, layer: torch.zeros((2, 1, capacity))})
+    with pytest.raises(ValueError, match="layer 5"):
+        batch(store, tables, held=held, weights={5: torch.zeros((2, 1, 64))})

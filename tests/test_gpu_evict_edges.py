@@ -1,0 +1,36 @@
+"""Calls of the eviction at the edges of what it takes."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def layer(gpu, pages, page=16, heads=2, dim=64, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    keys, values = (torch.randn((pages, heads, page, dim), generator=g).half().to(gpu)
+                    for _ in range(2))
+    return keys, values, g
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+def test_weights_and_tables_hold_the_longest(gpu, in_place):
+    """Rows past either were lost without an error; nothing is touched."""
+    from instinct_amd.eviction import evict_rows
+
+    keys, values, _ = layer(gpu, 8)
+    before = keys.clone(), values.clone()
+    tables = torch.arange(4, dtype=torch.int32, device=gpu)[None]
+    lengths = torch.tensor([60], dtype=torch.int32, device=gpu)
+    kw = dict(page_size=16, longest=60, keep=32, recent=8,
+              out_tables=None if in_place else tables + 4)
+    for capacity in (59, 31):
+        w = torch.ones((1, 2, capacity), device=gpu)
+        with pytest.raises(ValueError, match=f"weights of {capacity} positions"):
+            evict_rows(keys, values, w, tables, lengths, **kw)
+    w = torch.ones((1, 2, 60), device=gpu)
+    with pytest.raises(ValueError, match="tables of 3 pages"):
+        evict_rows(keys, values, w, tables[:, :3], lengths, **kw)
+    assert torch.equal(keys, before[0]) and torch.equal(values, before[1])
+    n, kept = evict_rows(keys, values, w, tables, lengths, **kw)
+    assert n.tolist() == [32] and kept[0, 0, -8:].tolist() == list(range(52, 60))
