@@ -33,8 +33,9 @@ def _check_index(name: str, t: torch.Tensor, shape: tuple, device: torch.device)
     return t.contiguous()
 
 
-def _check_weights(name: str, t: torch.Tensor, batch: int, kv_heads: int,
-                   device: torch.device) -> int:
+def check_weights(name: str, t: torch.Tensor, batch: int, kv_heads: int,
+                  device: torch.device) -> int:
+    """The capacity of float32 weights ``[batch, kv_heads, capacity]``."""
     if t.dtype != torch.float32:
         raise TypeError(f"{name} must be float32")
     if t.dim() != 3 or t.shape[0] != batch or t.shape[1] != kv_heads or t.shape[2] == 0:
@@ -96,10 +97,10 @@ def paged_attention_weights(queries: torch.Tensor, keys: torch.Tensor, tables: t
             raise ValueError("key_scales must have one scale per row and kv head")
     tables = _check_index("tables", tables, (batch, None), device)
     lengths = _check_index("lengths", lengths, (batch,), device)
-    capacity = _check_weights("weights", weights, batch, kv_heads, device)
+    capacity = check_weights("weights", weights, batch, kv_heads, device)
     if out is None:
         out = weights
-    elif _check_weights("out", out, batch, kv_heads, device) != capacity:
+    elif check_weights("out", out, batch, kv_heads, device) != capacity:
         raise ValueError("out must have the weights' shape")
     if batch == 0:
         return out
@@ -161,7 +162,7 @@ def evict_rows(keys: torch.Tensor, values: torch.Tensor | None, weights: torch.T
         raise ValueError("an int8 cache needs its scales")
     device = keys.device
     batch = int(weights.shape[0])
-    capacity = _check_weights("weights", weights, batch, kv_heads, device)
+    capacity = check_weights("weights", weights, batch, kv_heads, device)
     tables = _check_index("tables", tables, (batch, None), device)
     lengths = _check_index("lengths", lengths, (batch,), device)
     if int(longest) > capacity:
@@ -177,7 +178,7 @@ def evict_rows(keys: torch.Tensor, values: torch.Tensor | None, weights: torch.T
             raise ValueError("out_tables must have pages for the kept rows")
     if out_weights is None:
         out_weights = weights
-    out_capacity = _check_weights("out_weights", out_weights, batch, kv_heads, device)
+    out_capacity = check_weights("out_weights", out_weights, batch, kv_heads, device)
     kept = torch.empty((batch, kv_heads, max(keep, 0)), dtype=torch.int32, device=device)
     new_lengths = torch.empty(batch, dtype=torch.int32, device=device)
     lib = _lib.library()

@@ -190,6 +190,12 @@ class PagePool:
             raise RuntimeError("cannot share a page that is not allocated")
         self._refs[unique] += counts
 
+    def holds(self, pages: Iterable[int]) -> bool:
+        """Whether every listed page has a reference for each time it is listed
+        (:meth:`release` would take the list)."""
+        unique, counts = self._held(pages)
+        return not np.any(self._refs[unique] < counts)
+
     def held_only_by(self, counts: np.ndarray) -> int:
         """Pages that would come free if ``counts[page]`` of each page's
         references were dropped: those held by exactly that many references
@@ -332,10 +338,11 @@ class KVCache:
         (:func:`instinct_amd.eviction.evict_rows`). Pages no longer needed go
         back to the pool. Where a cut sequence shares a page it would write
         (a common prefix), the cut sequences move to fresh pages instead.
-        Returns the new page lists and lengths; the next token of a sequence
-        goes to row ``lengths[b]`` while its position counts on
+        What is wrong with the arguments is found before any layer or page
+        changes. Returns the new page lists and lengths; the next token of a
+        sequence goes to row ``lengths[b]`` while its position counts on
         (``DecodeBatch(held=...)``). No counterpart in the reference."""
-        from .eviction import evict_rows
+        from .eviction import check_weights, evict_rows
 
         group, pool = self.groups[name], self.pools[name]
         if group.window:
@@ -344,6 +351,8 @@ class KVCache:
             raise ValueError("keep must be positive and hold recent and sinks")
         lengths = np.asarray(lengths, dtype=np.int64)
         tables = [np.asarray(t, dtype=np.int64) for t in tables]
+        if lengths.shape != (len(tables),):
+            raise ValueError("lengths must be those of the tables")
         need = [-(-int(n) // self.page_size) for n in lengths]
         for table, pages in zip(tables, need):
             if len(table) < pages or np.any(table[:pages] < 0):
@@ -351,28 +360,43 @@ class KVCache:
         cut = [b for b, n in enumerate(lengths) if n > keep]
         if not cut:
             return tables, lengths
+        if not pool.holds(np.concatenate([tables[b] for b in cut])):
+            raise RuntimeError("a sequence to evict from lists pages that it does not hold")
         front = -(-keep // self.page_size)
         packed = np.zeros((len(tables), max(need)), dtype=np.int32)
         for b, pages in enumerate(need):
             packed[b, :pages] = tables[b][:pages]
         # Pages that more than one place of these tables, or another holder, has.
         shared = any(pool.shared(int(page)) for b in cut for page in tables[b][:front])
-        out, fresh = None, {}
-        if shared:
-            taken = pool.allocate_many(front * len(cut), reserved=False).reshape(len(cut), front)
-            fresh = dict(zip(cut, taken))
-            out = np.zeros_like(packed)
-            for b, pages in enumerate(need):
-                new = fresh.get(b, tables[b][:pages])
-                out[b, :len(new)] = new
-        put = lambda a: torch.as_tensor(a.astype(np.int32), device=self.device)  # noqa: E731
-        dev_tables, dev_lengths = put(packed), put(lengths)
-        dev_out = None if out is None else put(out)
-        for layer in group.layers:
-            evict_rows(self.keys[layer], self.values[layer], weights[layer], dev_tables,
-                       dev_lengths, page_size=self.page_size, longest=int(lengths.max()),
-                       keep=keep, recent=recent, sinks=sinks, scales=self.scales(layer),
-                       out_tables=dev_out)
+        taken = pool.allocate_many(front * len(cut) if shared else 0, reserved=False)
+        try:
+            # Every layer's weights before the first layer is packed.
+            for layer in group.layers:
+                w = weights.get(layer)
+                if w is None:
+                    raise ValueError(f"no weights of layer {layer}")
+                capacity = check_weights(f"weights of layer {layer}", w, len(tables),
+                                         group.kv_heads, self.keys[layer].device)
+                if capacity < int(lengths.max()):
+                    raise ValueError(f"weights of layer {layer} must hold its longest sequence")
+            out, fresh = None, {}
+            if shared:
+                fresh = dict(zip(cut, taken.reshape(len(cut), front)))
+                out = np.zeros_like(packed)
+                for b, pages in enumerate(need):
+                    new = fresh.get(b, tables[b][:pages])
+                    out[b, :len(new)] = new
+            put = lambda a: torch.as_tensor(a.astype(np.int32), device=self.device)  # noqa: E731
+            dev_tables, dev_lengths = put(packed), put(lengths)
+            dev_out = None if out is None else put(out)
+            for layer in group.layers:
+                evict_rows(self.keys[layer], self.values[layer], weights[layer], dev_tables,
+                           dev_lengths, page_size=self.page_size, longest=int(lengths.max()),
+                           keep=keep, recent=recent, sinks=sinks, scales=self.scales(layer),
+                           out_tables=dev_out)
+        except BaseException:
+            pool.release(taken)
+            raise
         # (On this stream the rows are read before anything that follows writes
         # the pages given back.)
         for b in cut:
