@@ -756,7 +756,8 @@ int pda_attention_weights_q8_bf16(const void* queries, const void* keys,
  *   out_weights [batch, kv_heads, out_capacity] (may be NULL, or weights
  *               itself): the kept positions' weights, in that order; the rest
  *               is left as it was
- * recent + sinks <= keep. One launch, no workspace. */
+ * recent + sinks <= keep; capacity and keep below 2^31 - 8192. One launch, no
+ * workspace. */
 int pda_evict_select(const float* weights, float* out_weights,
                      const int32_t* tables, const int32_t* lengths, int32_t* kept,
                      int32_t* new_lengths, int32_t batch, int32_t kv_heads,

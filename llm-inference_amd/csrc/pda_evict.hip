@@ -524,6 +524,11 @@ int attention_weights(const void* queries, const void* keys, const void* key_sca
 
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectWaves = kSelectThreads / 64;
+constexpr int kSelectEach = 8;  // positions a thread holds
+constexpr int kSelectBlock = kSelectEach * kSelectThreads;
+// Positions and kept rows of a sequence: the loops go on by a block at most past
+// the last, in 32 bits.
+constexpr int kMaxPositions = INT32_MAX - kSelectBlock;
 constexpr int kBins = 2048;
 
 struct SelectParams {
@@ -574,7 +579,7 @@ __device__ __forceinline__ int scan64(int x) {
 // by its chain of reads and meetings: 1100 positions 12 us, 128 times up to 8079
 // 16 us.
 __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const SelectParams p) {
-  constexpr int kEach = 8, kBlock = kEach * kSelectThreads;
+  constexpr int kEach = kSelectEach, kBlock = kSelectBlock;
   constexpr int kGroups = kEach * kSelectWaves;  // ballots of a block
   // (Two of each, so that a digit's need no meeting before the next one's.)
   __shared__ int s_hist[2][kBins];
@@ -802,7 +807,7 @@ __global__ __launch_bounds__(256) void evict_copy_kernel(const MoveParams p) {
   char* arena = p.arena[blockIdx.y / p.hkv];
   const int pieces = p.width / (int)sizeof(V);
   const int across = min(pieces, 256), rows = 256 / across;  // threads a row, rows a pass
-  const int total = p.new_lengths[b];
+  const int total = min(p.new_lengths[b], p.keep);
   const int32_t* kept = p.kept + ((int64_t)b * p.hkv + kvh) * p.keep;
   const int32_t* from = p.tables + (int64_t)b * p.table_stride;
   const int32_t* to = p.out_tables + (int64_t)b * p.out_stride;
@@ -857,7 +862,7 @@ __global__ __launch_bounds__(256) void evict_pack_kernel(const MoveParams p) {
   const int kvh = blockIdx.y, b = blockIdx.z;
   const int c = slice * kSlice + (threadIdx.x % kPieces) * (int)sizeof(V);
   const bool mine = c < p.width;
-  const int total = p.new_lengths[b];
+  const int total = min(p.new_lengths[b], p.keep);
   const int32_t* kept = p.kept + ((int64_t)b * p.hkv + kvh) * p.keep;
   const int32_t* table = p.tables + (int64_t)b * p.table_stride;
   for (int r0 = 0; r0 < total; r0 += kRows * kEach) {
@@ -980,8 +985,8 @@ int pda_evict_select(const float* weights, float* out_weights, const int32_t* ta
   if (arena_rows < page_size)
     return fail(PDA_ERR_INVALID_ARGUMENT, "arena_rows %lld holds no whole page",
                 (long long)arena_rows);
-  if (capacity > INT32_MAX - 4 * kSelectThreads)
-    return fail(PDA_ERR_TOO_LONG, "capacity %d next to 2^31", capacity);
+  if (capacity > kMaxPositions || keep > kMaxPositions)
+    return fail(PDA_ERR_TOO_LONG, "capacity %d or keep %d next to 2^31", capacity, keep);
   if (((uintptr_t)weights | (uintptr_t)out_weights | (uintptr_t)tables | (uintptr_t)lengths |
        (uintptr_t)kept | (uintptr_t)new_lengths) & 3)
     return fail(PDA_ERR_ALIGNMENT, "all buffers must be 4-byte aligned");
@@ -1028,6 +1033,7 @@ int pda_evict_move(void* arena, void* arena2, int32_t width, const int32_t* kept
   if (arena_rows < page_size)
     return fail(PDA_ERR_INVALID_ARGUMENT, "arena_rows %lld holds no whole page",
                 (long long)arena_rows);
+  if (keep > kMaxPositions) return fail(PDA_ERR_TOO_LONG, "keep %d next to 2^31", keep);
   if (((uintptr_t)kept | (uintptr_t)new_lengths | (uintptr_t)tables | (uintptr_t)out_tables) & 3)
     return fail(PDA_ERR_ALIGNMENT, "index buffers must be 4-byte aligned");
   MoveParams prm;
