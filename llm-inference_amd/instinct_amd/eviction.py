@@ -33,6 +33,12 @@ def _check_index(name: str, t: torch.Tensor, shape: tuple, device: torch.device)
     return t.contiguous()
 
 
+def _same_columns(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two matrices of as many rows begin with the same columns in memory."""
+    return (a.data_ptr() == b.data_ptr() and a.shape[0] == b.shape[0]
+            and a.stride(-1) == b.stride(-1) and (a.shape[0] < 2 or a.stride(0) == b.stride(0)))
+
+
 def check_weights(name: str, t: torch.Tensor, batch: int, kv_heads: int,
                   device: torch.device) -> int:
     """The capacity of float32 weights ``[batch, kv_heads, capacity]``."""
@@ -137,13 +143,13 @@ def evict_rows(keys: torch.Tensor, values: torch.Tensor | None, weights: torch.T
     None: ``keys`` alone, as for one arena of latent rows), int8 with their
     ``scales`` at 8 bits. ``out_tables`` int32 ``[batch, width]`` names pages
     that no row is read from (a position that stays where it is excepted);
-    without it the rows move to the front of their own pages, which then must
-    not be shared with another sequence. ``out_weights`` (``weights`` itself
-    unless given) receives the kept positions' weights; its other entries are
-    left. ``longest`` is the host-side largest length, which tables and weights
-    must hold: rows past either could not be kept. Returns (new lengths int32
-    ``[batch]``, kept positions int32 ``[batch, kv_heads, keep]``, -1 past a
-    sequence's last)."""
+    without it, or where it is ``tables`` or its first columns, the rows move to
+    the front of their own pages, which then must not be shared with another
+    sequence. ``out_weights`` (``weights`` itself unless given) receives the kept
+    positions' weights; its other entries are left. ``longest`` is the host-side
+    largest length, which tables and weights must hold: rows past either could
+    not be kept. Returns (new lengths int32 ``[batch]``, kept positions int32
+    ``[batch, kv_heads, keep]``, -1 past a sequence's last)."""
     layout, arena_rows, kv_heads, head_dim = _arena_geometry(keys, page_size)
     dtype = torch.int8 if scales is not None else keys.dtype
     if dtype not in (torch.int8, torch.float16, torch.bfloat16):
@@ -163,6 +169,7 @@ def evict_rows(keys: torch.Tensor, values: torch.Tensor | None, weights: torch.T
     device = keys.device
     batch = int(weights.shape[0])
     capacity = check_weights("weights", weights, batch, kv_heads, device)
+    given = tables  # (the library compares addresses, which a copy would change)
     tables = _check_index("tables", tables, (batch, None), device)
     lengths = _check_index("lengths", lengths, (batch,), device)
     if int(longest) > capacity:
@@ -176,6 +183,8 @@ def evict_rows(keys: torch.Tensor, values: torch.Tensor | None, weights: torch.T
         to = _check_index("out_tables", out_tables, (batch, None), device)
         if int(to.shape[1]) * page_size < min(keep, capacity, int(longest)):
             raise ValueError("out_tables must have pages for the kept rows")
+        if _same_columns(out_tables, given):
+            to = tables
     if out_weights is None:
         out_weights = weights
     out_capacity = check_weights("out_weights", out_weights, batch, kv_heads, device)

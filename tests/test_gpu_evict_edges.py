@@ -34,3 +34,23 @@ def test_weights_and_tables_hold_the_longest(gpu, in_place):
     assert torch.equal(keys, before[0]) and torch.equal(values, before[1])
     n, kept = evict_rows(keys, values, w, tables, lengths, **kw)
     assert n.tolist() == [32] and kept[0, 0, -8:].tolist() == list(range(52, 60))
+
+
+def test_tables_in_a_wider_one_are_in_place(gpu):
+    """Columns of a wider table as both tables, or their first ones: rows move to the front of their own
+    pages, as without out_tables."""
+    from instinct_amd.eviction import evict_rows
+
+    wide = torch.randperm(24, generator=torch.Generator().manual_seed(3)).int().view(2, 12).to(gpu)
+    tables = wide[:, 2:10]
+    lengths = torch.tensor([128, 90], dtype=torch.int32, device=gpu)
+    kw = dict(page_size=16, longest=128, keep=70, recent=8, sinks=2)
+    results = []
+    for out_tables in (None, tables, wide[:, 2:10], wide[:, 2:7]):
+        keys, values, g = layer(gpu, 24)
+        w = torch.rand((2, 2, 128), generator=g).to(gpu)
+        n, kept = evict_rows(keys, values, w, tables, lengths, out_tables=out_tables, **kw)
+        results.append((n, kept, w, keys, values))
+    assert results[0][0].tolist() == [70, 70]
+    for got in results[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(got, results[0]))
