@@ -1036,6 +1036,7 @@ int pda_evict_move(void* arena, void* arena2, int32_t width, const int32_t* kept
   if (keep > kMaxPositions) return fail(PDA_ERR_TOO_LONG, "keep %d next to 2^31", keep);
   if (((uintptr_t)kept | (uintptr_t)new_lengths | (uintptr_t)tables | (uintptr_t)out_tables) & 3)
     return fail(PDA_ERR_ALIGNMENT, "index buffers must be 4-byte aligned");
+  if (arena2 == arena) arena2 = nullptr;  // (once: two walks of one slice would race)
   MoveParams prm;
   prm.arena[0] = static_cast<char*>(arena);
   prm.arena[1] = static_cast<char*>(arena2);

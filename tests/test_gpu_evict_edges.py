@@ -54,3 +54,20 @@ def test_tables_in_a_wider_one_are_in_place(gpu):
     assert results[0][0].tolist() == [70, 70]
     for got in results[1:]:
         assert all(torch.equal(a, b) for a, b in zip(got, results[0]))
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+def test_one_arena_as_keys_and_values(gpu, in_place):
+    """Rows move once, as with the keys alone."""
+    from instinct_amd.eviction import evict_rows
+
+    tables = torch.randperm(80, generator=torch.Generator().manual_seed(4)).int().to(gpu)[None]
+    lengths = torch.tensor([1000], dtype=torch.int32, device=gpu)
+    stores = []
+    for both in (False, True):
+        keys, _, g = layer(gpu, 80, seed=5)
+        w = torch.rand((1, 2, 1000), generator=g).to(gpu)
+        evict_rows(keys, keys if both else None, w, tables[:, :63], lengths, page_size=16,
+                   longest=1000, keep=260, out_tables=None if in_place else tables[:, 63:])
+        stores.append(keys)
+    assert torch.equal(*stores)
