@@ -349,7 +349,7 @@ __global__ __launch_bounds__(256) void attention_weights_kernel(const WeightPara
 #pragma unroll
         for (int d = 32; d; d >>= 1)
           all = join(all, make_float2(__shfl_xor(all.x, d), __shfl_xor(all.y, d)));
-        // (A head that sees no key gives nothing; its sum is 0, or NaN.)
+        // (A head that sees no key gives nothing.)
         if (lane == 0)
           s_stats[i] = make_float2(all.x == -INFINITY ? 0.0f : all.x,
                                    all.y == 0.0f ? 0.0f : 1.0f / all.y);
@@ -361,7 +361,10 @@ __global__ __launch_bounds__(256) void attention_weights_kernel(const WeightPara
         const float2 st = s_stats[j];
 #pragma unroll
         for (int i = 0; i < kEach; ++i)
-          acc[i] = fmaf(__builtin_amdgcn_exp2f(x[j][i] - st.x), st.y, acc[i]);
+          // (A hidden key gets nothing, also beside a visible one that is NaN.)
+          acc[i] = x[j][i] == -INFINITY
+                       ? acc[i]
+                       : fmaf(__builtin_amdgcn_exp2f(x[j][i] - st.x), st.y, acc[i]);
       }
     }
 #pragma unroll

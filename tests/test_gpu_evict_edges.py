@@ -71,3 +71,25 @@ def test_one_arena_as_keys_and_values(gpu, in_place):
                    longest=1000, keep=260, out_tables=None if in_place else tables[:, 63:])
         stores.append(keys)
     assert torch.equal(*stores)
+
+
+def test_hidden_keys_beside_a_nan(gpu):
+    """A visible key of NaN makes the visible credits NaN; keys that the window or
+    their page hides keep what they had."""
+    from instinct_amd.eviction import paged_attention_weights
+
+    keys, _, g = layer(gpu, 8)
+    tables = torch.arange(8, dtype=torch.int32, device=gpu)[None].contiguous()
+    tables[0, 5] = -1
+    keys[6, 0, 3] = float("nan")  # position 99 of kv head 0
+    q = torch.randn((1, 4, 64), generator=g).half().to(gpu)
+    w = torch.rand((1, 2, 128), generator=g).to(gpu)
+    lengths = torch.tensor([120], dtype=torch.int32, device=gpu)
+    out = paged_attention_weights(q, keys, tables, lengths, w, page_size=16, longest=120, scale=0.1,
+                                  window=60, out=torch.zeros_like(w))
+    hidden = [t for t in range(119) if t < 60 or 80 <= t < 96]
+    seen = [t for t in range(120) if t not in hidden]
+    assert torch.equal(out[0, :, hidden], w[0, :, hidden])
+    assert bool(out[0, 0, seen].isnan().all())
+    # The other kv head's weights: two heads that each sum to 1.
+    assert abs(float((out[0, 1, seen] - w[0, 1, seen]).sum() + w[0, 1, 119]) - 2) < 1e-4
