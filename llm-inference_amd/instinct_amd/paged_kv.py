@@ -335,7 +335,7 @@ class KVCache:
         ``recent`` and the heaviest other rows by ``weights[layer]`` (``[batch,
         kv_heads, capacity]``, as ``DecodeBatch`` accumulates them), packed in
         order at the front of the sequence's pages, the weights with them
-        (:func:`instinct_amd.eviction.evict_rows`). Pages no longer needed go
+        (:func:`instinct_amd.eviction.evict_rows`) and zeros behind. Pages no longer needed go
         back to the pool. Where a cut sequence shares a page it would write
         (a common prefix), the cut sequences move to fresh pages instead.
         What is wrong with the arguments is found before any layer or page
@@ -394,6 +394,10 @@ class KVCache:
                            dev_lengths, page_size=self.page_size, longest=int(lengths.max()),
                            keep=keep, recent=recent, sinks=sinks, scales=self.scales(layer),
                            out_tables=dev_out)
+            # What the dropped keys were given, which rows to come would start from.
+            which = torch.as_tensor(cut, device=self.device)
+            for layer in group.layers:
+                weights[layer][..., keep:].index_fill_(0, which, 0.0)
         except BaseException:
             pool.release(taken)
             raise

@@ -77,3 +77,23 @@ def test_one_group_cut(gpu):
             credits[b][j] = [credits[b][j][t] for t in pick]
     for _ in range(3):
         step()
+
+
+@pytest.mark.parametrize("shared", [False, True])
+def test_rows_to_come_start_from_nothing(gpu, shared):
+    """The credits behind a cut sequence's rows are zeros, not those of dropped
+    keys; other sequences' are left."""
+    cache = KVCache([KVGroup("full", (0, 1), KV, DIM)], page_size=PAGE, capacities={"full": 16},
+                    device=gpu)
+    pool = cache.pools["full"]
+    tables = [pool.allocate_many(4, reserved=False) for _ in range(2)]
+    if shared:
+        pool.retain(tables[0][:1])
+    g = torch.Generator().manual_seed(6)
+    weights = {i: torch.rand((2, KV, 70), generator=g).to(gpu) for i in range(2)}
+    before = {i: w.clone() for i, w in weights.items()}
+    _, held = cache.evict("full", tables, np.array([60, 30]), weights, keep=32, recent=4)
+    assert held.tolist() == [32, 30]
+    for i, w in weights.items():
+        assert bool((w[0, :, :32] > 0).all()) and bool((w[0, :, 32:] == 0).all())
+        assert torch.equal(w[1], before[i][1])
