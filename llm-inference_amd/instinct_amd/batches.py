@@ -37,6 +37,23 @@ def pack_tables(tables: list[np.ndarray] | list[list[int]], count: int) -> np.nd
     return packed
 
 
+def rows_by_group(cache: KVCache, held: Any, shape: tuple[int, ...]) -> dict[str, np.ndarray]:
+    """The rows that sequences hold, int64 of ``shape``, by group name; one value
+    for a cache of one group."""
+    groups = cache.groups
+    if not isinstance(held, dict):
+        if len(groups) > 1:
+            raise ValueError("held must name its groups in a cache of several")
+        held = dict.fromkeys(groups, held)
+    rows = {name: np.asarray(n).astype(np.int64) for name, n in held.items()}
+    for name, n in rows.items():
+        if name not in groups:
+            raise ValueError(f"held names no group {name!r}")
+        if n.shape != shape or np.any(n < 0):
+            raise ValueError("held must be the rows of each sequence")
+    return rows
+
+
 class DecodeBatch:
     prefill = False
 
@@ -66,7 +83,7 @@ class DecodeBatch:
         self.count = int(tokens.shape[0])
         positions = np.asarray(positions).astype(np.int64)
         self.offsets = torch.as_tensor(positions.astype(np.int32), device=device)
-        by_group = self._held_rows(held)
+        by_group = {} if held is None else rows_by_group(cache, held, (self.count,))
         if len(cache.groups) == 1:
             positions = by_group.get(next(iter(cache.groups)), positions)
         put = lambda n: torch.as_tensor((n + 1).astype(np.int32), device=device)  # noqa: E731
@@ -94,23 +111,6 @@ class DecodeBatch:
             group = cache.layer_group.get(layer)
             if group is None or w.shape[-1] < self._longest[group.name]:
                 raise ValueError(f"weights of layer {layer} must hold its longest sequence")
-
-    def _held_rows(self, held: np.ndarray | dict[str, np.ndarray] | None) -> dict[str, np.ndarray]:
-        """``held`` by group name, int64."""
-        groups = self.cache.groups
-        if held is None:
-            return {}
-        if not isinstance(held, dict):
-            if len(groups) > 1:
-                raise ValueError("held must name its groups in a cache of several")
-            held = dict.fromkeys(groups, held)
-        rows = {name: np.asarray(n).astype(np.int64) for name, n in held.items()}
-        for name, n in rows.items():
-            if name not in groups:
-                raise ValueError(f"held names no group {name!r}")
-            if n.shape != (self.count,) or np.any(n < 0):
-                raise ValueError("held must be the rows of each sequence")
-        return rows
 
     @property
     def positions(self) -> torch.Tensor:
@@ -194,7 +194,12 @@ class PrefillBatch:
     prefill = True
 
     def __init__(self, cache: KVCache, tokens: torch.Tensor, *, start: int,
-                 tables: dict[str, np.ndarray], images: Any = ()) -> None:
+                 tables: dict[str, np.ndarray], images: Any = (),
+                 held: int | dict[str, int] | None = None) -> None:
+        """``held``: the rows that the sequence's cache holds before the chunk,
+        where rows were evicted and it is no longer ``start``; by group name as
+        for :class:`DecodeBatch`. The chunk is rotated at its positions and
+        written behind the rows held, all of which it sees."""
         device = cache.device
         self.cache = cache
         self.tokens = tokens
@@ -202,14 +207,19 @@ class PrefillBatch:
         self.start = int(start)
         self.images = list(images)
         end = self.start + self.count
+        rows = {} if held is None else rows_by_group(cache, held, ())
+        # First row of the chunk in each group.
+        self._starts = {name: int(rows.get(name, self.start)) for name in cache.groups}
+        if self.images and set(self._starts.values()) != {self.start}:
+            raise ValueError("images need a cache from which no rows were evicted")
         self._spans = image_spans(
             [(at, x if isinstance(x, int) else int(x.shape[0])) for at, x in self.images], device)
         self.offsets = torch.arange(self.start, end, dtype=torch.int32, device=device)
         self._write: dict[str, torch.Tensor] = {}
         self._tables: dict[str, torch.Tensor] = {}
-        for name in cache.groups:
+        for name, first in self._starts.items():
             table = np.asarray(tables[name])
-            self._write[name] = torch.as_tensor(cache.rows(table, self.start, end),
+            self._write[name] = torch.as_tensor(cache.rows(table, first, first + self.count),
                                                 device=device)
             self._tables[name] = torch.as_tensor(table.astype(np.int32), device=device)
 
@@ -244,7 +254,8 @@ class PrefillBatch:
         out = paged_prefill_attention(
             q.to(self.cache.compute_dtype).contiguous(), self.cache.keys[layer],
             self.cache.values[layer],
-            self._tables[group.name], start=self.start, page_size=self.cache.page_size,
+            self._tables[group.name], start=self._starts[group.name],
+            page_size=self.cache.page_size,
             scale=scale, window=group.window, softcap=softcap,
             scales=self.cache.scales(layer),
             images=self._spans if self._spans is not None else ())

@@ -38,7 +38,9 @@ class DecodeStepGraph:
     value_scales)`` (8-bit); bf16 arenas take bf16 q/k/v and give bf16
     outputs, fp16 and 8-bit arenas fp16 ones; all layers share ``seq_tables``
     (``[num_slots, stride]`` int32 resident page lists), the page size, the
-    window and the head shape. ``dims``/``base``/``freqs``: the rotary
+    window and the head shape. A sequence holds a row for every position: steps
+    over an evicted cache, and steps that credit weights, are
+    :class:`instinct_amd.batches.DecodeBatch`'s. ``dims``/``base``/``freqs``: the rotary
     embedding (``dims`` = 0: none)."""
 
     def __init__(self, arenas: Sequence[tuple[torch.Tensor, ...]], seq_tables: torch.Tensor, *,
