@@ -771,9 +771,10 @@ int pda_evict_select(const float* weights, float* out_weights,
  * bytes: head_dim elements, or 2 for a scale arena. out_tables is tables itself
  * (the same pointer: the rows move to the front of their own pages) or names
  * pages that no row is read from, except where a position stays where it is. A
- * page that is written belongs to one sequence; rows whose place is not in the
- * arena or past out_stride pages are dropped. keep below 2^31 - 8192. One launch,
- * no workspace. */
+ * page that is written belongs to one sequence. Rows whose place is not in the
+ * arena or past out_stride pages are dropped, though new_lengths counts them:
+ * in place, pages that a sequence has released must lie past its kept rows.
+ * keep below 2^31 - 8192. One launch, no workspace. */
 int pda_evict_move(void* arena, void* arena2, int32_t width, const int32_t* kept,
                    const int32_t* new_lengths, const int32_t* tables,
                    const int32_t* out_tables, int32_t batch, int32_t kv_heads,

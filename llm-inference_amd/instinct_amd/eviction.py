@@ -145,7 +145,10 @@ def evict_rows(keys: torch.Tensor, values: torch.Tensor | None, weights: torch.T
     that no row is read from (a position that stays where it is excepted);
     without it, or where it is ``tables`` or its first columns, the rows move to
     the front of their own pages, which then must not be shared with another
-    sequence. ``out_weights`` (``weights`` itself unless given) receives the kept
+    sequence; the first ``keep`` rows' pages must all be there then, since a kept
+    row whose place lies on a page that is gone has nowhere to go and is lost
+    (it still counts: its place is hidden like any on that page). Sequences that
+    released their first pages need ``out_tables``. ``out_weights`` (``weights`` itself unless given) receives the kept
     positions' weights; its other entries are left. ``longest`` is the host-side
     largest length, which tables and weights must hold: rows past either could
     not be kept. Returns (new lengths int32 ``[batch]``, kept positions int32

@@ -93,3 +93,28 @@ def test_hidden_keys_beside_a_nan(gpu):
     assert bool(out[0, 0, seen].isnan().all())
     # The other kv head's weights: two heads that each sum to 1.
     assert abs(float((out[0, 1, seen] - w[0, 1, seen]).sum() + w[0, 1, 119]) - 2) < 1e-4
+
+
+@pytest.mark.parametrize("holes, in_place", [((5, 7), True), ((0, 2, 7), False)])
+def test_no_kept_row_is_lost_to_released_pages(gpu, holes, in_place):
+    """In place with the released pages past the kept rows, else on other pages with
+    any released: every kept row is found at its place."""
+    from instinct_amd.eviction import evict_rows
+
+    keys, values, g = layer(gpu, 32)
+    before = keys.cpu(), values.cpu()
+    tables = torch.arange(16, dtype=torch.int32)[None]
+    tables[0, list(holes)] = -1
+    out = tables if in_place else torch.arange(16, 32, dtype=torch.int32)[None]
+    w = torch.rand((1, 2, 200), generator=g).to(gpu)
+    n, kept = evict_rows(keys, values, w, tables.to(gpu),
+                         torch.tensor([200], dtype=torch.int32, device=gpu), page_size=16,
+                         longest=200, keep=70, recent=6, sinks=3,
+                         out_tables=None if in_place else out.to(gpu))
+    assert n.tolist() == [70]
+    for old, new in zip(before, (keys.cpu(), values.cpu())):
+        for j in range(2):
+            for i, t in enumerate(kept[0, j].tolist()):
+                assert t // 16 not in holes
+                assert torch.equal(new[out[0, i // 16], j, i % 16],
+                                   old[tables[0, t // 16], j, t % 16])
