@@ -33,6 +33,7 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kMaxLatent = 512;  // latent width
 constexpr int kMaxRope = 64;     // rotary dims of a row
 constexpr int kMaxHead = 128;    // nope dims and value dims of a head
+constexpr int64_t kMaxGrid = UINT32_MAX / 256;  // workgroups of 256 threads a launch takes
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 

@@ -1013,8 +1013,8 @@ int latent_append(const void* q, void* q_out, const void* latent, int64_t latent
   prm.eps = eps;
   const int64_t blocks =
       (write ? ((int64_t)n + 3) / 4 : 0) + (queries ? (int64_t)n * prm.head_groups : 0);
-  if (blocks > INT32_MAX)
-    return fail(PDA_ERR_INVALID_ARGUMENT, "tokens x query heads exceeds 2^31 workgroups");
+  if (blocks > kMaxGrid)
+    return fail(PDA_ERR_INVALID_ARGUMENT, "tokens x query heads beyond one launch's workgroups");
   void* args[] = {&prm};
   const hipError_t err =
       hipLaunchKernel(bf ? (const void*)latent_append_kernel<true>

@@ -1074,7 +1074,7 @@ int latent_prefill(const void* queries, const void* arena, const void* kv_b, con
   const PrefillPlan plan = plan_for(start, count, q_heads, rope_dim, nope_dim, value_dim);
   const int64_t grid = (int64_t)plan.tiles * plan.splits * plan.heads;
   const int64_t join = ((int64_t)count * q_heads * (value_dim / 4) + 255) / 256;
-  if (grid > INT32_MAX || join > INT32_MAX)
+  if (grid > kMaxGrid || (plan.splits > 1 && join > kMaxGrid))
     return fail(PDA_ERR_INVALID_ARGUMENT, "queries x heads beyond one launch's workgroups");
   if (!workspace || workspace_bytes < plan.bytes)
     return fail(PDA_ERR_WORKSPACE, "a workspace of %zu bytes is needed (got %zu)", plan.bytes,
