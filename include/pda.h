@@ -613,7 +613,9 @@ int pda_latent_decode_workspace_bytes(int32_t batch, int32_t q_heads,
 /* Decode attention over latent rows, one new token per sequence, in the
  * absorbed form: the queries are projected into the latent (U_h^T q, rounded
  * to the element type), all heads attend over the rows themselves, and D_h is
- * applied to what comes out.
+ * applied to what comes out. (fp16: a query with elements from 2^7 on is taken
+ * down by a power of two on the way, so U_h^T q stays finite unless the
+ * magnitudes in a column of U_h sum to more than 512.)
  *   queries [batch, q_heads, nope_dim + rope_dim], out [batch, q_heads,
  *   value_dim]; tables, lengths, page_size, longest and the masking of
  *   negative or unknown pages as for pda_paged_decode_attention; a sequence

@@ -173,6 +173,7 @@ struct LatentDecodeParams {
   const int32_t* lengths;
   f16* out;              // [batch, hq, value]
   f16* q_lat;            // [batch, hq, latent + rope]: absorbed queries
+  float* q_size;         // [batch, hq]: the absorbed queries times this are true (fp16)
   int32_t* prefix;       // [batch + 1] tiles, kSequenceTiles a sequence, before each
   float* part_o;         // [groups + batch, hq, latent] unnormalised partial sums
   float2* part_ml;       // [groups + batch, hq] (running max, sum)
@@ -202,12 +203,23 @@ __device__ __forceinline__ int units_of(const LatentDecodeParams& p, int b) {
   return tiles ? tiles + kSequenceTiles : 0;
 }
 
+// The value of the lane kBy on in a row of 16 lanes.
+template <int kBy>
+__device__ __forceinline__ uint32_t row_turned(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x120 + kBy, 0xf, 0xf, false);
+}
+
 // Queries into the latent: q_lat[b, h] = [U_h^T q_nope | q_rope], rounded to
 // the element type, because the matrix cores take 16-bit operands (the products
 // and their sum are float32). It moves the result by about as much as the
-// output's own rounding: in bf16 1.6e-3 of its 2-norm beside 1.7e-3. As products: (U_h^T) (32 latent dims x nope) by
-// (q_nope)^T (nope x 32 sequences); a wave has 32 latent dims, whose columns of
-// U_h it keeps in LDS and reads transposed. U_h is read once per 32 sequences.
+// output's own rounding: in bf16 1.6e-3 of its 2-norm beside 1.7e-3. In fp16
+// q_lat may pass the type's range where queries and projections are far inside
+// it: a query with elements from 2^7 on is taken down by a power of two, which the
+// scores are multiplied by again (q_size); a latent dim whose |U_h| sum to less
+// than 512 then stays finite whatever the query. As products: (U_h^T) (32 latent
+// dims x nope) by (q_nope)^T (nope x 32 sequences); a wave has 32 latent dims,
+// whose columns of U_h it keeps in LDS and reads transposed. U_h is read once per
+// 32 sequences.
 // The first workgroup also leaves the sequences' tile prefix for the kernels
 // after it. 64 sequences of 128 heads 11 us (26 MB; the reads in turn of U_h, q
 // and the rows bound it), one of 16 heads 4 us.
@@ -216,6 +228,7 @@ __global__ __launch_bounds__(256) void latent_absorb_kernel(const LatentDecodePa
   __shared__ __align__(1024) f16 s_u[4][kMaxHead * 32];
   __shared__ __align__(16) f16 s_q[32 * (kMaxHead + 8)];
   __shared__ int s_scan[256];
+  __shared__ f16 s_down[32];
   const int tid = threadIdx.x, w = uniform(tid >> 6), lane = tid & 63;
   const int n = lane & 31, hh = lane >> 5;
   const int h = blockIdx.y, b0 = blockIdx.z * 32;
@@ -240,18 +253,14 @@ __global__ __launch_bounds__(256) void latent_absorb_kernel(const LatentDecodePa
     if (tid == 255) p.prefix[p.batch] = s_scan[255];
   }
   const int width = p.latent + p.rope, qwidth = p.nope + p.rope;
-  if (blockIdx.x == 0) {
-    // The rotary part is copied.
-    const int pieces = p.rope / 8;
-    for (int i = tid; i < 32 * pieces; i += 256) {
-      const int b = b0 + i / pieces, j = i % pieces;
-      if (b < p.batch) {
-        const int64_t e = (int64_t)b * p.hq + h;
-        *reinterpret_cast<f16x8*>(p.q_lat + e * width + p.latent + 8 * j) =
-            *reinterpret_cast<const f16x8*>(p.q + e * qwidth + p.nope + 8 * j);
-      }
-    }
-  }
+  // The rotary part is copied, in fp16 taken down like the rest: a piece a thread.
+  static_assert(32 * (kMaxRope / 8) <= 256, "a piece a thread");
+  const int pieces = max(p.rope / 8, 1), rot_row = tid / pieces;
+  const bool rotary = blockIdx.x == 0 && tid < 32 * (p.rope / 8) && b0 + rot_row < p.batch;
+  const int64_t rot_head = (int64_t)(b0 + rot_row) * p.hq + h;
+  const int rot_dim = 8 * (tid % pieces);
+  f16x8 rot = {};
+  if (rotary) rot = *reinterpret_cast<const f16x8*>(p.q + rot_head * qwidth + p.nope + rot_dim);
   const int d0 = (blockIdx.x * 4 + w) * 32;
   // The wave's columns of U_h: rows of 64 bytes, zeros past either edge.
   const f16* u = p.kv_b + (int64_t)h * (p.nope + p.value) * p.latent;
@@ -272,6 +281,27 @@ __global__ __launch_bounds__(256) void latent_absorb_kernel(const LatentDecodePa
     f16x8 x = {};
     if (b0 + r < p.batch && d < p.nope)
       x = *reinterpret_cast<const f16x8*>(p.q + ((int64_t)(b0 + r) * p.hq + h) * qwidth + d);
+    if constexpr (!BF) {
+      // The largest of a query's elements, whose 16 lanes are a row of the wave:
+      // without their signs fp16 numbers have the order of their bits.
+      u16x8 bits = __builtin_bit_cast(u16x8, x) & (unsigned short)0x7FFF;
+      unsigned int top = 0;
+#pragma unroll
+      for (int t = 0; t < 8; ++t) top = max(top, (unsigned int)bits[t]);
+      top = max(top, row_turned<8>(top));
+      top = max(top, row_turned<4>(top));
+      top = max(top, row_turned<2>(top));
+      top = max(top, row_turned<1>(top));
+      const int e = max(0, (int)(top >> 10) - (15 + 6));  // 2^7 and up: 1 and up
+      const f16 f = __builtin_bit_cast(f16, (unsigned short)((15 - e) << 10));
+#pragma unroll
+      for (int t = 0; t < 8; ++t) x[t] *= f;
+      if (d == 0) {
+        s_down[r] = f;
+        if (blockIdx.x == 0 && b0 + r < p.batch)
+          p.q_size[(int64_t)(b0 + r) * p.hq + h] = __uint_as_float((uint32_t)(127 + e) << 23);
+      }
+    }
     *reinterpret_cast<f16x8*>(s_q + r * kQPitch + d) = x;
   }
   f16* su = s_u[w];
@@ -310,6 +340,10 @@ __global__ __launch_bounds__(256) void latent_absorb_kernel(const LatentDecodePa
     if (b < p.batch && d < p.latent)
       *reinterpret_cast<f16x8*>(p.q_lat + ((int64_t)b * p.hq + h) * width + d) =
           *reinterpret_cast<const f16x8*>(so + (i / 16) * kPitch + 8 * (i % 16));
+  }
+  if (rotary) {
+    if constexpr (!BF) rot *= s_down[rot_row];
+    *reinterpret_cast<f16x8*>(p.q_lat + rot_head * width + p.latent + rot_dim) = rot;
   }
 }
 
@@ -401,7 +435,7 @@ __global__ __launch_bounds__(256, 1) void latent_decode_kernel(const LatentDecod
   // A positive scale is applied with the maximum's subtraction, another one to
   // the scores.
   const bool direct = p.scale_log2 > 0.0f;
-  const float c = direct ? p.scale_log2 : 1.0f;
+  float c = direct ? p.scale_log2 : 1.0f;
 
   for (; b < p.batch; ++b) {
     const int seq0 = scalar_load(p.prefix, b), seq1 = scalar_load(p.prefix, b + 1);
@@ -434,6 +468,8 @@ __global__ __launch_bounds__(256, 1) void latent_decode_kernel(const LatentDecod
       }
     };
     look_up(ta);
+    if constexpr (!BF)
+      c = (direct ? p.scale_log2 : 1.0f) * p.q_size[(int64_t)b * p.hq + min(h, p.hq - 1)];
     // The queries by way of the tiles' LDS, laid out as a tile: head group hg's in
     // slot hg, parts kg NHG .. copied by this wave. (Operands straight from memory,
     // 16 bytes of a row a lane, take the cache 4 times as long, each wave's anew: 32
@@ -902,7 +938,7 @@ int waves_over_heads(int q_heads) { return q_heads <= 32 ? 1 : q_heads <= 64 ? 2
 struct Plan {
   int head_groups;  // grid y
   int groups;       // ranges of the stream: grid x
-  size_t q_lat, prefix, part_ml, part_o, bytes;
+  size_t q_lat, q_size, prefix, part_ml, part_o, bytes;
 };
 
 size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -922,6 +958,8 @@ Plan plan_for(int batch, int q_heads, int latent, int rope, int page_size, int t
   size_t at = 0;
   r.q_lat = at;
   at = up256(at + (size_t)batch * q_heads * (latent + rope) * 2);
+  r.q_size = at;
+  at = up256(at + (size_t)batch * q_heads * 4);
   r.prefix = at;
   at = up256(at + (size_t)(batch + 1) * 4);
   r.part_ml = at;
@@ -1062,6 +1100,7 @@ int latent_decode(const void* queries, const void* arena, const void* kv_b, cons
   prm.lengths = lengths;
   prm.out = static_cast<f16*>(out);
   prm.q_lat = reinterpret_cast<f16*>(ws + plan.q_lat);
+  prm.q_size = reinterpret_cast<float*>(ws + plan.q_size);
   prm.prefix = reinterpret_cast<int32_t*>(ws + plan.prefix);
   prm.part_ml = reinterpret_cast<float2*>(ws + plan.part_ml);
   prm.part_o = reinterpret_cast<float*>(ws + plan.part_o);
