@@ -246,13 +246,27 @@ __global__ __launch_bounds__(256, 2) void latent_expand_kernel(const PrefillPara
       __builtin_amdgcn_sched_barrier(0);
     }
     const int left = is_value(now) ? 32 : p.nope - dim_of(now);  // keys' dims of the block
+    // A token whose latent is not finite has no finite projection (an infinity or a
+    // NaN times 0 is one too). Its keys become NaN, its values zeros: queries that
+    // see it give NaN, and those that do not are left alone by 0 times its values.
+    f16x4 y[4];
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      f16x4 y;
+    for (int g = 0; g < 4; ++g)
 #pragma unroll
-      for (int v = 0; v < 4; ++v) y[v] = 8 * g < left ? round16<BF>(acc[4 * g + v]) : (f16)0.0f;
-      *reinterpret_cast<f16x4*>(so + n * kPitch + 8 * g + 4 * hh) = y;
+      for (int v = 0; v < 4; ++v) y[g][v] = 8 * g < left ? round16<BF>(acc[4 * g + v]) : (f16)0.0f;
+    bool bad = !(fabsf(acc[0]) < INFINITY);
+    if (__ballot(bad) != 0) {
+#pragma unroll
+      for (int v = 1; v < 16; ++v) bad &= !(fabsf(acc[v]) < INFINITY);  // (not a projection's row)
+      const f16 instead = is_value(now) ? (f16)0.0f : __builtin_bit_cast(f16, (short)0x7FFF);
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) y[g][v] = bad && 8 * g < left ? instead : y[g][v];
     }
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<f16x4*>(so + n * kPitch + 8 * g + 4 * hh) = y[g];
   }
   if (b0 < b1) {
     store(last, 0, load_out(0));
@@ -942,18 +956,16 @@ __global__ __launch_bounds__(256) void latent_join_kernel(const PrefillParams p)
   for (int s = 0; s < p.splits; ++s) top = fmaxf(top, p.part_ml[s * pairs + pair].x);
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float sum = 0.0f;
-  if (top != -INFINITY) {
-    for (int s = 0; s < p.splits; ++s) {
-      const float2 ml = p.part_ml[s * pairs + pair];
-      if (ml.x == -INFINITY) continue;
-      const float f = __builtin_amdgcn_exp2f(ml.x - top);
-      const float4 x = *reinterpret_cast<const float4*>(p.part_o + (s * pairs + pair) * p.value + d);
-      acc.x = fmaf(x.x, f, acc.x);
-      acc.y = fmaf(x.y, f, acc.y);
-      acc.z = fmaf(x.z, f, acc.z);
-      acc.w = fmaf(x.w, f, acc.w);
-      sum = fmaf(ml.y, f, sum);
-    }
+  for (int s = 0; s < p.splits; ++s) {
+    const float2 ml = p.part_ml[s * pairs + pair];
+    if (ml.x == -INFINITY && ml.y == 0.0f) continue;  // no key (not one of NaN)
+    const float f = __builtin_amdgcn_exp2f(ml.x - top);
+    const float4 x = *reinterpret_cast<const float4*>(p.part_o + (s * pairs + pair) * p.value + d);
+    acc.x = fmaf(x.x, f, acc.x);
+    acc.y = fmaf(x.y, f, acc.y);
+    acc.z = fmaf(x.z, f, acc.z);
+    acc.w = fmaf(x.w, f, acc.w);
+    sum = fmaf(ml.y, f, sum);
   }
   const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
   const f16x4 y = {round16<BF>(acc.x * inv), round16<BF>(acc.y * inv), round16<BF>(acc.z * inv),
