@@ -661,8 +661,8 @@ int pda_latent_prefill_workspace_bytes(int32_t start, int32_t count,
  *           chunk's own rows are already written
  * Query p sees the keys of positions 0 .. p that lie on a page of the arena; one
  * that sees none gives zeros. A row that is not finite reaches the queries that
- * see it alone (a latent that is not makes them NaN). Results are reproducible. A chunk of fewer than
- * some 170 queries over a long prefix is cheaper as a
+ * see it alone (a latent that is not makes them NaN). Results are reproducible.
+ * A chunk of fewer than some 170 queries over a long prefix is cheaper as a
  * pda_latent_decode_attention call with a batch row per token. Launches on
  * `stream`; calls that share a workspace must not overlap. */
 int pda_latent_prefill_attention(const void* queries, const void* arena,

@@ -288,8 +288,9 @@ __global__ __launch_bounds__(256, 2) void latent_expand_kernel(const PrefillPara
 // result's 2-norm), and the sum that divides it is of the rounded ones.
 // NP, VP: planes of 64 dims of the nope part and of the values; RS: 16-dim steps
 // of the rotary plane that are computed. 14 heads of 64 + 32 and 64 dims, 1531
-// queries after 389 keys 23 us: 168 workgroups of up to 30 tiles, whose length
-// bounds it.
+// queries after 389 keys 24 us: 504 workgroups (168 query tiles, their keys in 3
+// ranges) of up to 10 tiles, whose scores, weights and values come in turn, some
+// 2.4 us a tile, and bound it.
 template <int NP, int RS, int VP, bool BF>
 __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(const PrefillParams p) {
   constexpr int kPlane = kKeys * 64;  // halves of a 64-dim plane of a tile
@@ -520,9 +521,10 @@ __global__ __launch_bounds__(256, 2) void latent_prefill_kernel(const PrefillPar
 // tile's V is used an iteration after its K. The outputs (2 x 32 x 128, 128
 // registers a lane) and the queries live in accumulator registers.
 // What takes the running maximum past 2^8 is found from the weights' sum after
-// the fact and weighed again (settle). Rounded as above. 128 heads, 4096 tokens 780 to
-// 830 us for 687 GFLOP (0.83 to 0.88 PFLOP/s), 16 heads, 512 at 7777 54 us for 42
-// GFLOP; the matrix cores bound it at the clock that their load leaves.
+// the fact and weighed again (settle). Rounded as above. 128 heads, 4096 tokens 684
+// to 936 us for 687 GFLOP (0.73 to 1.0 PFLOP/s), by the clock that its load leaves
+// from dispatch to dispatch; 16 heads, 512 at 7777 55 us for 42 GFLOP; the matrix
+// cores bound it.
 template <bool BF>
 __global__ __launch_bounds__(256, 1) void latent_prefill_wide_kernel(const PrefillParams p) {
   constexpr int NP = 2, RP = 1, VP = 2, KP = NP + RP, OB = 2 * VP, QB = 2;
