@@ -851,7 +851,7 @@ __global__ __launch_bounds__(256) void evict_copy_kernel(const MoveParams p) {
 // it, and rows keep their order, so a workgroup that owns a slice of the rows
 // (kSlice bytes of every row of a sequence and kv head) may walk them in
 // stretches: a stretch's places hold no source of a later one. Within a stretch
-// all loads come before the first store. The rows above in place 84 us: one
+// all loads come before the first store. The rows above in place 102 us: one
 // workgroup walks each slice, where the copy has as many as there are rows.
 template <class V>
 __global__ __launch_bounds__(256) void evict_pack_kernel(const MoveParams p) {

@@ -79,8 +79,9 @@ struct PrefillParams {
 // 512 tokens 63 us a call against 59, 16 heads, 256 at 30000 272 against 257.)
 // The next block's copies and the last one's stores go out among the products:
 // issued together they held the wave for as long as the products. 16 heads of
-// 128 + 128 dims, 8289 tokens 48 us, 128 heads, 4096 tokens 159 us (860 TFLOP/s);
-// the products and the copies' rate into LDS bound it about alike.
+// 128 + 128 dims, 8289 tokens 49 us, 128 heads, 4096 tokens 150 to 162 us by the
+// clock (0.85 to 0.92 PFLOP/s); the products and the copies' rate into LDS bound it
+// about alike.
 // Results are stored a block late. Tokens without a row are zeros from the start.
 // The workgroups of the group's first heads also gather the rotary keys and the
 // mask of keys that have a row. PL: planes of 64 latent dims.
