@@ -785,6 +785,161 @@ int pda_evict_move(void* arena, void* arena2, int32_t width, const int32_t* kept
                    int64_t arena_rows, int32_t layout, int32_t keep,
                    void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Steps that take many tokens of every sequence: prompts packed one behind the
+ * other, and trees of drafted tokens. Such a step's tokens lie sequence after
+ * sequence; starts [batch + 1] int32 ascends from 0, sequence b's tokens are
+ * [starts[b], starts[b + 1]). No counterpart in the reference, whose steps take a
+ * chunk of one prompt or one token a sequence (batches.py:26-253).
+ * ------------------------------------------------------------------------- */
+
+/* Page tables and slot maps of a step, from the requests' lengths. Sequence b
+ * holds lengths[b] rows and pages[b] pages (its table's first entries) and brings
+ * counts[b] tokens (negative values count as 0); where its pages do not hold them
+ * it takes the next ones of `feed`, pages that the host set aside, in the order of
+ * the sequences:
+ *   tables      [batch, table_stride] in place: the taken pages behind those held
+ *   starts      [batch + 1]: prefix sums of counts
+ *   out_lengths [batch]: lengths + counts (below 2^31)
+ *   out_pages   [batch]: pages held now
+ *   out_drawn   [2]: drawn[0] + pages taken, and 0
+ *   rows        [tokens]: the arena row of each token
+ *   positions   [tokens]: its position: lengths[b] + its index or, with parents,
+ *               its depth in the tree
+ *   masks       [tokens], with parents: bit j set where node j of the sequence is
+ *               the node itself or one of its ancestors
+ * drawn [2]: how many of the feed's pages were taken before, and the library's
+ * counter (0 before the first call; every call leaves it 0). parents [tokens] or
+ * NULL (each sequence's tokens follow each other): a node's parent among its
+ * sequence's nodes, anything but an earlier node for none. Nodes past a tree's 64th
+ * have no mask and the position lengths[b].
+ * Where the feed runs out the taken pages are -1 (their tokens' rows too) and
+ * out_drawn counts on; tokens past the table's entries, or whose row passes 2^31,
+ * have row -1 as well. Tokens past `tokens` are dropped. Entries of rows and
+ * positions behind the last token are -1 and 0 (masks: 0). out_lengths, out_pages
+ * and out_drawn may be lengths, pages and drawn themselves. batch <= 4096.
+ * One launch on `stream`, no workspace; calls that share `drawn` must not overlap. */
+int pda_extend_tables(int32_t* tables, int32_t table_stride,
+                      const int32_t* lengths, const int32_t* counts,
+                      const int32_t* pages, const int32_t* feed,
+                      int32_t feed_len, int32_t* drawn, const int32_t* parents,
+                      int32_t batch, int32_t page_size, int32_t tokens,
+                      int32_t* starts, int32_t* out_lengths, int32_t* out_pages,
+                      int32_t* out_drawn, int32_t* rows, int32_t* positions,
+                      uint64_t* masks, void* stream);
+
+/* Causal attention of whole prompts, packed: token i of a prompt attends to the
+ * tokens max(0, i - window + 1) .. i of the same prompt (window 0: from its first).
+ *   queries [tokens, q_heads, head_dim], keys, values [tokens, kv_heads, head_dim]
+ *           with `*_token` elements from token to token and `*_head` from head to
+ *           head (multiples of 8, so that slices of one projection's output are read
+ *           where they are), the elements of a head side by side
+ *   out     [tokens, q_heads, head_dim], contiguous
+ * Rows of out behind the last prompt become zeros. A key or value that is not
+ * finite reaches the queries that see it alone. head_dim a multiple of 8 up to 256.
+ * fp16, or bf16 (_bf16). One launch on `stream`; results are reproducible. */
+int pda_packed_prompt_attention(const void* queries, int64_t q_token,
+                                int64_t q_head, const void* keys,
+                                int64_t k_token, int64_t k_head,
+                                const void* values, int64_t v_token,
+                                int64_t v_head, const int32_t* starts,
+                                void* out, int32_t tokens, int32_t batch,
+                                int32_t q_heads, int32_t kv_heads,
+                                int32_t head_dim, float scale, int32_t window,
+                                float softcap, void* stream);
+int pda_packed_prompt_attention_bf16(const void* queries, int64_t q_token,
+                                int64_t q_head, const void* keys,
+                                int64_t k_token, int64_t k_head,
+                                const void* values, int64_t v_token,
+                                int64_t v_head, const int32_t* starts,
+                                void* out, int32_t tokens, int32_t batch,
+                                int32_t q_heads, int32_t kv_heads,
+                                int32_t head_dim, float scale, int32_t window,
+                                float softcap, void* stream);
+
+/* Bytes of workspace of a tree attention call, whatever its lengths. */
+int pda_tree_workspace_bytes(int32_t batch, int32_t head_dim, size_t* bytes);
+
+/* Attention for trees of drafted tokens over the paged cache. Sequence b holds
+ * lengths[b] rows; its nodes' keys and values lie behind them, node j's in row
+ * lengths[b] + j (written before the call). Node i attends to the held rows and to
+ * the nodes j < 64 whose bit masks[starts[b] + i] has, its own included or not as
+ * the mask says; a node that sees nothing gives zeros. Its position is lengths[b] +
+ * max(0, bits of its mask - 1): with window > 0 it sees the held rows past position
+ * - window and the last `window` nodes of its mask.
+ *   queries, out [tokens, q_heads, head_dim]; keys, values, tables, layout, the
+ *   masking of pages, scale and softcap as for pda_paged_decode_attention
+ * Rows of out behind the last sequence become zeros; a value that is not finite
+ * reaches the nodes that see it alone. head_dim a multiple of 8 up to 256. fp16, or
+ * bf16 (_bf16); int8 keys and values with fp16 scales under fp16 (_q8) or bf16
+ * (_q8_bf16) queries. Two launches on `stream`; calls that share a workspace must
+ * not overlap. Results are reproducible. */
+int pda_tree_attention(const void* queries, const void* keys,
+                       const void* values,
+                       const int32_t* tables, const int32_t* lengths,
+                       const int32_t* starts, const uint64_t* masks, void* out,
+                       int32_t tokens, int32_t batch, int32_t q_heads,
+                       int32_t kv_heads, int32_t head_dim, int32_t page_size,
+                       int32_t table_stride, int64_t arena_rows, int32_t layout,
+                       float scale, int32_t window, float softcap,
+                       void* workspace, size_t workspace_bytes, void* stream);
+int pda_tree_attention_bf16(const void* queries, const void* keys,
+                       const void* values,
+                       const int32_t* tables, const int32_t* lengths,
+                       const int32_t* starts, const uint64_t* masks, void* out,
+                       int32_t tokens, int32_t batch, int32_t q_heads,
+                       int32_t kv_heads, int32_t head_dim, int32_t page_size,
+                       int32_t table_stride, int64_t arena_rows, int32_t layout,
+                       float scale, int32_t window, float softcap,
+                       void* workspace, size_t workspace_bytes, void* stream);
+int pda_tree_attention_q8(const void* queries, const void* keys,
+                       const void* values, const void* key_scales,
+                       const void* value_scales,
+                       const int32_t* tables, const int32_t* lengths,
+                       const int32_t* starts, const uint64_t* masks, void* out,
+                       int32_t tokens, int32_t batch, int32_t q_heads,
+                       int32_t kv_heads, int32_t head_dim, int32_t page_size,
+                       int32_t table_stride, int64_t arena_rows, int32_t layout,
+                       float scale, int32_t window, float softcap,
+                       void* workspace, size_t workspace_bytes, void* stream);
+int pda_tree_attention_q8_bf16(const void* queries, const void* keys,
+                       const void* values, const void* key_scales,
+                       const void* value_scales,
+                       const int32_t* tables, const int32_t* lengths,
+                       const int32_t* starts, const uint64_t* masks, void* out,
+                       int32_t tokens, int32_t batch, int32_t q_heads,
+                       int32_t kv_heads, int32_t head_dim, int32_t page_size,
+                       int32_t table_stride, int64_t arena_rows, int32_t layout,
+                       float scale, int32_t window, float softcap,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/* Keeps the drafted tokens that the model chose. A sequence's node 0 is its newest
+ * token and always kept; then, after every kept node, its first child whose drafted
+ * token is targets[the kept node], the model's choice there.
+ *   accepted    [batch]: nodes kept (0 for a sequence without nodes)
+ *   path        [batch, 64]: the kept nodes in order, then -1
+ *   following   [batch]: the model's choice after the last kept node (-1: no node)
+ *   out_lengths [batch]: lengths + accepted; not lengths itself
+ * and in every store the kept nodes' rows move to the rows lengths[b] ..
+ * lengths[b] + accepted[b] - 1 (rows of other nodes are left as they are).
+ *   stores  HOST array [layers, stores_per_layer] of device pointers: keys, values
+ *           and, with 4, their fp16 scales; one layout and shape for all, no two the
+ *           same memory. `width`: bytes of a row of keys or values of one head
+ *   drafted, targets [tokens], token_bytes 8 (int64) or 4 (int32)
+ * Nodes past a tree's 64th are never kept. A row whose page is not in the arena (or
+ * past the table) does not move. The pages of a tree's rows belong to one sequence.
+ * One launch on `stream` for 48 layers, no workspace. */
+int pda_commit_drafts(void* const* stores, int32_t layers,
+                      int32_t stores_per_layer, int32_t width,
+                      const int32_t* tables, const int32_t* lengths,
+                      const int32_t* starts, const int32_t* parents,
+                      const void* drafted, const void* targets,
+                      int32_t token_bytes, int32_t* out_lengths,
+                      int32_t* accepted, int32_t* path, int64_t* following,
+                      int32_t tokens, int32_t batch, int32_t kv_heads,
+                      int32_t page_size, int32_t table_stride,
+                      int64_t arena_rows, int32_t layout, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,376 @@
+// Attention of 32 query rows a wave over key tiles of 64 in LDS: what packed
+// prompts (pda_prompts.hip) and drafted trees (pda_drafts.hip) have in common.
+//
+//   o_r = sum_k w_rk v_k / sum_k w_rk,  w_rk = exp(f(q_r . k)) over the keys that
+//   row r sees; f scales and, where asked, caps: f(x) = cap tanh(scale x / cap).
+//
+// A wave holds 32 rows and computes S^T = K Q^T and O^T += V^T W^T on
+// v_mfma_f32_32x32x16: the scores of a product come out with a lane holding 16
+// keys of one row, which after the exponential are the second product's operand as
+// they lie (nothing moves between lanes). Weights are taken in the log2 domain
+// against a running maximum that moves only when a block's weights sum past 2^8
+// (so that 16-bit weights stay finite), and rounded to the element type, to
+// nearest; their sum is that of the rounded weights, in float32, as are the
+// outputs.
+//
+// LDS: planes of 64 bytes a key (32 dims), 64 keys a plane. V as it lies, for the
+// transposing reads; K with the four 16-byte chunks of a key's plane permuted by
+// (key / 4) % 4, so that the 16 lanes of a read touch each bank once.
+#ifndef PDA_ROWS_H
+#define PDA_ROWS_H
+
+#include <hip/hip_runtime.h>
+
+#include <math.h>
+#include <stdint.h>
+
+#include <type_traits>
+#include <utility>
+
+namespace pda_rows {
+
+typedef _Float16 f16;
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16;
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kSlack = 8.0f;
+constexpr int kKeys = 64;            // keys of a tile: two blocks of 32
+constexpr int kPlane = kKeys * 32;   // halves of a plane
+
+// The kernel width that serves a head dim (zeros past it); 0: none does.
+constexpr int width_for(int dim) {
+  return dim <= 0 || dim % 8 ? 0 : dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128
+         : dim <= 256 ? 256 : 0;
+}
+
+// How scores become weights' exponents.
+struct Shape {
+  float scale_log2;
+  float cap_in;   // 2 log2(e) scale / softcap
+  float cap_out;  // softcap log2(e); 0: no softcap
+};
+inline Shape shape_of(float scale, float softcap) {
+  return {scale * kLog2e, softcap > 0.0f ? 2.0f * kLog2e * scale / softcap : 0.0f,
+          softcap * kLog2e};
+}
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+  return (int64_t)((uint64_t)(uint32_t)uniform((int)x) | (uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32);
+}
+
+__device__ __forceinline__ f16x4 read_tr(const f16* p) {
+  return __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)p));
+}
+
+// LDS byte address of a shared object.
+__device__ __forceinline__ uint32_t lds_address(const void* at) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)at;
+}
+
+// 16 bytes per lane from global memory straight into LDS: lane i's to dst + 16 i
+// (dst: wave-uniform). The caller waits (wait_vmem) before the barrier that
+// publishes them.
+__device__ __forceinline__ void copy_to_lds(const void* src, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src)
+               : "memory", "m0");
+}
+
+// Until at most kLeft of the wave's loads and copies are under way.
+template <int kLeft>
+__device__ __forceinline__ void wait_vmem() {
+  static_assert(kLeft < 64, "the count has six bits");
+  __builtin_amdgcn_s_waitcnt(0x0F70 | (kLeft & 15) | (kLeft >> 4) << 14);
+}
+
+template <bool BF>
+__device__ __forceinline__ f32x16 mfma16(const f16x8& a, const f16x8& b, const f32x16& c) {
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// f32 -> the 16-bit element type (to nearest even), as an fp16 bit pattern.
+template <bool BF>
+__device__ __forceinline__ f16 round16(float x) {
+  if constexpr (BF)
+    return __builtin_bit_cast(f16, (bf16)x);
+  else
+    return (f16)x;
+}
+template <bool BF>
+__device__ __forceinline__ float widen16(f16 x) {
+  if constexpr (BF)
+    return (float)__builtin_bit_cast(bf16, x);
+  else
+    return (float)x;
+}
+
+// Whether one of eight elements is an infinity or a NaN: all ones in the exponent.
+template <bool BF>
+__device__ __forceinline__ bool not_finite(const f16x8& x) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  const u32x4 y = __builtin_bit_cast(u32x4, x);
+  constexpr uint32_t kExp = BF ? 0x7F80u : 0x7C00u;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    bad |= (y[i] & kExp) == kExp || ((y[i] >> 16) & kExp) == kExp;
+  return bad;
+}
+
+template <bool BF>
+__device__ __forceinline__ float4 widen4(const f16* p) {
+  const f16x4 x = *reinterpret_cast<const f16x4*>(p);
+  return make_float4(widen16<BF>(x[0]), widen16<BF>(x[1]), widen16<BF>(x[2]), widen16<BF>(x[3]));
+}
+
+// Zeros in the place of elements that are not finite.
+template <bool BF>
+__device__ __forceinline__ f16x8 finite_only(f16x8 x) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (!(fabsf(widen16<BF>(x[j])) < INFINITY)) x[j] = (f16)0.0f;
+  return x;
+}
+
+// One bit a key from a ballot with four lanes a key.
+__device__ __forceinline__ uint32_t keys_of(uint64_t lanes) {
+  if (lanes == 0) return 0;
+  lanes |= lanes >> 1;
+  lanes |= lanes >> 2;
+  uint32_t keys = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) keys |= (uint32_t)(lanes >> (4 * i) & 1) << i;
+  return keys;
+}
+
+// Bits 0 .. n - 1 (none for n <= 0, all from 32 on).
+__device__ __forceinline__ uint32_t below(int n) {
+  const uint32_t ones = n >= 32 ? 32u : n > 0 ? (uint32_t)n : 0u;
+  return (uint32_t)((1ull << ones) - 1);
+}
+
+// 32 rows of one wave: lane l holds row l % 32, half l / 32 of its keys and dims
+// (of every 8 the first or the last four).
+template <int D, bool BF>
+struct Rows {
+  f16x8 q[D / 16];
+  f32x16 o[D / 32];
+  float m, l;  // running maximum (log2 units), sum of this lane's weights
+  float c;     // what a shaped score is multiplied by
+  int n, hh;
+  int k_lane0, k_lane1, v_lane;
+
+  __device__ __forceinline__ void init(const Shape& f) {
+    const int lane = threadIdx.x & 63;
+    n = lane & 31;
+    hh = lane >> 5;
+    const int ksw = (n >> 2) & 3;
+    k_lane0 = 32 * n + 8 * (hh ^ ksw);
+    k_lane1 = 32 * n + 8 * ((2 + hh) ^ ksw);
+    const int g16 = lane >> 4, s16 = lane & 15;
+    v_lane = (4 * (g16 >> 1) + (s16 >> 2)) * 32 + 16 * (g16 & 1) + 4 * (s16 & 3);
+    c = f.cap_out <= 0.0f && f.scale_log2 > 0.0f ? f.scale_log2 : 1.0f;
+    clear();
+  }
+
+  __device__ __forceinline__ void clear() {
+    m = -INFINITY;
+    l = 0.0f;
+#pragma unroll
+    for (int b = 0; b < D / 32; ++b) o[b] = f32x16{};
+  }
+
+  // This lane's row of queries; `dim` elements of it, zeros past them.
+  __device__ __forceinline__ void load(const f16* row, int dim, bool live) {
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      const int d = 16 * i + 8 * hh;
+      const bool in = live && d < dim;
+      const f16x8 x = *reinterpret_cast<const f16x8*>(row + (in ? d : 0));
+      q[i] = in ? x : f16x8{};
+    }
+  }
+
+  // Scores of the 32 keys from kt on.
+  __device__ __forceinline__ void scores(f32x16& x, const f16* kt) const {
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      const f16x8 a = *reinterpret_cast<const f16x8*>(kt + (i & 1 ? k_lane1 : k_lane0) +
+                                                      kPlane * (i >> 1));
+      x = mfma16<BF>(a, q[i], i == 0 ? f32x16{} : x);
+    }
+  }
+
+  // Caps and scales that are not one positive factor.
+  __device__ __forceinline__ void shape(f32x16& x, const Shape& f) const {
+    if (f.cap_out > 0.0f) {
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        const float e = __builtin_amdgcn_exp2f(x[v] * f.cap_in);
+        x[v] = (1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f)) * f.cap_out;
+      }
+    } else if (!(f.scale_log2 > 0.0f)) {
+#pragma unroll
+      for (int v = 0; v < 16; ++v) x[v] = x[v] * f.scale_log2;
+    }
+  }
+
+  // Hides the keys of a block whose bit in `see` is not set.
+  __device__ __forceinline__ void mask(f32x16& x, uint32_t see) const {
+    see >>= 4 * hh;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      const int bit = __builtin_amdgcn_sbfe((int)see, 8 * (v / 4) + (v % 4), 1);
+      const float y = x[v];  // (a bit cast of x[v] itself takes element 0)
+      x[v] = __builtin_bit_cast(float, (__builtin_bit_cast(int, y) & bit) |
+                                           (~bit & (int)0xFF800000));
+    }
+  }
+
+  // Weights 2 i, 2 i + 1 of a block, rounded to 16 bits and packed.
+  __device__ __forceinline__ static void put_pair(f16x8 (&w)[2], int i, float e0, float e1) {
+    f16x2 ph;
+    if constexpr (BF)
+      ph = __builtin_bit_cast(f16x2, bf16x2{(bf16)e0, (bf16)e1});
+    else
+      ph = f16x2{(f16)e0, (f16)e1};
+    w[i / 4][2 * (i % 4)] = ph[0];
+    w[i / 4][2 * (i % 4) + 1] = ph[1];
+  }
+
+  // Their sum.
+  __device__ __forceinline__ static float total(const f16x8 (&w)[2], float sum) {
+    float s2[2] = {sum, 0.0f};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const f16x2 ph = {w[i / 4][2 * (i % 4)], w[i / 4][2 * (i % 4) + 1]};
+      if constexpr (BF)
+        s2[i & 1] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, ph),
+                                                    bf16x2{(bf16)1.0f, (bf16)1.0f}, s2[i & 1],
+                                                    false);
+      else
+        s2[i & 1] = __builtin_amdgcn_fdot2(ph, f16x2{(f16)1.0f, (f16)1.0f}, s2[i & 1], false);
+    }
+    return s2[0] + s2[1];
+  }
+
+  __device__ __forceinline__ float weigh_against(const f32x16& x, f16x8 (&w)[2], float mu) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      put_pair(w, i, __builtin_amdgcn_exp2f(fmaf(x[2 * i], c, -mu)),
+               __builtin_amdgcn_exp2f(fmaf(x[2 * i + 1], c, -mu)));
+    return total(w, 0.0f);
+  }
+
+  // A block's weights w, summed in lb, were taken against the running maximum.
+  // Only where they sum past 2^8 (or no key was seen before: lb is infinite; or
+  // one is not a number) the maximum is taken and the block weighed again.
+  __device__ __forceinline__ void settle(const f32x16& x, f16x8 (&w)[2], float lb) {
+    if (__ballot(!(lb <= 256.0f)) != 0) {
+      float top = x[0];
+#pragma unroll
+      for (int v = 1; v < 16; ++v) top = fmaxf(top, x[v]);
+      top = fmaxf(top, __shfl_xor(top, 32)) * c;
+      if (top > m + kSlack) {
+        if (m != -INFINITY) {
+          const float f = __builtin_amdgcn_exp2f(m - top);
+          l *= f;
+#pragma unroll
+          for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) o[b][v] *= f;
+        }
+        m = top;
+      }
+      lb = weigh_against(x, w, m == -INFINITY ? 0.0f : m);
+    }
+    l += lb;
+  }
+
+  __device__ __forceinline__ void weigh(const f32x16& x, f16x8 (&w)[2]) {
+    settle(x, w, m == -INFINITY ? INFINITY : weigh_against(x, w, m));
+  }
+
+  // O^T += V^T W^T over the 32 keys from vt on.
+  __device__ __forceinline__ void accumulate(const f16x8 (&w)[2], const f16* vt) {
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+#pragma unroll
+      for (int b = 0; b < D / 32; ++b) {
+        const f16* vp = vt + v_lane + kPlane * b + 512 * ks;
+        const f16x4 lo4 = read_tr(vp);
+        const f16x4 hi4 = read_tr(vp + 256);
+        const f16x8 a = {lo4[0], lo4[1], lo4[2], lo4[3], hi4[0], hi4[1], hi4[2], hi4[3]};
+        o[b] = mfma16<BF>(a, w[ks], o[b]);
+      }
+    }
+  }
+
+  // Values that are not finite were taken as zeros (0 times one is no 0): adds
+  // them where the key is seen. `bad`: such keys of the block, `see` the keys that
+  // this lane's row sees, value4(k, d) values d .. d + 3 of key k as they are.
+  template <class F>
+  __device__ __forceinline__ void add_not_finite(const f16x8 (&w)[2], uint32_t bad, uint32_t see,
+                                                 int dim, F value4) {
+    while (bad) {
+      const int k = __builtin_ctz(bad);
+      bad &= bad - 1;
+      float mine = 0.0f;
+#pragma unroll
+      for (int v = 0; v < 16; ++v)
+        mine = v == 4 * (k / 8) + k % 4 ? widen16<BF>(w[v / 8][v % 8]) : mine;
+      const float other = __shfl_xor(mine, 32);
+      const float weight = (k >> 2 & 1) == hh ? mine : other;
+      const bool seen = see >> k & 1;
+#pragma unroll
+      for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int d = 32 * b + 8 * g + 4 * hh;
+          const float4 y = value4(k, min(d, dim - 4));
+          const float ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            o[b][4 * g + t] += seen && d < dim && !(fabsf(ys[t]) < INFINITY) ? weight * ys[t] : 0.0f;
+          __builtin_amdgcn_sched_barrier(0);  // (else all loads at once: registers of the common path)
+        }
+    }
+  }
+
+  // 1 / the row's sum, 0 where the row sees nothing (and NaN for NaN).
+  __device__ __forceinline__ float inverse() const {
+    const float sum = l + __shfl_xor(l, 32);
+    return sum == 0.0f ? 0.0f : 1.0f / sum;
+  }
+
+  // The row's outputs, normalised.
+  __device__ __forceinline__ void store(f16* row, int dim, float inv) const {
+#pragma unroll
+    for (int b = 0; b < D / 32; ++b) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = 32 * b + 8 * g + 4 * hh;
+        f16x4 y;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) y[t] = round16<BF>(o[b][4 * g + t] * inv);
+        if (d < dim) *reinterpret_cast<f16x4*>(row + d) = y;
+      }
+    }
+  }
+};
+
+}  // namespace pda_rows
+
+#endif  // PDA_ROWS_H

@@ -154,6 +154,24 @@ SIGNATURES["pda_evict_move"] = (
     ctypes.c_int, [c_void_p] * 2 + [c_int32] + [c_void_p] * 4 + [c_int32] * 5
     + [c_int64, c_int32, c_int32, c_void_p])
 
+# Steps of many tokens a sequence.
+SIGNATURES["pda_extend_tables"] = (
+    ctypes.c_int, [c_void_p, c_int32] + [c_void_p] * 4 + [c_int32] + [c_void_p] * 2
+    + [c_int32] * 3 + [c_void_p] * 8)
+_PACKED_ARGS = ([c_void_p, c_int64, c_int64] * 3 + [c_void_p] * 2 + [c_int32] * 5
+                + [c_float, c_int32, c_float, c_void_p])
+_TREE_TAIL = ([c_void_p] * 5 + [c_int32] * 7 + [c_int64, c_int32, c_float, c_int32, c_float,
+                                                 c_void_p, c_size_t, c_void_p])
+for _suffix in ("", "_bf16"):
+    SIGNATURES["pda_packed_prompt_attention" + _suffix] = (ctypes.c_int, _PACKED_ARGS)
+    SIGNATURES["pda_tree_attention" + _suffix] = (ctypes.c_int, [c_void_p] * 3 + _TREE_TAIL)
+    SIGNATURES["pda_tree_attention_q8" + _suffix] = (ctypes.c_int, [c_void_p] * 5 + _TREE_TAIL)
+SIGNATURES["pda_tree_workspace_bytes"] = (
+    ctypes.c_int, [c_int32] * 2 + [ctypes.POINTER(c_size_t)])
+SIGNATURES["pda_commit_drafts"] = (
+    ctypes.c_int, [ctypes.POINTER(c_void_p)] + [c_int32] * 3 + [c_void_p] * 6 + [c_int32]
+    + [c_void_p] * 4 + [c_int32] * 5 + [c_int64, c_int32, c_void_p])
+
 _lib: ctypes.CDLL | None = None
 
 
@@ -243,6 +261,12 @@ def attention_weights_workspace_bytes(batch, q_heads, capacity) -> int:
     out = c_size_t(0)
     check(library().pda_attention_weights_workspace_bytes(batch, q_heads, capacity,
                                                           ctypes.byref(out)))
+    return out.value
+
+
+def tree_workspace_bytes(batch, head_dim) -> int:
+    out = c_size_t(0)
+    check(library().pda_tree_workspace_bytes(batch, head_dim, ctypes.byref(out)))
     return out.value
 
 

@@ -1,0 +1,93 @@
+"""Page tables and slot maps of a step, built on the GPU from the requests' lengths.
+
+The reference gives a step's tokens their rows in host loops (``KVCache.rows``,
+python/instinct/paged_kv.py:259-265; ``DecodeBatch.__init__``, batches.py:148-179)
+after drawing the pages that they need one by one. Here the host sets pages aside
+ahead of time (:meth:`instinct_amd.paged_kv.KVCache.reserve_feed`) and
+:func:`extend_tables` does the rest of a step in one launch: it lengthens the page
+tables out of that feed and gives every token its row and its position, and the nodes
+of drafted trees the mask of their ancestors. Nothing crosses PCIe, so the launch can
+sit in a captured graph and be replayed while the feed lasts.
+
+The work happens in libpda.so (``csrc/pda_paging.hip``).
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+from .eviction import _check_index
+from .hip_kernels import on_device
+
+
+class StepRows(NamedTuple):
+    """What :func:`extend_tables` gives a step (int32 but for the masks)."""
+
+    starts: torch.Tensor     # [batch + 1] first token of each sequence, and the end
+    lengths: torch.Tensor    # [batch] rows held with the step's tokens
+    pages: torch.Tensor      # [batch] pages held
+    drawn: torch.Tensor      # [2] pages drawn from the feed, and 0
+    rows: torch.Tensor       # [tokens] arena row of each token
+    positions: torch.Tensor  # [tokens]
+    masks: torch.Tensor | None  # [tokens] int64, with parents
+
+
+def extend_tables(tables: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor,
+                  pages: torch.Tensor, feed: torch.Tensor, drawn: torch.Tensor, *,
+                  page_size: int, tokens: int, parents: torch.Tensor | None = None,
+                  out: StepRows | None = None) -> StepRows:
+    """Lengthen the page tables ``[batch, width]`` (in place) for a step that brings
+    ``counts[b]`` tokens to a sequence that holds ``lengths[b]`` rows on ``pages[b]``
+    pages, taking what is missing from ``feed`` (page ids) from entry ``drawn[0]`` on,
+    in the order of the sequences; and the step's slot map (:class:`StepRows`).
+
+    ``tokens``: entries of the per-token results, at least ``counts.sum()``; those
+    behind the last token have row -1 (the append writes nothing there), position 0
+    and mask 0. ``parents`` (int32 ``[tokens]``): each sequence's tokens are a tree of
+    up to 64 nodes and ``parents`` names each node's parent among them (-1: none); a
+    node's position then goes by its depth and its mask has the bits of its ancestors
+    and its own. ``drawn`` is int32 ``[2]``, zeros for a new feed. A feed that runs
+    out leaves -1 as page and row and ``drawn`` past its end. All are int32 on one
+    GPU; ``out`` may hold ``lengths``, ``pages`` and ``drawn`` themselves (a step
+    replayed from a graph). No counterpart in the reference."""
+    if not tables.is_cuda:
+        raise ValueError("tables must be on a GPU")
+    device = tables.device
+    if tables.dtype != torch.int32 or tables.dim() != 2 or not tables.is_contiguous():
+        raise ValueError("tables must be contiguous int32 [batch, width]")
+    batch, width = tables.shape
+    for name, t, shape in (("lengths", lengths, (batch,)), ("counts", counts, (batch,)),
+                           ("pages", pages, (batch,)), ("feed", feed, (feed.shape[0],)),
+                           ("drawn", drawn, (2,))):
+        if not _check_index(name, t, shape, device).is_contiguous() or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+    if tokens < 0:
+        raise ValueError("tokens must not be negative")
+    if parents is not None:
+        parents = _check_index("parents", parents, (tokens,), device)
+    if out is None:
+        new = lambda n, dtype=torch.int32: torch.empty(n, dtype=dtype, device=device)  # noqa: E731
+        out = StepRows(new(batch + 1), new(batch), new(batch), new(2), new(tokens), new(tokens),
+                       None if parents is None else new(tokens, torch.int64))
+    else:
+        for name, t, n in zip(StepRows._fields, out, (batch + 1, batch, batch, 2, tokens, tokens,
+                                                      tokens)):
+            if t is None and name == "masks" and parents is None:
+                continue
+            dtype = torch.int64 if name == "masks" else torch.int32
+            if (t is None or t.dtype != dtype or t.shape != (n,) or t.device != device
+                    or not t.is_contiguous()):
+                raise ValueError(f"out.{name} must be contiguous {dtype} [{n}] on {device}")
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    with on_device(device):
+        rc = _lib.library().pda_extend_tables(
+            tables.data_ptr(), width, lengths.data_ptr(), counts.data_ptr(), pages.data_ptr(),
+            feed.data_ptr(), feed.shape[0], drawn.data_ptr(), ptr(parents), batch, page_size,
+            tokens, out.starts.data_ptr(), out.lengths.data_ptr(), out.pages.data_ptr(),
+            out.drawn.data_ptr(), out.rows.data_ptr(), out.positions.data_ptr(), ptr(out.masks),
+            torch.cuda.current_stream(device).cuda_stream)
+    _lib.check(rc)
+    return out
