@@ -22,10 +22,13 @@ from typing import Any
 import numpy as np
 import torch
 
+from .drafts import NODES, Committed, commit_drafts, tree_attention
 from .eviction import paged_attention_weights
 from .hip_kernels import (image_spans, paged_decode_attention, paged_prefill_attention, rope,
                           rope_append)
 from .paged_kv import KVCache
+from .paging import StepRows, extend_tables
+from .prompts import packed_prompt_attention
 
 
 def pack_tables(tables: list[np.ndarray] | list[list[int]], count: int) -> np.ndarray:
@@ -260,3 +263,155 @@ class PrefillBatch:
             scales=self.cache.scales(layer),
             images=self._spans if self._spans is not None else ())
         return out.reshape(self.count, -1).to(self.cache.dtype)
+
+
+class _ManyTokens:
+    """What steps that bring several tokens of several sequences have in common: the
+    rows of the new tokens in every group, made on the GPU, and the calls that write
+    them. ``held``: rows of each sequence before the step, by group."""
+
+    prefill = True
+
+    def _place(self, cache: KVCache, counts: np.ndarray, held: dict[str, np.ndarray],
+               tables: dict[str, list[np.ndarray]], parents: torch.Tensor | None,
+               tokens: int) -> None:
+        device, page = cache.device, cache.page_size
+        pages = {name: np.array([len(t) for t in tables[name]], dtype=np.int64)
+                 for name in cache.groups}
+        for name, have in pages.items():
+            if have.shape != counts.shape:
+                raise ValueError(f"group {name!r}: a table for each sequence")
+            short = (-(-(held[name] + counts) // page) > have) & (counts > 0)
+            if np.any(short):
+                b = int(np.argmax(short))
+                raise ValueError(f"group {name!r}: no page for row {held[name][b] + counts[b] - 1} "
+                                 f"of sequence {b}")
+        put = lambda a: torch.as_tensor(np.asarray(a).astype(np.int32), device=device)  # noqa: E731
+        self._tables: dict[str, torch.Tensor] = {}
+        self._held: dict[str, torch.Tensor] = {}
+        self._steps: dict[str, StepRows] = {}
+        none, drawn = put([]), put([0, 0])
+        for name, have in pages.items():
+            packed = pack_tables(tables[name], len(counts)) if len(counts) else np.zeros((0, 1))
+            self._tables[name], self._held[name] = put(packed), put(held[name])
+            self._steps[name] = extend_tables(
+                self._tables[name], self._held[name], put(counts), put(have), none, drawn,
+                page_size=page, tokens=tokens, parents=parents)
+
+    @property
+    def positions(self) -> torch.Tensor:
+        return self.offsets
+
+    def rope(self, x: torch.Tensor, dims: int, *, base: float | None = None,
+             freqs: Any = None) -> torch.Tensor:
+        """Rotate ``[tokens, heads, head_dim]`` at the tokens' positions
+        (batches.py:70-81)."""
+        return rope(x.to(self.cache.dtype).contiguous(), self.offsets, dims, base=base,
+                    freqs=freqs)
+
+    def _write(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> str:
+        group = self.cache.layer_group[layer]
+        self.cache.write(layer, self._steps[group.name].rows, k, v)
+        return group.name
+
+
+class PackedPrefillBatch(_ManyTokens):
+    """Whole prompts of several sequences in one step: ``tokens`` holds them one behind
+    the other, ``counts[b]`` of sequence b, which holds nothing yet. Their keys and
+    values go to the cache, and every prompt attends to itself as it was projected (in
+    an 8-bit cache too: what later steps read is rounded, what the prompt sees is not).
+    ``tables``: per group the pages of each sequence. Outputs ``[tokens, q_heads *
+    head_dim]``; ``ends`` are the rows of the prompts' last tokens. The reference
+    prefills one sequence a step (``PrefillBatch``, batches.py:26-132)."""
+
+    def __init__(self, cache: KVCache, tokens: torch.Tensor, *, counts: np.ndarray,
+                 tables: dict[str, list[np.ndarray]]) -> None:
+        counts = np.asarray(counts).astype(np.int64)
+        if counts.ndim != 1 or np.any(counts < 0) or int(counts.sum()) != int(tokens.shape[0]):
+            raise ValueError("counts must be the tokens of each prompt")
+        self.cache, self.tokens, self.count = cache, tokens, int(tokens.shape[0])
+        zero = np.zeros_like(counts)
+        self._place(cache, counts, dict.fromkeys(cache.groups, zero), tables, None, self.count)
+        step = next(iter(self._steps.values()))
+        self.offsets, self.starts = step.positions, step.starts
+        self.ends = torch.as_tensor(np.cumsum(counts)[counts > 0] - 1, device=cache.device)
+
+    def attend(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
+               scale: float, softcap: float = 0.0) -> torch.Tensor:
+        """Write the prompts' K/V, then their attention. ``q`` ``[tokens, q_heads,
+        head_dim]``, ``k`` and ``v`` ``[tokens, kv_heads, head_dim]``; slices of one
+        projection are read where they are."""
+        self._write(layer, k, v)
+        dtype = self.cache.dtype
+        out = packed_prompt_attention(
+            q.to(dtype), k.to(dtype), v.to(dtype), self.starts, scale=scale,
+            window=self.cache.layer_group[layer].window, softcap=softcap)
+        return out.reshape(self.count, -1)
+
+
+class DraftBatch(_ManyTokens):
+    """A step that verifies a tree of drafted tokens for every sequence: ``tokens``
+    holds the trees one behind the other, ``counts[b]`` nodes (up to 64) of sequence b,
+    node 0 its newest token, and ``parents`` each node's parent among its sequence's
+    nodes (-1: none). ``positions``: of each sequence's node 0. ``held``: the rows held
+    before the step where rows were evicted, as for :class:`DecodeBatch`. ``tables``:
+    per group the pages of each sequence, with room for all nodes. After the layers,
+    :meth:`commit` keeps the nodes that the model agrees with. No counterpart in the
+    reference."""
+
+    def __init__(self, cache: KVCache, tokens: torch.Tensor, *, counts: np.ndarray,
+                 parents: np.ndarray, positions: np.ndarray,
+                 tables: dict[str, list[np.ndarray]],
+                 held: np.ndarray | dict[str, np.ndarray] | None = None) -> None:
+        counts = np.asarray(counts).astype(np.int64)
+        parents = np.asarray(parents).astype(np.int64)
+        positions = np.asarray(positions).astype(np.int64)
+        if counts.ndim != 1 or np.any(counts < 0) or int(counts.sum()) != int(tokens.shape[0]):
+            raise ValueError("counts must be the nodes of each tree")
+        if np.any(counts > NODES):
+            raise ValueError(f"a tree holds up to {NODES} nodes")
+        if positions.shape != counts.shape or np.any(positions < 0):
+            raise ValueError("positions must be those of each sequence's first node")
+        index = np.arange(len(tokens)) - np.repeat(np.cumsum(counts) - counts, counts)
+        if parents.shape != index.shape or np.any((parents < -1) | (parents >= index)):
+            raise ValueError("a node's parent is an earlier node of its tree, or -1")
+        self.cache, self.tokens, self.count = cache, tokens, int(tokens.shape[0])
+        rows = {} if held is None else rows_by_group(cache, held, counts.shape)
+        for name, n in rows.items():
+            if cache.groups[name].window and np.any(n != positions):
+                raise ValueError("a windowed group releases its pages by position")
+        self.parents = torch.as_tensor(parents.astype(np.int32), device=cache.device)
+        self._place(cache, counts, {name: rows.get(name, positions) for name in cache.groups},
+                    tables, self.parents, self.count)
+        name, step = next(iter(self._steps.items()))
+        self.starts, self.masks, self.offsets = step.starts, step.masks, step.positions
+        if name in rows:  # (positions count on where rows were evicted)
+            ahead = np.repeat(positions - rows[name], counts).astype(np.int32)
+            self.offsets = self.offsets + torch.as_tensor(ahead, device=cache.device)
+
+    def attend(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
+               scale: float, softcap: float = 0.0) -> torch.Tensor:
+        """Write the nodes' K/V behind the rows held, then attention over those and the
+        nodes' ancestors, ``[tokens, q_heads * head_dim]``."""
+        name = self._write(layer, k, v)
+        cache = self.cache
+        out = tree_attention(
+            q.to(cache.decode_dtype).contiguous(), cache.keys[layer], cache.values[layer],
+            self._tables[name], self._held[name], self.starts, self.masks,
+            page_size=cache.page_size, scale=scale, window=cache.groups[name].window,
+            softcap=softcap, scales=cache.scales(layer))
+        return out.reshape(self.count, -1).to(cache.dtype)
+
+    def commit(self, targets: torch.Tensor) -> dict[str, Committed]:
+        """Keep each tree's line of nodes that the model agrees with: ``targets`` is its
+        choice after every node, of the tokens' type. Moves the kept rows in every
+        layer; returns what was kept by group (the same but for ``lengths``, the rows
+        held now). The sequences' pages stay theirs."""
+        done = {}
+        for name, group in self.cache.groups.items():
+            arenas = [(self.cache.keys[i], self.cache.values[i], *(self.cache.scales(i) or ()))
+                      for i in group.layers]
+            done[name] = commit_drafts(
+                arenas, self._tables[name], self._held[name], self.starts, self.parents,
+                self.tokens.to(self.cache.device), targets, page_size=self.cache.page_size)
+        return done

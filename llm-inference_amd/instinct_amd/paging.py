@@ -3,7 +3,7 @@
 The reference gives a step's tokens their rows in host loops (``KVCache.rows``,
 python/instinct/paged_kv.py:259-265; ``DecodeBatch.__init__``, batches.py:148-179)
 after drawing the pages that they need one by one. Here the host sets pages aside
-ahead of time (:meth:`instinct_amd.paged_kv.KVCache.reserve_feed`) and
+ahead of time (:class:`PageFeed`) and
 :func:`extend_tables` does the rest of a step in one launch: it lengthens the page
 tables out of that feed and gives every token its row and its position, and the nodes
 of drafted trees the mask of their ancestors. Nothing crosses PCIe, so the launch can
@@ -14,13 +14,56 @@ The work happens in libpda.so (``csrc/pda_paging.hip``).
 
 from __future__ import annotations
 
-from typing import NamedTuple
+from typing import TYPE_CHECKING, NamedTuple
 
+import numpy as np
 import torch
 
 from . import _lib
 from .eviction import _check_index
 from .hip_kernels import on_device
+
+if TYPE_CHECKING:
+    from .paged_kv import KVCache
+
+
+class PageFeed:
+    """Pages of a group's pool set aside for steps that take them on the GPU: ``pages``
+    and ``drawn`` are what :func:`extend_tables` takes. The pages that were drawn belong
+    to the sequences whose tables have them and go back with those
+    (``PagePool.release``); :meth:`refill` and :meth:`close` read ``drawn`` (and wait
+    for the GPU)."""
+
+    def __init__(self, cache: "KVCache", group: str, count: int) -> None:
+        self._cache, self._pool = cache, cache.pools[group]
+        self._ids = self._pool.allocate_many(count, reserved=False)
+        self._put()
+
+    def _put(self) -> None:
+        device = self._cache.device
+        self.pages = torch.as_tensor(self._ids.astype(np.int32), device=device)
+        self.drawn = torch.zeros(2, dtype=torch.int32, device=device)
+
+    def _left(self) -> np.ndarray:
+        drawn = int(self.drawn[0])
+        if drawn > len(self._ids):
+            raise RuntimeError(f"steps asked for {drawn} pages of a feed of {len(self._ids)}: "
+                               "some of their tokens have no row")
+        return self._ids[drawn:]
+
+    def refill(self, count: int) -> None:
+        """``count`` pages to draw again, in new tensors."""
+        left = self._left()
+        more = max(0, count - len(left))
+        self._ids = np.concatenate([left, self._pool.allocate_many(more, reserved=False)])
+        self._put()
+
+    def close(self) -> None:
+        """Gives the pages that were not drawn back to the pool."""
+        left = self._left()
+        self._ids = self._ids[:0]
+        self._put()
+        self._pool.release(left)
 
 
 class StepRows(NamedTuple):
