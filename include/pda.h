@@ -857,8 +857,8 @@ int pda_packed_prompt_attention_bf16(const void* queries, int64_t q_token,
                                 int32_t head_dim, float scale, int32_t window,
                                 float softcap, void* stream);
 
-/* Bytes of workspace of a tree attention call, whatever its lengths. */
-int pda_tree_workspace_bytes(int32_t batch, int32_t head_dim, size_t* bytes);
+/* Bytes of workspace of a tree attention call, whatever its batch and lengths. */
+int pda_tree_workspace_bytes(int32_t head_dim, size_t* bytes);
 
 /* Attention for trees of drafted tokens over the paged cache. Sequence b holds
  * lengths[b] rows; its nodes' keys and values lie behind them, node j's in row

@@ -6,13 +6,13 @@
 // Node i of a sequence's tree lies behind the l rows that the sequence holds, in
 // row l + i, and attends to the held rows and to the nodes whose bits its mask has
 // (itself and its ancestors): flops 4 D a (query head, node, visible key); the
-// rows of a kv head are read once for up to 128 (node, query head) pairs of it.
+// rows of a kv head are read once for up to 256 (node, query head) pairs of it.
 //
-// Rows of queries. A unit is (sequence, kv head, 128 of its node and head pairs);
-// its keys come in tiles of 64. The tiles of all units form one stream that is cut
-// into equal ranges, one a workgroup, whatever the lengths: a unit inside one range
-// is written at once, the pieces of one that is cut are joined by a second kernel.
-// The cuts depend on the lengths alone, so repeated calls give the same bits.
+// Rows of queries. A unit is (sequence, kv head, 128 or 256 of its node and head
+// pairs); its keys come in tiles of 64. The tiles of all units form one stream that is
+// cut into equal ranges, one a workgroup, whatever the lengths: a unit inside one
+// range is written at once, the pieces of one that is cut are joined by a second
+// kernel. The cuts depend on the lengths alone, so repeated calls give the same bits.
 
 #include <hip/hip_runtime.h>
 
@@ -34,11 +34,25 @@ using pda_internal::ok;
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kThreads = 256;
-constexpr int kRows = 128;   // of a unit
-constexpr int kNodes = 64;   // of a tree
+constexpr int kThreads = 256;  // of a workgroup of four waves, and of the join's
+constexpr int kNodes = 64;     // of a tree
 constexpr int kCus = 256;
-constexpr int groups_for(int width) { return width <= 128 ? 2 * kCus : kCus; }
+// Workgroups: as many as the GPU holds at once.
+constexpr int groups_for(int width, int waves) { return width <= 128 && waves == 4 ? 2 * kCus : kCus; }
+// Tiles that a range has at least.
+constexpr int kLeastTiles = 2;
+
+// What the join has to know of a unit that ends in a workgroup's range and began in
+// an earlier one.
+struct Cut {
+  int32_t rows;     // of the unit (0: no such unit)
+  int32_t first;    // its first (token, query head) row, without the kv head's
+  int32_t token;    // the sequence's first token
+  int32_t kvh;
+  int32_t piece;    // its first piece
+  int32_t group;    // the workgroup after that piece's
+  int32_t pad[2];
+};
 
 struct TreeParams {
   const f16* q;          // [tokens, hq, dim]
@@ -51,10 +65,9 @@ struct TreeParams {
   const int32_t* starts;   // [batch + 1]
   const uint64_t* masks;   // [tokens]
   f16* out;                // [tokens, hq, dim]
-  int64_t* seq_tiles;      // [batch + 1] first tile of each sequence in the stream,
-  int32_t* seq_units;      // [batch + 1]   and its first unit
-  float* part_o;           // [2 groups, 4 waves, D / 8, 64 lanes, 4]
-  float2* part_ml;         // [2 groups, 128]
+  float* part_o;           // [2 groups, waves, D / 8, 64 lanes, 4]
+  float2* part_ml;         // [2 groups, waves, 32]
+  Cut* cuts;               // [groups]
   int64_t arena_pages;
   int64_t page_elems, scale_page;  // elements between pages,
   int32_t head_elems, scale_head;  //   kv heads of a page,
@@ -64,6 +77,7 @@ struct TreeParams {
   int32_t tokens;
   int32_t batch;
   int32_t groups;  // workgroups that take ranges
+  int32_t rows;    // of a unit: 32 a wave
   int32_t hq;
   int32_t hkv;
   int32_t dim;
@@ -86,7 +100,7 @@ __device__ __forceinline__ Seq seq_of(const TreeParams& p, int b) {
   s.t0 = p.window > 0 ? max(0, s.held - p.window + 1) / kKeys : 0;
   const int end = s.held + min(s.n, kNodes);
   s.nt = s.n > 0 ? (end + kKeys - 1) / kKeys - s.t0 : 0;
-  s.blocks = (int)(((int64_t)s.n * (p.hq / p.hkv) + kRows - 1) / kRows);
+  s.blocks = (int)(((int64_t)s.n * (p.hq / p.hkv) + p.rows - 1) / p.rows);
   return s;
 }
 __device__ __forceinline__ Seq uniform_seq(const Seq& s) {
@@ -99,81 +113,54 @@ __device__ __forceinline__ int64_t tiles_of(const TreeParams& p, const Seq& s) {
 
 // Workgroups that take ranges of a stream of `tiles`, and the first tile of one's.
 __device__ __forceinline__ int64_t ranges(const TreeParams& p, int64_t tiles) {
-  return min(tiles, (int64_t)p.groups);
+  return min((tiles + kLeastTiles - 1) / kLeastTiles, (int64_t)p.groups);
 }
 __device__ __forceinline__ int64_t range_begin(int64_t tiles, int64_t n, int64_t g) {
   return tiles * g / n;
 }
 
-// Prefix sums over the sequences: the stream's length, and sequence `seq` that
-// holds tile x, which is its `rest`-th. Workgroup 0 leaves the sums for the join.
-// (x is past the stream's end: seq is batch.)
-template <class F>
-__device__ __forceinline__ int64_t locate(const TreeParams& p, F pick, int& seq, int64_t& rest) {
-  __shared__ int64_t s_tiles[kThreads / 64];
-  __shared__ int32_t s_units[kThreads / 64];
-  __shared__ int s_seq;
-  __shared__ int64_t s_rest;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const int per = (p.batch + kThreads - 1) / kThreads;
-  const int b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
+// The workgroup's range of the stream of all sequences' tiles, and the sequence that
+// its first tile belongs to, of which it is the `rest`-th. Every wave finds them by
+// itself, a lane for a few sequences.
+struct Range {
+  int64_t all, n, begin, end, rest;
+  int seq;
+};
+__device__ __forceinline__ Range range_of(const TreeParams& p) {
+  const int lane = threadIdx.x & 63;
+  const int per = (p.batch + 63) / 64;
+  const int b0 = min(lane * per, p.batch), b1 = min(b0 + per, p.batch);
   int64_t mine = 0;
-  int32_t units = 0;
-  for (int b = b0; b < b1; ++b) {
-    const Seq s = seq_of(p, b);
-    mine += tiles_of(p, s);
-    units += s.blocks * p.hkv;
-  }
+  for (int b = b0; b < b1; ++b) mine += tiles_of(p, seq_of(p, b));
   int64_t upto = mine;
-  int32_t upto_units = units;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
     const int64_t y = __shfl_up(upto, d);
-    const int32_t z = __shfl_up(upto_units, d);
-    if (lane >= d) upto += y, upto_units += z;
+    if (lane >= d) upto += y;
   }
-  if (lane == 63) s_tiles[w] = upto, s_units[w] = upto_units;
-  if (tid == 0) s_seq = p.batch;
-  __syncthreads();
-  int64_t before = upto - mine, all = 0;
-  int32_t before_units = upto_units - units, all_units = 0;
-  for (int i = 0; i < kThreads / 64; ++i) {
-    if (i < w) before += s_tiles[i], before_units += s_units[i];
-    all += s_tiles[i];
-    all_units += s_units[i];
+  Range r;
+  r.all = uniform64(__shfl(upto, 63));
+  r.n = ranges(p, r.all);
+  if (blockIdx.x >= r.n) {
+    r.begin = r.end = r.rest = 0;
+    r.seq = 0;
+    return r;
   }
-  const int64_t x = pick(uniform64(all));
-  if (blockIdx.x == 0) {
-    int64_t t = before;
-    int32_t u = before_units;
-    for (int b = b0; b < b1; ++b) {
-      const Seq s = seq_of(p, b);
-      p.seq_tiles[b] = t;
-      p.seq_units[b] = u;
-      t += tiles_of(p, s);
-      u += s.blocks * p.hkv;
-    }
-    if (tid == 0) {
-      p.seq_tiles[p.batch] = all;
-      p.seq_units[p.batch] = all_units;
-    }
-  }
-  if (x >= before && x < before + mine) {
-    int64_t left = x - before;
-    for (int b = b0; b < b1; ++b) {
-      const int64_t n = tiles_of(p, seq_of(p, b));
-      if (left < n) {
-        s_seq = b;
-        s_rest = left;
-        break;
-      }
+  r.begin = range_begin(r.all, r.n, blockIdx.x);
+  r.end = range_begin(r.all, r.n, blockIdx.x + 1);
+  const bool here = r.begin >= upto - mine && r.begin < upto;
+  int64_t left = r.begin - (upto - mine);
+  int seq = b0;
+  if (here)
+    for (; seq < b1 - 1; ++seq) {
+      const int64_t n = tiles_of(p, seq_of(p, seq));
+      if (left < n) break;
       left -= n;
     }
-  }
-  __syncthreads();
-  seq = uniform(s_seq);
-  rest = uniform64(s_rest);
-  return uniform64(all);
+  const int owner = __builtin_ctzll(__ballot(here));
+  r.seq = uniform(__shfl(seq, owner));
+  r.rest = uniform64(__shfl(left, owner));
+  return r;
 }
 
 // Eight int8 values as elements of the queries' type, exactly.
@@ -195,263 +182,363 @@ __device__ __forceinline__ f16x8 from_bytes(const u32x2& y, float scale) {
   return x;
 }
 
-template <int D, bool BF, bool Q8>
-__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void tree_attention_kernel(
+// A unit's keys and values on their way from the pages through LDS, and their masks.
+// W waves: with eight the first four copy V and the others K.
+template <int D, bool BF, bool Q8, int W>
+struct TreeTiles {
+  static constexpr int kPlanes = D / 32;
+  static constexpr int kHalves = kPlanes * kPlane;  // of a tile
+  static constexpr int kCopies = W == 4 ? 2 * kPlanes : kPlanes;
+
+  const TreeParams& p;
+  f16* s_k;          // [2][kHalves]
+  f16* s_v;
+  float* s_scale;    // [4][64] the keys' scales, by tile
+  uint16_t* s_ok;    // [4][4] usable keys, by tile and wave
+  int* s_left;       // whether values that are not finite were taken as zeros
+  bool special;
+  int lane, w, gk, kchunk, vchunk;
+  uint32_t k_dst, v_dst, pages;
+
+  // The piece's.
+  const int32_t* table;
+  int kvh, held, last;
+  uint64_t mask;  // nodes that the lane's row sees
+  int lo;         // and the first row held
+  // This thread's key of the tiles whose V and K are copied next, and the looked-up
+  // page of the tile after them.
+  int64_t at_v, at_k, scale_v, scale_k;
+  bool ok_v, ok_k, in;
+  int page;
+  uint32_t slot;
+  uint64_t usable, usable_before;  // keys of the tile that is scored, and of the last
+  u32x2 raw_k[Q8 ? kPlanes : 1], raw_v[Q8 ? kPlanes : 1];
+  f16 raw_ks, raw_vs;
+
+  __device__ __forceinline__ bool moves_v() const { return W == 4 || w < 4; }
+  __device__ __forceinline__ bool moves_k() const { return W == 4 || w >= 4; }
+
+  __device__ __forceinline__ void init() {
+    const int tid = threadIdx.x;
+    lane = tid & 63;
+    w = uniform(tid >> 6);
+    // Copies: a thread moves key (tid / 4) % 64 of a tile, one 8-element chunk a plane.
+    gk = (tid >> 2) & 63;
+    kchunk = 8 * ((lane & 3) ^ ((lane >> 4) & 3));
+    vchunk = 8 * (lane & 3);
+    k_dst = uniform(lds_address(s_k) + 1024 * (w & 3));
+    v_dst = uniform(lds_address(s_v) + 1024 * (w & 3));
+    pages = (uint32_t)min(p.arena_pages, (int64_t)INT32_MAX);
+    special = p.shape.cap_out > 0.0f || !(p.shape.scale_log2 > 0.0f);
+    if (p.dim != D) {  // what no copy writes
+      for (int i = 8 * tid; i < 2 * kHalves; i += 8 * 64 * W) {
+        *reinterpret_cast<f16x8*>(s_k + i) = f16x8{};
+        *reinterpret_cast<f16x8*>(s_v + i) = f16x8{};
+      }
+      __syncthreads();
+    }
+  }
+  __device__ __forceinline__ const f16* keys(int t) const { return s_k + (t & 1) * kHalves; }
+  __device__ __forceinline__ const f16* values(int t) const { return s_v + (t & 1) * kHalves; }
+
+  __device__ __forceinline__ void lookup(int t) {
+    const uint32_t kp = (uint32_t)t * kKeys + gk;
+    const uint32_t pi = kp / (uint32_t)p.page_size;
+    slot = kp - pi * (uint32_t)p.page_size;
+    in = kp <= (uint32_t)last && pi < (uint32_t)p.stride;
+    page = table[min(pi, (uint32_t)p.stride - 1)];
+  }
+  // The looked-up tile becomes the next K to copy, the one before it the next V.
+  __device__ __forceinline__ void turn() {
+    at_v = at_k;
+    ok_v = ok_k;
+    ok_k = in && (uint32_t)page < pages;
+    const int64_t from = ok_k ? page : 0;
+    at_k = from * p.page_elems + (int64_t)slot * p.row_elems + (int64_t)kvh * p.head_elems;
+    if constexpr (Q8) {
+      scale_v = scale_k;
+      scale_k = from * p.scale_page + (int64_t)slot * p.scale_row + (int64_t)kvh * p.scale_head;
+    }
+  }
+  __device__ __forceinline__ void copy_k(int t, int i) {
+    if constexpr (Q8) {
+      if (i == 0) raw_ks = p.kscale[scale_k];
+    }
+    if (D != p.dim && 32 * i + kchunk >= p.dim) return;
+    if constexpr (Q8) {
+      raw_k[i] = *reinterpret_cast<const u32x2*>(static_cast<const int8_t*>(p.k) + at_k + kchunk + 32 * i);
+    } else {
+      copy_to_lds(static_cast<const f16*>(p.k) + at_k + kchunk + 32 * i,
+                  k_dst + (t & 1) * (2 * kHalves) + 2 * kPlane * i);
+    }
+  }
+  __device__ __forceinline__ void copy_v(int t, int i) {
+    if (D != p.dim && 32 * i + vchunk >= p.dim) return;
+    if constexpr (Q8) {
+      raw_v[i] = *reinterpret_cast<const u32x2*>(static_cast<const int8_t*>(p.v) + at_v + vchunk + 32 * i);
+      if (i == 0) raw_vs = p.vscale[scale_v];
+    } else {
+      copy_to_lds(static_cast<const f16*>(p.v) + at_v + vchunk + 32 * i,
+                  v_dst + (t & 1) * (2 * kHalves) + 2 * kPlane * i);
+    }
+  }
+  template <int j>
+  __device__ __forceinline__ void copy(int t) {
+    if constexpr (W == 4) {
+      if constexpr (j < kPlanes)
+        copy_v(t, j);
+      else
+        copy_k(t + 1, j - kPlanes);
+    } else {
+      if (w < 4)
+        copy_v(t, j);
+      else
+        copy_k(t + 1, j);
+    }
+  }
+  // 8 bits: what was loaded goes to LDS, the keys as they are (their scales beside
+  // them, for the scores), the values times their scale.
+  __device__ __forceinline__ void put_k(int t) {
+    if constexpr (Q8) {
+      if (!moves_k()) return;
+      f16* dst = s_k + (t & 1) * kHalves + 32 * gk + 8 * (lane & 3);
+      if ((lane & 3) == 0) s_scale[kKeys * (t & 3) + gk] = (float)raw_ks;
+#pragma unroll
+      for (int i = 0; i < kPlanes; ++i)
+        if (D == p.dim || 32 * i + kchunk < p.dim)
+          *reinterpret_cast<f16x8*>(dst + kPlane * i) = from_bytes<BF>(raw_k[i]);
+    }
+  }
+
+  // Tiles with keys that not every row sees.
+  __device__ __forceinline__ bool edge(int t) const {
+    return t * kKeys + kKeys > held || (p.window > 0 && t * kKeys < held + kNodes - p.window);
+  }
+  // V of tile t as it arrived: rows that are not usable become zeros (their weight is
+  // 0, but 0 times what an arena holds there need not be); on an edge, values that are
+  // not finite too.
+  __device__ __forceinline__ void put_v(int t) {
+    if (!moves_v()) return;
+    const bool check = edge(t);
+    f16* dst = s_v + (t & 1) * kHalves + 32 * gk + 8 * (lane & 3);
+    if constexpr (Q8) {
+      const float vs = (float)raw_vs;
+#pragma unroll
+      for (int i = 0; i < kPlanes; ++i) {
+        if (D != p.dim && 32 * i + vchunk >= p.dim) continue;
+        f16x8 x = from_bytes<BF>(raw_v[i], vs);
+        if (!ok_v) x = f16x8{};
+        if (check && not_finite<BF>(x)) {
+          *s_left = 1;
+          x = finite_only<BF>(x);
+        }
+        *reinterpret_cast<f16x8*>(dst + kPlane * i) = x;
+      }
+    } else if (!ok_v) {
+#pragma unroll
+      for (int i = 0; i < kPlanes; ++i) *reinterpret_cast<f16x8*>(dst + kPlane * i) = f16x8{};
+    } else if (check) {
+#pragma unroll
+      for (int i = 0; i < kPlanes; ++i) {
+        const f16x8 x = *reinterpret_cast<const f16x8*>(dst + kPlane * i);
+        if (not_finite<BF>(x)) {
+          *s_left = 1;
+          *reinterpret_cast<f16x8*>(dst + kPlane * i) = finite_only<BF>(x);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void put_usable(int t) {
+    if (!moves_k()) return;
+    const uint32_t flags = keys_of(__ballot(ok_k));
+    if (lane == 0) s_ok[4 * (t & 3) + (w & 3)] = (uint16_t)flags;
+  }
+  __device__ __forceinline__ void take_usable(int t) {
+    usable_before = usable;
+    usable = (uint64_t)uniform64((int64_t)*reinterpret_cast<const uint64_t*>(s_ok + 4 * (t & 3)));
+  }
+
+  __device__ __forceinline__ void first(int t) {
+    lookup(t);
+    turn();
+    lookup(t + 1);
+    if (moves_k())
+#pragma unroll
+      for (int i = 0; i < kPlanes; ++i) copy_k(t, i);
+    put_usable(t);
+    if constexpr (Q8) put_k(t);
+    turn();
+    auto one = [&](auto j) { copy<j.value>(t); };
+    each(one, std::make_integer_sequence<int, kCopies>{});
+    if (!Q8 && D == p.dim && W == 4)
+      wait_vmem<kCopies>();  // the first K alone
+    else
+      wait_vmem<0>();
+    __syncthreads();
+    take_usable(t);
+    lookup(t + 2);
+  }
+  __device__ __forceinline__ void close(int t) {
+    wait_vmem<0>();
+    put_v(t);
+    put_k(t + 1);
+    put_usable(t + 1);
+    __syncthreads();
+    take_usable(t + 1);
+    turn();
+    lookup(t + 3);
+  }
+
+  __device__ __forceinline__ uint32_t visible(int k0, uint32_t ok) const {
+    const int d = held - k0;  // the tree's first row in the block
+    uint32_t nodes = 0;
+    if (d >= 0 && d < 32) nodes = (uint32_t)(mask << d);
+    if (d < 0 && d > -kNodes) nodes = (uint32_t)(mask >> -d);
+    return ok & ((below(d) & ~below(lo - k0)) | nodes);
+  }
+  // Usable keys of the block from k0 on, of the tile that is scored or the one before.
+  __device__ __forceinline__ uint32_t ok_of(int k0) const {
+    return k0 & 32 ? (uint32_t)(usable_before >> 32) : (uint32_t)usable;
+  }
+  __device__ __forceinline__ bool rough(int t) const {
+    return Q8 || special || edge(t) || edge(t - 1) ||
+           ((uint32_t)usable & (uint32_t)(usable_before >> 32)) != 0xFFFFFFFFu;
+  }
+  __device__ __forceinline__ void shape(f32x16& x, int k0) const {
+    if constexpr (Q8) {
+      const float* ks = s_scale + (k0 & (4 * kKeys - 1)) + 4 * (lane >> 5);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float4 y = *reinterpret_cast<const float4*>(ks + 8 * g);
+        x[4 * g] *= y.x;
+        x[4 * g + 1] *= y.y;
+        x[4 * g + 2] *= y.z;
+        x[4 * g + 3] *= y.w;
+      }
+    }
+    if (special) Rows<D, BF>::shape(x, p.shape);
+    const uint32_t ok = ok_of(k0);
+    if (edge(k0 / kKeys) || ok != 0xFFFFFFFFu) Rows<D, BF>::mask(x, visible(k0, ok));
+  }
+  // After the piece's last tile: the values that were taken as zeros, to the rows that
+  // see them.
+  __device__ __forceinline__ void add_left_out(Rows<D, BF>& r, int ta, int tb) const {
+    __syncthreads();
+    if (uniform(*s_left) == 0) return;
+    for (int t = ta; t < tb; ++t) {
+      if (!edge(t)) continue;
+      for (int k = t * kKeys; k <= min(t * kKeys + kKeys - 1, last); ++k) {
+        const uint32_t pi = (uint32_t)k / (uint32_t)p.page_size;
+        const uint32_t sl = (uint32_t)k - pi * (uint32_t)p.page_size;
+        const int from = pi < (uint32_t)p.stride ? table[pi] : -1;
+        if ((uint32_t)from >= pages) continue;
+        const int64_t at = from * p.page_elems + (int64_t)sl * p.row_elems +
+                           (int64_t)kvh * p.head_elems;
+        const bool seen = k < held ? k >= lo : (mask >> (k - held) & 1) != 0;
+        r.add_not_finite(seen, p.dim, [&](int d) {
+          if constexpr (Q8) {
+            const float vs = (float)p.vscale[from * p.scale_page + (int64_t)sl * p.scale_row +
+                                             (int64_t)kvh * p.scale_head];
+            const int8_t* y = static_cast<const int8_t*>(p.v) + at + d;
+            return make_float4(y[0] * vs, y[1] * vs, y[2] * vs, y[3] * vs);
+          } else {
+            return widen4<BF>(static_cast<const f16*>(p.v) + at + d);
+          }
+        });
+      }
+    }
+  }
+};
+
+template <int D, bool BF, bool Q8, int W>
+__global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void tree_attention_kernel(
     const TreeParams p) {
-  constexpr int kPlanes = D / 32;
-  constexpr int kTileHalves = kPlanes * kPlane;
-  __shared__ __align__(1024) f16 s_k[2][kTileHalves];
-  __shared__ __align__(1024) f16 s_v[2][kTileHalves];
-  __shared__ __align__(16) float s_scale[2][kKeys];  // the keys' scales
-  __shared__ uint16_t s_ok[2][4], s_bad[2][4];  // usable keys; values not finite
+  using Tiles = TreeTiles<D, BF, Q8, W>;
+  __shared__ __align__(1024) f16 s_k[2 * Tiles::kHalves];
+  __shared__ __align__(1024) f16 s_v[2 * Tiles::kHalves];
+  __shared__ __align__(16) float s_scale[Q8 ? 4 * kKeys : 4];
+  __shared__ __align__(8) uint16_t s_ok[4 * 4];
+  __shared__ int s_left;
 
   const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
   const int G = p.hq / p.hkv;
-
   // Rows behind the last sequence: zeros.
   {
     const int real = p.batch > 0 ? max(0, min(p.starts[p.batch], p.tokens)) : 0;
     const int64_t from = (int64_t)real * p.hq * p.dim / 8, to = (int64_t)p.tokens * p.hq * p.dim / 8;
-    for (int64_t i = from + blockIdx.x * kThreads + tid; i < to; i += (int64_t)gridDim.x * kThreads)
+    for (int64_t i = from + blockIdx.x * (64 * W) + tid; i < to; i += (int64_t)gridDim.x * (64 * W))
       reinterpret_cast<f16x8*>(p.out)[i] = f16x8{};
   }
-  int seq;
-  int64_t rest, begin = 0, end = 0;
-  locate(p, [&](int64_t all) -> int64_t {
-    const int64_t n = ranges(p, all);
-    if (blockIdx.x >= n) return all;
-    begin = range_begin(all, n, blockIdx.x);
-    end = range_begin(all, n, blockIdx.x + 1);
-    return begin;
-  }, seq, rest);
-  if (begin >= end) return;
-
-  if (p.dim != D) {  // what no copy writes
-    f16* flat_k = &s_k[0][0];
-    f16* flat_v = &s_v[0][0];
-    for (int i = 8 * tid; i < 2 * kTileHalves; i += 8 * kThreads) {
-      *reinterpret_cast<f16x8*>(flat_k + i) = f16x8{};
-      *reinterpret_cast<f16x8*>(flat_v + i) = f16x8{};
-    }
-    __syncthreads();
-  }
-
+  const Range range = range_of(p);
+  Cut cut = {};  // of the unit that the first piece ends, if it began before
+  int64_t left = range.end - range.begin, rest = range.rest;
+  int seq = range.seq;
   Rows<D, BF> r;
   r.init(p.shape);
-  const bool special = p.shape.cap_out > 0.0f || !(p.shape.scale_log2 > 0.0f);
-  const uint32_t pages = (uint32_t)min(p.arena_pages, (int64_t)INT32_MAX);
-
-  // Copies: thread tid moves key tid / 4 of a tile, one 8-element chunk a plane.
-  const int gk = tid >> 2;
-  const int kchunk = 8 * ((lane & 3) ^ ((lane >> 4) & 3)), vchunk = 8 * (lane & 3);
-  const uint32_t k_dst = uniform(lds_address(&s_k[0][0]) + 1024 * w);
-  const uint32_t v_dst = uniform(lds_address(&s_v[0][0]) + 1024 * w);
-
-  int64_t left = end - begin;
+  Tiles x{p, s_k, s_v, s_scale, s_ok, &s_left};
+  if (left > 0) x.init();
   bool first_piece = true;
   while (left > 0) {
     const Seq s = uniform_seq(seq_of(p, seq));
     const int unit = uniform((int)(rest / s.nt));
-    const int ta = s.t0 + (int)(rest - (int64_t)unit * s.nt);
-    const int tb = s.t0 + (int)min((int64_t)s.nt, rest - (int64_t)unit * s.nt + left);
+    const int begin = (int)(rest - (int64_t)unit * s.nt);
+    const int end = (int)min((int64_t)s.nt, begin + left);
     const int kvh = uniform(unit / s.blocks), block = unit - kvh * s.blocks;
-    const int32_t* table = p.tables + (int64_t)seq * p.stride;
 
     // This lane's row: a node and a query head. (Rows past the last see what that
     // one sees, and are not stored.)
-    const int all_rows = s.n * G;
-    const int row = kRows * block + 32 * w + (lane & 31);
-    const bool wave_live = kRows * block + 32 * w < all_rows;
-    const bool live = row < all_rows;
+    const int first_row = 32 * W * block, all_rows = s.n * G;
+    const int row = first_row + 32 * w + (lane & 31);
+    const bool wave_live = first_row + 32 * w < all_rows;
     const int at = min(row, all_rows - 1);
     const int node = at / G;
     const int64_t q_row = (int64_t)(s.first + node) * p.hq + kvh * G + at % G;
     r.clear();
     r.load(p.q + q_row * p.dim, p.dim, true);
-    uint64_t mask = p.masks[s.first + node];
-    const int depth = max(0, (int)__popcll(mask) - 1);
-    int lo = 0;  // first held row the node sees
+    x.mask = p.masks[s.first + node];
+    const int depth = max(0, (int)__popcll(x.mask) - 1);
+    x.lo = 0;
     if (p.window > 0) {
-      lo = max(0, s.held + depth - p.window + 1);
-      while ((int)__popcll(mask) > p.window) mask &= mask - 1;
+      x.lo = max(0, s.held + depth - p.window + 1);
+      while ((int)__popcll(x.mask) > p.window) x.mask &= x.mask - 1;
     }
-    const int last = s.held + min(s.n, kNodes) - 1;
+    x.table = p.tables + (int64_t)seq * p.stride;
+    x.kvh = kvh;
+    x.held = s.held;
+    x.last = s.held + min(s.n, kNodes) - 1;
+    const int ta = s.t0 + begin, tb = s.t0 + end;
+    if (!first_piece) __syncthreads();  // (others may still read the last tile)
+    if (tid == 0) s_left = 0;
+    attend(r, x, ta, tb, ta, wave_live ? tb : ta, x.last >= (tb - 1) * kKeys + 32);
+    x.add_left_out(r, ta, tb);
 
-    int page = 0;
-    bool in = false;
-    uint32_t slot = 0;
-    auto lookup = [&](int t) {
-      const uint32_t kp = (uint32_t)t * kKeys + gk;
-      const uint32_t pi = kp / (uint32_t)p.page_size;
-      slot = kp - pi * (uint32_t)p.page_size;
-      in = kp <= (uint32_t)last && pi < (uint32_t)p.stride;
-      page = table[min(pi, (uint32_t)p.stride - 1)];
-    };
-    u32x2 raw_k[kPlanes], raw_v[kPlanes];
-    f16 raw_ks = (f16)0.0f, raw_vs = (f16)0.0f;
-    bool mine_ok = false;  // this thread's key of the tile under way
-    auto copies = [&](int t) {
-      const uint32_t buf = (t - ta) & 1;
-      mine_ok = in && (uint32_t)page < pages;
-      const int64_t from = mine_ok ? page : 0;
-      const int64_t src = from * p.page_elems + (int64_t)slot * p.row_elems + (int64_t)kvh * p.head_elems;
-      if constexpr (Q8) {
-        const int64_t sc = from * p.scale_page + (int64_t)slot * p.scale_row + (int64_t)kvh * p.scale_head;
-        raw_ks = p.kscale[sc];
-        raw_vs = p.vscale[sc];
-#pragma unroll
-        for (int i = 0; i < kPlanes; ++i) {
-          if (D == p.dim || 32 * i + kchunk < p.dim)
-            raw_k[i] = *reinterpret_cast<const u32x2*>(static_cast<const int8_t*>(p.k) + src + kchunk + 32 * i);
-          if (D == p.dim || 32 * i + vchunk < p.dim)
-            raw_v[i] = *reinterpret_cast<const u32x2*>(static_cast<const int8_t*>(p.v) + src + vchunk + 32 * i);
-        }
-      } else {
-        const f16* src_k = static_cast<const f16*>(p.k) + src + kchunk;
-        const f16* src_v = static_cast<const f16*>(p.v) + src + vchunk;
-        const uint32_t off = buf * (2 * kTileHalves);
-#pragma unroll
-        for (int i = 0; i < kPlanes; ++i) {
-          if (D == p.dim || 32 * i + kchunk < p.dim)
-            copy_to_lds(src_k + 32 * i, k_dst + off + 2 * kPlane * i);
-          if (D == p.dim || 32 * i + vchunk < p.dim)
-            copy_to_lds(src_v + 32 * i, v_dst + off + 2 * kPlane * i);
-        }
-      }
-    };
-    // Tiles with keys that not every row sees.
-    auto edge = [&](int t) {
-      return t * kKeys + kKeys > s.held ||
-             (p.window > 0 && t * kKeys < s.held + kNodes - p.window);
-    };
-    // What was copied becomes readable: rows that are not usable as zeros (their
-    // weight is 0, but 0 times what an arena holds there need not be); on an edge,
-    // values that are not finite as zeros too, their keys remembered.
-    auto arrive = [&](int t) {
-      const int buf = (t - ta) & 1;
-      wait_vmem<0>();
-      const bool check = edge(t);
-      bool bad = false;
-      f16* dst_k = &s_k[buf][32 * gk + 8 * (lane & 3)];
-      f16* dst_v = &s_v[buf][32 * gk + 8 * (lane & 3)];
-      if constexpr (Q8) {
-        if ((lane & 3) == 0) s_scale[buf][gk] = (float)raw_ks;
-        const float vs = (float)raw_vs;
-#pragma unroll
-        for (int i = 0; i < kPlanes; ++i) {
-          if (D == p.dim || 32 * i + kchunk < p.dim)
-            *reinterpret_cast<f16x8*>(dst_k + kPlane * i) = from_bytes<BF>(raw_k[i]);
-          if (D == p.dim || 32 * i + vchunk < p.dim) {
-            f16x8 x = from_bytes<BF>(raw_v[i], vs);
-            if (!mine_ok) x = f16x8{};
-            if (check && not_finite<BF>(x)) {
-              bad = true;
-              x = finite_only<BF>(x);
-            }
-            *reinterpret_cast<f16x8*>(dst_v + kPlane * i) = x;
-          }
-        }
-      } else if (!mine_ok) {
-#pragma unroll
-        for (int i = 0; i < kPlanes; ++i)
-          *reinterpret_cast<f16x8*>(dst_v + kPlane * i) = f16x8{};
-      } else if (check) {
-#pragma unroll
-        for (int i = 0; i < kPlanes; ++i) {
-          const f16x8 x = *reinterpret_cast<const f16x8*>(dst_v + kPlane * i);
-          if (not_finite<BF>(x)) {
-            bad = true;
-            *reinterpret_cast<f16x8*>(dst_v + kPlane * i) = finite_only<BF>(x);
-          }
-        }
-      }
-      const uint32_t usable = keys_of(__ballot(mine_ok)), not_fin = keys_of(__ballot(bad));
-      if (lane == 0) {
-        s_ok[buf][w] = (uint16_t)usable;
-        s_bad[buf][w] = (uint16_t)not_fin;
-      }
-    };
-
-    lookup(ta);
-    copies(ta);
-    if (ta + 1 < tb) lookup(ta + 1);
-    arrive(ta);
-    __syncthreads();
-    for (int t = ta; t < tb; ++t) {
-      if (t + 1 < tb) copies(t + 1);
-      if (t + 2 < tb) lookup(t + 2);
-      const int buf = (t - ta) & 1;
-      if (wave_live) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int k0 = t * kKeys + 32 * j;
-          f32x16 x;
-          f16x8 weights[2];
-          r.scores(x, s_k[buf] + 1024 * j);
-          if constexpr (Q8) {
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const float4 ks = *reinterpret_cast<const float4*>(&s_scale[buf][32 * j + 8 * g + 4 * r.hh]);
-              x[4 * g] *= ks.x;
-              x[4 * g + 1] *= ks.y;
-              x[4 * g + 2] *= ks.z;
-              x[4 * g + 3] *= ks.w;
-            }
-          }
-          if (special) r.shape(x, p.shape);
-          const uint32_t usable = uniform((int)(s_ok[buf][2 * j] | s_ok[buf][2 * j + 1] << 16));
-          uint32_t see = usable;
-          if (usable != 0xFFFFFFFFu || edge(t)) {
-            const int d = s.held - k0;  // the tree's first row in the block
-            uint32_t nodes = 0;
-            if (d >= 0 && d < 32) nodes = (uint32_t)(mask << d);
-            if (d < 0 && d > -64) nodes = (uint32_t)(mask >> -d);
-            see &= (below(d) & ~below(lo - k0)) | nodes;
-            r.mask(x, see);
-          }
-          r.weigh(x, weights);
-          r.accumulate(weights, s_v[buf] + 1024 * j);
-          if (edge(t)) {
-            const uint32_t bad = uniform((int)(s_bad[buf][2 * j] | s_bad[buf][2 * j + 1] << 16));
-            if (bad)
-              r.add_not_finite(weights, bad, see, p.dim, [&](int k, int d) {
-                const uint32_t pi = (uint32_t)(k0 + k) / (uint32_t)p.page_size;
-                const uint32_t sl = (uint32_t)(k0 + k) - pi * (uint32_t)p.page_size;
-                const int64_t from = table[pi];  // (the key is usable)
-                const int64_t src = from * p.page_elems + (int64_t)sl * p.row_elems +
-                                    (int64_t)kvh * p.head_elems + d;
-                if constexpr (Q8) {
-                  const float vs = (float)p.vscale[from * p.scale_page + (int64_t)sl * p.scale_row +
-                                                   (int64_t)kvh * p.scale_head];
-                  const int8_t* y = static_cast<const int8_t*>(p.v) + src;
-                  return make_float4(y[0] * vs, y[1] * vs, y[2] * vs, y[3] * vs);
-                } else {
-                  return widen4<BF>(static_cast<const f16*>(p.v) + src);
-                }
-              });
-          }
-        }
-      }
-      if (t + 1 < tb) arrive(t + 1);
-      __syncthreads();
-    }
-
-    if (tb - ta == s.nt) {
+    if (end - begin == s.nt) {
       const float inv = r.inverse();
-      if (live) r.store(p.out + q_row * p.dim, p.dim, inv);
+      if (row < all_rows) r.store(p.out + q_row * p.dim, p.dim, inv);
     } else if (wave_live) {
       // A piece of a unit that is cut, as it is.
-      const int64_t piece = 2 * (int64_t)blockIdx.x + (first_piece ? 0 : 1);
+      const int64_t piece = (2 * (int64_t)blockIdx.x + (first_piece ? 0 : 1)) * W + w;
       const float sum = r.l + __shfl_xor(r.l, 32);
-      if (lane < 32) p.part_ml[piece * kRows + 32 * w + lane] = make_float2(r.m, sum);
-      float4* dst = reinterpret_cast<float4*>(p.part_o) + (piece * 4 + w) * (D / 8 * 64) + lane;
+      if (lane < 32) p.part_ml[piece * 32 + lane] = make_float2(r.m, sum);
+      float4* dst = reinterpret_cast<float4*>(p.part_o) + piece * (D / 8 * 64) + lane;
 #pragma unroll
       for (int i = 0; i < D / 8; ++i)
         dst[64 * i] = make_float4(r.o[i / 4][4 * (i % 4)], r.o[i / 4][4 * (i % 4) + 1],
                                   r.o[i / 4][4 * (i % 4) + 2], r.o[i / 4][4 * (i % 4) + 3]);
     }
-    left -= tb - ta;
-    rest += tb - ta;
+    if (first_piece && begin > 0 && end == s.nt) {
+      // The unit's first tile, and the workgroup that has it.
+      const int64_t from = range.begin - begin;
+      const int64_t g = ((from + 1) * range.n - 1) / range.all;
+      cut.rows = min(all_rows - first_row, 32 * W);
+      cut.first = first_row;
+      cut.token = s.first;
+      cut.kvh = kvh;
+      cut.piece = (int)(2 * g + (from > range_begin(range.all, range.n, g) ? 1 : 0));
+      cut.group = (int)g + 1;
+    }
+    left -= end - begin;
+    rest += end - begin;
     if (rest >= tiles_of(p, s)) {  // the next sequence that has a tree
       rest = 0;
       ++seq;
@@ -459,65 +546,78 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void tree_attention_ker
     }
     first_piece = false;
   }
+  if (tid == 0) p.cuts[blockIdx.x] = cut;
 }
 
-// Joins the pieces of a cut unit: with M the largest of their maxima, the outputs
-// are sum 2^(m - M) o / sum 2^(m - M) l. A wave takes 32 rows and a few of their
-// dims, the lanes as in the kernel that left them.
+// Joins the pieces of the unit that is cut and ends in a workgroup's range: with M the
+// largest of their maxima, the outputs are sum 2^(m - M) o / sum 2^(m - M) l. A wave
+// takes 32 rows and a quarter of their dims, the lanes as in the kernel that left them.
 template <int D, bool BF>
 __global__ __launch_bounds__(kThreads) void tree_join_kernel(const TreeParams p) {
-  constexpr int kShare = D / 8 / 4;  // groups of 8 dims a wave takes: a quarter
-  const int unit = blockIdx.x >> 2;
-  const int lane = threadIdx.x & 63, w = blockIdx.x & 3, part = threadIdx.x >> 6;
-  if (unit >= p.seq_units[p.batch]) return;
-  int lo = 0, hi = p.batch - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (p.seq_units[mid] <= unit)
-      lo = mid;
-    else
-      hi = mid - 1;
-  }
-  const Seq s = seq_of(p, lo);
-  const int64_t all = p.seq_tiles[p.batch];
-  const int64_t n = ranges(p, all);
-  const int64_t begin = p.seq_tiles[lo] + (int64_t)(unit - p.seq_units[lo]) * s.nt;
-  const int64_t end = begin + s.nt;
-  const int64_t g0 = ((begin + 1) * n - 1) / all, g1 = (end * n - 1) / all;
-  if (g0 == g1) return;  // written where it was computed
-  const int G = p.hq / p.hkv;
-  const int kvh = (unit - p.seq_units[lo]) / s.blocks, block = (unit - p.seq_units[lo]) % s.blocks;
-  const int row = kRows * block + 32 * w + (lane & 31);
-  if (kRows * block + 32 * w >= s.n * G) return;
-  auto piece = [&](int64_t g) {
-    return 2 * g + (g == g0 && begin > range_begin(all, n, g) ? 1 : 0);
+  constexpr int kShare = D / 8 / 4;  // groups of 8 dims a wave takes
+  constexpr int kAtOnce = 4;         // pieces loaded together
+  const int g = blockIdx.x, w = blockIdx.y, waves = gridDim.y;
+  const int lane = threadIdx.x & 63, part = threadIdx.x >> 6;
+  const Cut cut = p.cuts[g];
+  if (cut.rows <= 32 * w) return;
+  // Its pieces: the first, then those of the workgroups up to this one.
+  const int count = g - cut.group + 2;
+  auto piece = [&](int i) {
+    return (int64_t)(i == 0 ? cut.piece : 2 * (cut.group + i - 1)) * waves + w;
   };
   float top = -INFINITY;
-  for (int64_t g = g0; g <= g1; ++g)
-    top = fmaxf(top, p.part_ml[piece(g) * kRows + 32 * w + (lane & 31)].x);
   float4 acc[kShare];
 #pragma unroll
   for (int i = 0; i < kShare; ++i) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float sum = 0.0f;
-  for (int64_t g = g0; g <= g1; ++g) {
-    const float2 ml = p.part_ml[piece(g) * kRows + 32 * w + (lane & 31)];
-    // (A piece of which the row sees nothing holds zeros. One of NaN is not empty.)
-    const float f = ml.x == -INFINITY && ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml.x - top);
-    const float4* src = reinterpret_cast<const float4*>(p.part_o) +
-                        (piece(g) * 4 + w) * (D / 8 * 64) + part * kShare * 64 + lane;
+  for (int i0 = 0; i0 < count; i0 += kAtOnce) {
+    float2 ml[kAtOnce];
+    float4 o[kAtOnce][kShare];
 #pragma unroll
-    for (int i = 0; i < kShare; ++i) {
-      const float4 x = src[64 * i];
-      acc[i].x = fmaf(x.x, f, acc[i].x);
-      acc[i].y = fmaf(x.y, f, acc[i].y);
-      acc[i].z = fmaf(x.z, f, acc[i].z);
-      acc[i].w = fmaf(x.w, f, acc[i].w);
+    for (int j = 0; j < kAtOnce; ++j) {
+      const int64_t at = piece(min(i0 + j, count - 1));
+      ml[j] = p.part_ml[at * 32 + (lane & 31)];
+      const float4* src = reinterpret_cast<const float4*>(p.part_o) + at * (D / 8 * 64) +
+                          part * kShare * 64 + lane;
+#pragma unroll
+      for (int i = 0; i < kShare; ++i) o[j][i] = src[64 * i];
     }
-    sum = fmaf(ml.y, f, sum);
+    float now = top;
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) now = fmaxf(now, ml[j].x);
+    const float f0 = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - now);
+    top = now;
+    // (Before any key was seen sums and outputs are zeros, or NaN where a piece was.)
+    if (f0 != 0.0f || sum == 0.0f) {
+      sum *= f0;
+#pragma unroll
+      for (int i = 0; i < kShare; ++i) {
+        acc[i].x *= f0;
+        acc[i].y *= f0;
+        acc[i].z *= f0;
+        acc[i].w *= f0;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      // (A piece of which the row sees nothing holds zeros. One of NaN is not empty.)
+      const bool empty = i0 + j >= count || (ml[j].x == -INFINITY && ml[j].y == 0.0f);
+      const float f = empty ? 0.0f : __builtin_amdgcn_exp2f(ml[j].x - top);
+#pragma unroll
+      for (int i = 0; i < kShare; ++i) {
+        acc[i].x = fmaf(empty ? 0.0f : o[j][i].x, f, acc[i].x);
+        acc[i].y = fmaf(empty ? 0.0f : o[j][i].y, f, acc[i].y);
+        acc[i].z = fmaf(empty ? 0.0f : o[j][i].z, f, acc[i].z);
+        acc[i].w = fmaf(empty ? 0.0f : o[j][i].w, f, acc[i].w);
+      }
+      sum = empty ? sum : fmaf(ml[j].y, f, sum);
+    }
   }
-  if (row >= s.n * G) return;
+  const int r = 32 * w + (lane & 31);
+  if (r >= cut.rows) return;
+  const int G = p.hq / p.hkv, row = cut.first + r;
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  f16* dst = p.out + ((int64_t)(s.first + row / G) * p.hq + kvh * G + row % G) * p.dim;
+  f16* dst = p.out + ((int64_t)(cut.token + row / G) * p.hq + cut.kvh * G + row % G) * p.dim;
 #pragma unroll
   for (int i = 0; i < kShare; ++i) {
     const int d = 8 * (part * kShare + i) + 4 * (lane >> 5);
@@ -528,11 +628,15 @@ __global__ __launch_bounds__(kThreads) void tree_join_kernel(const TreeParams p)
 }
 
 template <bool BF, bool Q8>
-const void* tree_kernel_for(int width) {
-  return width == 64    ? reinterpret_cast<const void*>(tree_attention_kernel<64, BF, Q8>)
-         : width == 96  ? reinterpret_cast<const void*>(tree_attention_kernel<96, BF, Q8>)
-         : width == 128 ? reinterpret_cast<const void*>(tree_attention_kernel<128, BF, Q8>)
-                        : reinterpret_cast<const void*>(tree_attention_kernel<256, BF, Q8>);
+const void* tree_kernel_for(int width, int waves) {
+  if (waves == 8)
+    return width == 64   ? reinterpret_cast<const void*>(tree_attention_kernel<64, BF, Q8, 8>)
+           : width == 96 ? reinterpret_cast<const void*>(tree_attention_kernel<96, BF, Q8, 8>)
+                         : reinterpret_cast<const void*>(tree_attention_kernel<128, BF, Q8, 8>);
+  return width == 64    ? reinterpret_cast<const void*>(tree_attention_kernel<64, BF, Q8, 4>)
+         : width == 96  ? reinterpret_cast<const void*>(tree_attention_kernel<96, BF, Q8, 4>)
+         : width == 128 ? reinterpret_cast<const void*>(tree_attention_kernel<128, BF, Q8, 4>)
+                        : reinterpret_cast<const void*>(tree_attention_kernel<256, BF, Q8, 4>);
 }
 template <bool BF>
 const void* tree_join_for(int width) {
@@ -542,12 +646,11 @@ const void* tree_join_for(int width) {
                         : reinterpret_cast<const void*>(tree_join_kernel<256, BF>);
 }
 
-constexpr size_t aligned(size_t n) { return (n + 255) & ~(size_t)255; }
-
-size_t tree_workspace(int64_t batch, int width) {
-  const size_t pieces = 2 * (size_t)groups_for(width);
-  return aligned((batch + 1) * 8) + aligned((batch + 1) * 4) + pieces * kRows * 8 +
-         pieces * kRows * width * 4;
+// Pieces' outputs, (max, sum) pairs and the cuts: 2 pieces a workgroup, of 32 rows a
+// wave. As many rows with four waves a workgroup as with eight.
+size_t tree_workspace(int width) {
+  const size_t rows = 2 * (size_t)groups_for(width, 4) * 4 * 32;
+  return rows * width * 4 + rows * 8 + groups_for(width, 4) * sizeof(Cut);
 }
 
 int tree_attention(const void* queries, const void* keys, const void* values,
@@ -578,10 +681,9 @@ int tree_attention(const void* queries, const void* keys, const void* values,
   if (arena_rows < page_size)
     return fail(PDA_ERR_INVALID_ARGUMENT, "arena_rows %lld holds no whole page",
                 (long long)arena_rows);
-  // Rows of a sequence's tree, and all units, are counted in 32 bits.
+  // Rows of a sequence's trees are counted in 32 bits.
   const int G = q_heads / kv_heads;
-  const int64_t units = ((int64_t)tokens * G + (int64_t)(kRows - 1) * batch) / kRows * kv_heads;
-  if ((int64_t)tokens * G > INT32_MAX || units >= (int64_t)1 << 22)
+  if ((int64_t)tokens * q_heads > INT32_MAX)
     return fail(PDA_ERR_TOO_LONG, "%d nodes of %d query heads exceed one launch", tokens, q_heads);
   if (tokens == 0) return ok();
   if (!queries || !out || (batch > 0 && (!keys || !values || !tables || !lengths || !starts ||
@@ -595,7 +697,7 @@ int tree_attention(const void* queries, const void* keys, const void* values,
     return fail(PDA_ERR_ALIGNMENT, "fp16 scale arenas must be 2-byte aligned");
   if ((((uintptr_t)tables | (uintptr_t)lengths | (uintptr_t)starts) & 3) || ((uintptr_t)masks & 7))
     return fail(PDA_ERR_ALIGNMENT, "int32 buffers must be 4-byte aligned, masks 8-byte aligned");
-  const size_t need = tree_workspace(batch, width);
+  const size_t need = tree_workspace(width);
   if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255))
     return fail(PDA_ERR_WORKSPACE, "a 256-byte aligned workspace of %zu bytes is needed (got %zu)",
                 need, workspace ? workspace_bytes : (size_t)0);
@@ -611,15 +713,18 @@ int tree_attention(const void* queries, const void* keys, const void* values,
   prm.starts = starts;
   prm.masks = masks;
   prm.out = static_cast<f16*>(out);
-  const size_t pieces = 2 * (size_t)groups_for(width);
+  // Eight waves, two to a SIMD, where the sequences' trees have more rows than four
+  // waves hold: their keys and values are then read once where they were read twice.
+  const int waves = width <= 128 && (int64_t)tokens * G > 4 * 32 * (int64_t)batch ? 8 : 4;
+  prm.groups = groups_for(width, waves);
+  prm.rows = 32 * waves;
+  const size_t pieces = 2 * (size_t)prm.groups * prm.rows;
   char* ws = static_cast<char*>(workspace);
   prm.part_o = reinterpret_cast<float*>(ws);
-  ws += pieces * kRows * width * 4;
+  ws += pieces * width * 4;
   prm.part_ml = reinterpret_cast<float2*>(ws);
-  ws += pieces * kRows * 8;
-  prm.seq_tiles = reinterpret_cast<int64_t*>(ws);
-  ws += aligned(((size_t)batch + 1) * 8);
-  prm.seq_units = reinterpret_cast<int32_t*>(ws);
+  ws += pieces * 8;
+  prm.cuts = reinterpret_cast<Cut*>(ws);
   prm.arena_pages = arena_rows / page_size;
   prm.page_elems = (int64_t)page_size * kv_heads * head_dim;
   prm.scale_page = (int64_t)page_size * kv_heads;
@@ -632,7 +737,6 @@ int tree_attention(const void* queries, const void* keys, const void* values,
   prm.page_size = page_size;
   prm.tokens = tokens;
   prm.batch = batch;
-  prm.groups = groups_for(width);
   prm.hq = q_heads;
   prm.hkv = kv_heads;
   prm.dim = head_dim;
@@ -640,16 +744,16 @@ int tree_attention(const void* queries, const void* keys, const void* values,
   prm.shape = shape_of(scale, softcap);
   void* args[] = {&prm};
   const hipStream_t hs = static_cast<hipStream_t>(stream);
-  const void* fn = q8 ? (bf16_elems ? tree_kernel_for<true, true>(width)
-                                    : tree_kernel_for<false, true>(width))
-                      : (bf16_elems ? tree_kernel_for<true, false>(width)
-                                    : tree_kernel_for<false, false>(width));
-  hipError_t err = hipLaunchKernel(fn, dim3(prm.groups), dim3(kThreads), args, 0, hs);
+  const void* fn = q8 ? (bf16_elems ? tree_kernel_for<true, true>(width, waves)
+                                    : tree_kernel_for<false, true>(width, waves))
+                      : (bf16_elems ? tree_kernel_for<true, false>(width, waves)
+                                    : tree_kernel_for<false, false>(width, waves));
+  hipError_t err = hipLaunchKernel(fn, dim3(prm.groups), dim3(64 * waves), args, 0, hs);
   if (err != hipSuccess)
     return fail(PDA_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(err));
   if (batch == 0) return ok();
   err = hipLaunchKernel(bf16_elems ? tree_join_for<true>(width) : tree_join_for<false>(width),
-                        dim3((unsigned)(4 * units)), dim3(kThreads), args, 0, hs);
+                        dim3(prm.groups, waves), dim3(kThreads), args, 0, hs);
   if (err != hipSuccess)
     return fail(PDA_ERR_HIP, "join launch failed: %s", hipGetErrorString(err));
   return ok();
@@ -792,13 +896,13 @@ __global__ __launch_bounds__(kThreads) void commit_drafts_kernel(const CommitPar
 
 extern "C" {
 
-int pda_tree_workspace_bytes(int32_t batch, int32_t head_dim, size_t* bytes) {
-  if (batch < 0 || !bytes) return fail(PDA_ERR_INVALID_ARGUMENT, "batch=%d", batch);
+int pda_tree_workspace_bytes(int32_t head_dim, size_t* bytes) {
+  if (!bytes) return fail(PDA_ERR_INVALID_ARGUMENT, "null pointer");
   const int width = width_for(head_dim);
   if (width == 0)
     return fail(PDA_ERR_HEAD_DIM, "head_dim %d: trees are served at multiples of 8 up to 256",
                 head_dim);
-  *bytes = tree_workspace(batch, width);
+  *bytes = tree_workspace(width);
   return ok();
 }
 

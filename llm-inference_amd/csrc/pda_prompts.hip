@@ -53,10 +53,46 @@ __device__ __forceinline__ void bounds(const PromptParams& p, int b, int& a, int
   z = b < p.batch ? max(a, min(p.starts[b + 1], p.tokens)) : p.tokens;
 }
 
-// The sequence and the tile of the packed tiles' x-th; sequence -1: there is none.
-__device__ __forceinline__ void locate(const PromptParams& p, int x, int& seq, int& tile) {
+__device__ __forceinline__ int sum64(int x) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d);
+  return x;
+}
+
+struct Place {
+  int seq, tile, a, z;  // the sequence (-1: none), the tile of its tokens [a, z)
+};
+
+// The x-th query tile of all sequences, those that see the most keys first: tile i of
+// any sequence before tile i - 1 of any. Every wave finds it by itself, a lane for a
+// sequence: count(i) = sum of max(0, tiles - i) is how many lie at i or above.
+__device__ __forceinline__ Place locate_few(const PromptParams& p, int x) {
+  const int lane = threadIdx.x & 63;
+  int a = 0, z = 0;
+  if (lane <= p.batch) bounds(p, lane, a, z);
+  const int mine = lane <= p.batch ? (z - a + kTile - 1) / kTile : 0;
+  int lo = 0, hi = p.tiles, above = 0;  // count(lo) > x >= count(hi) = above
+  const int all = sum64(mine);
+  if (x >= all) return {-1, 0, 0, 0};
+  while (hi - lo > 1) {
+    const int mid = lo + (hi - lo) / 2;
+    const int n = sum64(max(0, mine - mid));
+    if (n > x)
+      lo = mid;
+    else
+      hi = mid, above = n;
+  }
+  const uint64_t here = __ballot(mine > lo);
+  const int rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(here >> 32),
+                                             __builtin_amdgcn_mbcnt_lo((uint32_t)here, 0));
+  const int seq = __builtin_ctzll(__ballot(mine > lo && rank == x - above));
+  return {seq, lo, __shfl(a, seq), __shfl(z, seq)};
+}
+
+// For more sequences than lanes: sequence after sequence, each from its last tile.
+__device__ __forceinline__ Place locate_many(const PromptParams& p, int x) {
   __shared__ int s_sum[kThreads / 64];
-  __shared__ int s_found[2];
+  __shared__ Place s_found;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int per = (p.batch + kThreads) / kThreads;  // of batch + 1
   const int b0 = tid * per, b1 = min(b0 + per, p.batch + 1);
@@ -73,7 +109,7 @@ __device__ __forceinline__ void locate(const PromptParams& p, int x, int& seq, i
     if (lane >= d) upto += y;
   }
   if (lane == 63) s_sum[w] = upto;
-  if (tid == 0) s_found[0] = -1;
+  if (tid == 0) s_found.seq = -1;
   __syncthreads();
   int before = upto - mine;
   for (int i = 0; i < w; ++i) before += s_sum[i];
@@ -84,28 +120,147 @@ __device__ __forceinline__ void locate(const PromptParams& p, int x, int& seq, i
       bounds(p, b, a, z);
       const int n = (z - a + kTile - 1) / kTile;
       if (left < n) {
-        s_found[0] = b;
-        s_found[1] = left;
+        s_found = {b, n - 1 - left, a, z};
         break;
       }
       left -= n;
     }
   }
   __syncthreads();
-  seq = uniform(s_found[0]);
-  tile = uniform(s_found[1]);
+  return s_found;
 }
+
+// A query tile's keys and values on their way through LDS, and their masks.
+template <int D, bool BF>
+struct PromptTiles {
+  static constexpr int kPlanes = D / 32;
+  static constexpr int kHalves = kPlanes * kPlane;  // of a tile
+  static constexpr int kCopies = 2 * kPlanes;
+
+  const PromptParams& p;
+  f16* s_k;          // [2][kHalves]
+  f16* s_v;
+  int* s_left;       // whether values that are not finite were taken as zeros
+  const f16* kb;     // the prompt's first key and value of the kv head
+  const f16* vb;
+  int q0, last;      // first query and last key of the workgroup
+  int wq0, wlast;    // first and last query of the wave
+  int at;            // this lane's query
+  bool special;      // a softcap, or a scale that is no positive factor
+  int lane, w, gk, kchunk, vchunk;
+  uint32_t k_dst, v_dst;
+
+  __device__ __forceinline__ void init() {
+    const int tid = threadIdx.x;
+    lane = tid & 63;
+    w = uniform(tid >> 6);
+    // Copies: thread tid moves key tid / 4 of a tile, one 16-byte chunk a plane.
+    gk = tid >> 2;
+    kchunk = 8 * ((lane & 3) ^ ((lane >> 4) & 3));
+    vchunk = 8 * (lane & 3);
+    k_dst = uniform(lds_address(s_k) + 1024 * w);
+    v_dst = uniform(lds_address(s_v) + 1024 * w);
+    special = p.shape.cap_out > 0.0f || !(p.shape.scale_log2 > 0.0f);
+    if (tid == 0) *s_left = 0;
+    if (p.dim != D) {  // what no copy writes
+      for (int i = 8 * tid; i < 2 * kHalves; i += 8 * kThreads) {
+        *reinterpret_cast<f16x8*>(s_k + i) = f16x8{};
+        *reinterpret_cast<f16x8*>(s_v + i) = f16x8{};
+      }
+      __syncthreads();
+    }
+  }
+  __device__ __forceinline__ const f16* keys(int t) const { return s_k + (t & 1) * kHalves; }
+  __device__ __forceinline__ const f16* values(int t) const { return s_v + (t & 1) * kHalves; }
+
+  __device__ __forceinline__ void copy_k(int t, int i) const {
+    if (D == p.dim || 32 * i + kchunk < p.dim)
+      copy_to_lds(kb + (int64_t)min(t * kKeys + gk, last) * p.k_token + kchunk + 32 * i,
+                  k_dst + (t & 1) * (2 * kHalves) + 2 * kPlane * i);
+  }
+  template <int j>
+  __device__ __forceinline__ void copy(int t) const {
+    if constexpr (j >= kPlanes)
+      copy_k(t + 1, j - kPlanes);
+    else if (D == p.dim || 32 * j + vchunk < p.dim)
+      copy_to_lds(vb + (int64_t)min(t * kKeys + gk, last) * p.v_token + vchunk + 32 * j,
+                  v_dst + (t & 1) * (2 * kHalves) + 2 * kPlane * j);
+  }
+  __device__ __forceinline__ void first(int t) {
+#pragma unroll
+    for (int i = 0; i < kPlanes; ++i) copy_k(t, i);
+    auto one = [&](auto j) { copy<j.value>(t); };
+    each(one, std::make_integer_sequence<int, kCopies>{});
+    if (D == p.dim)
+      wait_vmem<kCopies>();  // the first K alone
+    else
+      wait_vmem<0>();  // (planes that no lane copies are not counted)
+    __syncthreads();
+  }
+
+  // Tiles that a row of the workgroup does not see whole.
+  __device__ __forceinline__ bool edge(int t) const {
+    return t * kKeys + kKeys - 1 > q0 || (p.window > 0 && t * kKeys <= last - p.window);
+  }
+  // There, values that are not finite become zeros (a weight of 0 would make them NaN
+  // in rows that do not see them).
+  __device__ __forceinline__ void close(int t) {
+    wait_vmem<0>();
+    if (edge(t)) {
+      f16* mine = s_v + (t & 1) * kHalves + 32 * gk + 8 * (lane & 3);
+#pragma unroll
+      for (int i = 0; i < kPlanes; ++i) {
+        const f16x8 x = *reinterpret_cast<const f16x8*>(mine + kPlane * i);
+        if (not_finite<BF>(x)) {
+          *s_left = 1;
+          *reinterpret_cast<f16x8*>(mine + kPlane * i) = finite_only<BF>(x);
+        }
+      }
+    }
+    __syncthreads();
+  }
+
+  // What the lane's row sees of the 32 keys from k0 on; whether a row of the wave does
+  // not see them all.
+  __device__ __forceinline__ uint32_t visible(int k0) const {
+    uint32_t see = below(at - k0 + 1);
+    if (p.window > 0) see &= ~below(at - k0 - p.window + 1);
+    return see;
+  }
+  __device__ __forceinline__ bool partly(int k0) const {
+    return k0 + 31 > wq0 || (p.window > 0 && k0 <= wlast - p.window);
+  }
+  __device__ __forceinline__ bool rough(int t) const {
+    return special || partly(t * kKeys) || partly(t * kKeys - 32);
+  }
+  __device__ __forceinline__ void shape(f32x16& x, int k0) const {
+    if (special) Rows<D, BF>::shape(x, p.shape);
+    if (partly(k0)) Rows<D, BF>::mask(x, visible(k0));
+  }
+  // After the last tile: the values that were taken as zeros, to the rows that see
+  // them.
+  __device__ __forceinline__ void add_left_out(Rows<D, BF>& r, int t0, int t1) const {
+    __syncthreads();
+    if (uniform(*s_left) == 0) return;
+    for (int t = t0; t < t1; ++t) {
+      if (!edge(t)) continue;
+      for (int k = t * kKeys; k <= min(t * kKeys + kKeys - 1, last); ++k)
+        r.add_not_finite(k <= at && (p.window == 0 || k > at - p.window), p.dim, [&](int d) {
+          return widen4<BF>(vb + (int64_t)k * p.v_token + d);
+        });
+    }
+  }
+};
 
 template <int D, bool BF>
 __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void packed_prompt_kernel(
     const PromptParams p) {
-  constexpr int kPlanes = D / 32;
-  constexpr int kTileHalves = kPlanes * kPlane;
-  __shared__ __align__(1024) f16 s_k[2][kTileHalves];
-  __shared__ __align__(1024) f16 s_v[2][kTileHalves];
-  __shared__ uint16_t s_bad[2][4];  // keys whose values are not finite, by wave
+  using Tiles = PromptTiles<D, BF>;
+  __shared__ __align__(1024) f16 s_k[2 * Tiles::kHalves];
+  __shared__ __align__(1024) f16 s_v[2 * Tiles::kHalves];
+  __shared__ int s_left;
 
-  const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
+  const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6);
   const int G = p.hq / p.hkv;
   // The G query heads of a kv head follow each other on one XCD (workgroups go
   // round robin over the XCDs): its L2 serves their keys and values.
@@ -117,15 +272,11 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void packed_prompt_kern
   }
   const int run = item / G;
   const int kvh = run % p.hkv, h = kvh * G + item % G;
-  int seq, tile;
-  locate(p, run / p.hkv, seq, tile);
+  const Place place = p.batch < 64 ? locate_few(p, run / p.hkv) : locate_many(p, run / p.hkv);
+  const int seq = uniform(place.seq);
   if (seq < 0) return;
-  int a, z;
-  bounds(p, seq, a, z);
-  a = uniform(a);
-  z = uniform(z);
-  const int q0 = tile * kTile, len = z - a;
-  const int wq0 = q0 + 32 * w, row = wq0 + (lane & 31);
+  const int a = uniform(place.a), len = uniform(place.z) - a;
+  const int q0 = uniform(place.tile) * kTile, wq0 = q0 + 32 * w, row = wq0 + (lane & 31);
   f16* out = p.out + ((int64_t)(a + row) * p.hq + h) * p.dim;
   Rows<D, BF> r;
   r.init(p.shape);
@@ -138,104 +289,16 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void packed_prompt_kern
   r.load(p.q + (int64_t)(a + at) * p.q_token + (int64_t)h * p.q_head, p.dim, true);
 
   const int last = min(q0 + kTile, len) - 1;
-  const int first = p.window > 0 ? max(0, q0 - p.window + 1) : 0;
-  const int t0 = first / kKeys, t1 = last / kKeys + 1;
-  // Tiles that this wave's rows see.
-  const bool wave_live = wq0 < len;
+  const int t0 = p.window > 0 ? max(0, q0 - p.window + 1) / kKeys : 0, t1 = last / kKeys + 1;
   const int wlast = min(wq0 + 31, len - 1);
-  const int wa = p.window > 0 ? max(t0, max(0, wq0 - p.window + 1) / kKeys) : t0;
-  const int wb = wave_live ? wlast / kKeys + 1 : 0;
-
-  // Copies: thread tid moves key tid / 4 of a tile, one 16-byte chunk a plane.
-  const int gk = tid >> 2;
-  const int kchunk = 8 * ((lane & 3) ^ ((lane >> 4) & 3)), vchunk = 8 * (lane & 3);
-  const f16* kb = p.k + (int64_t)a * p.k_token + (int64_t)kvh * p.k_head;
-  const f16* vb = p.v + (int64_t)a * p.v_token + (int64_t)kvh * p.v_head;
-  const uint32_t k_dst = uniform(lds_address(&s_k[0][0]) + 1024 * w);
-  const uint32_t v_dst = uniform(lds_address(&s_v[0][0]) + 1024 * w);
-  if (p.dim != D) {  // what no copy writes
-    f16* flat_k = &s_k[0][0];
-    f16* flat_v = &s_v[0][0];
-    for (int i = 8 * tid; i < 2 * kTileHalves; i += 8 * kThreads) {
-      *reinterpret_cast<f16x8*>(flat_k + i) = f16x8{};
-      *reinterpret_cast<f16x8*>(flat_v + i) = f16x8{};
-    }
-    __syncthreads();
-  }
-  auto copies = [&](int t) {
-    const int key = min(t * kKeys + gk, last);
-    const f16* src_k = kb + (int64_t)key * p.k_token + kchunk;
-    const f16* src_v = vb + (int64_t)key * p.v_token + vchunk;
-    const uint32_t off = ((t - t0) & 1) * (2 * kTileHalves);
-#pragma unroll
-    for (int i = 0; i < kPlanes; ++i) {
-      if (D == p.dim || 32 * i + kchunk < p.dim)
-        copy_to_lds(src_k + 32 * i, k_dst + off + 2 * kPlane * i);
-      if (D == p.dim || 32 * i + vchunk < p.dim)
-        copy_to_lds(src_v + 32 * i, v_dst + off + 2 * kPlane * i);
-    }
-  };
-  // Tiles that a row of the workgroup does not see whole.
-  auto edge = [&](int t) {
-    return t * kKeys + kKeys - 1 > q0 || (p.window > 0 && t * kKeys <= last - p.window);
-  };
-  // There, values that are not finite become zeros (a weight of 0 would make them
-  // NaN in rows that do not see them) and their keys are remembered.
-  auto clean = [&](int t) {
-    if (!edge(t)) return;
-    const int buf = (t - t0) & 1;
-    bool bad = false;
-    f16* mine = &s_v[buf][32 * gk + 8 * (lane & 3)];
-#pragma unroll
-    for (int i = 0; i < kPlanes; ++i) {
-      const f16x8 x = *reinterpret_cast<const f16x8*>(mine + kPlane * i);
-      if (not_finite<BF>(x)) {
-        bad = true;
-        *reinterpret_cast<f16x8*>(mine + kPlane * i) = finite_only<BF>(x);
-      }
-    }
-    const uint32_t keys = keys_of(__ballot(bad));
-    if (lane == 0) s_bad[buf][w] = (uint16_t)keys;
-  };
-
-  const bool special = p.shape.cap_out > 0.0f || !(p.shape.scale_log2 > 0.0f);
-  copies(t0);
-  wait_vmem<0>();
-  clean(t0);
-  __syncthreads();
-  for (int t = t0; t < t1; ++t) {
-    if (t + 1 < t1) copies(t + 1);
-    if (t >= wa && t < wb) {
-      const int buf = (t - t0) & 1;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int k0 = t * kKeys + 32 * j;
-        f32x16 x;
-        f16x8 weights[2];
-        r.scores(x, s_k[buf] + 1024 * j);
-        if (special) r.shape(x, p.shape);
-        const bool masks = k0 + 31 > wq0 || (p.window > 0 && k0 <= wlast - p.window);
-        uint32_t see = 0xFFFFFFFFu;
-        if (masks) {
-          see = below(at - k0 + 1);
-          if (p.window > 0) see &= ~below(at - k0 - p.window + 1);
-          r.mask(x, see);
-        }
-        r.weigh(x, weights);
-        r.accumulate(weights, s_v[buf] + 1024 * j);
-        if (edge(t)) {
-          const uint32_t bad = uniform((int)(s_bad[buf][2 * j] | s_bad[buf][2 * j + 1] << 16));
-          if (bad)
-            r.add_not_finite(weights, bad, see, p.dim, [&](int k, int d) {
-              return widen4<BF>(vb + (int64_t)min(k0 + k, last) * p.v_token + d);
-            });
-        }
-      }
-    }
-    wait_vmem<0>();
-    if (t + 1 < t1) clean(t + 1);
-    __syncthreads();
-  }
+  Tiles x{p, s_k, s_v, &s_left, p.k + (int64_t)a * p.k_token + (int64_t)kvh * p.k_head,
+          p.v + (int64_t)a * p.v_token + (int64_t)kvh * p.v_head, q0, last, wq0, wlast, at};
+  x.init();
+  // Tiles that this wave's rows see.
+  const int wa = p.window > 0 ? max(0, wq0 - p.window + 1) / kKeys : 0;
+  const int wb = wq0 < len ? wlast / kKeys + 1 : 0;
+  attend(r, x, t0, t1, wa, wb, wlast >= (wb - 1) * kKeys + 32);
+  x.add_left_out(r, t0, t1);
   const float inv = r.inverse();
   if (row < len) r.store(out, p.dim, inv);
 }

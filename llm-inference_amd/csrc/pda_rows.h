@@ -84,6 +84,12 @@ __device__ __forceinline__ void copy_to_lds(const void* src, uint32_t dst) {
                : "memory", "m0");
 }
 
+// f(0), f(1), ... with compile-time arguments.
+template <class F, int... kI>
+__device__ __forceinline__ void each(F& f, std::integer_sequence<int, kI...>) {
+  (f(std::integral_constant<int, kI>{}), ...);
+}
+
 // Until at most kLeft of the wave's loads and copies are under way.
 template <int kLeft>
 __device__ __forceinline__ void wait_vmem() {
@@ -201,6 +207,12 @@ struct Rows {
       const f16x8 x = *reinterpret_cast<const f16x8*>(row + (in ? d : 0));
       q[i] = in ? x : f16x8{};
     }
+    // Only matrix-core operands: where the outputs take half the vector registers,
+    // they go to accumulator registers.
+    if constexpr (D > 128) {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) asm volatile("" : "+a"(q[i]));
+    }
   }
 
   // Scores of the 32 keys from kt on.
@@ -214,7 +226,7 @@ struct Rows {
   }
 
   // Caps and scales that are not one positive factor.
-  __device__ __forceinline__ void shape(f32x16& x, const Shape& f) const {
+  __device__ __forceinline__ static void shape(f32x16& x, const Shape& f) {
     if (f.cap_out > 0.0f) {
 #pragma unroll
       for (int v = 0; v < 16; ++v) {
@@ -228,8 +240,8 @@ struct Rows {
   }
 
   // Hides the keys of a block whose bit in `see` is not set.
-  __device__ __forceinline__ void mask(f32x16& x, uint32_t see) const {
-    see >>= 4 * hh;
+  __device__ __forceinline__ static void mask(f32x16& x, uint32_t see) {
+    see >>= 4 * ((threadIdx.x & 63) >> 5);
 #pragma unroll
     for (int v = 0; v < 16; ++v) {
       const int bit = __builtin_amdgcn_sbfe((int)see, 8 * (v / 4) + (v % 4), 1);
@@ -318,34 +330,84 @@ struct Rows {
     }
   }
 
-  // Values that are not finite were taken as zeros (0 times one is no 0): adds
-  // them where the key is seen. `bad`: such keys of the block, `see` the keys that
-  // this lane's row sees, value4(k, d) values d .. d + 3 of key k as they are.
+  // The pipeline's step: the products of a 32-key block's V (weights pv, values vt)
+  // alternate with the scores of a later block (xn, keys kt), and the weights of the
+  // block between them (x, into w, summed in lb) are spread over those D / 8 matrix
+  // instructions, so that one wave alone keeps the matrix core busy while its
+  // exponentials run. Operands are read four ahead. beside(i) is called at slot i for
+  // what else is to be issued there.
   template <class F>
-  __device__ __forceinline__ void add_not_finite(const f16x8 (&w)[2], uint32_t bad, uint32_t see,
-                                                 int dim, F value4) {
-    while (bad) {
-      const int k = __builtin_ctz(bad);
-      bad &= bad - 1;
-      float mine = 0.0f;
+  __device__ __forceinline__ void step(const f32x16& x, f16x8 (&w)[2], const f16x8 (&pv)[2],
+                                       f32x16& xn, float& lb, const f16* kt, const f16* vt,
+                                       F beside) {
+    constexpr int kSlots = D / 8, kAhead = 4;
+    const float mu = m == -INFINITY ? 0.0f : m;
+    lb = m == -INFINITY ? INFINITY : 0.0f;
+    float e[16];
+    f16x8 a[kSlots];
+    auto read = [&](int i) {
+      if (i & 1) {
+        const int c = i >> 1;
+        a[i] = *reinterpret_cast<const f16x8*>(kt + (c & 1 ? k_lane1 : k_lane0) + kPlane * (c >> 1));
+      } else {
+        const int b = (i >> 1) % (D / 32), ks = (i >> 1) / (D / 32);
+        const f16* vp = vt + v_lane + kPlane * b + 512 * ks;
+        const f16x4 lo4 = read_tr(vp);
+        const f16x4 hi4 = read_tr(vp + 256);
+        a[i] = f16x8{lo4[0], lo4[1], lo4[2], lo4[3], hi4[0], hi4[1], hi4[2], hi4[3]};
+      }
+    };
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int v = 0; v < 16; ++v)
-        mine = v == 4 * (k / 8) + k % 4 ? widen16<BF>(w[v / 8][v % 8]) : mine;
-      const float other = __shfl_xor(mine, 32);
-      const float weight = (k >> 2 & 1) == hh ? mine : other;
-      const bool seen = see >> k & 1;
+    for (int i = 0; i < kAhead; ++i) read(i);
+    e[0] = fmaf(x[0], c, -mu);
+    __builtin_amdgcn_sched_barrier(0);
+    auto slot = [&](auto sc) {
+      constexpr int i = sc.value;
+      if constexpr (i & 1) {
+        constexpr int cc = i >> 1;
+        xn = mfma16<BF>(a[i], q[cc], cc == 0 ? f32x16{} : xn);
+      } else {
+        constexpr int b = (i >> 1) % (D / 32), ks = (i >> 1) / (D / 32);
+        o[b] = mfma16<BF>(a[i], pv[ks], o[b]);
+      }
+      if constexpr (i + kAhead < kSlots) read(i + kAhead);
+      beside(sc);
+      // The argument of the next exponential, this one, the pair before; done two
+      // slots early.
+      constexpr int v0 = 16 * i / (kSlots - 2), v1 = 16 * (i + 1) / (kSlots - 2);
 #pragma unroll
-      for (int b = 0; b < D / 32; ++b)
+      for (int v = v0 < 16 ? v0 : 16; v < (v1 < 16 ? v1 : 16); ++v) {
+        if (v + 1 < 16) e[v + 1] = fmaf(x[v + 1], c, -mu);
+        e[v] = __builtin_amdgcn_exp2f(e[v]);
+        if ((v & 1) && v >= 3) put_pair(w, (v - 3) / 2, e[v - 3], e[v - 2]);
+      }
+      if constexpr (i == kSlots - 2) put_pair(w, 7, e[14], e[15]);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    each(slot, std::make_integer_sequence<int, kSlots>{});
+    lb = total(w, lb);
+    // Keeps the products of the step in it (they would sink past the branch of
+    // settle, away from the weights they are to overlap).
+    asm volatile("" : "+v"(xn), "+v"(w[0]), "+v"(w[1]), "+v"(lb));
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int d = 32 * b + 8 * g + 4 * hh;
-          const float4 y = value4(k, min(d, dim - 4));
-          const float ys[4] = {y.x, y.y, y.z, y.w};
+    for (int b = 0; b < D / 32; ++b) asm volatile("" : "+v"(o[b]));
+  }
+
+  // A key's values that are not finite were taken as zeros (0 times one is no 0): adds
+  // them where the lane's row sees the key (any weight of them comes to the same).
+  // value4(d): values d .. d + 3 of the key as they are.
+  template <class F>
+  __device__ __forceinline__ void add_not_finite(bool seen, int dim, F value4) {
 #pragma unroll
-          for (int t = 0; t < 4; ++t)
-            o[b][4 * g + t] += seen && d < dim && !(fabsf(ys[t]) < INFINITY) ? weight * ys[t] : 0.0f;
-          __builtin_amdgcn_sched_barrier(0);  // (else all loads at once: registers of the common path)
-        }
+    for (int i = 0; i < D / 8; ++i) {
+      const int d = 8 * i + 4 * hh;
+      const float4 y = value4(min(d, dim - 4));
+      const float ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        o[i / 4][4 * (i % 4) + t] += seen && d < dim && !(fabsf(ys[t]) < INFINITY) ? ys[t] : 0.0f;
+      __builtin_amdgcn_sched_barrier(0);  // (else all loads at once)
     }
   }
 
@@ -370,6 +432,78 @@ struct Rows {
     }
   }
 };
+
+// The tiles [t0, t1) of a workgroup, of which this wave's rows see [wa, wb) (the last
+// one's odd block only with odd_last). `x` moves and shapes them:
+//   first(t0)     K of the first tile is readable, its V and the next K under way
+//   copy<j>(t)    for all j < T::kCopies: V of tile t and K of tile t + 1
+//   close(t)      they are readable by all waves; all are done with V of t - 1, K of t
+//   shape(s, k0)  caps and masks of the scores of the keys from k0 on, with rough(t)
+//                 telling whether the odd block before tile t or its even one need it
+// V runs one tile behind K, so that two LDS tiles of each serve the pipeline with one
+// barrier a tile.
+template <class R, class T>
+__device__ __forceinline__ void attend(R& r, T& x, int t0, int t1, int wa, int wb, bool odd_last) {
+  int t = t0;
+  x.first(t);
+  auto copies = [&]() {
+    auto one = [&](auto j) { x.template copy<j.value>(t); };
+    each(one, std::make_integer_sequence<int, T::kCopies>{});
+  };
+  auto idle = [&]() {  // a tile that this wave's rows do not see
+    if (t > t0) copies();
+    x.close(t);
+  };
+  const int from = wa < wb ? wa : t1;
+  for (; t < from; ++t) idle();
+  if (t < t1) {
+    f32x16 s0, s1 = {};
+    f16x8 w0[2], w1[2] = {};
+    float lb;
+    // First tile: scores of both blocks, weights of the even one.
+    if (t > t0) copies();
+    {
+      const f16* kt = x.keys(t);
+      r.scores(s0, kt);
+      x.shape(s0, t * kKeys);
+      if (wb - wa > 1 || odd_last) r.scores(s1, kt + 1024);
+      r.weigh(s0, w0);
+      x.close(t);
+    }
+    // Scores of tile t, weights of its even block and of tile t - 1's odd one,
+    // products of tile t - 1's V.
+    for (++t; t < wb; ++t) {
+      const int k0 = t * kKeys;
+      const f16* kt = x.keys(t);
+      const f16* vt = x.values(t - 1);
+      const bool rough = x.rough(t);
+      if (rough) x.shape(s1, k0 - 32);
+      r.step(s1, w1, w0, s0, lb, kt, vt, [&](auto i) {
+        // (Every other slot: a copy is two instructions and an address.)
+        if constexpr (i.value % 2 == 0 && i.value / 2 < T::kCopies) x.template copy<i.value / 2>(t);
+      });
+      r.settle(s1, w1, lb);
+      if (rough) x.shape(s0, k0);
+      r.step(s0, w0, w1, s1, lb, kt + 1024, vt + 1024, [](auto) {});
+      r.settle(s0, w0, lb);
+      x.close(t);
+    }
+    // Past the last tile: weights of its odd block, products of its V.
+    if (t < t1) copies();
+    const f16* vt = x.values(t - 1);
+    r.accumulate(w0, vt);
+    if (odd_last) {
+      x.shape(s1, (t - 1) * kKeys + 32);
+      r.weigh(s1, w1);
+      r.accumulate(w1, vt + 1024);
+    }
+    if (t < t1) x.close(t);
+    for (++t; t < t1; ++t) idle();
+  }
+  // (Where no tile was closed the copies under way have to land before the LDS is
+  // used anew.)
+  wait_vmem<0>();
+}
 
 }  // namespace pda_rows
 

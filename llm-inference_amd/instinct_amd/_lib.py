@@ -167,7 +167,7 @@ for _suffix in ("", "_bf16"):
     SIGNATURES["pda_tree_attention" + _suffix] = (ctypes.c_int, [c_void_p] * 3 + _TREE_TAIL)
     SIGNATURES["pda_tree_attention_q8" + _suffix] = (ctypes.c_int, [c_void_p] * 5 + _TREE_TAIL)
 SIGNATURES["pda_tree_workspace_bytes"] = (
-    ctypes.c_int, [c_int32] * 2 + [ctypes.POINTER(c_size_t)])
+    ctypes.c_int, [c_int32, ctypes.POINTER(c_size_t)])
 SIGNATURES["pda_commit_drafts"] = (
     ctypes.c_int, [ctypes.POINTER(c_void_p)] + [c_int32] * 3 + [c_void_p] * 6 + [c_int32]
     + [c_void_p] * 4 + [c_int32] * 5 + [c_int64, c_int32, c_void_p])
@@ -264,9 +264,9 @@ def attention_weights_workspace_bytes(batch, q_heads, capacity) -> int:
     return out.value
 
 
-def tree_workspace_bytes(batch, head_dim) -> int:
+def tree_workspace_bytes(head_dim) -> int:
     out = c_size_t(0)
-    check(library().pda_tree_workspace_bytes(batch, head_dim, ctypes.byref(out)))
+    check(library().pda_tree_workspace_bytes(head_dim, ctypes.byref(out)))
     return out.value
 
 

@@ -28,9 +28,10 @@ from .hip_kernels import _arena_geometry, _given_workspace, on_device, stream_wo
 NODES = 64  # of a tree: a mask has a bit for each
 
 
-def tree_workspace_bytes(batch: int, head_dim: int) -> int:
-    """Bytes of workspace :func:`tree_attention` needs (``pda_tree_workspace_bytes``)."""
-    return _lib.tree_workspace_bytes(int(batch), int(head_dim))
+def tree_workspace_bytes(head_dim: int) -> int:
+    """Bytes of workspace :func:`tree_attention` needs, whatever its batch and lengths
+    (``pda_tree_workspace_bytes``)."""
+    return _lib.tree_workspace_bytes(int(head_dim))
 
 
 def tree_attention(queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
@@ -89,7 +90,7 @@ def tree_attention(queries: torch.Tensor, keys: torch.Tensor, values: torch.Tens
     elif (out.dtype != queries.dtype or out.shape != queries.shape or out.device != device
           or not out.is_contiguous()):
         raise ValueError("out must be contiguous and match the queries' shape, dtype and device")
-    need = _lib.tree_workspace_bytes(batch, head_dim)
+    need = _lib.tree_workspace_bytes(head_dim)
     stream = int(torch.cuda.current_stream(device).cuda_stream)
     with on_device(device):
         ws = (stream_workspace(device, need, stream) if workspace is None

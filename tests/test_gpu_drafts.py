@@ -203,7 +203,7 @@ def test_repeated_captured_and_other_streams(gpu):
             dev(case.masks.view(np.int64), np.int64))
     kw = dict(page_size=16, scale=0.09)
     first = drafts.tree_attention(*args, **kw)
-    ws = torch.empty(drafts.tree_workspace_bytes(3, 128), dtype=torch.uint8, device="cuda")
+    ws = torch.empty(drafts.tree_workspace_bytes(128), dtype=torch.uint8, device="cuda")
     out = torch.empty_like(first)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):

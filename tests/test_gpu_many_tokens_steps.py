@@ -192,7 +192,7 @@ def test_captured_draft_steps(gpu):
                      k=torch.zeros((layers, batch * most, 2, 64), dtype=torch.float16, device="cuda"),
                      drafted=torch.zeros(batch * most, dtype=torch.int64, device="cuda"),
                      targets=torch.zeros(batch * most, dtype=torch.int64, device="cuda"),
-                     ws=torch.empty(drafts.tree_workspace_bytes(batch, 64), dtype=torch.uint8,
+                     ws=torch.empty(drafts.tree_workspace_bytes(64), dtype=torch.uint8,
                                     device="cuda"))
         return state
 

@@ -86,10 +86,9 @@ def test_tree_rejects(overrides, code):
 def test_tree_workspace():
     size = ctypes.c_size_t(0)
     call = _lib.library().pda_tree_workspace_bytes
-    assert call(4, 128, ctypes.byref(size)) == 0 and size.value % 256 == 0
-    rejected(call(-1, 128, ctypes.byref(size)), BAD)
-    rejected(call(4, 10, ctypes.byref(size)), _lib.PDA_ERR_HEAD_DIM)
-    rejected(call(4, 128, None), BAD)
+    assert call(128, ctypes.byref(size)) == 0 and size.value % 256 == 0
+    rejected(call(10, ctypes.byref(size)), _lib.PDA_ERR_HEAD_DIM)
+    rejected(call(128, None), BAD)
 
 
 def commit(**overrides):
