@@ -184,7 +184,8 @@ __device__ __forceinline__ f16x8 from_bytes(const u32x2& y, float scale) {
 
 // A unit's keys and values on their way from the pages through LDS, and their masks.
 // W waves: with eight the first four copy V and the others K.
-template <int D, bool BF, bool Q8, int W>
+// EXACT: the head dim is D.
+template <int D, bool BF, bool Q8, int W, bool EXACT>
 struct TreeTiles {
   static constexpr int kPlanes = D / 32;
   static constexpr int kHalves = kPlanes * kPlane;  // of a tile
@@ -230,7 +231,7 @@ struct TreeTiles {
     v_dst = uniform(lds_address(s_v) + 1024 * (w & 3));
     pages = (uint32_t)min(p.arena_pages, (int64_t)INT32_MAX);
     special = p.shape.cap_out > 0.0f || !(p.shape.scale_log2 > 0.0f);
-    if (p.dim != D) {  // what no copy writes
+    if constexpr (!EXACT) {  // what no copy writes
       for (int i = 8 * tid; i < 2 * kHalves; i += 8 * 64 * W) {
         *reinterpret_cast<f16x8*>(s_k + i) = f16x8{};
         *reinterpret_cast<f16x8*>(s_v + i) = f16x8{};
@@ -264,7 +265,7 @@ struct TreeTiles {
     if constexpr (Q8) {
       if (i == 0) raw_ks = p.kscale[scale_k];
     }
-    if (D != p.dim && 32 * i + kchunk >= p.dim) return;
+    if (!EXACT && 32 * i + kchunk >= p.dim) return;
     if constexpr (Q8) {
       raw_k[i] = *reinterpret_cast<const u32x2*>(static_cast<const int8_t*>(p.k) + at_k + kchunk + 32 * i);
     } else {
@@ -273,7 +274,7 @@ struct TreeTiles {
     }
   }
   __device__ __forceinline__ void copy_v(int t, int i) {
-    if (D != p.dim && 32 * i + vchunk >= p.dim) return;
+    if (!EXACT && 32 * i + vchunk >= p.dim) return;
     if constexpr (Q8) {
       raw_v[i] = *reinterpret_cast<const u32x2*>(static_cast<const int8_t*>(p.v) + at_v + vchunk + 32 * i);
       if (i == 0) raw_vs = p.vscale[scale_v];
@@ -305,7 +306,7 @@ struct TreeTiles {
       if ((lane & 3) == 0) s_scale[kKeys * (t & 3) + gk] = (float)raw_ks;
 #pragma unroll
       for (int i = 0; i < kPlanes; ++i)
-        if (D == p.dim || 32 * i + kchunk < p.dim)
+        if (EXACT || 32 * i + kchunk < p.dim)
           *reinterpret_cast<f16x8*>(dst + kPlane * i) = from_bytes<BF>(raw_k[i]);
     }
   }
@@ -325,7 +326,7 @@ struct TreeTiles {
       const float vs = (float)raw_vs;
 #pragma unroll
       for (int i = 0; i < kPlanes; ++i) {
-        if (D != p.dim && 32 * i + vchunk >= p.dim) continue;
+        if (!EXACT && 32 * i + vchunk >= p.dim) continue;
         f16x8 x = from_bytes<BF>(raw_v[i], vs);
         if (!ok_v) x = f16x8{};
         if (check && not_finite<BF>(x)) {
@@ -370,7 +371,7 @@ struct TreeTiles {
     turn();
     auto one = [&](auto j) { copy<j.value>(t); };
     each(one, std::make_integer_sequence<int, kCopies>{});
-    if (!Q8 && D == p.dim && W == 4)
+    if constexpr (!Q8 && EXACT && W == 4)
       wait_vmem<kCopies>();  // the first K alone
     else
       wait_vmem<0>();
@@ -450,10 +451,16 @@ struct TreeTiles {
   }
 };
 
-template <int D, bool BF, bool Q8, int W>
+// What a piece leaves to the one after it; in LDS, for the registers are the tiles'.
+struct Walk {
+  int64_t left, rest;  // tiles of the range, and where in the sequence's
+  int seq, pieces;
+};
+
+template <int D, bool BF, bool Q8, int W, bool EXACT>
 __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void tree_attention_kernel(
     const TreeParams p) {
-  using Tiles = TreeTiles<D, BF, Q8, W>;
+  using Tiles = TreeTiles<D, BF, Q8, W, EXACT>;
   __shared__ __align__(1024) f16 s_k[2 * Tiles::kHalves];
   __shared__ __align__(1024) f16 s_v[2 * Tiles::kHalves];
   __shared__ __align__(16) float s_scale[Q8 ? 4 * kKeys : 4];
@@ -469,55 +476,71 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void tree_attention_kerne
     for (int64_t i = from + blockIdx.x * (64 * W) + tid; i < to; i += (int64_t)gridDim.x * (64 * W))
       reinterpret_cast<f16x8*>(p.out)[i] = f16x8{};
   }
-  const Range range = range_of(p);
-  Cut cut = {};  // of the unit that the first piece ends, if it began before
-  int64_t left = range.end - range.begin, rest = range.rest;
-  int seq = range.seq;
+  __shared__ Walk s_walk;
+  {
+    const Range range = range_of(p);
+    if (tid == 0) {
+      p.cuts[blockIdx.x] = Cut{};
+      s_walk = {range.end - range.begin, range.rest, range.seq, 0};
+    }
+    if (range.begin >= range.end) return;
+  }
   Rows<D, BF> r;
   r.init(p.shape);
   Tiles x{p, s_k, s_v, s_scale, s_ok, &s_left};
-  if (left > 0) x.init();
-  bool first_piece = true;
-  while (left > 0) {
-    const Seq s = uniform_seq(seq_of(p, seq));
-    const int unit = uniform((int)(rest / s.nt));
-    const int begin = (int)(rest - (int64_t)unit * s.nt);
-    const int end = (int)min((int64_t)s.nt, begin + left);
-    const int kvh = uniform(unit / s.blocks), block = unit - kvh * s.blocks;
-
-    // This lane's row: a node and a query head. (Rows past the last see what that
-    // one sees, and are not stored.)
-    const int first_row = 32 * W * block, all_rows = s.n * G;
-    const int row = first_row + 32 * w + (lane & 31);
-    const bool wave_live = first_row + 32 * w < all_rows;
-    const int at = min(row, all_rows - 1);
-    const int node = at / G;
-    const int64_t q_row = (int64_t)(s.first + node) * p.hq + kvh * G + at % G;
-    r.clear();
-    r.load(p.q + q_row * p.dim, p.dim, true);
-    x.mask = p.masks[s.first + node];
-    const int depth = max(0, (int)__popcll(x.mask) - 1);
-    x.lo = 0;
-    if (p.window > 0) {
-      x.lo = max(0, s.held + depth - p.window + 1);
-      while ((int)__popcll(x.mask) > p.window) x.mask &= x.mask - 1;
+  x.init();
+  __syncthreads();
+  for (;;) {
+    int ta, tb;
+    {
+      const int64_t left = uniform64(s_walk.left), rest = uniform64(s_walk.rest);
+      const int seq = uniform(s_walk.seq);
+      const Seq s = uniform_seq(seq_of(p, seq));
+      const int unit = uniform((int)(rest / s.nt));
+      const int begin = (int)(rest - (int64_t)unit * s.nt);
+      ta = s.t0 + begin;
+      tb = s.t0 + (int)min((int64_t)s.nt, begin + left);
+      x.kvh = uniform(unit / s.blocks);
+      x.held = s.held;
+      x.last = s.held + min(s.n, kNodes) - 1;
+      x.table = p.tables + (int64_t)seq * p.stride;
+      // This lane's row: a node and a query head. (Rows past the last see what that
+      // one sees, and are not stored.)
+      const int row = 32 * W * (unit - x.kvh * s.blocks) + 32 * w + (lane & 31);
+      const int at = min(row, s.n * G - 1);
+      const int node = at / G;
+      r.clear();
+      r.load(p.q + ((int64_t)(s.first + node) * p.hq + x.kvh * G + at % G) * p.dim, p.dim, true);
+      x.mask = p.masks[s.first + node];
+      x.lo = 0;
+      if (p.window > 0) {
+        x.lo = max(0, s.held + max(0, (int)__popcll(x.mask) - 1) - p.window + 1);
+        while ((int)__popcll(x.mask) > p.window) x.mask &= x.mask - 1;
+      }
+      // (A wave that has no row sees no tile.)
+      const bool live = uniform(row - (lane & 31)) < s.n * G;
+      if (tid == 0) s_left = 0;
+      attend(r, x, ta, tb, ta, live ? tb : ta, x.last >= (tb - 1) * kKeys + 32);
     }
-    x.table = p.tables + (int64_t)seq * p.stride;
-    x.kvh = kvh;
-    x.held = s.held;
-    x.last = s.held + min(s.n, kNodes) - 1;
-    const int ta = s.t0 + begin, tb = s.t0 + end;
-    if (!first_piece) __syncthreads();  // (others may still read the last tile)
-    if (tid == 0) s_left = 0;
-    attend(r, x, ta, tb, ta, wave_live ? tb : ta, x.last >= (tb - 1) * kKeys + 32);
     x.add_left_out(r, ta, tb);
 
+    // (All of it anew: what was held over the tiles cost their registers.)
+    const int64_t left = uniform64(s_walk.left), rest = uniform64(s_walk.rest);
+    const int seq = uniform(s_walk.seq), pieces = uniform(s_walk.pieces);
+    const Seq s = uniform_seq(seq_of(p, seq));
+    const int unit = uniform((int)(rest / s.nt));
+    const int begin = ta - s.t0, end = tb - s.t0;
+    const int kvh = uniform(unit / s.blocks);
+    const int first_row = 32 * W * (unit - kvh * s.blocks), all_rows = s.n * G;
+    const int row = first_row + 32 * w + (lane & 31);
     if (end - begin == s.nt) {
       const float inv = r.inverse();
-      if (row < all_rows) r.store(p.out + q_row * p.dim, p.dim, inv);
-    } else if (wave_live) {
+      if (row < all_rows)
+        r.store(p.out + ((int64_t)(s.first + row / G) * p.hq + kvh * G + row % G) * p.dim, p.dim,
+                inv);
+    } else if (first_row + 32 * w < all_rows) {
       // A piece of a unit that is cut, as it is.
-      const int64_t piece = (2 * (int64_t)blockIdx.x + (first_piece ? 0 : 1)) * W + w;
+      const int64_t piece = (2 * (int64_t)blockIdx.x + (pieces ? 1 : 0)) * W + w;
       const float sum = r.l + __shfl_xor(r.l, 32);
       if (lane < 32) p.part_ml[piece * 32 + lane] = make_float2(r.m, sum);
       float4* dst = reinterpret_cast<float4*>(p.part_o) + piece * (D / 8 * 64) + lane;
@@ -526,27 +549,29 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void tree_attention_kerne
         dst[64 * i] = make_float4(r.o[i / 4][4 * (i % 4)], r.o[i / 4][4 * (i % 4) + 1],
                                   r.o[i / 4][4 * (i % 4) + 2], r.o[i / 4][4 * (i % 4) + 3]);
     }
-    if (first_piece && begin > 0 && end == s.nt) {
-      // The unit's first tile, and the workgroup that has it.
+    if (pieces == 0 && begin > 0 && end == s.nt) {
+      // The unit began in an earlier range: its first tile, and the workgroup of that.
+      const Range range = range_of(p);
       const int64_t from = range.begin - begin;
       const int64_t g = ((from + 1) * range.n - 1) / range.all;
-      cut.rows = min(all_rows - first_row, 32 * W);
-      cut.first = first_row;
-      cut.token = s.first;
-      cut.kvh = kvh;
-      cut.piece = (int)(2 * g + (from > range_begin(range.all, range.n, g) ? 1 : 0));
-      cut.group = (int)g + 1;
+      if (tid == 0)
+        p.cuts[blockIdx.x] = {min(all_rows - first_row, 32 * W), first_row, s.first, kvh,
+                              (int)(2 * g + (from > range_begin(range.all, range.n, g) ? 1 : 0)),
+                              (int)g + 1, {}};
     }
-    left -= end - begin;
-    rest += end - begin;
-    if (rest >= tiles_of(p, s)) {  // the next sequence that has a tree
-      rest = 0;
-      ++seq;
-      while (left > 0 && uniform(seq_of(p, seq).nt) == 0) ++seq;
+    const int64_t now = left - (end - begin);
+    if (now <= 0) break;
+    int64_t on = rest + (end - begin);
+    int next = seq;
+    if (on >= tiles_of(p, s)) {  // the next sequence that has a tree
+      on = 0;
+      do ++next;
+      while (uniform(seq_of(p, next).nt) == 0);
     }
-    first_piece = false;
+    __syncthreads();  // (others may still read the state and the last tile)
+    if (tid == 0) s_walk = {now, on, next, pieces + 1};
+    __syncthreads();
   }
-  if (tid == 0) p.cuts[blockIdx.x] = cut;
 }
 
 // Joins the pieces of the unit that is cut and ends in a workgroup's range: with M the
@@ -627,16 +652,23 @@ __global__ __launch_bounds__(kThreads) void tree_join_kernel(const TreeParams p)
   }
 }
 
+// Other head dims than the widths take the four-wave kernels.
 template <bool BF, bool Q8>
-const void* tree_kernel_for(int width, int waves) {
+const void* tree_kernel_for(int width, int waves, bool exact) {
+  if (!exact)
+    return width == 64   ? reinterpret_cast<const void*>(tree_attention_kernel<64, BF, Q8, 4, false>)
+           : width == 96 ? reinterpret_cast<const void*>(tree_attention_kernel<96, BF, Q8, 4, false>)
+           : width == 128
+               ? reinterpret_cast<const void*>(tree_attention_kernel<128, BF, Q8, 4, false>)
+               : reinterpret_cast<const void*>(tree_attention_kernel<256, BF, Q8, 4, false>);
   if (waves == 8)
-    return width == 64   ? reinterpret_cast<const void*>(tree_attention_kernel<64, BF, Q8, 8>)
-           : width == 96 ? reinterpret_cast<const void*>(tree_attention_kernel<96, BF, Q8, 8>)
-                         : reinterpret_cast<const void*>(tree_attention_kernel<128, BF, Q8, 8>);
-  return width == 64    ? reinterpret_cast<const void*>(tree_attention_kernel<64, BF, Q8, 4>)
-         : width == 96  ? reinterpret_cast<const void*>(tree_attention_kernel<96, BF, Q8, 4>)
-         : width == 128 ? reinterpret_cast<const void*>(tree_attention_kernel<128, BF, Q8, 4>)
-                        : reinterpret_cast<const void*>(tree_attention_kernel<256, BF, Q8, 4>);
+    return width == 64   ? reinterpret_cast<const void*>(tree_attention_kernel<64, BF, Q8, 8, true>)
+           : width == 96 ? reinterpret_cast<const void*>(tree_attention_kernel<96, BF, Q8, 8, true>)
+                         : reinterpret_cast<const void*>(tree_attention_kernel<128, BF, Q8, 8, true>);
+  return width == 64    ? reinterpret_cast<const void*>(tree_attention_kernel<64, BF, Q8, 4, true>)
+         : width == 96  ? reinterpret_cast<const void*>(tree_attention_kernel<96, BF, Q8, 4, true>)
+         : width == 128 ? reinterpret_cast<const void*>(tree_attention_kernel<128, BF, Q8, 4, true>)
+                        : reinterpret_cast<const void*>(tree_attention_kernel<256, BF, Q8, 4, true>);
 }
 template <bool BF>
 const void* tree_join_for(int width) {
@@ -715,7 +747,9 @@ int tree_attention(const void* queries, const void* keys, const void* values,
   prm.out = static_cast<f16*>(out);
   // Eight waves, two to a SIMD, where the sequences' trees have more rows than four
   // waves hold: their keys and values are then read once where they were read twice.
-  const int waves = width <= 128 && (int64_t)tokens * G > 4 * 32 * (int64_t)batch ? 8 : 4;
+  const bool exact = width == head_dim;
+  const int waves =
+      exact && width <= 128 && (int64_t)tokens * G > 4 * 32 * (int64_t)batch ? 8 : 4;
   prm.groups = groups_for(width, waves);
   prm.rows = 32 * waves;
   const size_t pieces = 2 * (size_t)prm.groups * prm.rows;
@@ -744,10 +778,10 @@ int tree_attention(const void* queries, const void* keys, const void* values,
   prm.shape = shape_of(scale, softcap);
   void* args[] = {&prm};
   const hipStream_t hs = static_cast<hipStream_t>(stream);
-  const void* fn = q8 ? (bf16_elems ? tree_kernel_for<true, true>(width, waves)
-                                    : tree_kernel_for<false, true>(width, waves))
-                      : (bf16_elems ? tree_kernel_for<true, false>(width, waves)
-                                    : tree_kernel_for<false, false>(width, waves));
+  const void* fn = q8 ? (bf16_elems ? tree_kernel_for<true, true>(width, waves, exact)
+                                    : tree_kernel_for<false, true>(width, waves, exact))
+                      : (bf16_elems ? tree_kernel_for<true, false>(width, waves, exact)
+                                    : tree_kernel_for<false, false>(width, waves, exact));
   hipError_t err = hipLaunchKernel(fn, dim3(prm.groups), dim3(64 * waves), args, 0, hs);
   if (err != hipSuccess)
     return fail(PDA_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(err));

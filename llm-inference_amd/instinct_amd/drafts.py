@@ -135,14 +135,18 @@ def commit_drafts(arenas: Sequence[tuple[torch.Tensor, ...]], tables: torch.Tens
     keys = arenas[0][0]
     layout, arena_rows, kv_heads, head_dim = _arena_geometry(keys, page_size)
     device = keys.device
+    if len(arenas[0]) not in (2, 4) or any(len(a) != len(arenas[0]) for a in arenas):
+        raise ValueError("a layer is (keys, values) or those and their scales")
+    # (One test for what is all right: with some dozens of stores the call waits for it.)
+    index, kind, shape = keys.get_device(), keys.dtype, keys.shape
+    forms = ((kind, shape),) * 2 + ((torch.float16, shape[:-1]),) * 2
     stores = []
     for arena in arenas:
-        if len(arena) != len(arenas[0]) or len(arena) not in (2, 4):
-            raise ValueError("a layer is (keys, values) or those and their scales")
-        for name, t in zip(("keys", "values", "key_scales", "value_scales"), arena):
-            scale = name.endswith("scales")
-            _check_arena(name, t, keys, torch.float16 if scale else keys.dtype)
-            if t.dim() != keys.dim() - scale or t.shape != keys.shape[:t.dim()]:
+        for t, (dtype, size) in zip(arena, forms):
+            if (t.dtype is not dtype or t.shape != size or t.get_device() != index
+                    or index < 0 or not t.is_contiguous()):
+                name = ("keys", "values", "key_scales", "value_scales")[len(stores) % len(arena)]
+                _check_arena(name, t, keys, dtype)
                 raise ValueError(f"{name} must have the first layer's shape")
             stores.append(t.data_ptr())
     if len(set(stores)) < len(stores):
@@ -164,9 +168,9 @@ def commit_drafts(arenas: Sequence[tuple[torch.Tensor, ...]], tables: torch.Tens
             raise ValueError(f"{name} must be on {device}")
     drafted, targets = drafted.contiguous(), targets.contiguous()
     if out is None:
-        i32 = dict(dtype=torch.int32, device=device)
-        out = Committed(torch.empty(batch, **i32), torch.empty(batch, **i32),
-                        torch.empty((batch, NODES), **i32),
+        new, accepted, path = torch.empty((2 + NODES) * batch, dtype=torch.int32,
+                                          device=device).split((batch, batch, NODES * batch))
+        out = Committed(new, accepted, path.view(batch, NODES),
                         torch.empty(batch, dtype=torch.int64, device=device))
     else:
         for name, t, shape in zip(Committed._fields, out, ((batch,), (batch,), (batch, NODES),
