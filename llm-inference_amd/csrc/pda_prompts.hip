@@ -173,22 +173,23 @@ struct PromptTiles {
   __device__ __forceinline__ const f16* keys(int t) const { return s_k + (t & 1) * kHalves; }
   __device__ __forceinline__ const f16* values(int t) const { return s_v + (t & 1) * kHalves; }
 
-  __device__ __forceinline__ void copy_k(int t, int i) const {
+  template <int i>
+  __device__ __forceinline__ void copy_k(int t) const {
     if (D == p.dim || 32 * i + kchunk < p.dim)
-      copy_to_lds(kb + (int64_t)min(t * kKeys + gk, last) * p.k_token + kchunk + 32 * i,
-                  k_dst + (t & 1) * (2 * kHalves) + 2 * kPlane * i);
+      copy_plane_to_lds<i>(kb + (int64_t)min(t * kKeys + gk, last) * p.k_token + kchunk,
+                           k_dst + (t & 1) * (2 * kHalves));
   }
   template <int j>
   __device__ __forceinline__ void copy(int t) const {
     if constexpr (j >= kPlanes)
-      copy_k(t + 1, j - kPlanes);
+      copy_k<j - kPlanes>(t + 1);
     else if (D == p.dim || 32 * j + vchunk < p.dim)
-      copy_to_lds(vb + (int64_t)min(t * kKeys + gk, last) * p.v_token + vchunk + 32 * j,
-                  v_dst + (t & 1) * (2 * kHalves) + 2 * kPlane * j);
+      copy_plane_to_lds<j>(vb + (int64_t)min(t * kKeys + gk, last) * p.v_token + vchunk,
+                           v_dst + (t & 1) * (2 * kHalves));
   }
   __device__ __forceinline__ void first(int t) {
-#pragma unroll
-    for (int i = 0; i < kPlanes; ++i) copy_k(t, i);
+    auto of_k = [&](auto i) { copy_k<i.value>(t); };
+    each(of_k, std::make_integer_sequence<int, kPlanes>{});
     auto one = [&](auto j) { copy<j.value>(t); };
     each(one, std::make_integer_sequence<int, kCopies>{});
     if (D == p.dim)

@@ -76,12 +76,16 @@ __device__ __forceinline__ uint32_t lds_address(const void* at) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)at;
 }
 
-// 16 bytes per lane from global memory straight into LDS: lane i's to dst + 16 i
-// (dst: wave-uniform). The caller waits (wait_vmem) before the barrier that
-// publishes them.
-__device__ __forceinline__ void copy_to_lds(const void* src, uint32_t dst) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src)
-               : "memory", "m0");
+// 16 bytes per lane from global memory straight into LDS, plane `kAt` of a key's row:
+// lane i's from src + 64 kAt to dst + 2 kPlane kAt + 16 i (dst: of the tile, wave-
+// uniform; the instruction adds its offset to both addresses). The caller waits
+// (wait_vmem) before the barrier that publishes them.
+template <int kAt>
+__device__ __forceinline__ void copy_plane_to_lds(const void* src, uint32_t dst) {
+  asm volatile("s_add_u32 m0, %0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off offset:%3" ::"s"(
+                   dst),
+               "v"(src), "n"((2 * kPlane - 64) * kAt), "n"(64 * kAt)
+               : "memory", "m0", "scc");
 }
 
 // f(0), f(1), ... with compile-time arguments.
@@ -153,6 +157,7 @@ __device__ __forceinline__ f16x8 finite_only(f16x8 x) {
 // One bit a key from a ballot with four lanes a key.
 __device__ __forceinline__ uint32_t keys_of(uint64_t lanes) {
   if (lanes == 0) return 0;
+  if (lanes == ~0ull) return 0xFFFFu;
   lanes |= lanes >> 1;
   lanes |= lanes >> 2;
   uint32_t keys = 0;
