@@ -212,8 +212,10 @@ struct Rows {
       const f16x8 x = *reinterpret_cast<const f16x8*>(row + (in ? d : 0));
       q[i] = in ? x : f16x8{};
     }
-    // Only matrix-core operands: where the outputs take half the vector registers,
-    // they go to accumulator registers.
+  }
+  // Before their first use. Only matrix-core operands: where the outputs take half the
+  // vector registers, they go to accumulator registers.
+  __device__ __forceinline__ void settle_queries() {
     if constexpr (D > 128) {
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) asm volatile("" : "+a"(q[i]));
@@ -441,7 +443,8 @@ struct Rows {
 // The tiles [t0, t1) of a workgroup, of which this wave's rows see [wa, wb) (the last
 // one's odd block only with odd_last). `x` moves and shapes them:
 //   first(t0)     K of the first tile is readable, its V and the next K under way
-//   copy<j>(t)    for all j < T::kCopies: V of tile t and K of tile t + 1
+//   ahead(r)      once no more scores are taken: what comes after may load its queries
+//   aim(t), copy<j>(t) for all j < T::kCopies: V of tile t and K of tile t + 1
 //   close(t)      they are readable by all waves; all are done with V of t - 1, K of t
 //   shape(s, k0)  caps and masks of the scores of the keys from k0 on, with rough(t)
 //                 telling whether the odd block before tile t or its even one need it
@@ -452,6 +455,7 @@ __device__ __forceinline__ void attend(R& r, T& x, int t0, int t1, int wa, int w
   int t = t0;
   x.first(t);
   auto copies = [&]() {
+    x.aim(t);
     auto one = [&](auto j) { x.template copy<j.value>(t); };
     each(one, std::make_integer_sequence<int, T::kCopies>{});
   };
@@ -481,6 +485,7 @@ __device__ __forceinline__ void attend(R& r, T& x, int t0, int t1, int wa, int w
       const int k0 = t * kKeys;
       const f16* kt = x.keys(t);
       const f16* vt = x.values(t - 1);
+      x.aim(t);
       const bool rough = x.rough(t);
       if (rough) x.shape(s1, k0 - 32);
       r.step(s1, w1, w0, s0, lb, kt, vt, [&](auto i) {
@@ -495,6 +500,7 @@ __device__ __forceinline__ void attend(R& r, T& x, int t0, int t1, int wa, int w
     }
     // Past the last tile: weights of its odd block, products of its V.
     if (t < t1) copies();
+    x.ahead(r);
     const f16* vt = x.values(t - 1);
     r.accumulate(w0, vt);
     if (odd_last) {
@@ -504,10 +510,9 @@ __device__ __forceinline__ void attend(R& r, T& x, int t0, int t1, int wa, int w
     }
     if (t < t1) x.close(t);
     for (++t; t < t1; ++t) idle();
+  } else {
+    x.ahead(r);
   }
-  // (Where no tile was closed the copies under way have to land before the LDS is
-  // used anew.)
-  wait_vmem<0>();
 }
 
 }  // namespace pda_rows

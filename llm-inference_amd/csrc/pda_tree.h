@@ -372,6 +372,8 @@ struct TreeTiles {
     take_usable(t);
     lookup(t + 2);
   }
+  __device__ __forceinline__ void aim(int) const {}  // (turn has)
+  __device__ __forceinline__ void ahead(Rows<D, BF>&) const {}
   __device__ __forceinline__ void close(int t) {
     wait_vmem<0>();
     put_v(t);
@@ -504,6 +506,7 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void tree_attention_kerne
       const int node = at / G;
       r.clear();
       r.load(p.q + ((int64_t)(s.first + node) * p.hq + x.kvh * G + at % G) * p.dim, p.dim, true);
+      r.settle_queries();
       x.mask = p.masks[s.first + node];
       x.lo = 0;
       if (p.window > 0) {
