@@ -206,6 +206,7 @@ struct PromptTiles {
   static constexpr int kPlanes = D / 32;
   static constexpr int kHalves = kPlanes * kPlane;  // of a tile
   static constexpr int kCopies = 2 * kPlanes;
+  static constexpr bool kSpread = true;  // (the copies are there long before they are needed)
 
   const PromptParams& p;
   f16* s_k;          // [2][kHalves]

@@ -174,7 +174,8 @@ __device__ __forceinline__ uint32_t below(int n) {
 
 // 32 rows of one wave: lane l holds row l % 32, half l / 32 of its keys and dims
 // (of every 8 the first or the last four).
-template <int D, bool BF>
+// BF: queries, keys and outputs are bf16 (else fp16); VBF: values and weights are.
+template <int D, bool BF, bool VBF = BF>
 struct Rows {
   f16x8 q[D / 16];
   f32x16 o[D / 32];
@@ -261,7 +262,7 @@ struct Rows {
   // Weights 2 i, 2 i + 1 of a block, rounded to 16 bits and packed.
   __device__ __forceinline__ static void put_pair(f16x8 (&w)[2], int i, float e0, float e1) {
     f16x2 ph;
-    if constexpr (BF)
+    if constexpr (VBF)
       ph = __builtin_bit_cast(f16x2, bf16x2{(bf16)e0, (bf16)e1});
     else
       ph = f16x2{(f16)e0, (f16)e1};
@@ -275,7 +276,7 @@ struct Rows {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const f16x2 ph = {w[i / 4][2 * (i % 4)], w[i / 4][2 * (i % 4) + 1]};
-      if constexpr (BF)
+      if constexpr (VBF)
         s2[i & 1] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, ph),
                                                     bf16x2{(bf16)1.0f, (bf16)1.0f}, s2[i & 1],
                                                     false);
@@ -332,7 +333,7 @@ struct Rows {
         const f16x4 lo4 = read_tr(vp);
         const f16x4 hi4 = read_tr(vp + 256);
         const f16x8 a = {lo4[0], lo4[1], lo4[2], lo4[3], hi4[0], hi4[1], hi4[2], hi4[3]};
-        o[b] = mfma16<BF>(a, w[ks], o[b]);
+        o[b] = mfma16<VBF>(a, w[ks], o[b]);
       }
     }
   }
@@ -376,7 +377,7 @@ struct Rows {
         xn = mfma16<BF>(a[i], q[cc], cc == 0 ? f32x16{} : xn);
       } else {
         constexpr int b = (i >> 1) % (D / 32), ks = (i >> 1) / (D / 32);
-        o[b] = mfma16<BF>(a[i], pv[ks], o[b]);
+        o[b] = mfma16<VBF>(a[i], pv[ks], o[b]);
       }
       if constexpr (i + kAhead < kSlots) read(i + kAhead);
       beside(sc);
@@ -448,6 +449,7 @@ struct Rows {
 //   close(t)      they are readable by all waves; all are done with V of t - 1, K of t
 //   shape(s, k0)  caps and masks of the scores of the keys from k0 on, with rough(t)
 //                 telling whether the odd block before tile t or its even one need it
+// T::kSpread: the copies go beside a step's products, else in front of them.
 // V runs one tile behind K, so that two LDS tiles of each serve the pipeline with one
 // barrier a tile.
 template <class R, class T>
@@ -485,12 +487,16 @@ __device__ __forceinline__ void attend(R& r, T& x, int t0, int t1, int wa, int w
       const int k0 = t * kKeys;
       const f16* kt = x.keys(t);
       const f16* vt = x.values(t - 1);
-      x.aim(t);
+      if constexpr (T::kSpread)
+        x.aim(t);
+      else
+        copies();
       const bool rough = x.rough(t);
       if (rough) x.shape(s1, k0 - 32);
       r.step(s1, w1, w0, s0, lb, kt, vt, [&](auto i) {
         // (Every other slot: a copy is two instructions and an address.)
-        if constexpr (i.value % 2 == 0 && i.value / 2 < T::kCopies) x.template copy<i.value / 2>(t);
+        if constexpr (T::kSpread && i.value % 2 == 0 && i.value / 2 < T::kCopies)
+          x.template copy<i.value / 2>(t);
       });
       r.settle(s1, w1, lb);
       if (rough) x.shape(s0, k0);

@@ -173,6 +173,12 @@ struct TreeTiles {
   static constexpr int kPlanes = D / 32;
   static constexpr int kHalves = kPlanes * kPlane;  // of a tile
   static constexpr int kCopies = W == 4 ? 2 * kPlanes : kPlanes;
+  static constexpr bool kSpread = false;  // the copies are issued at once: they are waited for
+  // 8 bits: the keys are exact in either type, the values times their scales are rounded,
+  // to fp16 also under bf16 queries (to bf16, and the weights with them, the outputs were
+  // 1.65 times as far from 64 bits as their own rounding puts them: 0.0028 and 0.0017).
+  static constexpr bool kVbf = BF && !Q8;
+  using R = Rows<D, BF, kVbf>;
 
   const TreeParams& p;
   f16* s_k;          // [2][kHalves]
@@ -319,11 +325,11 @@ struct TreeTiles {
 #pragma unroll
       for (int i = 0; i < kPlanes; ++i) {
         if (!EXACT && 32 * i + vchunk >= p.dim) continue;
-        f16x8 x = from_bytes<BF>(raw_v[i], vs);
+        f16x8 x = from_bytes<kVbf>(raw_v[i], vs);
         if (!ok_v) x = f16x8{};
-        if (check && not_finite<BF>(x)) {
+        if (check && not_finite<kVbf>(x)) {
           *s_left = 1;
-          x = finite_only<BF>(x);
+          x = finite_only<kVbf>(x);
         }
         *reinterpret_cast<f16x8*>(dst + kPlane * i) = x;
       }
@@ -334,9 +340,9 @@ struct TreeTiles {
 #pragma unroll
       for (int i = 0; i < kPlanes; ++i) {
         const f16x8 x = *reinterpret_cast<const f16x8*>(dst + kPlane * i);
-        if (not_finite<BF>(x)) {
+        if (not_finite<kVbf>(x)) {
           *s_left = 1;
-          *reinterpret_cast<f16x8*>(dst + kPlane * i) = finite_only<BF>(x);
+          *reinterpret_cast<f16x8*>(dst + kPlane * i) = finite_only<kVbf>(x);
         }
       }
     }
@@ -373,7 +379,7 @@ struct TreeTiles {
     lookup(t + 2);
   }
   __device__ __forceinline__ void aim(int) const {}  // (turn has)
-  __device__ __forceinline__ void ahead(Rows<D, BF>&) const {}
+  __device__ __forceinline__ void ahead(R&) const {}
   __device__ __forceinline__ void close(int t) {
     wait_vmem<0>();
     put_v(t);
@@ -412,13 +418,13 @@ struct TreeTiles {
         x[4 * g + 3] *= y.w;
       }
     }
-    if (special) Rows<D, BF>::shape(x, p.shape);
+    if (special) R::shape(x, p.shape);
     const uint32_t ok = ok_of(k0);
-    if (edge(k0 / kKeys) || ok != 0xFFFFFFFFu) Rows<D, BF>::mask(x, visible(k0, ok));
+    if (edge(k0 / kKeys) || ok != 0xFFFFFFFFu) R::mask(x, visible(k0, ok));
   }
   // After the piece's last tile: the values that were taken as zeros, to the rows that
   // see them.
-  __device__ __forceinline__ void add_left_out(Rows<D, BF>& r, int ta, int tb) const {
+  __device__ __forceinline__ void add_left_out(R& r, int ta, int tb) const {
     __syncthreads();
     if (uniform(*s_left) == 0) return;
     for (int t = ta; t < tb; ++t) {
@@ -436,7 +442,8 @@ struct TreeTiles {
             const float vs = (float)p.vscale[from * p.scale_page + (int64_t)sl * p.scale_row +
                                              (int64_t)kvh * p.scale_head];
             const int8_t* y = static_cast<const int8_t*>(p.v) + at + d;
-            return make_float4(y[0] * vs, y[1] * vs, y[2] * vs, y[3] * vs);
+            auto value = [&](int i) { return widen16<kVbf>(round16<kVbf>(y[i] * vs)); };
+            return make_float4(value(0), value(1), value(2), value(3));
           } else {
             return widen4<BF>(static_cast<const f16*>(p.v) + at + d);
           }
@@ -480,7 +487,7 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void tree_attention_kerne
     }
     if (range.begin >= range.end) return;
   }
-  Rows<D, BF> r;
+  typename Tiles::R r;
   r.init(p.shape);
   Tiles x{p, s_k, s_v, s_scale, s_ok, &s_left};
   x.init();
