@@ -836,8 +836,9 @@ int pda_extend_tables(int32_t* tables, int32_t table_stride,
  *           where they are), the elements of a head side by side
  *   out     [tokens, q_heads, head_dim], contiguous
  * Rows of out behind the last prompt become zeros. A key or value that is not
- * finite reaches the queries that see it alone. head_dim a multiple of 8 up to 256.
- * fp16, or bf16 (_bf16). One launch on `stream`; results are reproducible. */
+ * finite reaches the queries that see it alone. head_dim a multiple of 8 up to 256;
+ * tokens below 2^31 - 1024. fp16, or bf16 (_bf16). One launch on `stream`; results are
+ * reproducible. */
 int pda_packed_prompt_attention(const void* queries, int64_t q_token,
                                 int64_t q_head, const void* keys,
                                 int64_t k_token, int64_t k_head,
@@ -869,11 +870,12 @@ int pda_tree_workspace_bytes(int32_t head_dim, size_t* bytes);
  * - window and the last `window` nodes of its mask.
  *   queries, out [tokens, q_heads, head_dim]; keys, values, tables, layout, the
  *   masking of pages, scale and softcap as for pda_paged_decode_attention
- * Rows of out behind the last sequence become zeros; a value that is not finite
- * reaches the nodes that see it alone. head_dim a multiple of 8 up to 256. fp16, or
- * bf16 (_bf16); int8 keys and values with fp16 scales under fp16 (_q8) or bf16
- * (_q8_bf16) queries. Two launches on `stream`; calls that share a workspace must
- * not overlap. Results are reproducible. */
+ * Lengths are cut to what the table holds and to 2^31 - 1025. Rows of out behind the
+ * last sequence become zeros; a value that is not finite reaches the nodes that see it
+ * alone. head_dim a multiple of 8 up to 256. fp16, or bf16 (_bf16); int8 keys and
+ * values with fp16 scales under fp16 (_q8) or bf16 (_q8_bf16) queries (a value times
+ * its scale past 65504 is infinite). Two launches on `stream`; calls that share a
+ * workspace must not overlap. Results are reproducible. */
 int pda_tree_attention(const void* queries, const void* keys,
                        const void* values,
                        const int32_t* tables, const int32_t* lengths,

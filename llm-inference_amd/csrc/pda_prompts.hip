@@ -483,6 +483,8 @@ int packed_prompt(const void* queries, int64_t q_token, int64_t q_head, const vo
     return fail(PDA_ERR_ALIGNMENT, "query, K/V and output buffers must be 16-byte aligned");
   if ((uintptr_t)starts & 3)
     return fail(PDA_ERR_ALIGNMENT, "the starts must be 4-byte aligned");
+  if (tokens > INT32_MAX - 1024)  // (positions past a prompt's last tile are formed)
+    return fail(PDA_ERR_TOO_LONG, "%d tokens: below 2^31 - 1024 are taken", tokens);
   // As many query tiles as the prompts can have.
   const int64_t tiles = ((int64_t)tokens + (int64_t)(kTile - 1) * batch) / kTile;
   if (tiles * q_heads > INT32_MAX)

@@ -77,7 +77,7 @@ __device__ __forceinline__ Seq seq_of(const TreeParams& p, int b) {
   Seq s;
   s.first = max(0, min(p.starts[b], p.tokens));
   s.n = max(s.first, min(p.starts[b + 1], p.tokens)) - s.first;
-  const int64_t room = min((int64_t)p.stride * p.page_size, (int64_t)INT32_MAX - 2 * kNodes);
+  const int64_t room = min((int64_t)p.stride * p.page_size, (int64_t)INT32_MAX - 1024);
   s.held = (int)max((int64_t)0, min((int64_t)p.lengths[b], room));
   // (The first row that any node sees: a node is at least at position `held`.)
   s.t0 = p.window > 0 ? max(0, s.held - p.window + 1) / kKeys : 0;

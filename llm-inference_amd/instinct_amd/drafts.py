@@ -168,8 +168,9 @@ def commit_drafts(arenas: Sequence[tuple[torch.Tensor, ...]], tables: torch.Tens
             raise ValueError(f"{name} must be on {device}")
     drafted, targets = drafted.contiguous(), targets.contiguous()
     if out is None:
-        new, accepted, path = torch.empty((2 + NODES) * batch, dtype=torch.int32,
-                                          device=device).split((batch, batch, NODES * batch))
+        new, accepted, path = torch.empty(
+            (2 + NODES) * batch, dtype=torch.int32, device=device
+        ).split_with_sizes((batch, batch, NODES * batch))
         out = Committed(new, accepted, path.view(batch, NODES),
                         torch.empty(batch, dtype=torch.int64, device=device))
     else:

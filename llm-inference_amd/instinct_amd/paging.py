@@ -115,8 +115,8 @@ def extend_tables(tables: torch.Tensor, lengths: torch.Tensor, counts: torch.Ten
         parents = _check_index("parents", parents, (tokens,), device)
     if out is None:
         # (One allocation for the int32 results: seven took 9 us of a small step's 17.)
-        parts = torch.empty(3 * batch + 3 + 2 * tokens, dtype=torch.int32, device=device).split(
-            (batch + 1, batch, batch, 2, tokens, tokens))
+        parts = torch.empty(3 * batch + 3 + 2 * tokens, dtype=torch.int32, device=device
+                            ).split_with_sizes((batch + 1, batch, batch, 2, tokens, tokens))
         masks = (None if parents is None
                  else torch.empty(tokens, dtype=torch.int64, device=device))
         out = StepRows(*parts, masks)

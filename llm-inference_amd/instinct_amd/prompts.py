@@ -39,32 +39,35 @@ def packed_prompt_attention(queries: torch.Tensor, keys: torch.Tensor, values: t
     device = queries.device
     tokens, q_heads, head_dim = queries.shape
     kv_heads = keys.shape[1] if keys.dim() == 3 else 0
+    size = (tokens, kv_heads, head_dim)
     for name, t in (("keys", keys), ("values", values)):
-        if t.dtype != queries.dtype:
+        if t.dtype is not queries.dtype:
             raise TypeError(f"{name} must be {queries.dtype}, got {t.dtype}")
         if t.device != device:
             raise ValueError(f"{name} must be on {device}")
-        if t.dim() != 3 or t.shape != (tokens, kv_heads, head_dim) or not kv_heads:
+        if t.shape != size or not kv_heads:
             raise ValueError(f"{name} must be [tokens, kv_heads, head_dim] beside the queries")
     if q_heads == 0 or q_heads % kv_heads:
         raise ValueError("query heads must be a multiple of kv heads")
-    for name, t in (("queries", queries), ("keys", keys), ("values", values)):
-        if t.stride(2) != 1:
-            raise ValueError(f"the elements of a head of {name} must lie side by side")
+    q_token, q_head, q_one = queries.stride()
+    k_token, k_head, k_one = keys.stride()
+    v_token, v_head, v_one = values.stride()
+    if head_dim > 1 and (q_one != 1 or k_one != 1 or v_one != 1):
+        raise ValueError("the elements of a head must lie side by side")
     if starts.dim() != 1 or starts.shape[0] == 0:
         raise ValueError("starts must be int32 [batch + 1]")
     starts = _check_index("starts", starts, (starts.shape[0],), device)
     if out is None:
-        out = torch.empty((tokens, q_heads, head_dim), dtype=queries.dtype, device=device)
+        out = torch.empty_like(queries, memory_format=torch.contiguous_format)
     elif (out.dtype != queries.dtype or out.shape != queries.shape or out.device != device
           or not out.is_contiguous()):
         raise ValueError("out must be contiguous and match the queries' shape, dtype and device")
     entry = ("pda_packed_prompt_attention_bf16" if queries.dtype == torch.bfloat16
              else "pda_packed_prompt_attention")
-    place = lambda t: (t.data_ptr(), t.stride(0), t.stride(1))  # noqa: E731
     with on_device(device):
         rc = getattr(_lib.library(), entry)(
-            *place(queries), *place(keys), *place(values), starts.data_ptr(), out.data_ptr(),
+            queries.data_ptr(), q_token, q_head, keys.data_ptr(), k_token, k_head,
+            values.data_ptr(), v_token, v_head, starts.data_ptr(), out.data_ptr(),
             tokens, starts.shape[0] - 1, q_heads, kv_heads, head_dim, float(scale), int(window),
             float(softcap), torch.cuda.current_stream(device).cuda_stream)
     _lib.check(rc)
