@@ -169,7 +169,7 @@ for _suffix in ("", "_bf16"):
 SIGNATURES["pda_tree_workspace_bytes"] = (
     ctypes.c_int, [c_int32, ctypes.POINTER(c_size_t)])
 SIGNATURES["pda_commit_drafts"] = (
-    ctypes.c_int, [ctypes.POINTER(c_void_p)] + [c_int32] * 3 + [c_void_p] * 6 + [c_int32]
+    ctypes.c_int, [c_void_p] + [c_int32] * 3 + [c_void_p] * 6 + [c_int32]
     + [c_void_p] * 4 + [c_int32] * 5 + [c_int64, c_int32, c_void_p])
 
 _lib: ctypes.CDLL | None = None

@@ -15,8 +15,9 @@ The work happens in libpda.so (``csrc/pda_drafts.hip``).
 
 from __future__ import annotations
 
-import ctypes
+from array import array
 from collections.abc import Sequence
+from operator import attrgetter
 from typing import Any, NamedTuple
 
 import torch
@@ -26,6 +27,9 @@ from .eviction import _check_arena, _check_index
 from .hip_kernels import _arena_geometry, _given_workspace, on_device, stream_workspace
 
 NODES = 64  # of a tree: a mask has a bit for each
+
+_contiguous, _device = torch.Tensor.is_contiguous, torch.Tensor.get_device
+_size, _dtype = torch.Tensor.size, attrgetter("dtype")
 
 
 def tree_workspace_bytes(head_dim: int) -> int:
@@ -137,18 +141,20 @@ def commit_drafts(arenas: Sequence[tuple[torch.Tensor, ...]], tables: torch.Tens
     device = keys.device
     if len(arenas[0]) not in (2, 4) or any(len(a) != len(arenas[0]) for a in arenas):
         raise ValueError("a layer is (keys, values) or those and their scales")
-    # (One test for what is all right: with some dozens of stores the call waits for it.)
-    index, kind, shape = keys.get_device(), keys.dtype, keys.shape
-    forms = ((kind, shape),) * 2 + ((torch.float16, shape[:-1]),) * 2
-    stores = []
-    for arena in arenas:
-        for t, (dtype, size) in zip(arena, forms):
-            if (t.dtype is not dtype or t.shape != size or t.get_device() != index
-                    or index < 0 or not t.is_contiguous()):
-                name = ("keys", "values", "key_scales", "value_scales")[len(stores) % len(arena)]
+    # (One test of a kind of store in all layers at once: with some dozens of stores the
+    # call waits for this code.)
+    shape = keys.shape
+    for name, dtype, size, of_layers in zip(
+            ("keys", "values", "key_scales", "value_scales"),
+            (keys.dtype, keys.dtype, torch.float16, torch.float16),
+            (shape, shape, shape[:-1], shape[:-1]), zip(*arenas)):
+        if (not all(map(_contiguous, of_layers)) or set(map(_device, of_layers)) != {device.index}
+                or set(map(_dtype, of_layers)) != {dtype}
+                or list(map(_size, of_layers)) != [size] * len(arenas)):
+            for t in of_layers:
                 _check_arena(name, t, keys, dtype)
-                raise ValueError(f"{name} must have the first layer's shape")
-            stores.append(t.data_ptr())
+            raise ValueError(f"{name} must have the first layer's shape")
+    stores = array("Q", [t.data_ptr() for arena in arenas for t in arena])
     if len(set(stores)) < len(stores):
         raise ValueError("a store given twice: its rows would move twice")
     if tables.dim() != 2:
@@ -182,7 +188,7 @@ def commit_drafts(arenas: Sequence[tuple[torch.Tensor, ...]], tables: torch.Tens
                 raise ValueError(f"out.{name} must be contiguous {dtype} {list(shape)}")
     with on_device(device):
         rc = _lib.library().pda_commit_drafts(
-            (ctypes.c_void_p * len(stores))(*stores), len(arenas), len(arenas[0]),
+            stores.buffer_info()[0], len(arenas), len(arenas[0]),
             head_dim * keys.element_size(), tables.data_ptr(), lengths.data_ptr(),
             starts.data_ptr(), parents.data_ptr(), drafted.data_ptr(), targets.data_ptr(),
             drafted.element_size(), out.lengths.data_ptr(), out.accepted.data_ptr(),

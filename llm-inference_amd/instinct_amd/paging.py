@@ -14,6 +14,7 @@ The work happens in libpda.so (``csrc/pda_paging.hip``).
 
 from __future__ import annotations
 
+from operator import attrgetter
 from typing import TYPE_CHECKING, NamedTuple
 
 import numpy as np
@@ -25,6 +26,9 @@ from .hip_kernels import on_device
 
 if TYPE_CHECKING:
     from .paged_kv import KVCache
+
+_contiguous, _device = torch.Tensor.is_contiguous, torch.Tensor.get_device
+_dtype = attrgetter("dtype")
 
 
 class PageFeed:
@@ -102,13 +106,18 @@ def extend_tables(tables: torch.Tensor, lengths: torch.Tensor, counts: torch.Ten
     if tables.dtype != torch.int32 or tables.dim() != 2 or not tables.is_contiguous():
         raise ValueError("tables must be contiguous int32 [batch, width]")
     batch, width = tables.shape
-    for name, t, n in (("lengths", lengths, batch), ("counts", counts, batch),
-                       ("pages", pages, batch), ("feed", feed, None), ("drawn", drawn, 2)):
-        # (One test for what is all right: small steps wait for this code.)
-        if (t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous()
-                or t.device != device or (n is not None and t.shape[0] != n)):
-            _check_index(name, t, (t.shape[0] if n is None and t.dim() else n,), device)
-            raise ValueError(f"{name} must be contiguous")
+    given = (lengths, counts, pages, feed, drawn)
+    # (One test for what is all right: small steps wait for this code.)
+    if (not all(map(_contiguous, given)) or set(map(_dtype, given)) != {torch.int32}
+            or set(map(_device, given)) != {device.index} or feed.dim() != 1
+            or not lengths.shape == counts.shape == pages.shape == (batch,)
+            or drawn.shape != (2,)):
+        for name, t, n in (("lengths", lengths, batch), ("counts", counts, batch),
+                           ("pages", pages, batch), ("feed", feed, None), ("drawn", drawn, 2)):
+            if t.dim() != 1:
+                raise ValueError(f"{name} must have one dimension")
+            if not _check_index(name, t, (t.shape[0] if n is None else n,), device) is t:
+                raise ValueError(f"{name} must be contiguous")
     if tokens < 0:
         raise ValueError("tokens must not be negative")
     if parents is not None:
