@@ -34,13 +34,68 @@ using namespace pda_tree;
 
 // Joins the pieces of the unit that is cut and ends in a workgroup's range: with M the
 // largest of their maxima, the outputs are sum 2^(m - M) o / sum 2^(m - M) l. A wave
-// takes 32 rows and a quarter of their dims, the lanes as in the kernel that left them.
-template <int D, bool BF>
-__global__ __launch_bounds__(kThreads) void tree_join_kernel(const TreeParams p) {
+// takes 32 rows, a quarter of their dims and every PHASES-th piece, the lanes as in the
+// kernel that left them; the waves' sums meet in LDS, in a fixed order.
+//
+// PHASES 1: a workgroup for each of the ranges, whether a cut unit ends there or not. 4:
+// where a few units have many pieces each, a workgroup for each unit, which looks for its
+// cut among the ranges' (one sequence of 40000 rows, 28/4 heads of 128, 78 pieces a unit:
+// 67 -> 48 us a call; 16 pieces a unit in ranges without one: 22 -> 31 us the join).
+constexpr int kManyPhases = 4;
+
+// (m, sum, outputs) of some pieces plus those of others.
+template <int N>
+struct Joined {
+  float top, sum;
+  float4 o[N];
+  __device__ __forceinline__ void clear() {
+    top = -INFINITY;
+    sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
+  // (Pieces of which the row sees nothing hold zeros; one of NaN is not empty.)
+  __device__ __forceinline__ void add(float m, float l, const float4 (&x)[N]) {
+    if (m == -INFINITY && l == 0.0f) return;
+    const float now = fmaxf(top, m);
+    const float f = sum == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(top - now);
+    const float g = __builtin_amdgcn_exp2f(m - now);
+    top = now;
+    sum = fmaf(sum, f, l * g);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      o[i].x = fmaf(o[i].x, f, x[i].x * g);
+      o[i].y = fmaf(o[i].y, f, x[i].y * g);
+      o[i].z = fmaf(o[i].z, f, x[i].z * g);
+      o[i].w = fmaf(o[i].w, f, x[i].w * g);
+    }
+  }
+};
+
+template <int D, bool BF, int PHASES>
+__global__ __launch_bounds__(256 * PHASES) void tree_join_kernel(const TreeParams p) {
   constexpr int kShare = D / 8 / 4;  // groups of 8 dims a wave takes
-  constexpr int kAtOnce = 4;         // pieces loaded together
-  const int g = blockIdx.x, w = blockIdx.y, waves = gridDim.y;
-  const int lane = threadIdx.x & 63, part = threadIdx.x >> 6;
+  constexpr int kAtOnce = kShare <= 4 ? 4 : 2;  // pieces loaded together
+  const int w = blockIdx.y, waves = gridDim.y;
+  const int lane = threadIdx.x & 63, part = (threadIdx.x >> 6) & 3, phase = threadIdx.x >> 8;
+  int g = blockIdx.x;
+  if constexpr (PHASES > 1) {
+    // The range in which the blockIdx.x-th of the cut units ends.
+    static_assert(256 * PHASES >= groups_for(128, 4), "a thread for each range");
+    __shared__ int s_before[4 * PHASES], s_found;
+    const int wave = threadIdx.x >> 6;
+    const bool mine = (int)threadIdx.x < p.groups && p.cuts[threadIdx.x].rows > 0;
+    const uint64_t all = __ballot(mine);
+    if (lane == 0) s_before[wave] = __popcll(all);
+    if (threadIdx.x == 0) s_found = -1;
+    __syncthreads();
+    int at = __popcll(all & ((1ull << lane) - 1));
+    for (int i = 0; i < wave; ++i) at += s_before[i];
+    if (mine && at == (int)blockIdx.x) s_found = threadIdx.x;
+    __syncthreads();
+    g = s_found;
+    if (g < 0) return;
+  }
   const Cut cut = p.cuts[g];
   if (cut.rows <= 32 * w) return;
   // Its pieces: the first, then those of the workgroups up to this one.
@@ -48,74 +103,70 @@ __global__ __launch_bounds__(kThreads) void tree_join_kernel(const TreeParams p)
   auto piece = [&](int i) {
     return (int64_t)(i == 0 ? cut.piece : 2 * (cut.group + i - 1)) * waves + w;
   };
-  float top = -INFINITY;
-  float4 acc[kShare];
-#pragma unroll
-  for (int i = 0; i < kShare; ++i) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  float sum = 0.0f;
-  for (int i0 = 0; i0 < count; i0 += kAtOnce) {
+  Joined<kShare> all;
+  all.clear();
+  for (int i0 = phase; i0 < count; i0 += PHASES * kAtOnce) {
     float2 ml[kAtOnce];
     float4 o[kAtOnce][kShare];
 #pragma unroll
     for (int j = 0; j < kAtOnce; ++j) {
-      const int64_t at = piece(min(i0 + j, count - 1));
+      const int64_t at = piece(min(i0 + PHASES * j, count - 1));
       ml[j] = p.part_ml[at * 32 + (lane & 31)];
       const float4* src = reinterpret_cast<const float4*>(p.part_o) + at * (D / 8 * 64) +
                           part * kShare * 64 + lane;
 #pragma unroll
       for (int i = 0; i < kShare; ++i) o[j][i] = src[64 * i];
     }
-    float now = top;
 #pragma unroll
-    for (int j = 0; j < kAtOnce; ++j) now = fmaxf(now, ml[j].x);
-    const float f0 = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - now);
-    top = now;
-    // (Before any key was seen sums and outputs are zeros, or NaN where a piece was.)
-    if (f0 != 0.0f || sum == 0.0f) {
-      sum *= f0;
+    for (int j = 0; j < kAtOnce; ++j)
+      if (i0 + PHASES * j < count) all.add(ml[j].x, ml[j].y, o[j]);
+  }
+  if constexpr (PHASES > 1) {
+    __shared__ float s_join[PHASES - 1][4][kShare * 4 + 2][64];
+    if (phase > 0) {
+      float (&to)[kShare * 4 + 2][64] = s_join[phase - 1][part];
+      to[0][lane] = all.top;
+      to[1][lane] = all.sum;
 #pragma unroll
       for (int i = 0; i < kShare; ++i) {
-        acc[i].x *= f0;
-        acc[i].y *= f0;
-        acc[i].z *= f0;
-        acc[i].w *= f0;
+        to[2 + 4 * i][lane] = all.o[i].x;
+        to[3 + 4 * i][lane] = all.o[i].y;
+        to[4 + 4 * i][lane] = all.o[i].z;
+        to[5 + 4 * i][lane] = all.o[i].w;
       }
     }
+    __syncthreads();
+    if (phase > 0) return;
+    for (int f = 1; f < min(PHASES, count); ++f) {
+      const float (&from)[kShare * 4 + 2][64] = s_join[f - 1][part];
+      float4 o[kShare];
 #pragma unroll
-    for (int j = 0; j < kAtOnce; ++j) {
-      // (A piece of which the row sees nothing holds zeros. One of NaN is not empty.)
-      const bool empty = i0 + j >= count || (ml[j].x == -INFINITY && ml[j].y == 0.0f);
-      const float f = empty ? 0.0f : __builtin_amdgcn_exp2f(ml[j].x - top);
-#pragma unroll
-      for (int i = 0; i < kShare; ++i) {
-        acc[i].x = fmaf(empty ? 0.0f : o[j][i].x, f, acc[i].x);
-        acc[i].y = fmaf(empty ? 0.0f : o[j][i].y, f, acc[i].y);
-        acc[i].z = fmaf(empty ? 0.0f : o[j][i].z, f, acc[i].z);
-        acc[i].w = fmaf(empty ? 0.0f : o[j][i].w, f, acc[i].w);
-      }
-      sum = empty ? sum : fmaf(ml[j].y, f, sum);
+      for (int i = 0; i < kShare; ++i)
+        o[i] = make_float4(from[2 + 4 * i][lane], from[3 + 4 * i][lane], from[4 + 4 * i][lane],
+                           from[5 + 4 * i][lane]);
+      all.add(from[0][lane], from[1][lane], o);
     }
   }
   const int r = 32 * w + (lane & 31);
   if (r >= cut.rows) return;
   const int G = p.hq / p.hkv, row = cut.first + r;
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const float inv = all.sum == 0.0f ? 0.0f : 1.0f / all.sum;
   f16* dst = p.out + ((int64_t)(cut.token + row / G) * p.hq + cut.kvh * G + row % G) * p.dim;
 #pragma unroll
   for (int i = 0; i < kShare; ++i) {
     const int d = 8 * (part * kShare + i) + 4 * (lane >> 5);
-    const f16x4 y = {round16<BF>(acc[i].x * inv), round16<BF>(acc[i].y * inv),
-                     round16<BF>(acc[i].z * inv), round16<BF>(acc[i].w * inv)};
+    const f16x4 y = {round16<BF>(all.o[i].x * inv), round16<BF>(all.o[i].y * inv),
+                     round16<BF>(all.o[i].z * inv), round16<BF>(all.o[i].w * inv)};
     if (d < p.dim) *reinterpret_cast<f16x4*>(dst + d) = y;
   }
 }
 
-template <bool BF>
+template <bool BF, int PHASES>
 const void* tree_join_for(int width) {
-  return width == 64    ? reinterpret_cast<const void*>(tree_join_kernel<64, BF>)
-         : width == 96  ? reinterpret_cast<const void*>(tree_join_kernel<96, BF>)
-         : width == 128 ? reinterpret_cast<const void*>(tree_join_kernel<128, BF>)
-                        : reinterpret_cast<const void*>(tree_join_kernel<256, BF>);
+  return width == 64    ? reinterpret_cast<const void*>(tree_join_kernel<64, BF, PHASES>)
+         : width == 96  ? reinterpret_cast<const void*>(tree_join_kernel<96, BF, PHASES>)
+         : width == 128 ? reinterpret_cast<const void*>(tree_join_kernel<128, BF, PHASES>)
+                        : reinterpret_cast<const void*>(tree_join_kernel<256, BF, PHASES>);
 }
 
 // Pieces' outputs, (max, sum) pairs and the cuts: 2 pieces a workgroup, of 32 rows a
@@ -224,8 +275,16 @@ int tree_attention(const void* queries, const void* keys, const void* values,
   if (err != hipSuccess)
     return fail(PDA_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(err));
   if (batch == 0) return ok();
-  err = hipLaunchKernel(bf16_elems ? tree_join_for<true>(width) : tree_join_for<false>(width),
-                        dim3(prm.groups, waves), dim3(kThreads), args, 0, hs);
+  // (As many units as there may be, each of some groups / units pieces.)
+  const int64_t units =
+      ((int64_t)tokens * G + (int64_t)(prm.rows - 1) * batch) / prm.rows * kv_heads;
+  const bool many = 8 * units < prm.groups;
+  const void* join = many ? (bf16_elems ? tree_join_for<true, kManyPhases>(width)
+                                        : tree_join_for<false, kManyPhases>(width))
+                          : (bf16_elems ? tree_join_for<true, 1>(width)
+                                        : tree_join_for<false, 1>(width));
+  err = hipLaunchKernel(join, dim3(many ? (unsigned)units : (unsigned)prm.groups, waves),
+                        dim3(many ? 256 * kManyPhases : 256), args, 0, hs);
   if (err != hipSuccess)
     return fail(PDA_ERR_HIP, "join launch failed: %s", hipGetErrorString(err));
   return ok();

@@ -17,13 +17,14 @@ using namespace pda_rows;
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kThreads = 256;  // of a workgroup of four waves, and of the join's
+constexpr int kThreads = 256;  // of a workgroup of four waves
 constexpr int kNodes = 64;     // of a tree
 constexpr int kCus = 256;
 // Workgroups: as many as the GPU holds at once.
 constexpr int groups_for(int width, int waves) { return width <= 128 && waves == 4 ? 2 * kCus : kCus; }
-// Tiles that a range has at least.
-constexpr int kLeastTiles = 2;
+// A unit of n tiles in ranges of r takes about r tiles' time and then n / r pieces', of
+// some kPieceCost tile times each, to join: least at r = sqrt(kPieceCost n).
+constexpr float kPieceCost = 0.2f;
 
 // What the join has to know of a unit that ends in a workgroup's range and began in
 // an earlier one.
@@ -94,9 +95,14 @@ __device__ __forceinline__ int64_t tiles_of(const TreeParams& p, const Seq& s) {
   return (int64_t)s.nt * s.blocks * p.hkv;
 }
 
-// Workgroups that take ranges of a stream of `tiles`, and the first tile of one's.
-__device__ __forceinline__ int64_t ranges(const TreeParams& p, int64_t tiles) {
-  return min((tiles + kLeastTiles - 1) / kLeastTiles, (int64_t)p.groups);
+// Workgroups that take ranges of a stream of `tiles` in `units`, and the first tile of
+// one's.
+__device__ __forceinline__ int64_t ranges(const TreeParams& p, int64_t tiles, int64_t units) {
+  const int64_t least = max(1, (int)sqrtf(kPieceCost * ((float)tiles / (float)max(units, (int64_t)1))));
+  const int64_t n = min((tiles + least - 1) / least, (int64_t)p.groups);
+  // (One workgroup a CU rather than a second one on some: 4 sequences of 1000-2000 rows,
+  // 32/8 heads of 128, 384 ranges 35 us a call, 256 30.)
+  return n > kCus && n < p.groups ? (int64_t)kCus : n;
 }
 __device__ __forceinline__ int64_t range_begin(int64_t tiles, int64_t n, int64_t g) {
   return tiles * g / n;
@@ -113,17 +119,22 @@ __device__ __forceinline__ Range range_of(const TreeParams& p) {
   const int lane = threadIdx.x & 63;
   const int per = (p.batch + 63) / 64;
   const int b0 = min(lane * per, p.batch), b1 = min(b0 + per, p.batch);
-  int64_t mine = 0;
-  for (int b = b0; b < b1; ++b) mine += tiles_of(p, seq_of(p, b));
+  int64_t mine = 0, units = 0;
+  for (int b = b0; b < b1; ++b) {
+    const Seq s = seq_of(p, b);
+    mine += tiles_of(p, s);
+    units += s.nt > 0 ? (int64_t)s.blocks * p.hkv : 0;
+  }
   int64_t upto = mine;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
     const int64_t y = __shfl_up(upto, d);
     if (lane >= d) upto += y;
+    units += __shfl_xor(units, d);
   }
   Range r;
   r.all = uniform64(__shfl(upto, 63));
-  r.n = ranges(p, r.all);
+  r.n = uniform64(ranges(p, r.all, uniform64(units)));
   if (blockIdx.x >= r.n) {
     r.begin = r.end = r.rest = 0;
     r.seq = 0;
@@ -357,8 +368,8 @@ struct TreeTiles {
     usable = (uint64_t)uniform64((int64_t)*reinterpret_cast<const uint64_t*>(s_ok + 4 * (t & 3)));
   }
 
+  // (Tile t was looked up, beside the loads of the piece's rows.)
   __device__ __forceinline__ void first(int t) {
-    lookup(t);
     turn();
     lookup(t + 1);
     if (moves_k()) {
@@ -506,6 +517,7 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void tree_attention_kerne
       x.held = s.held;
       x.last = s.held + min(s.n, kNodes) - 1;
       x.table = p.tables + (int64_t)seq * p.stride;
+      x.lookup(ta);
       // This lane's row: a node and a query head. (Rows past the last see what that
       // one sees, and are not stored.)
       const int row = 32 * W * (unit - x.kvh * s.blocks) + 32 * w + (lane & 31);
