@@ -368,8 +368,8 @@ struct TreeTiles {
     usable = (uint64_t)uniform64((int64_t)*reinterpret_cast<const uint64_t*>(s_ok + 4 * (t & 3)));
   }
 
-  // (Tile t was looked up, beside the loads of the piece's rows.)
   __device__ __forceinline__ void first(int t) {
+    lookup(t);
     turn();
     lookup(t + 1);
     if (moves_k()) {
@@ -517,7 +517,6 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void tree_attention_kerne
       x.held = s.held;
       x.last = s.held + min(s.n, kNodes) - 1;
       x.table = p.tables + (int64_t)seq * p.stride;
-      x.lookup(ta);
       // This lane's row: a node and a query head. (Rows past the last see what that
       // one sees, and are not stored.)
       const int row = 32 * W * (unit - x.kvh * s.blocks) + 32 * w + (lane & 31);
