@@ -7,6 +7,15 @@
 // prompt, whose keys and values lie beside the queries (slices of one projection's
 // output, read where they are): flops 4 D per (query head, query, key), every
 // operand read once.
+//
+// Bound by the matrix cores from a few hundred tokens on, as far as the exponentials
+// beside them let it: 16384 tokens, 28/4 heads of 128, bf16, 1.78 ms, 1.08 PFLOP/s (a
+// large bf16 matrix product of this GPU: 1.38), matrix cores 50% busy, VALU 42%, 5.7 VALU
+// instructions a product. Short prompts pay for their ends: an item of one tile of keys
+// takes as long as five tiles more (16 prompts of 128-2048: 236 us, 728 TFLOP/s), which
+// is why workgroups stay and load the next item's first keys and queries beside the end
+// of the one at hand (a workgroup an item: 285 us; heads of 256, window 1024, one
+// workgroup a CU: 280 and 248).
 
 #include <hip/hip_runtime.h>
 
@@ -389,7 +398,8 @@ struct PromptTiles {
   }
 };
 
-// Workgroups of four waves (kGroups a CU) that take item after item.
+// Workgroups of four waves that take item after item, as many as a CU holds: at D = 64
+// three (4 prompts of 3000 tokens, 14/2 heads: 105 us with two, 100 with three).
 template <int D>
 constexpr int groups_a_cu() { return D == 64 ? 3 : D <= 128 ? 2 : 1; }
 

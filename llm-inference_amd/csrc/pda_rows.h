@@ -15,7 +15,8 @@
 //
 // LDS: planes of 64 bytes a key (32 dims), 64 keys a plane. V as it lies, for the
 // transposing reads; K with the four 16-byte chunks of a key's plane permuted by
-// (key / 4) % 4, so that the 16 lanes of a read touch each bank once.
+// (key / 4) % 4, so that the 16 lanes of a read touch each bank once (no bank conflicts in
+// the counters).
 #ifndef PDA_ROWS_H
 #define PDA_ROWS_H
 
