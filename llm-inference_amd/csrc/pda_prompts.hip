@@ -10,7 +10,7 @@
 //
 // Bound by the matrix cores from a few hundred tokens on, as far as the exponentials
 // beside them let it: 16384 tokens, 28/4 heads of 128, bf16, 1.78 ms, 1.08 PFLOP/s (a
-// large bf16 matrix product of this GPU: 1.38), matrix cores 50% busy, VALU 42%, 5.7 VALU
+// large bf16 matrix product of this GPU: 1.38), matrix cores 55% busy, VALU 46%, 5.7 VALU
 // instructions a product. Short prompts pay for their ends: an item of one tile of keys
 // takes as long as five tiles more (16 prompts of 128-2048: 236 us, 728 TFLOP/s), which
 // is why workgroups stay and load the next item's first keys and queries beside the end
