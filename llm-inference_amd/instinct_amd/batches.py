@@ -286,6 +286,12 @@ class _ManyTokens:
                 b = int(np.argmax(short))
                 raise ValueError(f"group {name!r}: no page for row {held[name][b] + counts[b] - 1} "
                                  f"of sequence {b}")
+            for b in np.flatnonzero(counts):
+                first = int(held[name][b]) // page
+                new = np.asarray(tables[name][b])[first:-(-int(held[name][b] + counts[b]) // page)]
+                if np.any(new < 0):
+                    row = max(int(held[name][b]), (first + int(np.argmax(new < 0))) * page)
+                    raise ValueError(f"group {name!r}: no page for row {row} of sequence {b}")
         put = lambda a: torch.as_tensor(np.asarray(a).astype(np.int32), device=device)  # noqa: E731
         self._tables: dict[str, torch.Tensor] = {}
         self._held: dict[str, torch.Tensor] = {}

@@ -39,6 +39,20 @@ def test_draft_refuses(kw, match):
         batches.DraftBatch(cache(window=8), TOKENS, **dict(base, **kw))
 
 
+def test_new_rows_on_released_pages():
+    released = [np.array([-1, 2, 3]), np.array([4, -1])]
+    with pytest.raises(ValueError, match="'b': no page for row 0 of sequence 0"):
+        batches.PackedPrefillBatch(cache(), TOKENS, counts=[4, 2],
+                                   tables=dict(TABLES, b=released))
+    args = dict(counts=[4, 2], parents=[-1, 0, 1, 0, -1, 0])
+    tables = dict(a=[np.array([1, 2, 3]), np.array([4, 5])], b=released)
+    page = cache().page_size
+    with pytest.raises(ValueError, match=f"'b': no page for row {page} of sequence 1"):
+        batches.DraftBatch(cache(), TOKENS, positions=[page + 1, page - 1], tables=tables, **args)
+    with pytest.raises(ValueError, match=f"'b': no page for row {page + 2} of sequence 1"):
+        batches.DraftBatch(cache(), TOKENS, positions=[page + 1, page + 2], tables=tables, **args)
+
+
 def test_draft_of_more_than_64_nodes():
     with pytest.raises(ValueError, match="64 nodes"):
         batches.DraftBatch(cache(), torch.zeros(65, dtype=torch.int64), counts=[65],
