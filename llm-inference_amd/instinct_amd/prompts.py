@@ -52,6 +52,13 @@ def packed_prompt_attention(queries: torch.Tensor, keys: torch.Tensor, values: t
     q_token, q_head, q_one = queries.stride()
     k_token, k_head, k_one = keys.stride()
     v_token, v_head, v_one = values.stride()
+    # (A tensor's stride says nothing where its size is one.)
+    if tokens == 1:
+        q_token = k_token = v_token = 0
+    if q_heads == 1:
+        q_head = 0
+    if kv_heads == 1:
+        k_head = v_head = 0
     if head_dim > 1 and (q_one != 1 or k_one != 1 or v_one != 1):
         raise ValueError("the elements of a head must lie side by side")
     if starts.dim() != 1 or starts.shape[0] == 0:

@@ -85,6 +85,18 @@ def test_strides(gpu, heads):
     compare(got, q, one, one, starts, scale=0.1)
 
 
+def test_strides_of_dimensions_of_one(gpu):
+    """What a tensor's stride says of one token or one head does not matter."""
+    q, k, v, starts, dev = make(12, [70], 1, 1, 64, F16, fused=False)
+    odd = lambda t: t.as_strided(t.shape, (64, 3, 1))  # noqa: E731
+    got = prompts.packed_prompt_attention(odd(q), odd(k), odd(v), dev, scale=0.1)
+    compare(got, q, k, v, starts, scale=0.1)
+    q, k, v, starts, dev = make(13, [1], 4, 2, 64, F16, fused=False)
+    odd = lambda t: t.as_strided(t.shape, (5, 64, 1))  # noqa: E731
+    got = prompts.packed_prompt_attention(odd(q), odd(k), odd(v), dev, scale=0.1)
+    compare(got, q, k, v, starts, scale=0.1)
+
+
 def test_rows_behind_the_last_prompt_are_zeros(gpu):
     for behind in (1, 130, 300):
         q, k, v, starts, dev = make(5, [100, 60], 4, 2, 64, F16, behind=behind)
