@@ -32,14 +32,16 @@ _dtype = attrgetter("dtype")
 
 
 class PageFeed:
-    """Pages of a group's pool set aside for steps that take them on the GPU: ``pages``
-    and ``drawn`` are what :func:`extend_tables` takes. The pages that were drawn belong
+    """Pages of a group's pool set aside for steps that take them on the GPU.
+    :func:`extend_tables` takes the feed and moves it on: ``pages`` are its page ids and
+    ``drawn[0]`` how many of them were taken. The pages that were drawn belong
     to the sequences whose tables have them and go back with those
     (``PagePool.release``); :meth:`refill` and :meth:`close` read ``drawn`` (and wait
     for the GPU)."""
 
     def __init__(self, cache: "KVCache", group: str, count: int) -> None:
         self._cache, self._pool = cache, cache.pools[group]
+        self.page_size = cache.page_size
         self._ids = self._pool.allocate_many(count, reserved=False)
         self._put()
 
@@ -76,30 +78,42 @@ class StepRows(NamedTuple):
     starts: torch.Tensor     # [batch + 1] first token of each sequence, and the end
     lengths: torch.Tensor    # [batch] rows held with the step's tokens
     pages: torch.Tensor      # [batch] pages held
-    drawn: torch.Tensor      # [2] pages drawn from the feed, and 0
+    drawn: torch.Tensor      # [2] pages drawn from the feed, and 0 (a PageFeed's own)
     rows: torch.Tensor       # [tokens] arena row of each token
     positions: torch.Tensor  # [tokens]
     masks: torch.Tensor | None  # [tokens] int64, with parents
 
 
 def extend_tables(tables: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor,
-                  pages: torch.Tensor, feed: torch.Tensor, drawn: torch.Tensor, *,
-                  page_size: int, tokens: int, parents: torch.Tensor | None = None,
-                  out: StepRows | None = None) -> StepRows:
+                  pages: torch.Tensor, feed: PageFeed | torch.Tensor,
+                  drawn: torch.Tensor | None = None, *, page_size: int, tokens: int,
+                  parents: torch.Tensor | None = None, out: StepRows | None = None) -> StepRows:
     """Lengthen the page tables ``[batch, width]`` (in place) for a step that brings
     ``counts[b]`` tokens to a sequence that holds ``lengths[b]`` rows on ``pages[b]``
-    pages, taking what is missing from ``feed`` (page ids) from entry ``drawn[0]`` on,
-    in the order of the sequences; and the step's slot map (:class:`StepRows`).
+    pages, taking what is missing from ``feed`` in the order of the sequences; and the
+    step's slot map (:class:`StepRows`). A :class:`PageFeed` moves on by itself: the next
+    step goes on behind the pages that this one took. Of a tensor of page ids the call
+    takes those from entry ``drawn[0]`` on (int32 ``[2]``, zeros for a new one), which
+    stays as it is: the next step's is the result's ``drawn``, or both take the same pages.
 
     ``tokens``: entries of the per-token results, at least ``counts.sum()``; those
     behind the last token have row -1 (the append writes nothing there), position 0
     and mask 0. ``parents`` (int32 ``[tokens]``): each sequence's tokens are a tree of
     up to 64 nodes and ``parents`` names each node's parent among them (-1: none); a
     node's position then goes by its depth and its mask has the bits of its ancestors
-    and its own. ``drawn`` is int32 ``[2]``, zeros for a new feed. A feed that runs
-    out leaves -1 as page and row and ``drawn`` past its end. All are int32 on one
-    GPU; ``out`` may hold ``lengths``, ``pages`` and ``drawn`` themselves (a step
-    replayed from a graph). No counterpart in the reference."""
+    and its own. A feed that runs out leaves -1 as page and row and ``drawn`` past its
+    end. All are int32 on one GPU; ``out`` may hold ``lengths``, ``pages`` and ``drawn``
+    themselves (a step replayed from a graph; of a :class:`PageFeed` it has ``drawn``). No
+    counterpart in the reference."""
+    own = feed if isinstance(feed, PageFeed) else None
+    if own is not None:
+        if drawn is not None:
+            raise TypeError("a PageFeed counts for itself what was drawn")
+        if page_size != own.page_size:
+            raise ValueError(f"the feed's pages hold {own.page_size} rows")
+        feed, drawn = own.pages, own.drawn
+    elif drawn is None:
+        raise TypeError("drawn goes with a feed of page ids")
     if not tables.is_cuda:
         raise ValueError("tables must be on a GPU")
     device = tables.device
@@ -129,7 +143,11 @@ def extend_tables(tables: torch.Tensor, lengths: torch.Tensor, counts: torch.Ten
         masks = (None if parents is None
                  else torch.empty(tokens, dtype=torch.int64, device=device))
         out = StepRows(*parts, masks)
+        if own is not None:
+            out = out._replace(drawn=drawn)
     else:
+        if own is not None and out.drawn is not drawn:
+            raise ValueError("out.drawn must be the feed's: the next step goes by it")
         for name, t, n in zip(StepRows._fields, out, (batch + 1, batch, batch, 2, tokens, tokens,
                                                       tokens)):
             if t is None and name == "masks" and parents is None:
