@@ -37,18 +37,28 @@ class PageFeed:
     ``drawn[0]`` how many of them were taken. The pages that were drawn belong
     to the sequences whose tables have them and go back with those
     (``PagePool.release``); :meth:`refill` and :meth:`close` read ``drawn`` (and wait
-    for the GPU)."""
+    for the GPU). A step captured into a graph draws on the feed as it is at each replay,
+    refilled or closed, up to as many pages as the feed had room for at the capture."""
 
     def __init__(self, cache: "KVCache", group: str, count: int) -> None:
         self._cache, self._pool = cache, cache.pools[group]
         self.page_size = cache.page_size
         self._ids = self._pool.allocate_many(count, reserved=False)
+        self._make_room()
         self._put()
 
-    def _put(self) -> None:
+    def _make_room(self) -> None:
         device = self._cache.device
-        self.pages = torch.as_tensor(self._ids.astype(np.int32), device=device)
-        self.drawn = torch.zeros(2, dtype=torch.int32, device=device)
+        self._room = torch.empty(len(self._ids), dtype=torch.int32, device=device)
+        self.drawn = torch.empty(2, dtype=torch.int32, device=device)
+
+    def _put(self) -> None:
+        # (In place: steps that were captured read these tensors.)
+        ids = np.full(len(self._room), -1, dtype=np.int32)
+        ids[:len(self._ids)] = self._ids
+        self._room.copy_(torch.from_numpy(ids))
+        self.pages = self._room[:len(self._ids)]
+        self.drawn.zero_()
 
     def _left(self) -> np.ndarray:
         drawn = int(self.drawn[0])
@@ -58,10 +68,14 @@ class PageFeed:
         return self._ids[drawn:]
 
     def refill(self, count: int) -> None:
-        """``count`` pages to draw again, in new tensors."""
+        """``count`` pages to draw again. Past the most that the feed held so far it takes
+        new tensors, and a step that was captured before finds no page (row -1)."""
         left = self._left()
         more = max(0, count - len(left))
         self._ids = np.concatenate([left, self._pool.allocate_many(more, reserved=False)])
+        if len(self._ids) > len(self._room):
+            self._room.fill_(-1)
+            self._make_room()
         self._put()
 
     def close(self) -> None:
@@ -111,7 +125,8 @@ def extend_tables(tables: torch.Tensor, lengths: torch.Tensor, counts: torch.Ten
             raise TypeError("a PageFeed counts for itself what was drawn")
         if page_size != own.page_size:
             raise ValueError(f"the feed's pages hold {own.page_size} rows")
-        feed, drawn = own.pages, own.drawn
+        # (All of its room: a refilled feed's pages are there for a captured step.)
+        feed, drawn = own._room, own.drawn
     elif drawn is None:
         raise TypeError("drawn goes with a feed of page ids")
     if not tables.is_cuda:

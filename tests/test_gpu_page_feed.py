@@ -102,3 +102,39 @@ def test_out_has_the_feeds_count(gpu):
         extend_tables(*args, page_size=P, tokens=3, out=out)
     got = extend_tables(*args, page_size=P, tokens=3, out=out._replace(drawn=feed.drawn))
     assert got.drawn is feed.drawn and feed.drawn.tolist() == [1, 0]
+
+
+def test_a_captured_step_goes_on_after_a_refill(gpu):
+    """A graph that was captured when the feed held few pages draws what refills bring,
+    each page once, and nothing from a closed feed."""
+    cache, batch = make(256), 5
+    pool = cache.pools["main"]
+    feed = PageFeed(cache, "main", 12)
+    feed.refill(12)
+    feed.drawn[0] = 9
+    taken = feed.pages[:9].tolist()
+    feed.refill(4)  # (less than its room at the capture)
+    tables, counts = torch.zeros((batch, 40), **I32), torch.tensor([7, 16, 0, 1, 20], **I32)
+    new = lambda n: torch.zeros(n, **I32)  # noqa: E731
+    tokens = int(counts.sum())
+    out = StepRows(new(batch + 1), new(batch), new(batch), feed.drawn, new(tokens), new(tokens), None)
+    step = lambda: extend_tables(tables, out.lengths, counts, out.pages, feed,  # noqa: E731
+                                 page_size=P, tokens=tokens, out=out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for turn in range(10):
+        feed.refill(12 if turn % 3 else 5)
+        graph.replay()
+        torch.zeros(1000, device="cuda").sum()  # eager work between the replays
+        used = in_tables(tables, out.pages)
+        assert min(used) >= 0 and len(set(used + taken)) == len(used) + len(taken)
+        assert int(out.rows.min()) >= 0
+        assert pool.used == len(taken) + len(used) + len(feed._ids) - int(feed.drawn[0])
+    assert len(used) > 25
+    feed.close()
+    assert pool.used == len(taken) + len(used)
+    for _ in range(3):
+        graph.replay()
+    after = in_tables(tables, out.pages)
+    assert set(after) == set(used) | {-1}
