@@ -37,7 +37,7 @@ class PageFeed:
     ``drawn[0]`` how many of them were taken. The pages that were drawn belong
     to the sequences whose tables have them and go back with those
     (``PagePool.release``); :meth:`refill` and :meth:`close` read ``drawn`` (and wait
-    for the GPU). A step captured into a graph draws on the feed as it is at each replay,
+    for the GPU, whatever streams the steps run on). A step captured into a graph draws on the feed as it is at each replay,
     refilled or closed, up to as many pages as the feed had room for at the capture."""
 
     def __init__(self, cache: "KVCache", group: str, count: int) -> None:
@@ -59,8 +59,14 @@ class PageFeed:
         self._room.copy_(torch.from_numpy(ids))
         self.pages = self._room[:len(self._ids)]
         self.drawn.zero_()
+        self._wait()
+
+    def _wait(self) -> None:
+        if self.drawn.is_cuda:
+            torch.cuda.synchronize(self.drawn.device)
 
     def _left(self) -> np.ndarray:
+        self._wait()
         drawn = int(self.drawn[0])
         if drawn > len(self._ids):
             raise RuntimeError(f"steps asked for {drawn} pages of a feed of {len(self._ids)}: "

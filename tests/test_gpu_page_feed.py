@@ -138,3 +138,31 @@ def test_a_captured_step_goes_on_after_a_refill(gpu):
         graph.replay()
     after = in_tables(tables, out.pages)
     assert set(after) == set(used) | {-1}
+
+
+def test_steps_on_another_stream(gpu):
+    """refill and close wait for steps of any stream, and what they put is there for a step
+    that follows on one."""
+    cache = make()
+    pool = cache.pools["main"]
+    feed = PageFeed(cache, "main", 8)
+    tables, zero, counts = torch.zeros((2, 8), **I32), torch.zeros(2, **I32), torch.full((2,), 20, **I32)
+    slow = torch.ones((4096, 4096), device="cuda") / 4096
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+
+    def step():
+        with torch.cuda.stream(stream):
+            x = slow
+            for _ in range(60):  # some tens of milliseconds
+                x = slow @ x
+            return extend_tables(tables, zero, counts, zero, feed, page_size=P, tokens=40)
+
+    step()
+    feed.refill(8)
+    assert feed.pages.tolist() == list(range(4, 12))
+    step()
+    feed.close()
+    assert pool.used == 8
+    torch.cuda.synchronize()
+    assert in_tables(tables, torch.full((2,), 2, **I32)) == [4, 5, 6, 7]
