@@ -921,13 +921,14 @@ int pda_tree_attention_q8_bf16(const void* queries, const void* keys,
  *   accepted    [batch]: nodes kept (0 for a sequence without nodes)
  *   path        [batch, 64]: the kept nodes in order, then -1
  *   following   [batch]: the model's choice after the last kept node (-1: no node)
- *   out_lengths [batch]: lengths + accepted; not lengths itself
+ *   out_lengths [batch]: lengths + accepted
  * and in every store the kept nodes' rows move to the rows lengths[b] ..
  * lengths[b] + accepted[b] - 1 (rows of other nodes are left as they are).
  *   stores  HOST array [layers, stores_per_layer] of device pointers: keys, values
  *           and, with 4, their fp16 scales; one layout and shape for all, no two the
  *           same memory. `width`: bytes of a row of keys or values of one head
  *   drafted, targets [tokens], token_bytes 8 (int64) or 4 (int32)
+ * No result may overlap another or an input: workgroups of other stores still read those.
  * Nodes past a tree's 64th are never kept. A row whose page is not in the arena (or
  * past the table) does not move. The pages of a tree's rows belong to one sequence.
  * One launch on `stream` for 48 layers, no workspace. */

@@ -29,6 +29,8 @@ namespace {
 
 using pda_internal::fail;
 using pda_internal::ok;
+using pda_internal::overlap;
+using pda_internal::Span;
 
 using namespace pda_tree;
 
@@ -499,6 +501,24 @@ int pda_commit_drafts(void* const* stores, int32_t layers, int32_t stores_per_la
     return fail(PDA_ERR_ALIGNMENT, "int32 buffers must be 4-byte aligned");
   if ((((uintptr_t)drafted | (uintptr_t)targets) & (token_bytes - 1)) || ((uintptr_t)following & 7))
     return fail(PDA_ERR_ALIGNMENT, "tokens must be aligned to their size");
+  // (The workgroups of other stores read the inputs while one writes the results.)
+  const Span in[] = {{"tables", tables, 4 * (int64_t)batch * table_stride},
+                     {"lengths", lengths, 4 * (int64_t)batch},
+                     {"starts", starts, 4 * ((int64_t)batch + 1)},
+                     {"parents", parents, 4 * (int64_t)tokens},
+                     {"drafted", drafted, (int64_t)token_bytes * tokens},
+                     {"targets", targets, (int64_t)token_bytes * tokens}};
+  const Span results[] = {{"out_lengths", out_lengths, 4 * (int64_t)batch},
+                          {"accepted", accepted, 4 * (int64_t)batch},
+                          {"path", path, 4 * (int64_t)kNodes * batch},
+                          {"following", following, 8 * (int64_t)batch}};
+  for (const Span& r : results) {
+    for (const Span& x : in)
+      if (overlap(r, x)) return fail(PDA_ERR_INVALID_ARGUMENT, "%s overlaps %s", r.name, x.name);
+    for (const Span& x : results)
+      if (&x != &r && overlap(r, x))
+        return fail(PDA_ERR_INVALID_ARGUMENT, "%s overlaps %s", r.name, x.name);
+  }
   const int64_t count = (int64_t)layers * stores_per_layer;
   for (int64_t i = 0; i < count; ++i)
     if (!stores[i]) return fail(PDA_ERR_INVALID_ARGUMENT, "null arena pointer");

@@ -17,6 +17,17 @@ __attribute__((visibility("hidden"))) int ok();
 // The thread's message.
 __attribute__((visibility("hidden"))) const char* last_error();
 
+// What a call reads or writes of a buffer.
+struct Span {
+  const char* name;
+  const void* at;
+  int64_t bytes;
+};
+inline bool overlap(const Span& a, const Span& b) {
+  const uintptr_t x = (uintptr_t)a.at, y = (uintptr_t)b.at;
+  return a.bytes > 0 && b.bytes > 0 && x < y + (uintptr_t)b.bytes && y < x + (uintptr_t)a.bytes;
+}
+
 // Four int8 values (one dword, each byte's sign bit already flipped:
 // b + 128) as one fp16 pair, exactly: v_perm places two bytes under the fp16
 // exponent byte 0x64, which reads as 1024 + b + 128; subtracting 1152 leaves

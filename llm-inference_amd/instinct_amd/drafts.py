@@ -133,7 +133,7 @@ def commit_drafts(arenas: Sequence[tuple[torch.Tensor, ...]], tables: torch.Tens
     values, key_scales, value_scales)``, all of one shape and layout. Rows of other
     nodes stay as they are, to be overwritten; pages are kept (the next
     ``extend_tables`` takes as many fewer). A tree's rows lie on pages that no other
-    sequence holds."""
+    sequence holds. ``out`` overlaps no input."""
     if not arenas:
         raise ValueError("no layers given")
     keys = arenas[0][0]
