@@ -817,7 +817,8 @@ int pda_evict_move(void* arena, void* arena2, int32_t width, const int32_t* kept
  * out_drawn counts on; tokens past the table's entries, or whose row passes 2^31,
  * have row -1 as well. Tokens past `tokens` are dropped. Entries of rows and
  * positions behind the last token are -1 and 0 (masks: 0). out_lengths, out_pages
- * and out_drawn may be lengths, pages and drawn themselves. batch <= 4096.
+ * and out_drawn may be lengths, pages and drawn themselves; else no result overlaps
+ * another or an input. batch <= 4096.
  * One launch on `stream`, no workspace; calls that share `drawn` must not overlap. */
 int pda_extend_tables(int32_t* tables, int32_t table_stride,
                       const int32_t* lengths, const int32_t* counts,

@@ -24,6 +24,8 @@ namespace {
 
 using pda_internal::fail;
 using pda_internal::ok;
+using pda_internal::overlap;
+using pda_internal::Span;
 
 constexpr int kThreads = 256;
 constexpr int kNodes = 64;             // of a tree at most
@@ -264,6 +266,31 @@ int pda_extend_tables(int32_t* tables, int32_t table_stride, const int32_t* leng
                         (uintptr_t)positions;
   if ((mis & 3) || ((uintptr_t)masks & 7))
     return fail(PDA_ERR_ALIGNMENT, "int32 buffers must be 4-byte aligned, masks 8-byte aligned");
+  // (Workgroups read the inputs, and the pages that the tables hold, while others write; what
+  // may be in place is written by the last one, entry by entry.)
+  const int64_t n = 4 * (int64_t)batch, t = 4 * (int64_t)tokens;
+  const Span in[] = {{"lengths", lengths, n}, {"counts", counts, n},
+                     {"pages", pages, n},     {"feed", feed, 4 * (int64_t)feed_len},
+                     {"drawn", drawn, 8},     {"parents", parents, parents ? t : 0}};
+  const struct {
+    Span of;
+    const void* in_place;
+  } results[] = {{{"tables", tables, n * table_stride}, nullptr},
+                 {{"starts", starts, n + 4}, nullptr},
+                 {{"out_lengths", out_lengths, n}, lengths},
+                 {{"out_pages", out_pages, n}, pages},
+                 {{"out_drawn", out_drawn, 8}, drawn},
+                 {{"rows", rows, t}, nullptr},
+                 {{"positions", positions, t}, nullptr},
+                 {{"masks", masks, parents ? 2 * t : 0}, nullptr}};
+  for (const auto& r : results) {
+    for (const Span& x : in)
+      if (overlap(r.of, x) && !(r.of.at == x.at && x.at == r.in_place))
+        return fail(PDA_ERR_INVALID_ARGUMENT, "%s overlaps %s", r.of.name, x.name);
+    for (const auto& x : results)
+      if (&x != &r && overlap(r.of, x.of))
+        return fail(PDA_ERR_INVALID_ARGUMENT, "%s overlaps %s", r.of.name, x.of.name);
+  }
   ExtendParams prm{tables,    lengths,     counts,    pages,     feed,   drawn,
                    parents,   starts,      out_lengths, out_pages, out_drawn, rows,
                    positions, masks,       tokens,    table_stride, feed_len, batch,
