@@ -382,6 +382,7 @@ class DraftBatch(_ManyTokens):
         if parents.shape != index.shape or np.any((parents < -1) | (parents >= index)):
             raise ValueError("a node's parent is an earlier node of its tree, or -1")
         self.cache, self.tokens, self.count = cache, tokens, int(tokens.shape[0])
+        self._moved: set[int] = set()  # layers committed since they were written
         rows = {} if held is None else rows_by_group(cache, held, counts.shape)
         for name, n in rows.items():
             if cache.groups[name].window and np.any(n != positions):
@@ -400,6 +401,7 @@ class DraftBatch(_ManyTokens):
         """Write the nodes' K/V behind the rows held, then attention over those and the
         nodes' ancestors, ``[tokens, q_heads * head_dim]``."""
         name = self._write(layer, k, v)
+        self._moved.discard(layer)
         cache = self.cache
         out = tree_attention(
             q.to(cache.decode_dtype).contiguous(), cache.keys[layer], cache.values[layer],
@@ -412,7 +414,11 @@ class DraftBatch(_ManyTokens):
         """Keep each tree's line of nodes that the model agrees with: ``targets`` is its
         choice after every node, of the tokens' type. Moves the kept rows in every
         layer; returns what was kept by group (the same but for ``lengths``, the rows
-        held now). The sequences' pages stay theirs."""
+        held now). The sequences' pages stay theirs. Rows that have moved do not move
+        again: a step is committed once, or once more when every layer was attended
+        again."""
+        if self._moved:
+            raise RuntimeError(f"the rows of layers {sorted(self._moved)} have moved already")
         done = {}
         for name, group in self.cache.groups.items():
             arenas = [(self.cache.keys[i], self.cache.values[i], *(self.cache.scales(i) or ()))
@@ -420,4 +426,5 @@ class DraftBatch(_ManyTokens):
             done[name] = commit_drafts(
                 arenas, self._tables[name], self._held[name], self.starts, self.parents,
                 self.tokens.to(self.cache.device), targets, page_size=self.cache.page_size)
+            self._moved.update(group.layers)
         return done
