@@ -276,6 +276,10 @@ class _ManyTokens:
                tables: dict[str, list[np.ndarray]], parents: torch.Tensor | None,
                tokens: int) -> None:
         device, page = cache.device, cache.page_size
+        for name, group in cache.groups.items():  # (before any layer's K/V are written)
+            if group.head_dim % 8 or group.head_dim > 256:
+                raise ValueError(f"group {name!r}: steps of many tokens a sequence serve head dims "
+                                 f"that are multiples of 8 up to 256, not {group.head_dim}")
         pages = {name: np.array([len(t) for t in tables[name]], dtype=np.int64)
                  for name in cache.groups}
         for name, have in pages.items():
@@ -315,6 +319,13 @@ class _ManyTokens:
         return rope(x.to(self.cache.dtype).contiguous(), self.offsets, dims, base=base,
                     freqs=freqs)
 
+    def _check_queries(self, layer: int, q: torch.Tensor) -> None:
+        group = self.cache.layer_group[layer]
+        if (q.dim() != 3 or q.shape[0] != self.count or q.shape[2] != group.head_dim
+                or q.shape[1] == 0 or q.shape[1] % group.kv_heads):
+            raise ValueError(f"q must be [{self.count}, a multiple of {group.kv_heads}, "
+                             f"{group.head_dim}], got {list(q.shape)}")
+
     def _write(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> str:
         group = self.cache.layer_group[layer]
         self.cache.write(layer, self._steps[group.name].rows, k, v)
@@ -347,6 +358,7 @@ class PackedPrefillBatch(_ManyTokens):
         """Write the prompts' K/V, then their attention. ``q`` ``[tokens, q_heads,
         head_dim]``, ``k`` and ``v`` ``[tokens, kv_heads, head_dim]``; slices of one
         projection are read where they are."""
+        self._check_queries(layer, q)
         self._write(layer, k, v)
         dtype = self.cache.dtype
         out = packed_prompt_attention(
@@ -400,6 +412,7 @@ class DraftBatch(_ManyTokens):
                scale: float, softcap: float = 0.0) -> torch.Tensor:
         """Write the nodes' K/V behind the rows held, then attention over those and the
         nodes' ancestors, ``[tokens, q_heads * head_dim]``."""
+        self._check_queries(layer, q)
         name = self._write(layer, k, v)
         self._moved.discard(layer)
         cache = self.cache
