@@ -8,10 +8,12 @@
 // v_mfma_f32_32x32x16: the scores of a product come out with a lane holding 16
 // keys of one row, which after the exponential are the second product's operand as
 // they lie (nothing moves between lanes). Weights are taken in the log2 domain
-// against a running maximum that moves only when a block's weights sum past 2^8
-// (so that 16-bit weights stay finite), and rounded to the element type, to
-// nearest; their sum is that of the rounded weights, in float32, as are the
-// outputs.
+// against a running reference that moves only when a block's weights sum past 2^8 times
+// the weight its maximum was given (so that 16-bit weights stay finite), and rounded to
+// the element type, to nearest; their sum is that of the rounded weights, in float32, as
+// are the outputs. In fp16 that weight is 2^7: the sums stay finite up to 2^15, and keys
+// down to 2^-31 of the maximum still count, of which a long sequence has many (at a
+// weight of 1, 40000 keys of 2^-25 lost a quarter of their share). bf16 has float32's range.
 //
 // LDS: planes of 64 bytes a key (32 dims), 64 keys a plane. V as it lies, for the
 // transposing reads; K with the four 16-byte chunks of a key's plane permuted by
@@ -42,7 +44,7 @@ typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
 
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr float kSlack = 8.0f;
+constexpr float kSlack = 8.0f;       // log2 of how far weights pass their maximum's
 constexpr int kKeys = 64;            // keys of a tile: two blocks of 32
 constexpr int kPlane = kKeys * 32;   // halves of a plane
 
@@ -178,9 +180,12 @@ __device__ __forceinline__ uint32_t below(int n) {
 // BF: queries, keys and outputs are bf16 (else fp16); VBF: values and weights are.
 template <int D, bool BF, bool VBF = BF>
 struct Rows {
+  static constexpr float kTop = VBF ? 0.0f : 7.0f;  // log2 of a maximum's weight
+  static constexpr float kMost = VBF ? 256.0f : 32768.0f;  // 2^(kTop + kSlack)
+
   f16x8 q[D / 16];
   f32x16 o[D / 32];
-  float m, l;  // running maximum (log2 units), sum of this lane's weights
+  float m, l;  // running reference (log2 units), sum of this lane's weights
   float c;     // what a shaped score is multiplied by
   int n, hh;
   int k_lane0, k_lane1, v_lane;
@@ -295,15 +300,15 @@ struct Rows {
     return total(w, 0.0f);
   }
 
-  // A block's weights w, summed in lb, were taken against the running maximum.
-  // Only where they sum past 2^8 (or no key was seen before: lb is infinite; or
+  // A block's weights w, summed in lb, were taken against the running reference.
+  // Only where they sum past kMost (or no key was seen before: lb is infinite; or
   // one is not a number) the maximum is taken and the block weighed again.
   __device__ __forceinline__ void settle(const f32x16& x, f16x8 (&w)[2], float lb) {
-    if (__ballot(!(lb <= 256.0f)) != 0) {
+    if (__ballot(!(lb <= kMost)) != 0) {
       float top = x[0];
 #pragma unroll
       for (int v = 1; v < 16; ++v) top = fmaxf(top, x[v]);
-      top = fmaxf(top, __shfl_xor(top, 32)) * c;
+      top = fmaxf(top, __shfl_xor(top, 32)) * c - kTop;
       if (top > m + kSlack) {
         if (m != -INFINITY) {
           const float f = __builtin_amdgcn_exp2f(m - top);
