@@ -9,9 +9,9 @@
 // operand read once.
 //
 // Bound by the matrix cores from a few hundred tokens on, as far as the exponentials
-// beside them let it: 16384 tokens, 28/4 heads of 128, bf16, 1.78 ms, 1.08 PFLOP/s (a
-// large bf16 matrix product of this GPU: 1.38), matrix cores 55% busy, VALU 46%, 5.7 VALU
-// instructions a product. Short prompts pay for their ends: an item of one tile of keys
+// beside them let it: 16384 tokens, 28/4 heads of 128, bf16, 1.79 to 1.86 ms by
+// the card, 1.04 to 1.07 PFLOP/s (a large bf16 matrix product: 1.38), matrix cores 55%
+// busy, VALU 46%, 5.7 VALU instructions a product. Short prompts pay for their ends: an item of one tile of keys
 // takes as long as five tiles more (16 prompts of 128-2048: 236 us, 728 TFLOP/s), which
 // is why workgroups stay and load the next item's first keys and queries beside the end
 // of the one at hand (a workgroup an item: 285 us; heads of 256, window 1024, one
