@@ -159,7 +159,8 @@ def attention_tolerance(out, size, values, keys_seen, dtype, dequantized=False):
     up to 256 products in float32, times log2 e, capped and exponentiated there: for
     unit-variance inputs |score| stays below 2^4 and its error below 260 * 2^-24 *
     2^4 < 2^-11.9, on both the weight and the sum: 2^-10.9 sum p |v|. fp16 weights
-    below 2^-14 of the largest have an absolute error of 2^-25 each."""
+    that are subnormal have an absolute error of at most 2^-25 of the largest each
+    (2^-32 where the largest has the weight 2^7)."""
     u = half_step(dtype)
     small = 0.0 if "bfloat16" in str(dtype) else keys_seen * 2.0 ** -25 * np.abs(values).max()
     return (u * (size + 2 * np.abs(out)) + (u * size if dequantized else 0.0)
