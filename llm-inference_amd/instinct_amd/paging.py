@@ -37,13 +37,15 @@ class PageFeed:
     ``drawn[0]`` how many of them were taken. The pages that were drawn belong
     to the sequences whose tables have them and go back with those
     (``PagePool.release``); :meth:`refill` and :meth:`close` read ``drawn`` (and wait
-    for the GPU, whatever streams the steps run on). A step captured into a graph draws on the feed as it is at each replay,
-    refilled or closed, up to as many pages as the feed had room for at the capture."""
+    for the GPU, whatever streams the steps run on). A step captured into a graph draws on
+    the feed as it is at each replay, refilled or closed, up to as many pages as the feed
+    had room for at the capture; the feed outlives the graph."""
 
     def __init__(self, cache: "KVCache", group: str, count: int) -> None:
         self._cache, self._pool = cache, cache.pools[group]
         self.page_size = cache.page_size
         self._ids = self._pool.allocate_many(count, reserved=False)
+        self._outgrown: list[tuple[torch.Tensor, torch.Tensor]] = []
         self._make_room()
         self._put()
 
@@ -81,6 +83,7 @@ class PageFeed:
         self._ids = np.concatenate([left, self._pool.allocate_many(more, reserved=False)])
         if len(self._ids) > len(self._room):
             self._room.fill_(-1)
+            self._outgrown.append((self._room, self.drawn))  # (graphs may still read them)
             self._make_room()
         self._put()
 

@@ -166,3 +166,22 @@ def test_steps_on_another_stream(gpu):
     assert pool.used == 8
     torch.cuda.synchronize()
     assert in_tables(tables, torch.full((2,), 2, **I32)) == [4, 5, 6, 7]
+
+
+def test_a_captured_step_after_the_feed_outgrew_its_tensors(gpu):
+    """It finds no page, whatever was allocated since."""
+    feed = PageFeed(make(256), "main", 4)
+    tables, counts = torch.zeros((2, 8), **I32), torch.full((2,), 5, **I32)
+    new = lambda n: torch.zeros(n, **I32)  # noqa: E731
+    out = StepRows(new(3), new(2), new(2), feed.drawn, new(10), new(10), None)
+    zero = new(2)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        extend_tables(tables, zero, counts, zero, feed, page_size=P, tokens=10, out=out)
+    graph.replay()
+    assert out.rows.tolist() == list(range(5)) + list(range(16, 21))
+    feed.refill(100)
+    others = [torch.full((4,), 7, **I32) for _ in range(64)]
+    graph.replay()
+    assert out.rows.tolist() == [-1] * 10 and tables[:, 0].tolist() == [-1, -1]
+    assert feed.drawn.tolist() == [0, 0] and len(others) == 64

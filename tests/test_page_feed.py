@@ -1,5 +1,8 @@
 """A PageFeed and the calls that take it: what is refused, on the CPU."""
 
+import gc
+import weakref
+
 import pytest
 import torch
 
@@ -49,3 +52,14 @@ def test_refill_and_close_stay_in_place():
     assert c.pools["a"].free == 32 - 13
     feed.refill(3)  # a closed feed may go on
     assert feed.pages.tolist() == [13, 14, 15]
+
+
+def test_outgrown_tensors_stay():
+    """A graph captured on them holds addresses alone."""
+    feed = paging.PageFeed(cache(), "a", 4)
+    drawn = weakref.ref(feed.drawn)
+    address = feed.pages.data_ptr()
+    feed.refill(9)
+    gc.collect()
+    assert drawn() is not None and feed._outgrown[0][0].data_ptr() == address
+    assert feed._outgrown[0][0].tolist() == [-1] * 4
